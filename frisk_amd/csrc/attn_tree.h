@@ -1,0 +1,69 @@
+// Attention of new tokens over a cache of keys and values: what its kernels
+// share (attn_tree_rows.hip, attn_tree_mfma.h).
+#pragma once
+
+#include "kvcache.h"
+
+namespace frisk {
+namespace tree {
+
+constexpr int kBlock = plan::kTreeBlock;  // keys per block
+constexpr float kLog2eF = 1.4426950408889634f;
+constexpr float kLn2F = 0.6931471805599453f;
+
+// The rows of a launch with several key splits: O (f32, not divided by l),
+// then m (exp2 domain) and l, for row (b * heads + h) * tokens + t.
+struct Part {
+  float* o;   // [rows][splits][head_dim]
+  float* ml;  // [rows][splits][2]
+  int splits;
+  int min_blocks;  // a split has at least so many blocks
+};
+
+// Blocks per split of a sequence with `keys` keys: the launch's splits, or
+// fewer where they would fall short.
+__device__ __forceinline__ int blocks_per_split(const Part& p, int blocks) {
+  return max(p.min_blocks, (blocks + p.splits - 1) / p.splits);
+}
+
+// Whether new token t sees draft j.
+__device__ __forceinline__ bool sees(const TreeAttnArgs& a, int64_t b, int t, int j) {
+  if (!a.mask) return j <= t;
+  return (a.mask[b * a.mask_sb + t * a.mask_st + (j >> 6)] >> (j & 63)) & 1;
+}
+
+// Keys of sequence b that exist: up to the last new one, and the capacity.
+__device__ __forceinline__ int keys_of(const TreeAttnArgs& a, const kv::Span& sp) {
+  return (int)min(sp.ctx + sp.fresh, a.cache.capacity);
+}
+
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+// Natural-log sum from the exp2-domain maximum and the sum.
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.0f ? -__builtin_inff() : (m + __log2f(l)) * kLn2F;
+}
+
+template <Elt T> __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (T == Elt::BF16) {
+    return f32x2_to_bf16x2_bits(lo, hi);
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 v = {(_Float16)lo, (_Float16)hi};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
+// Four dims of an output row, in Q's type or f32.
+template <Elt T>
+__device__ __forceinline__ void store4(const TreeAttnArgs& a, int64_t at, f32x4 v) {
+  if (a.out == Elt::F32) *(f32x4*)((float*)a.o + at) = v;
+  else *(i32x2*)((uint16_t*)a.o + at) = i32x2{(int)pack16<T>(v[0], v[1]), (int)pack16<T>(v[2], v[3])};
+}
+
+}  // namespace tree
+
+// The launches of attn_tree_rows.hip: any head_dim, and the sum over splits.
+hipError_t tree_attn_rows(const TreeAttnArgs& a, const tree::Part& p, hipStream_t s);
+hipError_t tree_attn_sum(const TreeAttnArgs& a, const tree::Part& p, hipStream_t s);
+
+}  // namespace frisk

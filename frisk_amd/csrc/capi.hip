@@ -744,6 +744,423 @@ int frisk_probe_lds_transpose(int bits, uint16_t* out, int64_t out_elems, void* 
 
 }  // extern "C"
 
+namespace {
+
+// Sizes n and strides of three dims around rows of one length (elements).
+struct Rows {
+  const void* p;
+  int64_t n[3], s[3];
+};
+
+// Whether i * strides of a and j * strides of b, `gap` apart, meet within a
+// row: the dims d[0 .. k) by falling stride, equal in both.
+bool rows_meet(int64_t gap, const Rows& a, const Rows& b, const int* d, int k, int64_t row) {
+  if (k == 0) return gap < row && gap > -row;
+  const int64_t s = a.s[*d];
+  const int64_t q = gap >= 0 ? gap / s : -((-gap + s - 1) / s);
+  for (const int64_t i : {q, q + 1})  // index in a less index in b
+    if (i < a.n[*d] && -i < b.n[*d] && rows_meet(gap - i * s, a, b, d + 1, k - 1, row)) return true;
+  return false;
+}
+
+// Whether the rows of two tensors may share memory.  Exact for equal strides
+// each at least the extent of the dims below it (heads of one buffer); other
+// tensors must not reach into each other's range.
+bool rows_share(const Rows& a, const Rows& b, int64_t row, int es) {
+  int64_t ea = row, eb = row;
+  for (int i = 0; i < 3; ++i) ea += (a.n[i] - 1) * a.s[i], eb += (b.n[i] - 1) * b.s[i];
+  const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+  if (pa >= pb + (uintptr_t)(eb * es) || pb >= pa + (uintptr_t)(ea * es)) return false;
+  const int64_t bytes = (int64_t)(pb - pa);
+  int d[3], k = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (a.n[i] == 1 && b.n[i] == 1) continue;
+    if (a.s[i] != b.s[i] || a.s[i] == 0) return true;
+    d[k++] = i;
+  }
+  std::sort(d, d + k, [&](int i, int j) { return a.s[i] > a.s[j]; });
+  int64_t below = row;
+  for (int i = k - 1; i >= 0; --i) {
+    if (a.s[d[i]] < below) return true;
+    below += (std::max(a.n[d[i]], b.n[d[i]]) - 1) * a.s[d[i]];
+  }
+  if (bytes % es) return true;
+  return rows_meet(bytes / es, a, b, d, k, row);
+}
+// Sizes that keep every offset the kernels form inside 63 bits.
+constexpr int64_t kMaxDim = (int64_t)1 << 31, kMaxStride = (int64_t)1 << 40;
+
+int check_rope_tensor(const char* name, int64_t batch, int64_t heads, int64_t seq, int64_t head_dim,
+                      int es, const void* x, const int64_t (&xs)[3], void* out,
+                      const int64_t (&os)[3], frisk::RopeTensor& t) {
+  if (!x || !out) return fail(FRISK_EINVAL, "frisk_rope: null %s", name);
+  if ((uintptr_t)x % es || (uintptr_t)out % es)
+    return fail(FRISK_EINVAL, "frisk_rope: pointers must be element-aligned");
+  const int64_t n[3] = {batch, heads, seq};
+  for (int i = 0; i < 3; ++i) {
+    if (xs[i] < 0 || os[i] < 0 || xs[i] > kMaxStride || os[i] > kMaxStride)
+      return fail(FRISK_EINVAL, "frisk_rope: strides must be non-negative, up to 2^40 elements");
+    if (n[i] > 1 && os[i] < head_dim)
+      return fail(FRISK_EINVAL, "frisk_rope: the rows of %s's output overlap (stride %lld < head_dim %lld)",
+                  name, (long long)os[i], (long long)head_dim);
+  }
+  bool same = x == out;
+  for (int i = 0; i < 3; ++i) same = same && (n[i] == 1 || xs[i] == os[i]);
+  const Rows in{x, {batch, heads, seq}, {xs[0], xs[1], xs[2]}};
+  const Rows to{out, {batch, heads, seq}, {os[0], os[1], os[2]}};
+  if (!same && rows_share(in, to, head_dim, es))
+    return fail(FRISK_EINVAL, "frisk_rope: %s and its output overlap (in place: one pointer and its "
+                              "strides)", name);
+  t = {x, xs[0], xs[1], xs[2], out, os[0], os[1], os[2], (int)heads};
+  return FRISK_OK;
+}
+
+// Checks of a cache; 0 or an error code.
+int check_cache(const frisk_kv_cache& d, const char* fn, bool ptrs, int64_t batch, frisk::KvCache& c) {
+  if (d.pages <= 0 || d.kv_heads <= 0 || d.page_size <= 0 || d.head_dim <= 0)
+    return fail(FRISK_EINVAL, "%s: cache sizes must be positive", fn);
+  if (d.dtype != FRISK_BF16 && d.dtype != FRISK_F16 && d.dtype != FRISK_E4M3 && d.dtype != FRISK_I8)
+    return fail(FRISK_EINVAL, "%s: cache dtype must be bf16, f16, e4m3 or i8 (got %s)", fn,
+                dtype_name(d.dtype));
+  const int es = esize(d.dtype);
+  const bool k8 = es == 1;
+  if (d.head_dim % 16 || d.head_dim > 256)
+    return fail(FRISK_EUNSUP, "%s: head_dim %lld not supported (multiples of 16 up to 256)", fn,
+                (long long)d.head_dim);
+  if (d.pages >= kMaxDim || d.page_size >= kMaxDim || d.kv_heads >= 65536)
+    return fail(FRISK_EUNSUP, "%s: cache sizes beyond the kernels' index range", fn);
+  const int64_t n[3] = {d.pages, d.kv_heads, d.page_size};
+  const int64_t st[3] = {d.stride_page, d.stride_head, d.stride_slot};
+  const int64_t sc[3] = {d.scale_stride_page, d.scale_stride_head, d.scale_stride_slot};
+  for (int i = 0; i < 3; ++i) {
+    if (st[i] < 0 || st[i] > kMaxStride || (st[i] * es) % 16 || (n[i] > 1 && st[i] < d.head_dim))
+      return fail(FRISK_EINVAL, "%s: cache strides must be multiples of 16 bytes, at least head_dim "
+                                "and up to 2^40 elements", fn);
+    if (k8 && (sc[i] < 0 || sc[i] > kMaxStride || (n[i] > 1 && sc[i] < 1)))
+      return fail(FRISK_EINVAL, "%s: scale strides must be 1 to 2^40 elements", fn);
+  }
+  if (ptrs && (!d.k || !d.v)) return fail(FRISK_EINVAL, "%s: null cache", fn);
+  if (!aligned16(d.k) || !aligned16(d.v))
+    return fail(FRISK_EINVAL, "%s: the cache must be 16-byte aligned", fn);
+  if (ptrs && k8 && (!d.k_scale || !d.v_scale))
+    return fail(FRISK_EINVAL, "%s: an 8-bit cache needs k_scale and v_scale", fn);
+  if (!k8 && (d.k_scale || d.v_scale))
+    return fail(FRISK_EINVAL, "%s: scales are for 8-bit caches", fn);
+  if ((uintptr_t)d.k_scale % 4 || (uintptr_t)d.v_scale % 4 || (uintptr_t)d.block_table % 4)
+    return fail(FRISK_EINVAL, "%s: scales and block_table must be 4-byte aligned", fn);
+  c.page_shift = 0;
+  c.capacity = d.page_size;
+  if (d.block_table) {
+    if (d.page_size & (d.page_size - 1))
+      return fail(FRISK_EUNSUP, "%s: pages of a block table hold a power of two keys (got %lld)", fn,
+                  (long long)d.page_size);
+    if (d.max_pages <= 0 || d.table_stride < 0 || d.table_stride > kMaxStride ||
+        (batch > 1 && d.table_stride < d.max_pages))
+      return fail(FRISK_EINVAL, "%s: block_table needs max_pages > 0 and rows of at least that", fn);
+    while (((int64_t)1 << c.page_shift) < d.page_size) ++c.page_shift;
+    if (d.max_pages > (kMaxDim >> c.page_shift))
+      return fail(FRISK_EUNSUP, "%s: a sequence of more than 2^31 keys", fn);
+    c.capacity = d.max_pages << c.page_shift;
+  } else if (batch > d.pages) {
+    return fail(FRISK_EINVAL, "%s: without a block table every sequence needs its page (%lld > %lld)",
+                fn, (long long)batch, (long long)d.pages);
+  }
+  if (c.capacity > INT32_MAX - 8192)
+    return fail(FRISK_EUNSUP, "%s: a sequence of more than 2^31 - 8193 keys", fn);
+  c.kind = (frisk::Elt)d.dtype;
+  c.pages = (int)d.pages;
+  c.kv_heads = (int)d.kv_heads;
+  c.head_dim = (int)d.head_dim;
+  c.k = d.k; c.v = d.v;
+  c.sp = st[0]; c.sh = st[1]; c.ss = st[2];
+  c.k_scale = d.k_scale; c.v_scale = d.v_scale;
+  c.scp = sc[0]; c.sch = sc[1]; c.scs = sc[2];
+  c.table = d.block_table;
+  c.table_stride = d.table_stride;
+  return FRISK_OK;
+}
+
+int check_kv(const frisk_kv_desc* d, const char* fn, bool write, frisk::KvArgs& a) {
+  if (!d) return fail(FRISK_EINVAL, "%s: null descriptor", fn);
+  if (d->batch <= 0 || d->tokens <= 0) return fail(FRISK_EINVAL, "%s: sizes must be positive", fn);
+  if (d->batch >= kMaxDim || d->tokens >= kMaxDim)
+    return fail(FRISK_EUNSUP, "%s: sizes beyond the kernels' index range", fn);
+  if (d->dtype != FRISK_BF16 && d->dtype != FRISK_F16)
+    return fail(FRISK_EINVAL, "%s: dtype must be bf16 or f16 (got %s)", fn, dtype_name(d->dtype));
+  const int rc = check_cache(d->cache, fn, true, d->batch, a.cache);
+  if (rc) return rc;
+  if (esize(d->cache.dtype) == 2 && d->cache.dtype != d->dtype)
+    return fail(FRISK_EINVAL, "%s: a %s cache takes and gives that type (got %s)", fn,
+                dtype_name(d->cache.dtype), dtype_name(d->dtype));
+  if (!d->k || !d->v || !d->ctx_len) return fail(FRISK_EINVAL, "%s: null tensor", fn);
+  if (!aligned16(d->k) || !aligned16(d->v))
+    return fail(FRISK_EINVAL, "%s: k and v must be 16-byte aligned", fn);
+  if ((uintptr_t)d->ctx_len % 4 || (uintptr_t)d->new_len % 4)
+    return fail(FRISK_EINVAL, "%s: ctx_len and new_len must be 4-byte aligned", fn);
+  const int64_t n[3] = {d->batch, d->cache.kv_heads, d->tokens};
+  const int64_t st[2][3] = {{d->k_stride_b, d->k_stride_h, d->k_stride_s},
+                            {d->v_stride_b, d->v_stride_h, d->v_stride_s}};
+  for (int j = 0; j < 2; ++j)
+    for (int i = 0; i < 3; ++i) {
+      if (st[j][i] < 0 || st[j][i] > kMaxStride || st[j][i] % 8)
+        return fail(FRISK_EINVAL, "%s: strides must be non-negative multiples of 8 elements, up to "
+                                  "2^40", fn);
+      if (!write && n[i] > 1 && st[j][i] < d->cache.head_dim)
+        return fail(FRISK_EINVAL, "%s: the rows of k or v overlap", fn);
+    }
+  if (d->tokens > (((int64_t)1 << 46) / d->batch) / d->cache.kv_heads)
+    return fail(FRISK_EUNSUP, "%s: sizes beyond the kernels' index range", fn);
+  a.dtype = (frisk::Elt)d->dtype;
+  a.batch = d->batch; a.tokens = d->tokens;
+  a.k = d->k; a.ksb = st[0][0]; a.ksh = st[0][1]; a.kss = st[0][2];
+  a.v = d->v; a.vsb = st[1][0]; a.vsh = st[1][1]; a.vss = st[1][2];
+  a.ctx_len = d->ctx_len;
+  a.new_len = d->new_len;
+  return FRISK_OK;
+}
+
+int kv_call(const frisk_kv_desc* d, bool write, void* stream) {
+  const char* fn = write ? "frisk_kv_append" : "frisk_kv_read";
+  g_last_error.clear();
+  frisk::KvArgs a;
+  const int rc = check_kv(d, fn, write, a);
+  if (rc) return rc;
+  clear_stale_error();
+  const hipError_t e = write ? frisk::kv_append(a, (hipStream_t)stream) : frisk::kv_read(a, (hipStream_t)stream);
+  if (e == hipErrorInvalidConfiguration)
+    return fail(FRISK_EUNSUP, "%s: more rows than one launch takes", fn);
+  if (e != hipSuccess) return hip_fail(e, write ? "frisk_kv_append launch" : "frisk_kv_read launch");
+  return FRISK_OK;
+}
+
+// Checks of the tree attention entries; 0 or an error code.  With ptrs ==
+// false the tensors are not required.
+int check_tree(const frisk_tree_attn_desc* d, bool ptrs, frisk::TreeAttnArgs& a) {
+  const char* fn = "frisk_tree_attn";
+  if (!d) return fail(FRISK_EINVAL, "%s: null descriptor", fn);
+  if (d->batch <= 0 || d->heads <= 0 || d->tokens <= 0)
+    return fail(FRISK_EINVAL, "%s: sizes must be positive", fn);
+  if (d->dtype != FRISK_BF16 && d->dtype != FRISK_F16)
+    return fail(FRISK_EINVAL, "%s: dtype must be bf16 or f16 (got %s)", fn, dtype_name(d->dtype));
+  if (d->o_dtype != d->dtype && d->o_dtype != FRISK_F32)
+    return fail(FRISK_EINVAL, "%s: o_dtype must be q's dtype or f32 (got %s)", fn,
+                dtype_name(d->o_dtype));
+  const int rc = check_cache(d->cache, fn, ptrs, d->batch, a.cache);
+  if (rc) return rc;
+  if (esize(d->cache.dtype) == 2 && d->cache.dtype != d->dtype)
+    return fail(FRISK_EINVAL, "%s: a %s cache needs q of that type (got %s)", fn,
+                dtype_name(d->cache.dtype), dtype_name(d->dtype));
+  if (d->heads % d->cache.kv_heads)
+    return fail(FRISK_EINVAL, "%s: heads %lld is no multiple of kv_heads %lld", fn,
+                (long long)d->heads, (long long)d->cache.kv_heads);
+  if (d->heads >= 65536 || d->tokens > INT32_MAX / 4 ||
+      d->tokens > (int64_t)UINT32_MAX / 256 / d->heads ||
+      d->batch > (int64_t)UINT32_MAX / 256 / (d->heads * d->tokens))
+    return fail(FRISK_EUNSUP, "%s: more than 2^24 - 1 query rows", fn);
+  if (ptrs && (!d->q || !d->o || !d->ctx_len)) return fail(FRISK_EINVAL, "%s: null tensor", fn);
+  if (!aligned16(d->q) || !aligned16(d->o))
+    return fail(FRISK_EINVAL, "%s: q and o must be 16-byte aligned", fn);
+  if ((uintptr_t)d->ctx_len % 4 || (uintptr_t)d->new_len % 4 || (uintptr_t)d->lse % 4 ||
+      (uintptr_t)d->mask % 8)
+    return fail(FRISK_EINVAL, "%s: lengths and lse must be 4-byte, mask 8-byte aligned", fn);
+  const int64_t n[3] = {d->batch, d->heads, d->tokens};
+  const int64_t qs[3] = {d->q_stride_b, d->q_stride_h, d->q_stride_s};
+  const int64_t os[3] = {d->o_stride_b, d->o_stride_h, d->o_stride_s};
+  for (int i = 0; i < 3; ++i) {
+    if (qs[i] < 0 || os[i] < 0 || qs[i] > kMaxStride || os[i] > kMaxStride || qs[i] % 8 || os[i] % 8)
+      return fail(FRISK_EINVAL, "%s: strides must be non-negative multiples of 8 elements, up to 2^40", fn);
+    if (n[i] > 1 && os[i] < d->cache.head_dim)
+      return fail(FRISK_EINVAL, "%s: the rows of o overlap", fn);
+  }
+  if (d->mask && (d->mask_stride_b < 0 || d->mask_stride_t < 0 || d->mask_stride_b > kMaxStride ||
+                  d->mask_stride_t > kMaxStride))
+    return fail(FRISK_EINVAL, "%s: mask strides must be non-negative, up to 2^40 words", fn);
+  if (!(d->sm_scale > 0.0f) || !__builtin_isfinite(d->sm_scale))
+    return fail(FRISK_EINVAL, "%s: sm_scale must be positive and finite", fn);
+  if (d->max_ctx < 0) return fail(FRISK_EINVAL, "%s: negative max_ctx", fn);
+  if (d->workspace_bytes < 0) return fail(FRISK_EINVAL, "%s: negative workspace_bytes", fn);
+  a.dtype = (frisk::Elt)d->dtype;
+  a.out = (frisk::Elt)d->o_dtype;
+  a.batch = d->batch;
+  a.heads = (int)d->heads;
+  a.tokens = (int)d->tokens;
+  a.sm_scale = d->sm_scale;
+  a.q = d->q; a.q_sb = qs[0]; a.q_sh = qs[1]; a.q_ss = qs[2];
+  a.o = d->o; a.o_sb = os[0]; a.o_sh = os[1]; a.o_ss = os[2];
+  a.lse = d->lse;
+  a.ctx_len = d->ctx_len;
+  a.new_len = d->new_len;
+  a.mask = d->mask; a.mask_sb = d->mask_stride_b; a.mask_st = d->mask_stride_t;
+  const int64_t keys = d->max_ctx ? std::min(d->max_ctx + d->tokens, a.cache.capacity) : a.cache.capacity;
+  a.splits = frisk::plan::tree_splits(d->batch * d->heads * d->tokens, keys, frisk::device_cus());
+  a.workspace = nullptr;
+  return FRISK_OK;
+}
+
+int64_t tree_workspace(const frisk::TreeAttnArgs& a) {
+  return frisk::plan::tree_workspace(a.batch * a.heads * a.tokens, a.splits, a.cache.head_dim);
+}
+
+}  // namespace
+
+extern "C" {
+
+int frisk_rope(const frisk_rope_desc* d, void* stream) {
+  g_last_error.clear();
+  if (!d) return fail(FRISK_EINVAL, "frisk_rope: null descriptor");
+  if (d->batch <= 0 || d->seq <= 0 || d->heads <= 0 || d->head_dim <= 0 || d->rot_dim <= 0 ||
+      (d->k && d->k_heads <= 0))
+    return fail(FRISK_EINVAL, "frisk_rope: sizes must be positive");
+  if (d->dtype != FRISK_F32 && d->dtype != FRISK_F16 && d->dtype != FRISK_BF16)
+    return fail(FRISK_EINVAL, "frisk_rope: dtype must be f32, f16 or bf16 (got %s)", dtype_name(d->dtype));
+  if (d->rot_dim % 2 || d->rot_dim > d->head_dim)
+    return fail(FRISK_EINVAL, "frisk_rope: rot_dim %lld must be even and at most head_dim %lld",
+                (long long)d->rot_dim, (long long)d->head_dim);
+  if ((d->interleaved & ~1) || (d->backward & ~1))
+    return fail(FRISK_EINVAL, "frisk_rope: interleaved and backward must be 0 or 1");
+  if (!__builtin_isfinite(d->amplitude))
+    return fail(FRISK_EINVAL, "frisk_rope: amplitude must be finite");
+  if (!d->frequencies || (uintptr_t)d->frequencies % 8)
+    return fail(FRISK_EINVAL, "frisk_rope: frequencies must be an 8-byte aligned device array");
+  if (d->positions && d->position_bits != 32 && d->position_bits != 64)
+    return fail(FRISK_EINVAL, "frisk_rope: position_bits must be 32 or 64 (got %d)", (int)d->position_bits);
+  if (d->positions && (uintptr_t)d->positions % (d->position_bits / 8))
+    return fail(FRISK_EINVAL, "frisk_rope: positions must be element-aligned");
+  if ((uintptr_t)d->start % 4) return fail(FRISK_EINVAL, "frisk_rope: start must be 4-byte aligned");
+  if (d->pos_stride_b < 0 || d->pos_stride_s < 0 || d->pos_stride_b > kMaxStride || d->pos_stride_s > kMaxStride)
+    return fail(FRISK_EINVAL, "frisk_rope: position strides must be non-negative, up to 2^40");
+  if (d->batch >= kMaxDim || d->seq >= kMaxDim || d->batch * d->seq >= ((int64_t)1 << 40) ||
+      d->heads > 32767 || (d->k && d->k_heads > 32767) || d->head_dim > 4096)
+    return fail(FRISK_EUNSUP, "frisk_rope: sizes beyond the kernels' limits (2^40 tokens, 32767 "
+                              "heads, head_dim 4096)");
+  frisk::RopeArgs a;
+  const int es = esize(d->dtype);
+  const int64_t xs[3] = {d->x_stride_b, d->x_stride_h, d->x_stride_s};
+  const int64_t os[3] = {d->out_stride_b, d->out_stride_h, d->out_stride_s};
+  int rc = check_rope_tensor("x", d->batch, d->heads, d->seq, d->head_dim, es, d->x, xs, d->out, os, a.t[0]);
+  if (rc) return rc;
+  a.t[1] = frisk::RopeTensor{};
+  if (d->k) {
+    const int64_t ks[3] = {d->k_stride_b, d->k_stride_h, d->k_stride_s};
+    const int64_t kos[3] = {d->k_out_stride_b, d->k_out_stride_h, d->k_out_stride_s};
+    rc = check_rope_tensor("k", d->batch, d->k_heads, d->seq, d->head_dim, es, d->k, ks, d->k_out, kos, a.t[1]);
+    if (rc) return rc;
+    auto rows = [&](const void* p, int64_t heads, const int64_t (&st)[3]) {
+      return Rows{p, {d->batch, heads, d->seq}, {st[0], st[1], st[2]}};
+    };
+    const Rows x = rows(d->x, d->heads, xs), o = rows(d->out, d->heads, os);
+    const Rows k = rows(d->k, d->k_heads, ks), ko = rows(d->k_out, d->k_heads, kos);
+    if (rows_share(o, k, d->head_dim, es) || rows_share(x, ko, d->head_dim, es) ||
+        rows_share(o, ko, d->head_dim, es))
+      return fail(FRISK_EINVAL, "frisk_rope: the output of x or k overlaps the other tensor");
+  }
+  a.dtype = (frisk::Elt)d->dtype;
+  a.batch = d->batch; a.seq = d->seq;
+  a.head_dim = (int)d->head_dim; a.rot_dim = (int)d->rot_dim;
+  a.interleaved = d->interleaved; a.backward = d->backward;
+  a.amplitude = d->amplitude;
+  a.positions = d->positions; a.position_bits = d->position_bits;
+  a.pos_sb = d->pos_stride_b; a.pos_ss = d->pos_stride_s;
+  a.start = d->start;
+  a.freq = d->frequencies;
+  clear_stale_error();
+  const hipError_t e = frisk::rope(a, (hipStream_t)stream);
+  if (e == hipErrorInvalidConfiguration)
+    return fail(FRISK_EUNSUP, "frisk_rope: more tokens than one launch takes");
+  if (e != hipSuccess) return hip_fail(e, "frisk_rope launch");
+  return FRISK_OK;
+}
+
+int frisk_rope_frequencies(int64_t rot_dim, double base, int32_t scaling, double factor,
+                           double trained, double fast, double slow, uint64_t* out) {
+  g_last_error.clear();
+  const char* fn = "frisk_rope_frequencies";
+  const double pi = 3.14159265358979323846;
+  if (rot_dim <= 0 || rot_dim % 2 || rot_dim > 4096)
+    return fail(FRISK_EINVAL, "%s: rot_dim must be even, 2 to 4096 (got %lld)", fn, (long long)rot_dim);
+  if (!out) return fail(FRISK_EINVAL, "%s: null output", fn);
+  if (!(base > 1.0) || !std::isfinite(base)) return fail(FRISK_EINVAL, "%s: base must be above 1", fn);
+  if (scaling < FRISK_ROPE_NONE || scaling > FRISK_ROPE_INDEX)
+    return fail(FRISK_EINVAL, "%s: unknown scaling %d", fn, (int)scaling);
+  if (scaling != FRISK_ROPE_NONE && (!(factor >= 1.0) || !std::isfinite(factor)))
+    return fail(FRISK_EINVAL, "%s: factor must be at least 1", fn);
+  if (scaling == FRISK_ROPE_BASE && rot_dim == 2)
+    return fail(FRISK_EINVAL, "%s: a scaled base needs rot_dim above 2", fn);
+  if (scaling >= FRISK_ROPE_TURNS && (!(trained > 0.0) || !std::isfinite(trained) || !(slow > 0.0) ||
+                                      !(fast > slow) || !std::isfinite(fast)))
+    return fail(FRISK_EINVAL, "%s: trained > 0 and fast > slow > 0 are needed", fn);
+  if (scaling == FRISK_ROPE_BASE) base *= std::pow(factor, (double)rot_dim / (double)(rot_dim - 2));
+  // The (real) pair index whose frequency turns n times in the trained length.
+  auto index_of = [&](double n) { return rot_dim * std::log(trained / (2.0 * pi * n)) / (2.0 * std::log(base)); };
+  double lo = 0.0, hi = 0.0;
+  if (scaling == FRISK_ROPE_INDEX) {
+    lo = std::min(std::max(std::floor(index_of(fast)), 0.0), (double)(rot_dim - 1));
+    hi = std::min(std::max(std::ceil(index_of(slow)), 0.0), (double)(rot_dim - 1));
+    hi = std::max(hi, lo + 0.001);
+  }
+  for (int64_t i = 0; i < rot_dim / 2; ++i) {
+    double f = std::pow(base, -2.0 * (double)i / (double)rot_dim);
+    double keep = 1.0;  // of f, the rest of f / factor
+    if (scaling == FRISK_ROPE_LINEAR) keep = 0.0;
+    else if (scaling == FRISK_ROPE_TURNS) keep = (trained * f / (2.0 * pi) - slow) / (fast - slow);
+    else if (scaling == FRISK_ROPE_INDEX) keep = 1.0 - ((double)i - lo) / (hi - lo);
+    keep = std::min(std::max(keep, 0.0), 1.0);
+    if (keep < 1.0) f = keep * f + (1.0 - keep) * f / factor;
+    // f <= 1 radian: below 2^62 of the 2^64 units of a turn.
+    out[i] = (uint64_t)std::nearbyint(std::ldexp(f / (2.0 * pi), 64));
+  }
+  return FRISK_OK;
+}
+
+int frisk_kv_append(const frisk_kv_desc* d, void* stream) { return kv_call(d, true, stream); }
+int frisk_kv_read(const frisk_kv_desc* d, void* stream) { return kv_call(d, false, stream); }
+
+int frisk_tree_mask(int64_t batch, int64_t tokens, const int32_t* parents, uint64_t* mask,
+                    int32_t* depth, void* stream) {
+  g_last_error.clear();
+  if (batch <= 0 || tokens <= 0) return fail(FRISK_EINVAL, "frisk_tree_mask: sizes must be positive");
+  if (tokens > 4096 || batch > (int64_t)UINT32_MAX / 256)
+    return fail(FRISK_EUNSUP, "frisk_tree_mask: up to 4096 tokens and 2^24 - 1 trees");
+  if (!parents || !mask) return fail(FRISK_EINVAL, "frisk_tree_mask: null tensor");
+  if ((uintptr_t)parents % 4 || (uintptr_t)mask % 8 || (uintptr_t)depth % 4)
+    return fail(FRISK_EINVAL, "frisk_tree_mask: pointers must be element-aligned");
+  clear_stale_error();
+  const hipError_t e = frisk::tree_mask(batch, (int)tokens, parents, mask, depth, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "frisk_tree_mask launch");
+  return FRISK_OK;
+}
+
+int64_t frisk_tree_attn_workspace_size(const frisk_tree_attn_desc* d) {
+  g_last_error.clear();
+  frisk::TreeAttnArgs a;
+  const int rc = check_tree(d, false, a);
+  return rc ? rc : tree_workspace(a);
+}
+
+int frisk_tree_attn(const frisk_tree_attn_desc* d, void* stream) {
+  g_last_error.clear();
+  frisk::TreeAttnArgs a;
+  const int rc = check_tree(d, true, a);
+  if (rc) return rc;
+  const int64_t need = tree_workspace(a);
+  if (!d->workspace) {
+    a.splits = 1;
+  } else if (need > 0) {
+    if (d->workspace_bytes < need)
+      return fail(FRISK_EINVAL, "frisk_tree_attn: workspace of %lld bytes, this call takes %lld",
+                  (long long)d->workspace_bytes, (long long)need);
+    if (!aligned16(d->workspace))
+      return fail(FRISK_EINVAL, "frisk_tree_attn: workspace must be 16-byte aligned");
+    a.workspace = d->workspace;
+  }
+  clear_stale_error();
+  const hipError_t e = frisk::tree_attn(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "frisk_tree_attn launch");
+  return FRISK_OK;
+}
+
+}  // extern "C"
+
 // ---------------------------------------------------------------------------
 // Allocation-free GEMM.  frisk_gemm_noalloc runs exactly what frisk_gemm
 // runs with a workspace of frisk_gemm_workspace_size() bytes, but its

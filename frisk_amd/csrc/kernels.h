@@ -194,6 +194,84 @@ struct FillArgs {
 };
 hipError_t tile_fill(const FillArgs& a, hipStream_t s);
 
+// Rotary positions (rope.hip).  One tensor [batch, heads, seq, head_dim]; x
+// and out may be the same.
+struct RopeTensor {
+  const void* x;
+  int64_t sb, sh, ss;
+  void* out;
+  int64_t osb, osh, oss;
+  int heads;
+};
+struct RopeArgs {
+  Elt dtype;  // F32, F16 or BF16
+  int64_t batch, seq;
+  int head_dim, rot_dim;
+  int interleaved, backward;
+  float amplitude;
+  RopeTensor t[2];  // t[1].heads == 0: one tensor
+  const void* positions;  // null: s
+  int position_bits;      // 32 or 64
+  int64_t pos_sb, pos_ss;
+  const int32_t* start;  // null: 0
+  const uint64_t* freq;
+};
+hipError_t rope(const RopeArgs& a, hipStream_t s);
+
+// A validated cache of keys and values (kvcache.h has the device side).
+// Strides in elements.
+struct KvCache {
+  Elt kind;  // BF16, F16, E4M3 or I8
+  int pages, kv_heads, head_dim;
+  int page_shift;    // log2 of the page size with a table
+  int64_t capacity;  // keys a sequence holds
+  void* k;
+  void* v;
+  int64_t sp, sh, ss;
+  float* k_scale;
+  float* v_scale;
+  int64_t scp, sch, scs;
+  const int32_t* table;  // null: page b
+  int64_t table_stride;
+};
+struct KvArgs {
+  Elt dtype;  // of k and v: BF16 or F16
+  int64_t batch, tokens;
+  void* k;
+  int64_t ksb, ksh, kss;
+  void* v;
+  int64_t vsb, vsh, vss;
+  const int32_t* ctx_len;
+  const int32_t* new_len;  // null: tokens
+  KvCache cache;
+};
+hipError_t kv_append(const KvArgs& a, hipStream_t s);
+hipError_t kv_read(const KvArgs& a, hipStream_t s);
+hipError_t tree_mask(int64_t batch, int tokens, const int32_t* parents, uint64_t* mask,
+                     int32_t* depth, hipStream_t s);
+
+// Attention of new tokens over a cache.
+struct TreeAttnArgs {
+  Elt dtype;  // Q
+  Elt out;    // dtype or F32
+  int64_t batch;
+  int heads, tokens;
+  float sm_scale;
+  const void* q;
+  int64_t q_sb, q_sh, q_ss;
+  void* o;
+  int64_t o_sb, o_sh, o_ss;
+  float* lse;
+  const int32_t* ctx_len;
+  const int32_t* new_len;
+  const uint64_t* mask;  // null: token t sees the drafts up to t
+  int64_t mask_sb, mask_st;
+  KvCache cache;
+  int splits;       // key splits; more than one needs the workspace
+  void* workspace;  // plan::tree_workspace bytes
+};
+hipError_t tree_attn(const TreeAttnArgs& a, hipStream_t s);
+
 // MFMA fragment-layout probe (probe.hip): atom 0 = bf16 32x32x16,
 // 1 = bf16 16x16x32, 2 = i8 32x32x32; `out` holds mfma_probe_floats(atom)
 // floats.

@@ -617,6 +617,21 @@ inline int64_t attn_workspace(int64_t batch_heads, int64_t seq_q, int64_t seq_k,
 }
 
 // ---------------------------------------------------------------------------
+// Attention of new tokens over a cache (attn_tree_rows.hip): key splits, so
+// that four workgroups a CU have work.  `keys`: the most a sequence may hold.
+// ---------------------------------------------------------------------------
+constexpr int kTreeBlock = 64;  // keys per block
+constexpr int tree_min_blocks() { return 4; }
+inline int tree_splits(int64_t rows, int64_t keys, int cus) {
+  const int64_t blocks = (keys + kTreeBlock - 1) / kTreeBlock;
+  const int64_t want = (4 * (int64_t)cus + rows - 1) / rows;
+  return (int)std::max<int64_t>(1, std::min({want, blocks / tree_min_blocks(), (int64_t)64}));
+}
+inline int64_t tree_workspace(int64_t rows, int splits, int64_t head_dim) {
+  return splits > 1 ? rows * splits * (head_dim + 2) * 4 : 0;
+}
+
+// ---------------------------------------------------------------------------
 // Reductions along axis 0 (tileops.hip), of [rows, cols] in slots of 4 columns.
 //
 // One pass: a workgroup of `threads` owns a strip of 2^cvb_log2 slots; its

@@ -2,7 +2,8 @@
 
 This is the Python side of the C-ABI: it fills the descriptors from torch
 device tensors and calls frisk_gemm / frisk_attn_fwd / frisk_reduce /
-frisk_copy / frisk_fill on the current HIP stream.  There is no fallback: if the library is missing or a call fails,
+frisk_copy / frisk_fill, and frisk_rope / frisk_kv_append / frisk_kv_read /
+frisk_tree_mask / frisk_tree_attn, on the current HIP stream.  There is no fallback: if the library is missing or a call fails,
 a RuntimeError (or ValueError for rejected requests, matching the
 reference's ValueError on contract violations, ffi/ir.cpp:333-341) is raised.
 """
@@ -24,9 +25,11 @@ EXPORTS = ("frisk_gemm", "frisk_gemm_workspace_size", "frisk_gemm_plan", "frisk_
            "frisk_attn_fwd", "frisk_attn_fwd_ws", "frisk_attn_workspace_size",
            "frisk_reduce", "frisk_reduce_workspace_size",
            "frisk_copy", "frisk_fill",
+           "frisk_rope", "frisk_rope_frequencies", "frisk_kv_append", "frisk_kv_read",
+           "frisk_tree_mask", "frisk_tree_attn", "frisk_tree_attn_workspace_size",
            "frisk_last_error", "frisk_abi_version", "frisk_probe_mfma_layout",
            "frisk_probe_lds_transpose")
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 REDUCE_SUM, REDUCE_MAX, REDUCE_MIN = 0, 1, 2
 REDUCE_KINDS = {"sum": REDUCE_SUM, "add": REDUCE_SUM, "max": REDUCE_MAX, "min": REDUCE_MIN}
@@ -96,6 +99,53 @@ class FillDesc(ctypes.Structure):
     ]
 
 
+_i64, _i32, _ptr = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p
+
+
+def _strides(prefix, names):
+    return [(f"{prefix}_stride_{n}", _i64) for n in names]
+
+
+class RopeDesc(ctypes.Structure):
+    _fields_ = [
+        *((n, _i64) for n in ("batch", "seq", "heads", "k_heads", "head_dim", "rot_dim")),
+        ("dtype", _i32), ("interleaved", _i32), ("backward", _i32), ("amplitude", ctypes.c_float),
+        ("x", _ptr), *_strides("x", "bhs"), ("out", _ptr), *_strides("out", "bhs"),
+        ("k", _ptr), *_strides("k", "bhs"), ("k_out", _ptr), *_strides("k_out", "bhs"),
+        ("positions", _ptr), ("position_bits", _i32), *_strides("pos", "bs"),
+        ("start", _ptr), ("frequencies", _ptr),
+    ]
+
+
+class KvCacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("pages", _i64), ("kv_heads", _i64), ("page_size", _i64), ("head_dim", _i64),
+        ("dtype", _i32), ("k", _ptr), ("v", _ptr),
+        ("stride_page", _i64), ("stride_head", _i64), ("stride_slot", _i64),
+        ("k_scale", _ptr), ("v_scale", _ptr),
+        ("scale_stride_page", _i64), ("scale_stride_head", _i64), ("scale_stride_slot", _i64),
+        ("block_table", _ptr), ("table_stride", _i64), ("max_pages", _i64),
+    ]
+
+
+class KvDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("tokens", _i64), ("dtype", _i32),
+        ("k", _ptr), *_strides("k", "bhs"), ("v", _ptr), *_strides("v", "bhs"),
+        ("ctx_len", _ptr), ("new_len", _ptr), ("cache", KvCacheDesc),
+    ]
+
+
+class TreeAttnDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("heads", _i64), ("tokens", _i64), ("dtype", _i32), ("o_dtype", _i32),
+        ("sm_scale", ctypes.c_float), ("q", _ptr), *_strides("q", "bhs"),
+        ("o", _ptr), *_strides("o", "bhs"), ("lse", _ptr), ("ctx_len", _ptr), ("new_len", _ptr),
+        ("mask", _ptr), *_strides("mask", "bt"), ("max_ctx", _i64), ("cache", KvCacheDesc),
+        ("workspace", _ptr), ("workspace_bytes", _i64),
+    ]
+
+
 _lib = None
 
 
@@ -132,6 +182,20 @@ def load() -> ctypes.CDLL:
     lib.frisk_copy.restype = ctypes.c_int
     lib.frisk_fill.argtypes = [ctypes.POINTER(FillDesc), ctypes.c_void_p]
     lib.frisk_fill.restype = ctypes.c_int
+    lib.frisk_rope.argtypes = [ctypes.POINTER(RopeDesc), ctypes.c_void_p]
+    lib.frisk_rope.restype = ctypes.c_int
+    lib.frisk_rope_frequencies.argtypes = [_i64, ctypes.c_double, _i32, *[ctypes.c_double] * 4,
+                                           ctypes.POINTER(ctypes.c_uint64)]
+    lib.frisk_rope_frequencies.restype = ctypes.c_int
+    for fn in (lib.frisk_kv_append, lib.frisk_kv_read):
+        fn.argtypes = [ctypes.POINTER(KvDesc), ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+    lib.frisk_tree_mask.argtypes = [_i64, _i64, _ptr, _ptr, _ptr, _ptr]
+    lib.frisk_tree_mask.restype = ctypes.c_int
+    lib.frisk_tree_attn.argtypes = [ctypes.POINTER(TreeAttnDesc), ctypes.c_void_p]
+    lib.frisk_tree_attn.restype = ctypes.c_int
+    lib.frisk_tree_attn_workspace_size.argtypes = [ctypes.POINTER(TreeAttnDesc)]
+    lib.frisk_tree_attn_workspace_size.restype = ctypes.c_int64
     lib.frisk_last_error.argtypes = []
     lib.frisk_last_error.restype = ctypes.c_char_p
     lib.frisk_abi_version.argtypes = []
@@ -477,3 +541,290 @@ def fill(dst, value, *, stream=None):
     _check(load().frisk_fill(ctypes.byref(d), ctypes.c_void_p(_stream_handle(stream))),
            "frisk_fill")
     return dst
+
+
+# ---- Rotary positions, the cache of keys and values, drafted trees -------------
+
+ROPE_SCALINGS = {"none": 0, "linear": 1, "base": 2, "turns": 3, "index": 4}
+
+
+def rope_table(rot_dim, base=10000.0, *, scaling="none", factor=1.0, trained=0.0, fast=32.0,
+               slow=1.0, device="cuda"):
+    """The int64 [rot_dim / 2] frequencies rope() takes, made once: turns per
+    position in units of 2^-64.  `scaling` slows them down for contexts
+    longer than the `trained` length (frisk_rope_scaling): "linear" by
+    `factor`; "base" through the base; "turns" by `factor` where a pair turns
+    at most `slow` times in the trained length, not where it turns `fast`
+    times or more, evenly in turns between; "index" the same, evenly in the
+    pair's index."""
+    import torch
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"unknown scaling {scaling!r} ({', '.join(ROPE_SCALINGS)})")
+    buf = (ctypes.c_uint64 * max(int(rot_dim) // 2, 1))()
+    _check(load().frisk_rope_frequencies(int(rot_dim), float(base), ROPE_SCALINGS[scaling],
+                                         float(factor), float(trained), float(fast), float(slow), buf),
+           "frisk_rope_frequencies")
+    return torch.tensor([v - (1 << 64) if v >> 63 else v for v in buf], dtype=torch.int64).to(device)
+
+
+def _heads(t, name: str):
+    """Shape and strides of a [batch, heads, rows, head_dim] device tensor."""
+    sh, st = t.shape, t.stride()
+    if len(sh) != 4 or not t.is_cuda or (st[3] != 1 and sh[3] > 1):
+        raise ValueError(f"{name} must be a rank-4 device tensor with unit head_dim stride")
+    return sh, st
+
+
+def _same_device(*ts):
+    """Every tensor on the first one's device, which the call runs on."""
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices ({dev} and {t.device})")
+
+
+def _lengths(t, batch: int, name: str):
+    """The pointer of an int32 [batch] device tensor, or None."""
+    import torch
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or tuple(t.shape) != (batch,) or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"{name} must be a contiguous int32 device tensor of {batch} elements")
+    return t.data_ptr()
+
+
+def _run(fn, name: str, d, device, stream):
+    """fn(d, stream) with `device` current."""
+    import torch
+    if device.index is not None and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            _check(fn(ctypes.byref(d), _stream_handle(stream)), name)
+    else:
+        _check(fn(ctypes.byref(d), _stream_handle(stream)), name)
+
+
+def rope(x, out, positions, table, *, k=None, k_out=None, start=None, interleaved=False,
+         amplitude=1.0, backward=False, stream=None):
+    """out = x [batch, heads, seq, head_dim] with its first 2 * len(table) dims
+    rotated to their positions, and k_out = k (its own number of heads)
+    likewise, in one launch.  out may be x.  `positions` (int32 or int64,
+    [seq] or [batch, seq], or None: 0 .. seq - 1) are counted from `start`
+    (int32 [batch], or None: 0).  Pairs are dims (i, i + rot_dim / 2), or
+    (2i, 2i + 1) if `interleaved`.  backward=True is the gradient: the
+    transposed rotation."""
+    import torch
+    (b, h, s, d), xs = _heads(x, "x")
+    (ob, oh, os_, od), outs = _heads(out, "out")
+    if (ob, oh, os_, od) != (b, h, s, d) or out.dtype != x.dtype:
+        raise ValueError("x and out must have one shape and dtype")
+    if (k is None) != (k_out is None):
+        raise ValueError("k and k_out go together")
+    if table.dtype != torch.int64 or table.dim() != 1 or not table.is_contiguous() or not table.is_cuda:
+        raise ValueError("table must be a contiguous int64 device tensor (rope_table)")
+    desc = RopeDesc(b, s, h, 0, d, 2 * table.shape[0], torch_dtype_code(x.dtype),
+                    int(bool(interleaved)), int(bool(backward)), float(amplitude),
+                    x.data_ptr(), xs[0], xs[1], xs[2], out.data_ptr(), outs[0], outs[1], outs[2],
+                    start=_lengths(start, b, "start"), frequencies=table.data_ptr())
+    if k is not None:
+        (kb, kh, ks_, kd), ks = _heads(k, "k")
+        kosh, kos = _heads(k_out, "k_out")
+        if (kb, ks_, kd) != (b, s, d) or tuple(kosh) != (kb, kh, ks_, kd) or k.dtype != x.dtype \
+                or k_out.dtype != x.dtype:
+            raise ValueError("k and k_out must have one shape, and x's dtype, batch, seq and head_dim")
+        desc.k_heads = kh
+        desc.k, desc.k_stride_b, desc.k_stride_h, desc.k_stride_s = k.data_ptr(), ks[0], ks[1], ks[2]
+        desc.k_out, desc.k_out_stride_b, desc.k_out_stride_h, desc.k_out_stride_s = \
+            k_out.data_ptr(), kos[0], kos[1], kos[2]
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or not positions.is_cuda or \
+                tuple(positions.shape) not in ((s,), (b, s)):
+            raise ValueError("positions must be an int32 or int64 device tensor [seq] or [batch, seq]")
+        st = positions.stride()
+        desc.positions, desc.position_bits = positions.data_ptr(), 8 * positions.element_size()
+        desc.pos_stride_b, desc.pos_stride_s = (0, st[0]) if len(st) == 1 else st
+    _same_device(x, out, k, k_out, positions, table, start)
+    _run(load().frisk_rope, "frisk_rope", desc, x.device, stream)
+    return out if k is None else (out, k_out)
+
+
+class KvCache:
+    """A cache of keys and values (frisk_kv_cache) over tensors the caller
+    owns: k and v [pages, kv_heads, page_size, head_dim] of one layout, in
+    bf16 / f16, or in float8_e4m3fn / int8 with f32 k_scale and v_scale
+    [pages, kv_heads, page_size].  `block_table` (int32 [batch, max_pages])
+    names the pages of each sequence; without it page b is sequence b's."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "block_table", "desc")
+
+    def __init__(self, k, v, k_scale=None, v_scale=None, block_table=None):
+        import torch
+        ksh, kst = _heads(k, "k")
+        vsh, vst = _heads(v, "v")
+        if tuple(ksh) != tuple(vsh) or tuple(kst) != tuple(vst) or k.dtype != v.dtype:
+            raise ValueError("k and v must have one shape, layout and dtype")
+        if k.dtype not in (torch.bfloat16, torch.float16, torch.float8_e4m3fn, torch.int8):
+            raise ValueError(f"a cache holds bf16, f16, float8_e4m3fn or int8 (got {k.dtype})")
+        if (k_scale is None) != (k.element_size() == 2) or (v_scale is None) != (k_scale is None):
+            raise ValueError("an 8-bit cache has k_scale and v_scale, a 16-bit one none")
+        sst = (0, 0, 0)
+        if k_scale is not None:
+            for t in (k_scale, v_scale):
+                if t.dtype != torch.float32 or tuple(t.shape) != tuple(ksh[:3]) or not t.is_cuda:
+                    raise ValueError("scales must be f32 device tensors [pages, kv_heads, page_size]")
+            sst = k_scale.stride()
+            if v_scale.stride() != sst:
+                raise ValueError("k_scale and v_scale must have one layout")
+        if block_table is not None and (block_table.dtype != torch.int32 or block_table.dim() != 2 or
+                                        not block_table.is_cuda or
+                                        (block_table.stride(1) != 1 and block_table.shape[1] > 1)):
+            raise ValueError("block_table must be an int32 device tensor [batch, max_pages] with unit "
+                             "stride along the pages")
+        _same_device(k, v, k_scale, v_scale, block_table)
+        self.k, self.v, self.k_scale, self.v_scale, self.block_table = k, v, k_scale, v_scale, block_table
+        self.desc = KvCacheDesc(
+            *ksh, torch_dtype_code(k.dtype), k.data_ptr(), v.data_ptr(), *kst[:3],
+            None if k_scale is None else k_scale.data_ptr(),
+            None if v_scale is None else v_scale.data_ptr(), *sst,
+            None if block_table is None else block_table.data_ptr(),
+            0 if block_table is None else block_table.stride(0),
+            0 if block_table is None else block_table.shape[1])
+
+    @classmethod
+    def empty(cls, pages, kv_heads, page_size, head_dim, dtype, *, block_table=None, device="cuda"):
+        """A cache over new tensors (their contents undefined until written)."""
+        import torch
+        shape = (pages, kv_heads, page_size, head_dim)
+        k, v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        ks = vs = None
+        if k.element_size() == 1:
+            ks, vs = (torch.empty(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
+        return cls(k, v, ks, vs, block_table)
+
+    def _rows(self, batch: int):
+        if self.block_table is not None and self.block_table.shape[0] != batch:
+            raise ValueError(f"block_table has {self.block_table.shape[0]} rows for a batch of {batch}")
+
+
+def _kv(fn, name, k, v, cache, ctx_len, new_len, stream):
+    (b, h, t, d), ks = _heads(k, "k")
+    vsh, vs = _heads(v, "v")
+    c = cache.desc
+    if tuple(vsh) != (b, h, t, d) or v.dtype != k.dtype or h != c.kv_heads or d != c.head_dim:
+        raise ValueError(f"k and v must be [batch, {c.kv_heads}, tokens, {c.head_dim}] of one dtype "
+                         f"(got {tuple(k.shape)} and {tuple(v.shape)})")
+    cache._rows(b)
+    _same_device(k, v, cache.k, ctx_len, new_len)
+    desc = KvDesc(b, t, torch_dtype_code(k.dtype), k.data_ptr(), ks[0], ks[1], ks[2],
+                  v.data_ptr(), vs[0], vs[1], vs[2], _lengths(ctx_len, b, "ctx_len"),
+                  _lengths(new_len, b, "new_len"), c)
+    _run(fn, name, desc, k.device, stream)
+
+
+def kv_append(k, v, cache, ctx_len, *, new_len=None, stream=None):
+    """Write k and v [batch, kv_heads, tokens, head_dim] (bf16 or f16) into the
+    KvCache as keys ctx_len[b] .. of each sequence (int32 [batch] on the
+    device; negative: the sequence takes no part), the first new_len[b]
+    tokens of it.  An 8-bit cache quantises each row by its largest value."""
+    _kv(load().frisk_kv_append, "frisk_kv_append", k, v, cache, ctx_len, new_len, stream)
+    return cache
+
+
+def kv_read(cache, k, v, ctx_len, *, new_len=None, stream=None):
+    """Read keys ctx_len[b] .. of each sequence back into k and v [batch,
+    kv_heads, tokens, head_dim], the first new_len[b] rows of it; the other
+    rows are left as they were."""
+    _kv(load().frisk_kv_read, "frisk_kv_read", k, v, cache, ctx_len, new_len, stream)
+    return k, v
+
+
+def tree_mask(parents, mask=None, depth=None, *, stream=None):
+    """(mask, depth) of drafted trees: parents int32 [batch, tokens] (the
+    drafted token each one continues, -1: the context) to the int64 words
+    [batch, tokens, ceil(tokens / 64)] that tree_attn takes, and the int32
+    number of drafted tokens before each ([batch, tokens]; its position is
+    ctx_len + depth)."""
+    import torch
+    if parents.dtype != torch.int32 or parents.dim() != 2 or not parents.is_contiguous() or \
+            not parents.is_cuda:
+        raise ValueError("parents must be a contiguous int32 device tensor [batch, tokens]")
+    b, t = parents.shape
+    words = (t + 63) // 64
+    if mask is None:
+        mask = torch.empty((b, t, words), dtype=torch.int64, device=parents.device)
+    if depth is None:
+        depth = torch.empty((b, t), dtype=torch.int32, device=parents.device)
+    if mask.dtype != torch.int64 or tuple(mask.shape) != (b, t, words) or not mask.is_contiguous():
+        raise ValueError(f"mask must be a contiguous int64 tensor [{b}, {t}, {words}]")
+    if depth.dtype != torch.int32 or tuple(depth.shape) != (b, t) or not depth.is_contiguous():
+        raise ValueError(f"depth must be a contiguous int32 tensor [{b}, {t}]")
+    _same_device(parents, mask, depth)
+    with torch.cuda.device(parents.device):
+        _check(load().frisk_tree_mask(b, t, parents.data_ptr(), mask.data_ptr(), depth.data_ptr(),
+                                      _stream_handle(stream)), "frisk_tree_mask")
+    return mask, depth
+
+
+def tree_attn_desc(q, cache, ctx_len, o, *, mask=None, new_len=None, sm_scale=None, lse=None,
+                   max_ctx=0) -> TreeAttnDesc:
+    """Describe tree_attn's call."""
+    import torch
+    (b, h, t, d), qs = _heads(q, "q")
+    osh, os_ = _heads(o, "o")
+    c = cache.desc
+    if tuple(osh) != (b, h, t, d) or d != c.head_dim:
+        raise ValueError(f"q and o must have one shape and the cache's head_dim {c.head_dim} "
+                         f"(got {tuple(q.shape)} and {tuple(o.shape)})")
+    if lse is not None and (tuple(lse.shape) != (b, h, t) or not lse.is_contiguous()
+                            or lse.dtype != torch.float32):
+        raise ValueError("lse must be a contiguous f32 [batch, heads, tokens] tensor")
+    cache._rows(b)
+    _same_device(q, o, cache.k, ctx_len, new_len, mask, lse)
+    desc = TreeAttnDesc(b, h, t, torch_dtype_code(q.dtype), torch_dtype_code(o.dtype),
+                        float(d ** -0.5 if sm_scale is None else sm_scale),
+                        q.data_ptr(), qs[0], qs[1], qs[2], o.data_ptr(), os_[0], os_[1], os_[2],
+                        None if lse is None else lse.data_ptr(), _lengths(ctx_len, b, "ctx_len"),
+                        _lengths(new_len, b, "new_len"), max_ctx=int(max_ctx), cache=c)
+    if mask is not None:
+        words = (t + 63) // 64
+        if mask.dtype != torch.int64 or tuple(mask.shape) not in ((t, words), (b, t, words)) or \
+                (mask.stride(-1) != 1 and words > 1):
+            raise ValueError(f"mask must be int64 words [{t}, {words}] or [{b}, {t}, {words}] (tree_mask)")
+        st = mask.stride()
+        desc.mask = mask.data_ptr()
+        desc.mask_stride_b, desc.mask_stride_t = (0, st[0]) if len(st) == 2 else st[:2]
+    return desc
+
+
+def tree_attn_workspace_bytes(desc: TreeAttnDesc) -> int:
+    """frisk_tree_attn_workspace_size for a descriptor."""
+    need = int(load().frisk_tree_attn_workspace_size(ctypes.byref(desc)))
+    _check(need if need < 0 else OK, "frisk_tree_attn_workspace_size")
+    return need
+
+
+def tree_attn(q, cache, ctx_len, o, *, mask=None, new_len=None, sm_scale=None, lse=None, max_ctx=0,
+              workspace=True, stream=None):
+    """o = softmax(sm_scale . q K^T) V of new tokens q [batch, heads, tokens,
+    head_dim] over a KvCache that holds them (kv_append) behind the ctx_len[b]
+    keys every token sees.  Among themselves token t sees draft j where bit j
+    of mask[b][t] is set (tree_mask; [tokens, words] for one tree of all
+    sequences), without a mask where j <= t; tokens from new_len[b] on are
+    left out.  `max_ctx` hints at the largest ctx_len (0: the capacity).
+    `workspace`: True allocates the scratch of the key splits (torch's
+    caching allocator, on the call's stream), a device tensor supplies it,
+    False runs unsplit."""
+    import torch
+    if q.device.index is not None and q.device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return tree_attn(q, cache, ctx_len, o, mask=mask, new_len=new_len, sm_scale=sm_scale,
+                             lse=lse, max_ctx=max_ctx, workspace=workspace, stream=stream)
+    d = tree_attn_desc(q, cache, ctx_len, o, mask=mask, new_len=new_len, sm_scale=sm_scale, lse=lse,
+                       max_ctx=max_ctx)
+    lib, ws = load(), None
+    if workspace is not False:
+        need = tree_attn_workspace_bytes(d)
+        if need > 0:
+            ws = workspace if workspace is not True else _scratch(need, o.device, stream)
+            d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+    _check(lib.frisk_tree_attn(ctypes.byref(d), _stream_handle(stream)), "frisk_tree_attn")
+    return o

@@ -31,6 +31,11 @@
  *   frisk_fill      <- frisk.fill (FriskOps.td:400-422; builder ffi/ir.cpp:
  *                      439-454).
  *
+ * Beside attention, for serving and training around it (no counterpart in the
+ * reference): frisk_rope (rotary positions), frisk_kv_append / frisk_kv_read
+ * (a cache of keys and values in 16 or 8 bits), frisk_tree_mask and
+ * frisk_tree_attn (attention of new or drafted tokens over that cache).
+ *
  * Conventions: plain pointers and sizes only; every pointer is a device
  * pointer owned by the caller; `stream` is a hipStream_t (NULL = the null
  * stream).  Calls are stream-ordered and reentrant.  Every entry returns 0
@@ -46,7 +51,7 @@
 extern "C" {
 #endif
 
-#define FRISK_ABI_VERSION 7
+#define FRISK_ABI_VERSION 8
 
 /* Element types (the dtype strings of ffi/ir.cpp:399-411 plus bf16/i8/i32). */
 typedef enum frisk_dtype {
@@ -332,6 +337,178 @@ typedef struct frisk_fill_desc {
 } frisk_fill_desc;
 
 int frisk_fill(const frisk_fill_desc* desc, void* stream);
+
+/*
+ * Rotary positions.  For pair i < rot_dim / 2 of a row at position p, with
+ * phi = 2 pi p F_i / 2^64:
+ *   (a, b) -> amplitude * (a cos phi - b sin phi, a sin phi + b cos phi)
+ * where (a, b) are dims (2i, 2i + 1) when interleaved, else (i, i + rot_dim/2).
+ * Dims rot_dim .. head_dim - 1 are copied.  backward = 1 applies the
+ * transpose (phi negated): the gradient of x from that of out.  F_i
+ * (frequencies, a device array of rot_dim / 2 words) is the pair's turns per
+ * position in units of 2^-64, as frisk_rope_frequencies fills it: p F_i mod
+ * 2^64 is the exact phase of that frequency at any 64-bit position.  The
+ * rotation runs in f32 and is rounded once.
+ *
+ * One call rotates x and, if k is not NULL, k, by the same positions: two
+ * tensors [batch, heads, seq, head_dim] of one dtype (f32, f16 or bf16), unit
+ * innermost stride, other strides in elements.  out may be x itself (the same
+ * pointer and strides); no other rows of the four tensors may overlap an
+ * output.  The position of row (b, s) is
+ * start[b] (0 if start is NULL) + positions[b * pos_stride_b + s *
+ * pos_stride_s] (s if positions is NULL).
+ */
+typedef struct frisk_rope_desc {
+  int64_t batch, seq, heads, k_heads, head_dim, rot_dim;
+  int32_t dtype; /* frisk_dtype: FRISK_F32, FRISK_F16 or FRISK_BF16 */
+  int32_t interleaved, backward;
+  float amplitude;
+  const void* x;
+  int64_t x_stride_b, x_stride_h, x_stride_s;
+  void* out;
+  int64_t out_stride_b, out_stride_h, out_stride_s;
+  const void* k; /* optional second tensor */
+  int64_t k_stride_b, k_stride_h, k_stride_s;
+  void* k_out;
+  int64_t k_out_stride_b, k_out_stride_h, k_out_stride_s;
+  const void* positions; /* optional */
+  int32_t position_bits; /* 32 or 64 (signed) */
+  int64_t pos_stride_b, pos_stride_s;
+  const int32_t* start; /* optional, [batch] */
+  const uint64_t* frequencies;
+} frisk_rope_desc;
+
+int frisk_rope(const frisk_rope_desc* desc, void* stream);
+
+/* How frisk_rope_frequencies slows frequencies down for long contexts, from
+ * f_i = base^(-2 i / rot_dim) radians a position:
+ *   NONE    f_i
+ *   LINEAR  f_i / factor
+ *   BASE    base * factor^(rot_dim / (rot_dim - 2)) in the place of base
+ *   TURNS   w f_i + (1 - w) f_i / factor, w = clamp((t_i - slow) / (fast -
+ *           slow), 0, 1), t_i = trained f_i / (2 pi): turns in the trained length
+ *   INDEX   the same with w = 1 - clamp((i - lo) / (hi - lo), 0, 1), lo and hi
+ *           the pair indices that turn fast and slow times in the trained length
+ *           (lo rounded down, hi up, both held in 0 .. rot_dim - 1, hi at least lo +
+ *           0.001) */
+typedef enum frisk_rope_scaling {
+  FRISK_ROPE_NONE = 0,
+  FRISK_ROPE_LINEAR = 1,
+  FRISK_ROPE_BASE = 2,
+  FRISK_ROPE_TURNS = 3,
+  FRISK_ROPE_INDEX = 4
+} frisk_rope_scaling;
+
+/* Fills frequencies[0 .. rot_dim / 2) (HOST memory; copy it to the device
+ * once) for frisk_rope.  trained, fast and slow are read for TURNS and INDEX. */
+int frisk_rope_frequencies(int64_t rot_dim, double base, int32_t scaling, double factor,
+                           double trained, double fast, double slow, uint64_t* frequencies);
+
+/*
+ * A cache of keys and values.  k and v are [pages, kv_heads, page_size,
+ * head_dim] with the strides below (elements, shared by k and v; head_dim
+ * stride 1).  dtype bf16 or f16 holds them as they are; e4m3 or i8 holds
+ * codes and an f32 scale for each row (page, head, slot) of k and of v: a
+ * value is code * scale.
+ * Key n of sequence b is slot n % page_size of page block_table[b *
+ * table_stride + n / page_size] (page_size a power of two), or without a
+ * table slot n of page b; a sequence holds capacity = max_pages * page_size
+ * (without a table page_size) keys.  A page number outside 0 .. pages - 1 is
+ * no page: keys there are not written, not read and not seen.  Bases, and row
+ * and stride bytes, are multiples of 16.
+ */
+typedef struct frisk_kv_cache {
+  int64_t pages, kv_heads, page_size, head_dim;
+  int32_t dtype; /* frisk_dtype: FRISK_BF16, FRISK_F16, FRISK_E4M3 or FRISK_I8 */
+  void* k;
+  void* v;
+  int64_t stride_page, stride_head, stride_slot;
+  float* k_scale; /* 8-bit types only */
+  float* v_scale;
+  int64_t scale_stride_page, scale_stride_head, scale_stride_slot;
+  const int32_t* block_table; /* optional */
+  int64_t table_stride, max_pages;
+} frisk_kv_cache;
+
+/*
+ * frisk_kv_append writes rows [batch, kv_heads, tokens, head_dim] of k and v
+ * (bf16 or f16) into the cache: token t < new_len[b] (all, if new_len is NULL)
+ * of sequence b becomes key ctx_len[b] + t.  frisk_kv_read is its inverse:
+ * those keys, as code * scale rounded to dtype, into k and v; rows from
+ * new_len[b] on, and of keys the cache does not hold, are left as they were.
+ * A sequence with ctx_len[b] < 0 takes no part.
+ * A row x of an 8-bit cache, with top Q = 448 (e4m3) or 127 (i8): a = max |x|
+ * held at least 2^-126 Q, scale = a / Q, code = x Q / a rounded to nearest
+ * even.  A row that holds an infinity or a NaN has scale NaN and codes 0: it
+ * reads back as NaN.  A 16-bit cache takes and gives its own dtype.
+ * Pages written by one call must be distinct between its sequences.
+ */
+typedef struct frisk_kv_desc {
+  int64_t batch, tokens;
+  int32_t dtype; /* frisk_dtype of k and v: FRISK_BF16 or FRISK_F16 */
+  void* k;       /* read by append, written by read */
+  int64_t k_stride_b, k_stride_h, k_stride_s;
+  void* v;
+  int64_t v_stride_b, v_stride_h, v_stride_s;
+  const int32_t* ctx_len; /* [batch] */
+  const int32_t* new_len; /* optional, [batch] */
+  frisk_kv_cache cache;
+} frisk_kv_desc;
+
+int frisk_kv_append(const frisk_kv_desc* desc, void* stream);
+int frisk_kv_read(const frisk_kv_desc* desc, void* stream);
+
+/* Masks of drafted trees.  parents [batch, tokens]: the drafted token each one
+ * continues (an earlier one), or -1: the context.  Token t sees itself and its
+ * ancestors: bit j % 64 of word j / 64 of mask[b][t] ((tokens + 63) / 64 words
+ * a token) is set for those, and depth[b][t] (optional) counts the ancestors.
+ * A parent outside 0 .. t - 1 counts as -1.  Contiguous; tokens <= 4096. */
+int frisk_tree_mask(int64_t batch, int64_t tokens, const int32_t* parents, uint64_t* mask,
+                    int32_t* depth, void* stream);
+
+/*
+ * Attention of new tokens over a cache that holds them already (frisk_kv_append
+ * first): token t < new_len[b] (all, if NULL) of sequence b sees keys 0 ..
+ * ctx_len[b] - 1 and, of the new tokens' keys ctx_len[b] + j, those with j < new_len[b]
+ * and bit j set in mask[b][t] (without a mask: j <= t):
+ *   o[b,h,t,:] = softmax_n(sm_scale q[b,h,t,:] . K[b,h / group,n,:]) . V[b,h / group,n,:]
+ * with group = heads / cache.kv_heads.  One token is a decode step, a mask
+ * from frisk_tree_mask a step of drafted trees, no mask a prompt's chunk.
+ * q is bf16 or f16 [batch, heads, tokens, head_dim]; o is that dtype or f32; lse, if
+ * given, [batch, heads, tokens] contiguous f32 natural-log sums.  A 16-bit
+ * cache has q's dtype.  A token that sees no key has o = 0 and lse = -inf.
+ * What a hidden key or its value holds does not matter, NaN and infinities
+ * included.  Tokens from new_len[b] on, and sequences with ctx_len[b] < 0,
+ * are left as they were.  ctx_len and new_len are read on the device;
+ * max_ctx (0: the cache's capacity) is a hint of the largest ctx_len that
+ * only places the work.  head_dim is a multiple of 16 up to 256; 32, 64 and
+ * 128 run on the matrix cores.
+ * workspace: optional device scratch (16-byte aligned) of at least
+ * frisk_tree_attn_workspace_size() bytes, with which the keys are split over
+ * the whole GPU (f32 partial rows, added in split order).  Its contents
+ * before a call do not matter; calls that share one must not overlap.
+ */
+typedef struct frisk_tree_attn_desc {
+  int64_t batch, heads, tokens;
+  int32_t dtype, o_dtype; /* frisk_dtype */
+  float sm_scale;
+  const void* q;
+  int64_t q_stride_b, q_stride_h, q_stride_s;
+  void* o;
+  int64_t o_stride_b, o_stride_h, o_stride_s;
+  float* lse;
+  const int32_t* ctx_len;
+  const int32_t* new_len;
+  const uint64_t* mask;                 /* optional */
+  int64_t mask_stride_b, mask_stride_t; /* words */
+  int64_t max_ctx;
+  frisk_kv_cache cache;
+  void* workspace;
+  int64_t workspace_bytes;
+} frisk_tree_attn_desc;
+
+int frisk_tree_attn(const frisk_tree_attn_desc* desc, void* stream);
+int64_t frisk_tree_attn_workspace_size(const frisk_tree_attn_desc* desc);
 
 /* Description of the last failure on the calling thread ("" if none). */
 const char* frisk_last_error(void);
