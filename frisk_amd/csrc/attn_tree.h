@@ -62,6 +62,10 @@ __device__ __forceinline__ void store4(const TreeAttnArgs& a, int64_t at, f32x4 
 
 }  // namespace tree
 
+// The matrix-core kernels of one head_dim (attn_tree_d*.hip).
+hipError_t tree_attn_d32(const TreeAttnArgs& a, const tree::Part& p, hipStream_t s);
+hipError_t tree_attn_d64(const TreeAttnArgs& a, const tree::Part& p, hipStream_t s);
+hipError_t tree_attn_d128(const TreeAttnArgs& a, const tree::Part& p, hipStream_t s);
 // The launches of attn_tree_rows.hip: any head_dim, and the sum over splits.
 hipError_t tree_attn_rows(const TreeAttnArgs& a, const tree::Part& p, hipStream_t s);
 hipError_t tree_attn_sum(const TreeAttnArgs& a, const tree::Part& p, hipStream_t s);

@@ -1,0 +1,645 @@
+// Attention of new tokens over a cache on the matrix cores, head_dim 32, 64 or
+// 128.  attn_tree_d*.hip instantiate the kernels.
+//
+// The query rows of one kv head (tokens x the heads that share it) form tiles
+// of 32; a key block is 64 keys.  A block's arithmetic is that of attn.h: S^T =
+// K.Q^T on 32x32x16 MFMAs, so that a lane owns a query row and 32 of its scores;
+// online softmax in the exp2 domain with a lazily moving maximum; P rounded
+// to q's type feeds O^T += V^T.P^T from the registers it is in, and V^T comes
+// from transposing LDS reads in the matching key order.  The row sum is kept
+// over the unrounded P, so that the log-sum-exp is exact to f32.
+//
+// 8-bit rows: codes widen to q's type exactly (4 or 8 significant bits), the
+// key's scale multiplies its score column and the value's scale its column of
+// P, in f32; nothing is rounded that a 16-bit cache would not round.  In f16
+// P times a scale could leave the type's range, so those columns are in units
+// of u, a power of two near the largest scale a row has seen, which moves like
+// the maximum does.
+//
+// Where a key lies is computed once per key and block (a page number from the
+// table, loaded a block ahead), into LDS, as a 64-bit offset; the row loads go
+// straight to LDS from 64-bit addresses, so neither pages nor long caches
+// limit them.  A key behind the last, or on a page that is none, is loaded from
+// the cache's first row and hidden.
+//
+// Hidden keys must not matter whatever they hold, and 0 * NaN is NaN: in blocks
+// with a hidden key a V row that is not finite is taken out of the product and
+// added by itself to the rows that see it.
+#pragma once
+
+#include "attn_tree.h"
+
+namespace frisk {
+namespace tree {
+
+#define TREE_INLINE __device__ __forceinline__
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef __attribute__((address_space(1))) const void* global_ptr;
+
+constexpr float kSlack = 8.0f;      // log2 headroom before the running maximum moves
+constexpr float kUnitSlack = 16.0f;  // headroom before the unit of P moves
+
+template <Elt T> TREE_INLINE f32x16 mfma(i32x4 a, i32x4 b, f32x16 c) {
+  if constexpr (T == Elt::BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Lane l with lane l ^ 32 (both get the result).
+TREE_INLINE float pair_max(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+TREE_INLINE float pair_sum(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+constexpr bool is8(Elt c) { return c == Elt::E4M3 || c == Elt::I8; }
+constexpr int bytes_of(Elt c) { return is8(c) ? 1 : 2; }
+
+// LDS geometry of 64 rows (keys) of D elements: rows of kRB bytes, kKC chunks of
+// 16 B, chunk c of row r stored at c ^ swz(r).
+//  K: the 16 rows that one cycle of ds_read_b128 takes at one logical chunk
+//     land in 16 distinct chunks of the 256-B bank window.
+//  V: a transposing read takes 4 rows (r & 3) x 64 B in 16 bits, 8 rows (bits
+//     0, 1 and 3 of r vary) x 32 B in 8 bits, which land apart (rows of 32 B:
+//     two by two).
+template <Elt C, int D> struct Geom {
+  static constexpr int kRB = D * bytes_of(C), kKC = kRB / 16;
+  static constexpr int kShift = kKC == 16 ? 0 : kKC == 8 ? 1 : kKC == 4 ? 2 : 3;
+  static constexpr int kTile = kBlock * kRB;
+  static constexpr int kLoads = kTile / 1024;  // 1 KiB per load instruction
+  static constexpr int kRows = 1024 / kRB;     // rows per load
+  __device__ static int swz_k(int r) { return (r >> kShift) & (kKC - 1); }
+  __device__ static int swz_v(int r) {
+    if constexpr (is8(C)) {
+      if constexpr (kKC == 8) return (((r >> 1) & 1) | ((r >> 2) & 2)) << 1;
+      else if constexpr (kKC == 4) return ((r >> 3) & 1) << 1;
+      else return 0;
+    } else {
+      if constexpr (kKC == 16) return 4 * (r & 3);
+      else if constexpr (kKC == 8) return 2 * ((r >> 1) & 1);
+      else return 0;
+    }
+  }
+};
+
+// Eight codes as eight values of T (exact).
+template <Elt T, Elt C> TREE_INLINE i32x4 widen8(int w0, int w1) {
+  i32x4 out;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int w = i ? w1 : w0;
+    if constexpr (C == Elt::E4M3 && T == Elt::BF16) {
+      out[2 * i] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+      out[2 * i + 1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+    } else if constexpr (C == Elt::E4M3) {
+      out[2 * i] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+      out[2 * i + 1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+    } else {
+      float f[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(w >> (8 * e));
+      out[2 * i] = (int)pack16<T>(f[0], f[1]);
+      out[2 * i + 1] = (int)pack16<T>(f[2], f[3]);
+    }
+  }
+  return out;
+}
+
+// Q fragments of one row (B operand of S^T): step ds, lane half h holds dims
+// 16 ds + 8 h .. +7; over codes, whose lanes read 16 dims at a time, steps 2 j
+// and 2 j + 1 hold dims 16 (2 j + h) .. +7 and +8 .. +15.
+template <Elt C, int D> TREE_INLINE void load_q(const char* row, int half, i32x4 (&qf)[D / 16]) {
+#pragma unroll
+  for (int ds = 0; ds < D / 16; ++ds) {
+    const int d = is8(C) ? 16 * ((ds & ~1) + half) + 8 * (ds & 1) : 16 * ds + 8 * half;
+    qf[ds] = *(const i32x4*)(row + d * 2);
+  }
+}
+
+// K fragments of steps h0 .. h0 + N - 1 (N even over codes) of both 32-key tiles.
+template <Elt T, Elt C, int D, int N>
+TREE_INLINE void read_k(const char* ks, int h0, int l32, int half, i32x4 (&kf)[2][N]) {
+  using G = Geom<C, D>;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+    const int r = kt * 32 + l32;
+    if constexpr (is8(C)) {
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const i32x4 w = *(const i32x4*)(ks + r * G::kRB + (((h0 + i + half) ^ G::swz_k(r)) << 4));
+        kf[kt][i] = widen8<T, C>(w[0], w[1]);
+        kf[kt][i + 1] = widen8<T, C>(w[2], w[3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        kf[kt][i] = *(const i32x4*)(ks + r * G::kRB + (((2 * (h0 + i) + half) ^ G::swz_k(r)) << 4));
+    }
+  }
+}
+
+// Lane offsets of the transposing reads of V^T (attn.h and gemm_tile.h derive
+// them): the fragment of key step kk and dim tile dt holds, in lane (l32,
+// half), V[16 kk + (e < 4 ? 4 half + e : 4 + 4 half + e)][32 dt + l32], e = 0 .. 7.
+template <Elt C, int D> TREE_INLINE void v_offsets(int lane, int (&off)[D / 32]) {
+  using G = Geom<C, D>;
+  const int g = lane >> 4, h = g >> 1, dg = g & 1;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) {
+    if constexpr (is8(C)) {
+      const int e = (lane >> 1) & 7, b = lane & 1, r = e < 4 ? 4 * h + e : 4 + 4 * h + e;
+      off[dt] = r * G::kRB + (((2 * dt + dg) ^ G::swz_v(r)) << 4) + 8 * b;
+    } else {
+      const int e = (lane >> 2) & 3, q = lane & 3, r = 4 * h + e;
+      off[dt] = r * G::kRB + (((4 * dt + 2 * dg + (q >> 1)) ^ G::swz_v(r)) << 4) + 8 * (q & 1);
+    }
+  }
+}
+template <Elt T, Elt C, int D> TREE_INLINE i32x4 read_v(const char* vs, int off, int kk) {
+  using G = Geom<C, D>;
+  const char* p = vs + off + kk * 16 * G::kRB;
+  if constexpr (is8(C)) {
+    const i32x2 w = lds_read_tr8(p);
+    return widen8<T, C>(w[0], w[1]);
+  } else {
+    const i32x2 a = __builtin_bit_cast(i32x2, lds_read_tr16(p));
+    const i32x2 c = __builtin_bit_cast(i32x2, lds_read_tr16(p + 8 * G::kRB));
+    return i32x4{a[0], a[1], c[0], c[1]};
+  }
+}
+
+// ---- where keys lie ------------------------------------------------------------
+
+// Byte offset of a key's row and element offset of its scale, for one head.
+struct Place {
+  int64_t row;
+  int64_t scale;
+  bool there;
+};
+// The table entry of key n (any value without a table), n < the capacity.
+TREE_INLINE int entry_of(const TreeAttnArgs& a, int64_t b, int n) {
+  const int32_t* p = a.cache.table ? a.cache.table + b * a.cache.table_stride + (n >> a.cache.page_shift)
+                                   : a.ctx_len + b;
+  return *p;
+}
+template <Elt C>
+TREE_INLINE Place place_of(const TreeAttnArgs& a, int64_t b, int kvh, int n, int keys, int entry) {
+  const KvCache& c = a.cache;
+  const int page = c.table ? entry : (int)b;
+  const int slot = c.table ? n & ((1 << c.page_shift) - 1) : n;
+  Place p;
+  p.there = n < keys && page >= 0 && page < c.pages;
+  const int64_t pg = p.there ? page : 0, sl = p.there ? slot : 0;
+  p.row = (pg * c.sp + sl * c.ss + kvh * c.sh) * bytes_of(C);
+  p.scale = pg * c.scp + sl * c.scs + kvh * c.sch;
+  return p;
+}
+
+// ---- masks -----------------------------------------------------------------------
+
+// Which keys of the block from key n0 a token sees, as bits (all of the context;
+// `there`: keys that exist).
+TREE_INLINE uint64_t seen_bits(const TreeAttnArgs& a, int64_t b, int t, int64_t ctx, int n0,
+                               uint64_t there) {
+  const int64_t j0 = n0 - ctx;  // draft number of the first key
+  if (j0 + kBlock <= 0) return there;
+  uint64_t bits;
+  if (!a.mask) {
+    const int64_t n = t - j0 + 1;  // the first n keys
+    bits = n >= 64 ? ~0ull : n <= 0 ? 0 : (1ull << n) - 1;
+  } else {
+    const uint64_t* w = a.mask + (b * a.mask_sb + t * a.mask_st);
+    const int words = (a.tokens + 63) >> 6;
+    if (j0 < 0) {
+      const int n = (int)-j0;  // context keys in front, 1 .. 63
+      bits = ((1ull << n) - 1) | (w[0] << n);
+    } else {
+      const int i = (int)(j0 >> 6), s = (int)(j0 & 63);
+      bits = i < words ? w[i] >> s : 0;
+      if (s && i + 1 < words) bits |= w[i + 1] << (64 - s);
+    }
+  }
+  return bits & there;
+}
+// Key of score register r (of 16) of tile kt, less 4 half.
+constexpr int key_of(int kt, int r) { return kt * 32 + 8 * (r >> 2) + (r & 3); }
+
+// ---- softmax of one block -----------------------------------------------------------
+
+// A row's running state; u: unit of P and O over codes in f16, else 1.
+template <int D> struct State {
+  f32x16 o[D / 32];
+  float m, l, u;
+};
+template <int D> TREE_INLINE void clear(State<D>& st) {
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = f32x16{};
+  st.m = -__builtin_inff();
+  st.l = 0.0f;
+  st.u = 0x1p-126f;
+}
+
+// Scores s to P (in place, f32, and packed in pf).  seen: bits of the row's
+// keys shifted down by 4 half, read if masked (uniform).  sc: the block's 64 key
+// scales times scale_log2, then 64 value scales, over codes.
+template <Elt T, Elt C, int D>
+TREE_INLINE void softmax(f32x16 (&s)[2], i32x4 (&pf)[4], State<D>& st, float scale_log2,
+                         const float* sc, int half, bool masked, uint64_t seen) {
+  constexpr bool k8 = is8(C), unit = k8 && T == Elt::F16;
+  if constexpr (k8) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 f = *(const f32x4*)(sc + kt * 32 + 8 * g + 4 * half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[kt][4 * g + i] *= f[i];
+      }
+  }
+  if (masked) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[kt][r] = (seen >> key_of(kt, r)) & 1 ? s[kt][r] : -__builtin_inff();
+  }
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kt][r]);
+  top = pair_max(top);
+  if constexpr (!k8) top *= scale_log2;
+  const bool move = top > st.m + kSlack;
+  if (__builtin_amdgcn_ballot_w64(move)) {
+    const float alpha = move ? __builtin_amdgcn_exp2f(st.m - top) : 1.0f;
+    st.m = move ? top : st.m;
+    st.l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= alpha;
+  }
+  // A row that has seen no key keeps m = -inf: p = 0, not NaN.
+  const float nm = st.m == -__builtin_inff() ? 0.0f : -st.m;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float x = k8 ? s[kt][r] + nm : __builtin_fmaf(s[kt][r], scale_log2, nm);
+      s[kt][r] = __builtin_amdgcn_exp2f(x);
+    }
+  float l = st.l;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) l += s[kt][r];
+  st.l = l;
+  if constexpr (k8) {
+    f32x4 f[2][4];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) f[kt][g] = *(const f32x4*)(sc + 64 + kt * 32 + 8 * g + 4 * half);
+    if (masked) {  // a hidden key's scale may be anything
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          f[kt][r >> 2][r & 3] = (seen >> key_of(kt, r)) & 1 ? f[kt][r >> 2][r & 3] : 0.0f;
+    }
+    if constexpr (unit) {
+      float big = 0.0f;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float v = f[kt][r >> 2][r & 3];
+          big = fmaxf(big, v < __builtin_inff() ? v : 0.0f);
+        }
+      big = pair_max(big);
+      const bool grow = big > st.u * kUnitSlack;
+      if (__builtin_amdgcn_ballot_w64(grow)) {
+        const float next = grow ? __builtin_ldexpf(1.0f, __builtin_amdgcn_frexp_expf(big)) : st.u;
+        const float by = st.u / next;
+        st.u = next;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= by;
+      }
+      const float inv = 1.0f / st.u;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) f[kt][g] *= inv;
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kt][r] *= f[kt][r >> 2][r & 3];
+  }
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = 8 * (kk & 1) + 2 * e;
+      pf[kk][e] = (int)pack16<T>(s[kk >> 1][r], s[kk >> 1][r + 1]);
+    }
+}
+
+// ---- V rows that are not finite ----------------------------------------------------
+
+// Bits of the block's keys whose V row holds an infinity or NaN (lane = key).
+template <Elt T, Elt C, int D> TREE_INLINE uint64_t not_finite(const char* vs, int lane) {
+  using G = Geom<C, D>;
+  if constexpr (C == Elt::I8) return 0;
+  uint32_t bad = 0;
+#pragma unroll
+  for (int i = 0; i < G::kKC; ++i) {
+    const i32x4 w = *(const i32x4*)(vs + lane * G::kRB + 16 * ((i + lane) & (G::kKC - 1)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // A carry into the sign bit of each element from a full exponent (codes:
+      // from the NaN code).
+      const uint32_t x = (uint32_t)w[e];
+      if constexpr (C == Elt::E4M3) bad |= ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+      else if constexpr (T == Elt::BF16) bad |= ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+      else bad |= ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+    }
+  }
+  return __builtin_amdgcn_ballot_w64(bad != 0);
+}
+
+// o += p V of key `key` alone, for rows that see it.
+template <Elt T, Elt C, int D>
+TREE_INLINE void add_key(const char* vs, int key, const f32x16 (&p)[2], uint64_t seen, int l32, int half,
+                         State<D>& st) {
+  using G = Geom<C, D>;
+  float w = 0.0f;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w = key_of(kt, r) == (key & ~4) ? p[kt][r] : w;
+  const int from = l32 + 32 * ((key >> 2) & 1);  // the half that holds the key
+  w = __shfl(w, from);
+  const bool sees_it = __shfl((int)((seen >> (key & ~4)) & 1), from);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int d = dt * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+      const int at = key * G::kRB + (((d * bytes_of(C) >> 4) ^ G::swz_v(key)) << 4) + (d * bytes_of(C) & 15);
+      float v;
+      if constexpr (is8(C)) {
+        v = __builtin_amdgcn_cvt_f32_fp8((int)*(const uint8_t*)(vs + at), 0);
+      } else {
+        const uint16_t h = *(const uint16_t*)(vs + at);
+        v = T == Elt::BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+      }
+      st.o[dt][r] += sees_it ? w * v : 0.0f;
+    }
+}
+template <Elt C, int D> TREE_INLINE void clear_key(char* vs, int key, int lane) {
+  using G = Geom<C, D>;
+  if (lane < G::kKC) *(i32x4*)(vs + key * G::kRB + 16 * lane) = i32x4{0, 0, 0, 0};
+}
+
+// ---- few rows: the waves divide the keys ---------------------------------------------
+
+// Waves per workgroup: K and V tiles of all waves in LDS.
+template <Elt C, int D> constexpr int kKeyWaves = D == 128 ? 4 : 8;
+constexpr int kExtra = 1024;  // per wave: 64 row offsets (8 B), 2 x 64 scales
+template <Elt C, int D> constexpr int keys_lds() {
+  const int tiles = kKeyWaves<C, D> * (2 * Geom<C, D>::kTile + kExtra);
+  const int sum = kKeyWaves<C, D> * 32 * (D + 4 + 2) * 4;
+  return tiles > sum ? tiles : sum;
+}
+
+// One tile of 32 rows per workgroup; each wave takes every NW-th key block of
+// the split with K and V tiles of its own: no barrier in the loop, and a block's
+// bytes of loads in flight per wave.
+template <Elt T, Elt C, int D>
+__global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeAttnArgs a, Part part,
+                                                                         int row_tiles) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using G = Geom<C, D>;
+  constexpr int NW = kKeyWaves<C, D>;
+  constexpr bool k8 = is8(C);
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tile = (int)(blockIdx.x % (unsigned)row_tiles);
+  const unsigned bk = blockIdx.x / (unsigned)row_tiles;
+  const int64_t b = bk / (unsigned)a.cache.kv_heads;
+  const int kvh = (int)(bk % (unsigned)a.cache.kv_heads), split = blockIdx.y;
+  const int group = a.heads / a.cache.kv_heads;
+  const kv::Span sp = kv::span_of(a.ctx_len, a.new_len, a.tokens, b);
+  const int rows = sp.fresh * group;
+  if (sp.ctx < 0 || tile * 32 >= rows) return;
+  int keys = keys_of(a, sp);
+  const int blocks_all = (keys + kBlock - 1) / kBlock;
+  const int per = blocks_per_split(part, blocks_all);
+  if (split > 0 && split * per >= blocks_all) return;
+  const int row = min(tile * 32 + l32, rows - 1), t = row / group, h = kvh * group + row % group;
+  const int end = min(blocks_all, (split + 1) * per);
+
+  i32x4 qf[D / 16];
+  load_q<C, D>((const char*)a.q + (b * a.q_sb + h * a.q_sh + t * a.q_ss) * 2, half, qf);
+  const float scale_log2 = a.sm_scale * kLog2eF;
+
+  char* ks = smem + wave * (2 * G::kTile + kExtra);
+  char* vs = ks + G::kTile;
+  int64_t* offs = (int64_t*)(vs + G::kTile);
+  float* sc = (float*)(offs + 64);
+  const char* kbase = (const char*)a.cache.k;
+  const char* vbase = (const char*)a.cache.v;
+  const int lrow = lane / G::kKC, lchunk = lane % G::kKC;
+  auto issue = [&](const char* base, char* dst, bool is_v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < G::kLoads; ++i) {
+      const int r = i * G::kRows + lrow, c = lchunk ^ (is_v ? G::swz_v(r) : G::swz_k(r));
+      __builtin_amdgcn_global_load_lds((global_ptr)(base + offs[r] + (c << 4)), (lds_ptr)(dst + i * 1024),
+                                       16, 0, 0);
+    }
+  };
+  int vt[D / 32];
+  v_offsets<C, D>(lane, vt);
+  State<D> st;
+  clear(st);
+
+  // The key this lane looks up for block kb.
+  auto my_key = [&](int kb) { return min(kb * kBlock + lane, (int)a.cache.capacity - 1); };
+  int kb = split * per + wave;
+  int entry = 0;
+  uint64_t there = 0, there_next = 0;
+  float ksc = 0.0f, vsc = 0.0f;
+  auto place = [&](int block, int e) __attribute__((always_inline)) {
+    const Place p = place_of<C>(a, b, kvh, block * kBlock + lane, keys, e);
+    offs[lane] = p.row;
+    if constexpr (k8) {
+      ksc = a.cache.k_scale[p.scale];
+      vsc = a.cache.v_scale[p.scale];
+    }
+    return __builtin_amdgcn_ballot_w64(p.there);
+  };
+  // Table entries of the first two blocks; Q has landed with them, on every
+  // path into the loop, so that nothing in it waits for a load by accident.
+  const int first = entry_of(a, b, my_key(max(0, min(kb, end - 1))));
+  entry = entry_of(a, b, my_key(max(0, min(kb + NW, end - 1))));
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) asm volatile("" ::"v"(qf[i]), "v"(first), "v"(entry));
+  __builtin_amdgcn_s_waitcnt(0);
+  if (kb < end) {
+    there = place(kb, first);
+    __builtin_amdgcn_sched_barrier(0);
+    issue(kbase, ks, false);
+    issue(vbase, vs, true);
+  }
+  for (; kb < end; kb += NW) {
+    const bool more = kb + NW < end;
+    // K landed (V's loads may still be in flight), and with it the scales and
+    // the table entry, which were asked for before.
+    constexpr int nv = G::kLoads;
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt((nv & 15) | ((nv >> 4) << 14) | (7 << 4) | (15 << 8));
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (k8) {
+      sc[lane] = ksc * scale_log2;
+      sc[64 + lane] = vsc;
+    }
+    f32x16 s[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+    for (int h0 = 0; h0 < D / 16; h0 += 2) {
+      i32x4 kf[2][2];
+      read_k<T, C, D, 2>(ks, h0, l32, half, kf);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) s[kt] = mfma<T>(kf[kt][i], qf[h0 + i], s[kt]);
+    }
+    // Every K fragment has been read: the next block's K may land.
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    if (more) {
+      there_next = place(kb + NW, entry);
+      entry = entry_of(a, b, my_key(min(kb + 2 * NW, end - 1)));
+      __builtin_amdgcn_sched_barrier(0);
+      issue(kbase, ks, false);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    const bool masked = there != ~0ull || (int64_t)(kb + 1) * kBlock > sp.ctx;
+    i32x4 pf[4];
+    uint64_t seen = 0;
+    if (masked) seen = seen_bits(a, b, t, sp.ctx, kb * kBlock, there) >> (4 * half);
+    softmax<T, C, D>(s, pf, st, scale_log2, sc, half, masked, seen);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) asm volatile("" ::"v"(pf[kk]));  // P before the wait
+    // V landed (only the next block's K may be in flight).
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) __builtin_amdgcn_s_waitcnt((nv & 15) | ((nv >> 4) << 14) | (7 << 4) | (15 << 8));
+    else __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));
+    __builtin_amdgcn_sched_barrier(0);
+    if (masked) {
+      for (uint64_t bad = not_finite<T, C, D>(vs, lane); bad; bad &= bad - 1) {
+        const int key = __builtin_ctzll(bad);
+        add_key<T, C, D>(vs, key, s, seen, l32, half, st);
+        clear_key<C, D>(vs, key, lane);
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+        st.o[dt] = mfma<T>(read_v<T, C, D>(vs, vt[dt], kk), pf[kk], st.o[dt]);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    if (more) issue(vbase, vs, true);
+    there = there_next;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  const float l = pair_sum(st.l);
+  const float u = k8 && T == Elt::F16 ? st.u : 1.0f;
+
+  // Combine the waves: O_w as padded rows, then m and l.
+  __syncthreads();
+  constexpr int kPitch = D + 4;
+  float* po = (float*)smem;
+  float* pm = po + NW * 32 * kPitch;
+  {
+    float* w = po + (wave * 32 + l32) * kPitch;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(f32x4*)(w + dt * 32 + 8 * g + 4 * half) =
+            f32x4{st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]} * u;
+    if (half == 0) {
+      pm[(wave * 32 + l32) * 2] = st.m;
+      pm[(wave * 32 + l32) * 2 + 1] = l;
+    }
+  }
+  __syncthreads();
+  const int live = min(32, rows - tile * 32);
+  for (int idx = tid; idx < live * (D / 4); idx += 64 * NW) {
+    const int q = idx / (D / 4), d = idx % (D / 4) * 4;
+    float M = -__builtin_inff(), L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, pm[(w * 32 + q) * 2]);
+    const float nM = M == -__builtin_inff() ? 0.0f : M;
+    f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(pm[(w * 32 + q) * 2] - nM);
+      L = __builtin_fmaf(f, pm[(w * 32 + q) * 2 + 1], L);
+      acc += *(const f32x4*)(po + (w * 32 + q) * kPitch + d) * f;
+    }
+    const int r = tile * 32 + q, rt = r / group, rh = kvh * group + r % group;
+    const int64_t id = (b * a.heads + rh) * a.tokens + rt;
+    if (per < blocks_all) {
+      const int64_t at = id * part.splits + split;
+      *(f32x4*)(part.o + at * D + d) = acc;
+      if (d == 0) part.ml[2 * at] = M, part.ml[2 * at + 1] = L;
+      continue;
+    }
+    store4<T>(a, b * a.o_sb + rh * a.o_sh + rt * a.o_ss + d, acc * inverse_sum(L));
+    if (a.lse && d == 0) a.lse[id] = lse_of(M, L);
+  }
+#endif  // __HIP_DEVICE_COMPILE__
+}
+
+template <Elt T, Elt C, int D>
+static hipError_t launch_keys(const TreeAttnArgs& a, const Part& p, hipStream_t stream) {
+  auto kern = tree_keys_kernel<T, C, D>;
+  constexpr int lds = keys_lds<C, D>(), threads = 64 * kKeyWaves<C, D>;
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
+  static const hipError_t attr =
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (attr != hipSuccess) return attr;
+  const int group = a.heads / a.cache.kv_heads;
+  const int64_t tiles = ((int64_t)a.tokens * group + 31) / 32;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a.batch * a.cache.kv_heads * tiles), (unsigned)p.splits),
+                     dim3(threads), lds, stream, a, p, (int)tiles);
+  return hipGetLastError();
+}
+
+template <int D> hipError_t tree_mfma_dispatch(const TreeAttnArgs& a, const Part& p, hipStream_t s) {
+  const bool bf = a.dtype == Elt::BF16;
+  switch (a.cache.kind) {
+    case Elt::E4M3:
+      return bf ? launch_keys<Elt::BF16, Elt::E4M3, D>(a, p, s) : launch_keys<Elt::F16, Elt::E4M3, D>(a, p, s);
+    case Elt::I8:
+      return bf ? launch_keys<Elt::BF16, Elt::I8, D>(a, p, s) : launch_keys<Elt::F16, Elt::I8, D>(a, p, s);
+    default:
+      return bf ? launch_keys<Elt::BF16, Elt::BF16, D>(a, p, s) : launch_keys<Elt::F16, Elt::F16, D>(a, p, s);
+  }
+}
+
+}  // namespace tree
+}  // namespace frisk

@@ -204,12 +204,18 @@ hipError_t tree_attn_sum(const TreeAttnArgs& a, const tree::Part& p, hipStream_t
 }
 
 hipError_t tree_attn(const TreeAttnArgs& a, hipStream_t s) {
-  tree::Part p{nullptr, nullptr, a.splits, plan::tree_min_blocks()};
+  tree::Part p{nullptr, nullptr, a.splits, a.min_blocks};
   if (a.splits > 1) {
     p.o = (float*)a.workspace;
     p.ml = p.o + a.batch * a.heads * a.tokens * a.splits * a.cache.head_dim;
   }
-  const hipError_t e = tree_attn_rows(a, p, s);
+  hipError_t e;
+  switch (a.kernel == plan::TreeKernel::Rows ? 0 : a.cache.head_dim) {
+    case 32: e = tree_attn_d32(a, p, s); break;
+    case 64: e = tree_attn_d64(a, p, s); break;
+    case 128: e = tree_attn_d128(a, p, s); break;
+    default: e = tree_attn_rows(a, p, s);
+  }
   if (e != hipSuccess || a.splits <= 1) return e;
   return tree_attn_sum(a, p, s);
 }

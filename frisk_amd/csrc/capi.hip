@@ -992,7 +992,11 @@ int check_tree(const frisk_tree_attn_desc* d, bool ptrs, frisk::TreeAttnArgs& a)
   a.new_len = d->new_len;
   a.mask = d->mask; a.mask_sb = d->mask_stride_b; a.mask_st = d->mask_stride_t;
   const int64_t keys = d->max_ctx ? std::min(d->max_ctx + d->tokens, a.cache.capacity) : a.cache.capacity;
-  a.splits = frisk::plan::tree_splits(d->batch * d->heads * d->tokens, keys, frisk::device_cus());
+  const frisk::plan::TreePlan p = frisk::plan::tree_plan(
+      d->batch, d->heads, d->cache.kv_heads, d->tokens, d->cache.head_dim, keys, frisk::device_cus());
+  a.kernel = p.kernel;
+  a.splits = p.splits;
+  a.min_blocks = p.min_blocks;
   a.workspace = nullptr;
   return FRISK_OK;
 }

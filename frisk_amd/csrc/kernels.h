@@ -267,7 +267,9 @@ struct TreeAttnArgs {
   const uint64_t* mask;  // null: token t sees the drafts up to t
   int64_t mask_sb, mask_st;
   KvCache cache;
+  plan::TreeKernel kernel;
   int splits;       // key splits; more than one needs the workspace
+  int min_blocks;   // key blocks a split has at least
   void* workspace;  // plan::tree_workspace bytes
 };
 hipError_t tree_attn(const TreeAttnArgs& a, hipStream_t s);

@@ -617,15 +617,32 @@ inline int64_t attn_workspace(int64_t batch_heads, int64_t seq_q, int64_t seq_k,
 }
 
 // ---------------------------------------------------------------------------
-// Attention of new tokens over a cache (attn_tree_rows.hip): key splits, so
-// that four workgroups a CU have work.  `keys`: the most a sequence may hold.
+// Attention of new tokens over a cache (attn_tree_mfma.h, attn_tree_rows.hip).
+// Rows: one query row a workgroup, head dims without a matrix-core kernel.
+// Keys: a tile of 32 query rows of a kv head a workgroup, whose waves divide the
+// keys.
+// The keys are split so that every CU has workgroups; `keys` is the most a
+// sequence may hold, and the kernels use fewer splits for shorter ones.
 // ---------------------------------------------------------------------------
 constexpr int kTreeBlock = 64;  // keys per block
-constexpr int tree_min_blocks() { return 4; }
-inline int tree_splits(int64_t rows, int64_t keys, int cus) {
+enum class TreeKernel { Rows, Keys };
+struct TreePlan {
+  TreeKernel kernel;
+  int splits, min_blocks;
+};
+inline TreePlan tree_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t tokens, int64_t head_dim,
+                          int64_t keys, int cus) {
+  TreePlan p{TreeKernel::Rows, 1, 4};
   const int64_t blocks = (keys + kTreeBlock - 1) / kTreeBlock;
-  const int64_t want = (4 * (int64_t)cus + rows - 1) / rows;
-  return (int)std::max<int64_t>(1, std::min({want, blocks / tree_min_blocks(), (int64_t)64}));
+  int64_t want = (4 * (int64_t)cus + batch * heads * tokens - 1) / (batch * heads * tokens);
+  if (head_dim == 32 || head_dim == 64 || head_dim == 128) {
+    p.kernel = TreeKernel::Keys;
+    p.min_blocks = head_dim == 128 ? 4 : 8;  // one for every wave
+    const int64_t wgs = batch * kv_heads * ((tokens * (heads / kv_heads) + 31) / 32);
+    want = (cus + wgs - 1) / wgs;
+  }
+  p.splits = (int)std::max<int64_t>(1, std::min({want, blocks / p.min_blocks, (int64_t)64}));
+  return p;
 }
 inline int64_t tree_workspace(int64_t rows, int splits, int64_t head_dim) {
   return splits > 1 ? rows * splits * (head_dim + 2) * 4 : 0;
