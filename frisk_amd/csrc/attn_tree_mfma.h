@@ -230,6 +230,13 @@ TREE_INLINE uint64_t seen_bits(const TreeAttnArgs& a, int64_t b, int t, int64_t 
   }
   return bits & there;
 }
+// A copy of the bits that the compiler takes for another value, so that the 32
+// conditions of one use are not kept in scalar registers for the next.
+TREE_INLINE uint64_t again(uint64_t bits) {
+  uint32_t lo = (uint32_t)bits, hi = (uint32_t)(bits >> 32);
+  asm volatile("" : "+v"(lo), "+v"(hi));
+  return (uint64_t)hi << 32 | lo;
+}
 // Key of score register r (of 16) of tile kt, less 4 half.
 constexpr int key_of(int kt, int r) { return kt * 32 + 8 * (r >> 2) + (r & 3); }
 
@@ -303,26 +310,21 @@ TREE_INLINE void softmax(f32x16 (&s)[2], i32x4 (&pf)[4], State<D>& st, float sca
     for (int r = 0; r < 16; ++r) l += s[kt][r];
   st.l = l;
   if constexpr (k8) {
-    f32x4 f[2][4];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) f[kt][g] = *(const f32x4*)(sc + 64 + kt * 32 + 8 * g + 4 * half);
-    if (masked) {  // a hidden key's scale may be anything
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          f[kt][r >> 2][r & 3] = (seen >> key_of(kt, r)) & 1 ? f[kt][r >> 2][r & 3] : 0.0f;
-    }
+    float inv = 1.0f;
     if constexpr (unit) {
       float big = 0.0f;
+      const uint64_t bits = again(masked ? seen : ~0ull);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float v = f[kt][r >> 2][r & 3];
-          big = fmaxf(big, v < __builtin_inff() ? v : 0.0f);
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 f = *(const f32x4*)(sc + 64 + kt * 32 + 8 * g + 4 * half);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // (A hidden key's scale may be anything.)
+            const bool counts = f[i] < __builtin_inff() && ((bits >> key_of(kt, 4 * g + i)) & 1);
+            big = fmaxf(big, counts ? f[i] : 0.0f);
+          }
         }
       big = pair_max(big);
       const bool grow = big > st.u * kUnitSlack;
@@ -333,16 +335,23 @@ TREE_INLINE void softmax(f32x16 (&s)[2], i32x4 (&pf)[4], State<D>& st, float sca
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= by;
       }
-      const float inv = 1.0f / st.u;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) f[kt][g] *= inv;
+      inv = 1.0f / st.u;
     }
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[kt][r] *= f[kt][r >> 2][r & 3];
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 f = *(const f32x4*)(sc + 64 + kt * 32 + 8 * g + 4 * half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[kt][4 * g + i] *= unit ? f[i] * inv : f[i];
+      }
+    if (masked) {  // a hidden key's scale may be NaN
+      const uint64_t bits = again(seen);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kt][r] = (bits >> key_of(kt, r)) & 1 ? s[kt][r] : 0.0f;
+    }
   }
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk)
@@ -410,10 +419,23 @@ template <Elt C, int D> TREE_INLINE void clear_key(char* vs, int key, int lane) 
   if (lane < G::kKC) *(i32x4*)(vs + key * G::kRB + 16 * lane) = i32x4{0, 0, 0, 0};
 }
 
+// Workgroup pid as (unit: sequence, kv head and split; tile of its rows).  The
+// tiles of a unit run on one XCD (workgroups go round the 8 XCDs), next to each
+// other, so that its L2 holds the keys they share.
+TREE_INLINE void place_unit(int pid, int units, int tiles, int& unit, int& tile) {
+  if (units % 8 == 0) {
+    unit = ((pid >> 3) / tiles) * 8 + (pid & 7);
+    tile = (pid >> 3) % tiles;
+  } else {
+    unit = pid / tiles;
+    tile = pid % tiles;
+  }
+}
+
 // ---- few rows: the waves divide the keys ---------------------------------------------
 
 // Waves per workgroup: K and V tiles of all waves in LDS.
-template <Elt C, int D> constexpr int kKeyWaves = D == 128 ? 4 : 8;
+template <Elt C, int D> constexpr int kKeyWaves = plan::tree_key_waves(D);
 constexpr int kExtra = 1024;  // per wave: 64 row offsets (8 B), 2 x 64 scales
 template <Elt C, int D> constexpr int keys_lds() {
   const int tiles = kKeyWaves<C, D> * (2 * Geom<C, D>::kTile + kExtra);
@@ -426,7 +448,7 @@ template <Elt C, int D> constexpr int keys_lds() {
 // bytes of loads in flight per wave.
 template <Elt T, Elt C, int D>
 __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeAttnArgs a, Part part,
-                                                                         int row_tiles) {
+                                                                         int row_tiles, int units) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using G = Geom<C, D>;
   constexpr int NW = kKeyWaves<C, D>;
@@ -434,10 +456,11 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int tile = (int)(blockIdx.x % (unsigned)row_tiles);
-  const unsigned bk = blockIdx.x / (unsigned)row_tiles;
-  const int64_t b = bk / (unsigned)a.cache.kv_heads;
-  const int kvh = (int)(bk % (unsigned)a.cache.kv_heads), split = blockIdx.y;
+  int unit, tile;
+  place_unit(blockIdx.x, units, row_tiles, unit, tile);
+  const int split = unit % part.splits, bk = unit / part.splits;
+  const int64_t b = bk / a.cache.kv_heads;
+  const int kvh = bk % a.cache.kv_heads;
   const int group = a.heads / a.cache.kv_heads;
   const kv::Span sp = kv::span_of(a.ctx_len, a.new_len, a.tokens, b);
   const int rows = sp.fresh * group;
@@ -624,20 +647,302 @@ static hipError_t launch_keys(const TreeAttnArgs& a, const Part& p, hipStream_t 
   if (attr != hipSuccess) return attr;
   const int group = a.heads / a.cache.kv_heads;
   const int64_t tiles = ((int64_t)a.tokens * group + 31) / 32;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(a.batch * a.cache.kv_heads * tiles), (unsigned)p.splits),
-                     dim3(threads), lds, stream, a, p, (int)tiles);
+  const int64_t units = a.batch * a.cache.kv_heads * p.splits;
+  if (units * tiles > UINT32_MAX / 512) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(units * tiles)), dim3(threads), lds, stream, a, p, (int)tiles,
+                     (int)units);
   return hipGetLastError();
+}
+
+// ---- many rows: the waves share the keys ----------------------------------------------
+
+// NW tiles of 32 rows per workgroup, one a wave; K and V of a key block in LDS
+// for all of them, in q's type (codes are widened once, on their way), double
+// buffered.
+template <Elt T, Elt C, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, Part part, int row_blocks,
+                                                            int units) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using G = Geom<T, D>;
+  constexpr bool k8 = is8(C);
+  constexpr int kBuf = 2 * G::kTile;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  int64_t* offs = (int64_t*)(smem + 2 * kBuf);  // [2][64]
+  float* scales = (float*)(offs + 128);         // [2][128]
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int unit, rb;
+  place_unit(blockIdx.x, units, row_blocks, unit, rb);
+  rb = row_blocks - 1 - rb;  // the last rows, which see most keys, first
+  const int split = unit % part.splits, bk = unit / part.splits;
+  const int64_t b = bk / a.cache.kv_heads;
+  const int kvh = bk % a.cache.kv_heads, group = a.heads / a.cache.kv_heads;
+  const kv::Span sp = kv::span_of(a.ctx_len, a.new_len, a.tokens, b);
+  const int rows = sp.fresh * group;
+  if (sp.ctx < 0 || rb * 32 * NW >= rows) return;
+  const int keys = keys_of(a, sp);
+  const int blocks_all = (keys + kBlock - 1) / kBlock;
+  const int per = blocks_per_split(part, blocks_all);
+  if (split > 0 && split * per >= blocks_all) return;
+  const int row0 = (rb * NW + wave) * 32;  // this wave's first row
+  const int row = min(row0 + l32, rows - 1), t = row / group, h = kvh * group + row % group;
+  // Without a mask no row of the workgroup sees past its last token.
+  int end = min(blocks_all, (split + 1) * per);
+  int t_wave = sp.fresh;  // the last token of this wave
+  if (!a.mask) {
+    const int t_last = (min(rows, (rb + 1) * 32 * NW) - 1) / group;
+    end = min((int64_t)end, (sp.ctx + t_last + kBlock) / kBlock);
+    t_wave = min(row0 + 31, rows - 1) / group;
+  }
+  const int begin = split * per;
+
+  i32x4 qf[D / 16];
+  load_q<T, D>((const char*)a.q + (b * a.q_sb + h * a.q_sh + t * a.q_ss) * 2, half, qf);
+  const float scale_log2 = a.sm_scale * kLog2eF;
+  const char* kbase = (const char*)a.cache.k;
+  const char* vbase = (const char*)a.cache.v;
+
+  auto my_key = [&](int kb) { return max(0, min(kb * kBlock + lane, (int)a.cache.capacity - 1)); };
+  int64_t my_scale = 0;
+  // Row offsets of a block, by wave 0 for all; every wave keeps which keys exist.
+  auto place = [&](int kb, int entry) __attribute__((always_inline)) {
+    const Place p = place_of<C>(a, b, kvh, kb * kBlock + lane, keys, entry);
+    if (wave == 0) offs[(kb & 1) * 64 + lane] = p.row;
+    my_scale = p.scale;
+    return __builtin_amdgcn_ballot_w64(p.there);
+  };
+  // 16 bits: 1 KiB per load instruction to LDS.
+  constexpr int kIns = G::kLoads, kPer = (kIns + NW - 1) / NW;
+  const int lrow = lane / G::kKC, lchunk = lane % G::kKC;
+  auto issue = [&](int kb) __attribute__((always_inline)) {
+    char* dst = smem + (kb & 1) * kBuf;
+    const int64_t* o = offs + (kb & 1) * 64;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int n = wave * kPer + i;
+      if (n >= kIns) continue;  // wave-uniform
+      const int r = n * G::kRows + lrow;
+      const int64_t at = o[r];
+      __builtin_amdgcn_global_load_lds((global_ptr)(kbase + at + ((lchunk ^ G::swz_k(r)) << 4)),
+                                       (lds_ptr)(dst + n * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_ptr)(vbase + at + ((lchunk ^ G::swz_v(r)) << 4)),
+                                       (lds_ptr)(dst + G::kTile + n * 1024), 16, 0, 0);
+    }
+  };
+  // Codes: 16 of them per thread and piece, widened on the way to LDS.
+  constexpr int kPieces = 4 * D, kMine = (kPieces + 64 * NW - 1) / (64 * NW), kC8 = D / 16;
+  i32x4 kw[kMine], vw[kMine];
+  float my_value = 0.0f;
+  auto fetch = [&](int kb) __attribute__((always_inline)) {
+    const int64_t* o = offs + (kb & 1) * 64;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int p = i * 64 * NW + tid;
+      if (kPieces % (64 * NW) && p >= kPieces) continue;
+      const int64_t at = o[p / kC8] + (p % kC8) * 16;
+      kw[i] = *(const i32x4*)(kbase + at);
+      vw[i] = *(const i32x4*)(vbase + at);
+    }
+    if (wave < 2) my_value = (wave == 0 ? a.cache.k_scale : a.cache.v_scale)[my_scale];
+  };
+  auto widen = [&](int kb) __attribute__((always_inline)) {
+    char* dst = smem + (kb & 1) * kBuf;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int p = i * 64 * NW + tid;
+      if (kPieces % (64 * NW) && p >= kPieces) continue;
+      const int r = p / kC8, c = 2 * (p % kC8);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        *(i32x4*)(dst + r * G::kRB + (((c + e) ^ G::swz_k(r)) << 4)) =
+            widen8<T, C>(kw[i][2 * e], kw[i][2 * e + 1]);
+        *(i32x4*)(dst + G::kTile + r * G::kRB + (((c + e) ^ G::swz_v(r)) << 4)) =
+            widen8<T, C>(vw[i][2 * e], vw[i][2 * e + 1]);
+      }
+    }
+    if (wave < 2) scales[(kb & 1) * 128 + wave * 64 + lane] = wave == 0 ? my_value * scale_log2 : my_value;
+  };
+
+  int vt[D / 32];
+  v_offsets<T, D>(lane, vt);
+  State<D> st;
+  clear(st);
+  // Table entries of the first blocks; Q has landed with them, on every path
+  // into the loop, so that nothing in it waits for a load by accident.
+  const int entry0 = entry_of(a, b, my_key(begin)), entry1 = entry_of(a, b, my_key(begin + 1));
+  int entry = entry_of(a, b, my_key(begin + 2));
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) asm volatile("" ::"v"(qf[i]), "v"(entry0), "v"(entry1), "v"(entry));
+  __builtin_amdgcn_s_waitcnt(0);
+  uint64_t there = 0, there1 = 0;
+  if (begin < end) {
+    there = place(begin, entry0);
+    const int64_t scale0 = my_scale;
+    there1 = place(begin + 1, entry1);
+    const int64_t scale1 = my_scale;
+    __syncthreads();
+    if constexpr (k8) {
+      my_scale = scale0;
+      fetch(begin);
+      my_scale = scale1;
+      widen(begin);
+    } else {
+      issue(begin);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+  for (int kb = begin; kb < end; ++kb) {
+    const bool more = kb + 1 < end;
+    const char* ks = smem + (kb & 1) * kBuf;
+    char* vs = smem + (kb & 1) * kBuf + G::kTile;
+    const bool masked = there != ~0ull || (int64_t)(kb + 1) * kBlock > sp.ctx;
+    // The same in every wave: all of them look at the same tile.
+    uint64_t bad = 0;
+    if (masked) bad = not_finite<T, T, D>(vs, lane);
+    if (more) {
+      if constexpr (k8) fetch(kb + 1);
+      else issue(kb + 1);
+    }
+    const bool idle = row0 >= rows || (!a.mask && (int64_t)kb * kBlock > sp.ctx + t_wave);
+    if (!idle || bad) {
+      // V fragments read ahead of the softmax: as many key steps as registers
+      // allow (over codes the staged loads take some).
+      constexpr int kEarly = D < 128 ? 4 : k8 ? 0 : 2;
+      f32x16 s[2] = {f32x16{}, f32x16{}};
+      i32x4 vf[4][D / 32];
+      if constexpr (k8 && D == 128) {
+#pragma unroll
+        for (int h0 = 0; h0 < D / 16; h0 += 2) {
+          i32x4 kf[2][2];
+          read_k<T, T, D, 2>(ks, h0, l32, half, kf);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) s[kt] = mfma<T>(kf[kt][i], qf[h0 + i], s[kt]);
+        }
+      } else {
+        constexpr int H1 = D / 32;
+        i32x4 kf0[2][H1], kf1[2][H1];
+        read_k<T, T, D, H1>(ks, 0, l32, half, kf0);
+        __builtin_amdgcn_sched_barrier(0);
+        read_k<T, T, D, H1>(ks, H1, l32, half, kf1);
+#pragma unroll
+        for (int i = 0; i < H1; ++i)
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) s[kt] = mfma<T>(kf0[kt][i], qf[i], s[kt]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(vs, vt[dt], kk);
+#pragma unroll
+        for (int i = 0; i < H1; ++i)
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) s[kt] = mfma<T>(kf1[kt][i], qf[H1 + i], s[kt]);
+#pragma unroll
+        for (int kk = 2; kk < kEarly; ++kk)
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(vs, vt[dt], kk);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      i32x4 pf[4];
+      uint64_t seen = 0;
+      if (masked) seen = seen_bits(a, b, t, sp.ctx, kb * kBlock, there) >> (4 * half);
+      softmax<T, C, D>(s, pf, st, scale_log2, scales + (kb & 1) * 128, half, masked, seen);
+      if (bad) {
+        for (uint64_t left = bad; left; left &= left - 1)
+          add_key<T, T, D>(vs, __builtin_ctzll(left), s, seen, l32, half, st);
+        __syncthreads();
+        if (wave == 0)
+          for (uint64_t left = bad; left; left &= left - 1) clear_key<T, D>(vs, __builtin_ctzll(left), lane);
+        __syncthreads();
+#pragma unroll
+        for (int kk = 0; kk < kEarly; ++kk)
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(vs, vt[dt], kk);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kk = kEarly; kk < 4; ++kk)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(vs, vt[dt], kk);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = mfma<T>(vf[kk][dt], pf[kk], st.o[dt]);
+    }
+    if constexpr (k8)
+      if (more) widen(kb + 1);
+    // Offsets of the block after the next, whose place in LDS this block's had.
+    there = there1;
+    there1 = place(kb + 2, entry);
+    entry = entry_of(a, b, my_key(kb + 3));
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+
+  // Each lane holds half of its row's dims.
+  const float l = pair_sum(st.l);
+  const float u = k8 && T == Elt::F16 ? st.u : 1.0f;
+  if (row0 + l32 >= rows) return;
+  const int64_t id = (b * a.heads + h) * a.tokens + t;
+  if (per < blocks_all) {
+    const int64_t at = id * part.splits + split;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(f32x4*)(part.o + at * D + dt * 32 + 8 * g + 4 * half) =
+            f32x4{st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]} * u;
+    if (half == 0) part.ml[2 * at] = st.m, part.ml[2 * at + 1] = l;
+    return;
+  }
+  const float f = inverse_sum(l) * u;
+  const int64_t o_row = b * a.o_sb + h * a.o_sh + t * a.o_ss;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      store4<T>(a, o_row + dt * 32 + 8 * g + 4 * half,
+                f32x4{st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]} * f);
+  if (a.lse && half == 0) a.lse[id] = lse_of(st.m, l);
+#endif  // __HIP_DEVICE_COMPILE__
+}
+
+template <Elt T, Elt C, int D, int NW>
+static hipError_t launch_tile(const TreeAttnArgs& a, const Part& p, hipStream_t stream) {
+  auto kern = tree_tile_kernel<T, C, D, NW>;
+  constexpr int lds = 4 * Geom<T, D>::kTile + 2048;
+  static const hipError_t attr =
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (attr != hipSuccess) return attr;
+  const int group = a.heads / a.cache.kv_heads;
+  const int64_t blocks = ((int64_t)a.tokens * group + 32 * NW - 1) / (32 * NW);
+  const int64_t units = a.batch * a.cache.kv_heads * p.splits;
+  if (units * blocks > UINT32_MAX / 512) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(units * blocks)), dim3(64 * NW), lds, stream, a, p, (int)blocks,
+                     (int)units);
+  return hipGetLastError();
+}
+
+template <Elt T, Elt C, int D>
+static hipError_t launch_mfma(const TreeAttnArgs& a, const Part& p, hipStream_t s) {
+  if (a.kernel == plan::TreeKernel::Keys) return launch_keys<T, C, D>(a, p, s);
+  if constexpr (D == 128)
+    if (a.kernel == plan::TreeKernel::Tile8) return launch_tile<T, C, D, 8>(a, p, s);
+  return launch_tile<T, C, D, 4>(a, p, s);
 }
 
 template <int D> hipError_t tree_mfma_dispatch(const TreeAttnArgs& a, const Part& p, hipStream_t s) {
   const bool bf = a.dtype == Elt::BF16;
   switch (a.cache.kind) {
     case Elt::E4M3:
-      return bf ? launch_keys<Elt::BF16, Elt::E4M3, D>(a, p, s) : launch_keys<Elt::F16, Elt::E4M3, D>(a, p, s);
+      return bf ? launch_mfma<Elt::BF16, Elt::E4M3, D>(a, p, s) : launch_mfma<Elt::F16, Elt::E4M3, D>(a, p, s);
     case Elt::I8:
-      return bf ? launch_keys<Elt::BF16, Elt::I8, D>(a, p, s) : launch_keys<Elt::F16, Elt::I8, D>(a, p, s);
+      return bf ? launch_mfma<Elt::BF16, Elt::I8, D>(a, p, s) : launch_mfma<Elt::F16, Elt::I8, D>(a, p, s);
     default:
-      return bf ? launch_keys<Elt::BF16, Elt::BF16, D>(a, p, s) : launch_keys<Elt::F16, Elt::F16, D>(a, p, s);
+      return bf ? launch_mfma<Elt::BF16, Elt::BF16, D>(a, p, s) : launch_mfma<Elt::F16, Elt::F16, D>(a, p, s);
   }
 }
 

@@ -161,6 +161,7 @@ __global__ __launch_bounds__(256) void tree_sum_kernel(TreeAttnArgs a, tree::Par
   const float nM = M == -__builtin_inff() ? 0.0f : M;
   f32x4 acc = {0, 0, 0, 0};
   for (int s = 0; s < n; ++s) {
+    if (ml[2 * s + 1] == 0.0f) continue;  // no key of the split is seen
     const float g = __builtin_amdgcn_exp2f(ml[2 * s] - nM);
     L = __builtin_fmaf(ml[2 * s + 1], g, L);
     acc += *(const f32x4*)(part.o + (row * part.splits + s) * D + d) * g;

@@ -934,8 +934,8 @@ int kv_call(const frisk_kv_desc* d, bool write, void* stream) {
 }
 
 // Checks of the tree attention entries; 0 or an error code.  With ptrs ==
-// false the tensors are not required.
-int check_tree(const frisk_tree_attn_desc* d, bool ptrs, frisk::TreeAttnArgs& a) {
+// false the tensors are not required; `split`: the keys may be.
+int check_tree(const frisk_tree_attn_desc* d, bool ptrs, bool split, frisk::TreeAttnArgs& a) {
   const char* fn = "frisk_tree_attn";
   if (!d) return fail(FRISK_EINVAL, "%s: null descriptor", fn);
   if (d->batch <= 0 || d->heads <= 0 || d->tokens <= 0)
@@ -993,7 +993,8 @@ int check_tree(const frisk_tree_attn_desc* d, bool ptrs, frisk::TreeAttnArgs& a)
   a.mask = d->mask; a.mask_sb = d->mask_stride_b; a.mask_st = d->mask_stride_t;
   const int64_t keys = d->max_ctx ? std::min(d->max_ctx + d->tokens, a.cache.capacity) : a.cache.capacity;
   const frisk::plan::TreePlan p = frisk::plan::tree_plan(
-      d->batch, d->heads, d->cache.kv_heads, d->tokens, d->cache.head_dim, keys, frisk::device_cus());
+      d->batch, d->heads, d->cache.kv_heads, d->tokens, d->cache.head_dim, esize(d->cache.dtype) == 1, keys,
+      split, frisk::device_cus());
   a.kernel = p.kernel;
   a.splits = p.splits;
   a.min_blocks = p.min_blocks;
@@ -1137,19 +1138,17 @@ int frisk_tree_mask(int64_t batch, int64_t tokens, const int32_t* parents, uint6
 int64_t frisk_tree_attn_workspace_size(const frisk_tree_attn_desc* d) {
   g_last_error.clear();
   frisk::TreeAttnArgs a;
-  const int rc = check_tree(d, false, a);
+  const int rc = check_tree(d, false, true, a);
   return rc ? rc : tree_workspace(a);
 }
 
 int frisk_tree_attn(const frisk_tree_attn_desc* d, void* stream) {
   g_last_error.clear();
   frisk::TreeAttnArgs a;
-  const int rc = check_tree(d, true, a);
+  const int rc = check_tree(d, true, d && d->workspace, a);
   if (rc) return rc;
   const int64_t need = tree_workspace(a);
-  if (!d->workspace) {
-    a.splits = 1;
-  } else if (need > 0) {
+  if (need > 0) {
     if (d->workspace_bytes < need)
       return fail(FRISK_EINVAL, "frisk_tree_attn: workspace of %lld bytes, this call takes %lld",
                   (long long)d->workspace_bytes, (long long)need);

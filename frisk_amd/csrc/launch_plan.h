@@ -621,28 +621,70 @@ inline int64_t attn_workspace(int64_t batch_heads, int64_t seq_q, int64_t seq_k,
 // Rows: one query row a workgroup, head dims without a matrix-core kernel.
 // Keys: a tile of 32 query rows of a kv head a workgroup, whose waves divide the
 // keys.
+// Tile4, Tile8 (head_dim 128): 4 or 8 such tiles, one a wave, over shared keys.
 // The keys are split so that every CU has workgroups; `keys` is the most a
 // sequence may hold, and the kernels use fewer splits for shorter ones.
+//
+// Kernel and splits are the pair of least estimated time: 8 us to start, the
+// rounds of workgroups over the CUs, at least the bytes of K and V at 5.3
+// TB/s, and with splits 5 us of second launch and the f32 rows out and back at 3
+// TB/s.  A round is its steps (64 keys, under Keys 64 for each wave) times
+// the us below, fitted to calls with one and with two workgroups on a CU.  us, the choice of each kernel and its best splits:
+//   b8 h32/8 d128 8k keys        Keys        Tile4       Tile8
+//     bf16, 1 token              47.9 (2)    53.3 (8)    56.6 (4)
+//     bf16, 64 tokens            152 (1)     105 (4)     98 (4)
+//     e4m3, 16 tokens            43.4 (4)    62.7 (8)    75.3 (4)
+//     e4m3, 64 tokens            106 (1)     109 (4)     103 (4)
+//   b1 h32/8 d128 4k keys, 128 tokens: bf16 32.2 (2), 34.4 (8), 39.3 (8)
+//   b4 h16/16 d64 4k keys, 128 tokens: bf16 22.8 (1), 33.2 (4)
 // ---------------------------------------------------------------------------
 constexpr int kTreeBlock = 64;  // keys per block
-enum class TreeKernel { Rows, Keys };
+enum class TreeKernel { Rows, Keys, Tile4, Tile8 };
+constexpr int tree_key_waves(int64_t head_dim) { return head_dim == 128 ? 4 : 8; }
 struct TreePlan {
   TreeKernel kernel;
   int splits, min_blocks;
 };
 inline TreePlan tree_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t tokens, int64_t head_dim,
-                          int64_t keys, int cus) {
-  TreePlan p{TreeKernel::Rows, 1, 4};
-  const int64_t blocks = (keys + kTreeBlock - 1) / kTreeBlock;
-  int64_t want = (4 * (int64_t)cus + batch * heads * tokens - 1) / (batch * heads * tokens);
-  if (head_dim == 32 || head_dim == 64 || head_dim == 128) {
-    p.kernel = TreeKernel::Keys;
-    p.min_blocks = head_dim == 128 ? 4 : 8;  // one for every wave
-    const int64_t wgs = batch * kv_heads * ((tokens * (heads / kv_heads) + 31) / 32);
-    want = (cus + wgs - 1) / wgs;
+                          bool bits8, int64_t keys, bool split, int cus) {
+  const int64_t blocks = (keys + kTreeBlock - 1) / kTreeBlock, all = batch * heads * tokens;
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128) {
+    const int64_t want = (4 * (int64_t)cus + all - 1) / all;
+    const int64_t s = std::max<int64_t>(1, std::min({want, blocks / 4, (int64_t)64}));
+    return TreePlan{TreeKernel::Rows, split ? (int)s : 1, 4};
   }
-  p.splits = (int)std::max<int64_t>(1, std::min({want, blocks / p.min_blocks, (int64_t)64}));
-  return p;
+  struct Kind {
+    TreeKernel kernel;
+    int tile, waves, per_cu;  // rows and key-dividing waves of a workgroup, workgroups on a CU
+    double one, two;          // us a step
+  };
+  const bool d128 = head_dim == 128;
+  const Kind kinds[] = {
+      {TreeKernel::Keys, 32, tree_key_waves(head_dim), bits8 || head_dim == 32 ? 2 : 1,
+       d128 ? (bits8 ? 2.0 : 2.2) : bits8 ? 1.8 : 1.6, d128 ? 3.1 : head_dim == 64 ? 4.5 : bits8 ? 3.6 : 2.3},
+      {TreeKernel::Tile4, 128, 1, 2, d128 ? (bits8 ? 1.9 : 1.5) : bits8 ? 1.15 : 0.85,
+       d128 ? (bits8 ? 2.7 : 2.5) : bits8 ? 1.7 : 1.35},
+      {TreeKernel::Tile8, 256, 1, 1, bits8 ? 2.3 : 2.1, 0.0}};
+  const int64_t rows = tokens * (heads / kv_heads);  // of a kv head
+  const double bytes_us = 2.0 * batch * kv_heads * keys * head_dim * (bits8 ? 1 : 2) / 5.3e6;
+  TreePlan best{TreeKernel::Keys, 1, 1};
+  double best_us = -1.0;
+  for (const Kind& k : kinds) {
+    if (k.kernel == TreeKernel::Tile8 && !d128) continue;
+    const int64_t units = batch * kv_heads * ((rows + k.tile - 1) / k.tile);
+    const int least = k.kernel == TreeKernel::Keys ? k.waves : 4;
+    for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      if (s > 1 && (!split || blocks < (int64_t)least * s)) break;
+      const int64_t steps = ((blocks + s - 1) / s + k.waves - 1) / k.waves, load = (units * s + cus - 1) / cus;
+      const double work = (double)steps * ((load / k.per_cu) * (k.per_cu > 1 ? k.two : k.one) +
+                                           (load % k.per_cu ? k.one : 0.0));
+      const double us = std::max(work, bytes_us) + (s > 1 ? 5.0 + 8.0 * all * s * (head_dim + 2) / 3e6 : 0.0);
+      if (best_us >= 0 && us >= best_us) continue;
+      best_us = us;
+      best = TreePlan{k.kernel, s, least};
+    }
+  }
+  return best;
 }
 inline int64_t tree_workspace(int64_t rows, int splits, int64_t head_dim) {
   return splits > 1 ? rows * splits * (head_dim + 2) * 4 : 0;
