@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libfrisk_hip.so"
@@ -221,15 +222,20 @@ def _check(rc: int, what: str) -> None:
     raise RuntimeError(f"{what}: {msg}")
 
 
+_dtype_codes: dict = {}
+
+
 def torch_dtype_code(dt) -> int:
-    import torch
-    table = {
-        torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16,
-        torch.float8_e4m3fn: E4M3, torch.int8: I8, torch.int32: I32, torch.float64: F64,
-    }
-    if dt not in table:
+    if not _dtype_codes:
+        import torch
+        _dtype_codes.update({
+            torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16,
+            torch.float8_e4m3fn: E4M3, torch.int8: I8, torch.int32: I32, torch.float64: F64,
+        })
+    code = _dtype_codes.get(dt)
+    if code is None:
         raise ValueError(f"unsupported tensor dtype {dt}")
-    return table[dt]
+    return code
 
 
 def _stream_handle(stream) -> int:
@@ -567,6 +573,40 @@ def rope_table(rot_dim, base=10000.0, *, scaling="none", factor=1.0, trained=0.0
     return torch.tensor([v - (1 << 64) if v >> 63 else v for v in buf], dtype=torch.int64).to(device)
 
 
+# The calls below fill their descriptors with struct.pack, which takes a fifth
+# of the time of a ctypes.Structure's fields (a decode step's launches are short).
+
+def _packer(cls, until=None):
+    """struct.Struct of a descriptor's fields, up to the field `until`, padded
+    to its offset."""
+    codes = {_i64: "q", _i32: "i", ctypes.c_float: "f", _ptr: "P"}
+    fmt = "@"
+    for name, kind in cls._fields_:
+        if name == until:
+            break
+        fmt += codes[kind]
+    end = getattr(cls, until).offset if until else ctypes.sizeof(cls)
+    return struct.Struct(fmt + f"{end - struct.calcsize(fmt)}x")
+
+
+_rope_pack = _packer(RopeDesc)
+_kv_pack = _packer(KvDesc, "cache")
+_tree_pack = _packer(TreeAttnDesc, "cache")
+_ws_pack = struct.Struct("@Pq")
+_raw: dict = {}
+
+
+def _raw_fn(name: str):
+    """The library's function `name` taking a packed descriptor."""
+    fn = _raw.get(name)
+    if fn is None:
+        fn = load()[name]
+        fn.restype = ctypes.c_int64 if name.endswith("_size") else ctypes.c_int
+        fn.argtypes = [ctypes.c_char_p] + ([] if name.endswith("_size") else [ctypes.c_void_p])
+        _raw[name] = fn
+    return fn
+
+
 def _heads(t, name: str):
     """Shape and strides of a [batch, heads, rows, head_dim] device tensor."""
     sh, st = t.shape, t.stride()
@@ -575,32 +615,33 @@ def _heads(t, name: str):
     return sh, st
 
 
-def _same_device(*ts):
-    """Every tensor on the first one's device, which the call runs on."""
-    dev = ts[0].device
+def _same_device(*ts) -> int:
+    """The device index every tensor lies on, which the call runs on."""
+    dev = ts[0].get_device()
     for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on different devices ({dev} and {t.device})")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on different devices ({ts[0].device} and {t.device})")
+    return dev
 
 
-def _lengths(t, batch: int, name: str):
-    """The pointer of an int32 [batch] device tensor, or None."""
+def _lengths(t, batch: int, name: str) -> int:
+    """The pointer of an int32 [batch] device tensor, or 0."""
     import torch
     if t is None:
-        return None
-    if t.dtype != torch.int32 or tuple(t.shape) != (batch,) or not t.is_contiguous() or not t.is_cuda:
+        return 0
+    if t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous() or not t.is_cuda:
         raise ValueError(f"{name} must be a contiguous int32 device tensor of {batch} elements")
     return t.data_ptr()
 
 
-def _run(fn, name: str, d, device, stream):
-    """fn(d, stream) with `device` current."""
+def _run(name: str, desc: bytes, dev: int, stream):
+    """The library's `name` on a packed descriptor, with device `dev` current."""
     import torch
-    if device.index is not None and device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            _check(fn(ctypes.byref(d), _stream_handle(stream)), name)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            _check(_raw_fn(name)(desc, _stream_handle(stream)), name)
     else:
-        _check(fn(ctypes.byref(d), _stream_handle(stream)), name)
+        _check(_raw_fn(name)(desc, _stream_handle(stream)), name)
 
 
 def rope(x, out, positions, table, *, k=None, k_out=None, start=None, interleaved=False,
@@ -614,36 +655,33 @@ def rope(x, out, positions, table, *, k=None, k_out=None, start=None, interleave
     transposed rotation."""
     import torch
     (b, h, s, d), xs = _heads(x, "x")
-    (ob, oh, os_, od), outs = _heads(out, "out")
-    if (ob, oh, os_, od) != (b, h, s, d) or out.dtype != x.dtype:
+    osh, outs = _heads(out, "out")
+    if osh != x.shape or out.dtype != x.dtype:
         raise ValueError("x and out must have one shape and dtype")
-    if (k is None) != (k_out is None):
-        raise ValueError("k and k_out go together")
-    if table.dtype != torch.int64 or table.dim() != 1 or not table.is_contiguous() or not table.is_cuda:
+    if table.dtype != torch.int64 or table.dim() != 1 or not table.is_contiguous():
         raise ValueError("table must be a contiguous int64 device tensor (rope_table)")
-    desc = RopeDesc(b, s, h, 0, d, 2 * table.shape[0], torch_dtype_code(x.dtype),
-                    int(bool(interleaved)), int(bool(backward)), float(amplitude),
-                    x.data_ptr(), xs[0], xs[1], xs[2], out.data_ptr(), outs[0], outs[1], outs[2],
-                    start=_lengths(start, b, "start"), frequencies=table.data_ptr())
-    if k is not None:
+    kh, second = 0, (0,) * 8
+    if k is not None or k_out is not None:
+        if k is None or k_out is None:
+            raise ValueError("k and k_out go together")
         (kb, kh, ks_, kd), ks = _heads(k, "k")
         kosh, kos = _heads(k_out, "k_out")
-        if (kb, ks_, kd) != (b, s, d) or tuple(kosh) != (kb, kh, ks_, kd) or k.dtype != x.dtype \
-                or k_out.dtype != x.dtype:
+        if (kb, ks_, kd) != (b, s, d) or kosh != k.shape or k.dtype != x.dtype or k_out.dtype != x.dtype:
             raise ValueError("k and k_out must have one shape, and x's dtype, batch, seq and head_dim")
-        desc.k_heads = kh
-        desc.k, desc.k_stride_b, desc.k_stride_h, desc.k_stride_s = k.data_ptr(), ks[0], ks[1], ks[2]
-        desc.k_out, desc.k_out_stride_b, desc.k_out_stride_h, desc.k_out_stride_s = \
-            k_out.data_ptr(), kos[0], kos[1], kos[2]
+        second = (k.data_ptr(), ks[0], ks[1], ks[2], k_out.data_ptr(), kos[0], kos[1], kos[2])
+    at = (0, 0, 0, 0)
     if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64) or not positions.is_cuda or \
-                tuple(positions.shape) not in ((s,), (b, s)):
+        bits = 64 if positions.dtype == torch.int64 else 32
+        if (bits == 32 and positions.dtype != torch.int32) or positions.shape not in ((s,), (b, s)):
             raise ValueError("positions must be an int32 or int64 device tensor [seq] or [batch, seq]")
         st = positions.stride()
-        desc.positions, desc.position_bits = positions.data_ptr(), 8 * positions.element_size()
-        desc.pos_stride_b, desc.pos_stride_s = (0, st[0]) if len(st) == 1 else st
-    _same_device(x, out, k, k_out, positions, table, start)
-    _run(load().frisk_rope, "frisk_rope", desc, x.device, stream)
+        at = (positions.data_ptr(), bits, *((0, st[0]) if len(st) == 1 else st))
+    dev = _same_device(x, out, k, k_out, positions, table, start)
+    desc = _rope_pack.pack(b, s, h, kh, d, 2 * table.shape[0], torch_dtype_code(x.dtype),
+                           bool(interleaved), bool(backward), amplitude,
+                           x.data_ptr(), xs[0], xs[1], xs[2], out.data_ptr(), outs[0], outs[1], outs[2],
+                           *second, *at, _lengths(start, b, "start"), table.data_ptr())
+    _run("frisk_rope", desc, dev, stream)
     return out if k is None else (out, k_out)
 
 
@@ -654,7 +692,7 @@ class KvCache:
     [pages, kv_heads, page_size].  `block_table` (int32 [batch, max_pages])
     names the pages of each sequence; without it page b is sequence b's."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "block_table", "desc")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "block_table", "desc", "_packed", "_device")
 
     def __init__(self, k, v, k_scale=None, v_scale=None, block_table=None):
         import torch
@@ -679,7 +717,7 @@ class KvCache:
                                         (block_table.stride(1) != 1 and block_table.shape[1] > 1)):
             raise ValueError("block_table must be an int32 device tensor [batch, max_pages] with unit "
                              "stride along the pages")
-        _same_device(k, v, k_scale, v_scale, block_table)
+        self._device = _same_device(k, v, k_scale, v_scale, block_table)
         self.k, self.v, self.k_scale, self.v_scale, self.block_table = k, v, k_scale, v_scale, block_table
         self.desc = KvCacheDesc(
             *ksh, torch_dtype_code(k.dtype), k.data_ptr(), v.data_ptr(), *kst[:3],
@@ -688,6 +726,7 @@ class KvCache:
             None if block_table is None else block_table.data_ptr(),
             0 if block_table is None else block_table.stride(0),
             0 if block_table is None else block_table.shape[1])
+        self._packed = bytes(self.desc)
 
     @classmethod
     def empty(cls, pages, kv_heads, page_size, head_dim, dtype, *, block_table=None, device="cuda"):
@@ -700,24 +739,25 @@ class KvCache:
             ks, vs = (torch.empty(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
         return cls(k, v, ks, vs, block_table)
 
-    def _rows(self, batch: int):
+    def _check(self, batch: int, *ts) -> int:
+        """The device of the cache and `ts`, for a batch that fits the block table."""
         if self.block_table is not None and self.block_table.shape[0] != batch:
             raise ValueError(f"block_table has {self.block_table.shape[0]} rows for a batch of {batch}")
+        return _same_device(self.k, *ts)
 
 
-def _kv(fn, name, k, v, cache, ctx_len, new_len, stream):
+def _kv(name, k, v, cache, ctx_len, new_len, stream):
     (b, h, t, d), ks = _heads(k, "k")
     vsh, vs = _heads(v, "v")
-    c = cache.desc
-    if tuple(vsh) != (b, h, t, d) or v.dtype != k.dtype or h != c.kv_heads or d != c.head_dim:
-        raise ValueError(f"k and v must be [batch, {c.kv_heads}, tokens, {c.head_dim}] of one dtype "
+    csh = cache.k.shape
+    if vsh != k.shape or v.dtype != k.dtype or h != csh[1] or d != csh[3]:
+        raise ValueError(f"k and v must be [batch, {csh[1]}, tokens, {csh[3]}] of one dtype "
                          f"(got {tuple(k.shape)} and {tuple(v.shape)})")
-    cache._rows(b)
-    _same_device(k, v, cache.k, ctx_len, new_len)
-    desc = KvDesc(b, t, torch_dtype_code(k.dtype), k.data_ptr(), ks[0], ks[1], ks[2],
-                  v.data_ptr(), vs[0], vs[1], vs[2], _lengths(ctx_len, b, "ctx_len"),
-                  _lengths(new_len, b, "new_len"), c)
-    _run(fn, name, desc, k.device, stream)
+    dev = cache._check(b, k, v, ctx_len, new_len)
+    desc = _kv_pack.pack(b, t, torch_dtype_code(k.dtype), k.data_ptr(), ks[0], ks[1], ks[2],
+                         v.data_ptr(), vs[0], vs[1], vs[2], _lengths(ctx_len, b, "ctx_len"),
+                         _lengths(new_len, b, "new_len")) + cache._packed
+    _run(name, desc, dev, stream)
 
 
 def kv_append(k, v, cache, ctx_len, *, new_len=None, stream=None):
@@ -725,7 +765,7 @@ def kv_append(k, v, cache, ctx_len, *, new_len=None, stream=None):
     KvCache as keys ctx_len[b] .. of each sequence (int32 [batch] on the
     device; negative: the sequence takes no part), the first new_len[b]
     tokens of it.  An 8-bit cache quantises each row by its largest value."""
-    _kv(load().frisk_kv_append, "frisk_kv_append", k, v, cache, ctx_len, new_len, stream)
+    _kv("frisk_kv_append", k, v, cache, ctx_len, new_len, stream)
     return cache
 
 
@@ -733,7 +773,7 @@ def kv_read(cache, k, v, ctx_len, *, new_len=None, stream=None):
     """Read keys ctx_len[b] .. of each sequence back into k and v [batch,
     kv_heads, tokens, head_dim], the first new_len[b] rows of it; the other
     rows are left as they were."""
-    _kv(load().frisk_kv_read, "frisk_kv_read", k, v, cache, ctx_len, new_len, stream)
+    _kv("frisk_kv_read", k, v, cache, ctx_len, new_len, stream)
     return k, v
 
 
@@ -751,48 +791,53 @@ def tree_mask(parents, mask=None, depth=None, *, stream=None):
     words = (t + 63) // 64
     if mask is None:
         mask = torch.empty((b, t, words), dtype=torch.int64, device=parents.device)
+    elif mask.dtype != torch.int64 or mask.shape != (b, t, words) or not mask.is_contiguous():
+        raise ValueError(f"mask must be a contiguous int64 tensor [{b}, {t}, {words}]")
     if depth is None:
         depth = torch.empty((b, t), dtype=torch.int32, device=parents.device)
-    if mask.dtype != torch.int64 or tuple(mask.shape) != (b, t, words) or not mask.is_contiguous():
-        raise ValueError(f"mask must be a contiguous int64 tensor [{b}, {t}, {words}]")
-    if depth.dtype != torch.int32 or tuple(depth.shape) != (b, t) or not depth.is_contiguous():
+    elif depth.dtype != torch.int32 or depth.shape != (b, t) or not depth.is_contiguous():
         raise ValueError(f"depth must be a contiguous int32 tensor [{b}, {t}]")
-    _same_device(parents, mask, depth)
-    with torch.cuda.device(parents.device):
-        _check(load().frisk_tree_mask(b, t, parents.data_ptr(), mask.data_ptr(), depth.data_ptr(),
-                                      _stream_handle(stream)), "frisk_tree_mask")
+    dev = _same_device(parents, mask, depth)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return tree_mask(parents, mask, depth, stream=stream)
+    _check(load().frisk_tree_mask(b, t, parents.data_ptr(), mask.data_ptr(), depth.data_ptr(),
+                                  _stream_handle(stream)), "frisk_tree_mask")
     return mask, depth
+
+
+def _tree_values(q, cache, ctx_len, o, mask, new_len, sm_scale, lse, max_ctx):
+    """Device and the fields of TreeAttnDesc before its cache."""
+    import torch
+    (b, h, t, d), qs = _heads(q, "q")
+    osh, os_ = _heads(o, "o")
+    if osh != q.shape or d != cache.k.shape[3]:
+        raise ValueError(f"q and o must have one shape and the cache's head_dim {cache.k.shape[3]} "
+                         f"(got {tuple(q.shape)} and {tuple(o.shape)})")
+    if lse is not None and (lse.shape != (b, h, t) or not lse.is_contiguous()
+                            or lse.dtype != torch.float32):
+        raise ValueError("lse must be a contiguous f32 [batch, heads, tokens] tensor")
+    words = (0, 0, 0)
+    if mask is not None:
+        n = (t + 63) // 64
+        if mask.dtype != torch.int64 or mask.shape not in ((t, n), (b, t, n)) or \
+                (mask.stride(-1) != 1 and n > 1):
+            raise ValueError(f"mask must be int64 words [{t}, {n}] or [{b}, {t}, {n}] (tree_mask)")
+        st = mask.stride()
+        words = (mask.data_ptr(), *((0, st[0]) if len(st) == 2 else st[:2]))
+    dev = cache._check(b, q, o, ctx_len, new_len, mask, lse)
+    return dev, (b, h, t, torch_dtype_code(q.dtype), torch_dtype_code(o.dtype),
+                 d ** -0.5 if sm_scale is None else sm_scale,
+                 q.data_ptr(), qs[0], qs[1], qs[2], o.data_ptr(), os_[0], os_[1], os_[2],
+                 0 if lse is None else lse.data_ptr(), _lengths(ctx_len, b, "ctx_len"),
+                 _lengths(new_len, b, "new_len"), *words, max_ctx)
 
 
 def tree_attn_desc(q, cache, ctx_len, o, *, mask=None, new_len=None, sm_scale=None, lse=None,
                    max_ctx=0) -> TreeAttnDesc:
-    """Describe tree_attn's call."""
-    import torch
-    (b, h, t, d), qs = _heads(q, "q")
-    osh, os_ = _heads(o, "o")
-    c = cache.desc
-    if tuple(osh) != (b, h, t, d) or d != c.head_dim:
-        raise ValueError(f"q and o must have one shape and the cache's head_dim {c.head_dim} "
-                         f"(got {tuple(q.shape)} and {tuple(o.shape)})")
-    if lse is not None and (tuple(lse.shape) != (b, h, t) or not lse.is_contiguous()
-                            or lse.dtype != torch.float32):
-        raise ValueError("lse must be a contiguous f32 [batch, heads, tokens] tensor")
-    cache._rows(b)
-    _same_device(q, o, cache.k, ctx_len, new_len, mask, lse)
-    desc = TreeAttnDesc(b, h, t, torch_dtype_code(q.dtype), torch_dtype_code(o.dtype),
-                        float(d ** -0.5 if sm_scale is None else sm_scale),
-                        q.data_ptr(), qs[0], qs[1], qs[2], o.data_ptr(), os_[0], os_[1], os_[2],
-                        None if lse is None else lse.data_ptr(), _lengths(ctx_len, b, "ctx_len"),
-                        _lengths(new_len, b, "new_len"), max_ctx=int(max_ctx), cache=c)
-    if mask is not None:
-        words = (t + 63) // 64
-        if mask.dtype != torch.int64 or tuple(mask.shape) not in ((t, words), (b, t, words)) or \
-                (mask.stride(-1) != 1 and words > 1):
-            raise ValueError(f"mask must be int64 words [{t}, {words}] or [{b}, {t}, {words}] (tree_mask)")
-        st = mask.stride()
-        desc.mask = mask.data_ptr()
-        desc.mask_stride_b, desc.mask_stride_t = (0, st[0]) if len(st) == 2 else st[:2]
-    return desc
+    """Describe tree_attn's call (without a workspace)."""
+    _, values = _tree_values(q, cache, ctx_len, o, mask, new_len, sm_scale, lse, max_ctx)
+    return TreeAttnDesc(*values, cache.desc)
 
 
 def tree_attn_workspace_bytes(desc: TreeAttnDesc) -> int:
@@ -814,17 +859,19 @@ def tree_attn(q, cache, ctx_len, o, *, mask=None, new_len=None, sm_scale=None, l
     caching allocator, on the call's stream), a device tensor supplies it,
     False runs unsplit."""
     import torch
-    if q.device.index is not None and q.device.index != torch.cuda.current_device():
-        with torch.cuda.device(q.device):
+    dev, values = _tree_values(q, cache, ctx_len, o, mask, new_len, sm_scale, lse, max_ctx)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
             return tree_attn(q, cache, ctx_len, o, mask=mask, new_len=new_len, sm_scale=sm_scale,
                              lse=lse, max_ctx=max_ctx, workspace=workspace, stream=stream)
-    d = tree_attn_desc(q, cache, ctx_len, o, mask=mask, new_len=new_len, sm_scale=sm_scale, lse=lse,
-                       max_ctx=max_ctx)
-    lib, ws = load(), None
+    head = _tree_pack.pack(*values) + cache._packed
+    ws, tail = None, bytes(16)
     if workspace is not False:
-        need = tree_attn_workspace_bytes(d)
+        need = _raw_fn("frisk_tree_attn_workspace_size")(head + tail)
+        if need < 0:
+            _check(need, "frisk_tree_attn_workspace_size")
         if need > 0:
             ws = workspace if workspace is not True else _scratch(need, o.device, stream)
-            d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    _check(lib.frisk_tree_attn(ctypes.byref(d), _stream_handle(stream)), "frisk_tree_attn")
+            tail = _ws_pack.pack(ws.data_ptr(), ws.numel() * ws.element_size())
+    _check(_raw_fn("frisk_tree_attn")(head + tail, _stream_handle(stream)), "frisk_tree_attn")
     return o
