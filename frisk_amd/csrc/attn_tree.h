@@ -18,6 +18,9 @@ struct Part {
   float* ml;  // [rows][splits][2]
   int splits;
   int min_blocks;  // a split has at least so many blocks
+  // The Keys kernel, which sums its splits itself, lays o out by tiles of rows
+  // (keys_part) and has a word for each behind them.
+  unsigned long long* words;
 };
 
 // Blocks per split of a sequence with `keys` keys: the launch's splits, or

@@ -34,6 +34,7 @@ namespace tree {
 
 #define TREE_INLINE __device__ __forceinline__
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef __attribute__((address_space(1))) const void* global_ptr;
 
@@ -443,6 +444,43 @@ template <Elt C, int D> constexpr int keys_lds() {
   return tiles > sum ? tiles : sum;
 }
 
+// The f32 rows of a tile's splits: per split [32][D] of O (not divided by l),
+// then [32][2] of m and l; and the word its splits arrive at.  They are written
+// and read past the XCDs' L2 caches (device scope), the arrival is an atomic.
+constexpr int kDeviceScope = 0x10;  // SC1 of a buffer access
+struct KeysPart {
+  __amdgpu_buffer_rsrc_t rs;
+  int bytes;  // of a split
+  unsigned long long* word;
+};
+template <int D> TREE_INLINE KeysPart keys_part(const Part& p, int64_t tile) {
+  constexpr int kFloats = 32 * (D + 2);
+  KeysPart k;
+  k.bytes = kFloats * 4;
+  k.rs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.o + tile * p.splits * kFloats), (short)0,
+                                           p.splits * kFloats * 4, 0x00020000);
+  k.word = p.words + tile;
+  return k;
+}
+
+// Whether this is the last of n arrivals at a word, which is then 0 again.  Any
+// value but kArrived + count reads as no arrival yet, so a workspace needs no
+// clearing (one never used holds that with probability 2^-56).
+constexpr unsigned long long kArrived = 0x7AEE51EC0DE20000ull;
+TREE_INLINE int arrive(unsigned long long* word, int n) {
+  unsigned long long old = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // An exchange fails only when another arrival changed the word: at most n
+  // times.
+  for (int attempt = 0; attempt <= n; ++attempt) {
+    const int count = (old & ~0xffull) == kArrived ? (int)(old & 0xff) : 0;
+    const bool last = count + 1 == n;
+    if (__hip_atomic_compare_exchange_strong(word, &old, last ? 0ull : kArrived + count + 1, __ATOMIC_RELAXED,
+                                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+      return last;
+  }
+  return 0;
+}
+
 // One tile of 32 rows per workgroup; each wave takes every NW-th key block of
 // the split with K and V tiles of its own: no barrier in the loop, and a block's
 // bytes of loads in flight per wave.
@@ -610,6 +648,8 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
   }
   __syncthreads();
   const int live = min(32, rows - tile * 32);
+  const int splits = (blocks_all + per - 1) / per;  // of this sequence
+  const KeysPart kp = keys_part<D>(part, (int64_t)bk * row_tiles + tile);
   for (int idx = tid; idx < live * (D / 4); idx += 64 * NW) {
     const int q = idx / (D / 4), d = idx % (D / 4) * 4;
     float M = -__builtin_inff(), L = 0.0f;
@@ -623,16 +663,56 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
       L = __builtin_fmaf(f, pm[(w * 32 + q) * 2 + 1], L);
       acc += *(const f32x4*)(po + (w * 32 + q) * kPitch + d) * f;
     }
-    const int r = tile * 32 + q, rt = r / group, rh = kvh * group + r % group;
-    const int64_t id = (b * a.heads + rh) * a.tokens + rt;
-    if (per < blocks_all) {
-      const int64_t at = id * part.splits + split;
-      *(f32x4*)(part.o + at * D + d) = acc;
-      if (d == 0) part.ml[2 * at] = M, part.ml[2 * at + 1] = L;
+    if (splits > 1) {
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, acc), kp.rs, (q * D + d) * 4,
+                                             split * kp.bytes, kDeviceScope);
+      if (d == 0) {
+        const i32x2 ml = {__builtin_bit_cast(int, M), __builtin_bit_cast(int, L)};
+        __builtin_amdgcn_raw_buffer_store_b64(ml, kp.rs, (32 * D + 2 * q) * 4, split * kp.bytes, kDeviceScope);
+      }
       continue;
     }
+    const int r = tile * 32 + q, rt = r / group, rh = kvh * group + r % group;
     store4<T>(a, b * a.o_sb + rh * a.o_sh + rt * a.o_ss + d, acc * inverse_sum(L));
-    if (a.lse && d == 0) a.lse[id] = lse_of(M, L);
+    if (a.lse && d == 0) a.lse[(b * a.heads + rh) * a.tokens + rt] = lse_of(M, L);
+  }
+  if (splits <= 1) return;
+  // The last workgroup of the tile's splits to arrive sums them, in split order.
+  __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));  // vmcnt(0): the stores are acknowledged
+  __syncthreads();
+  int* last = (int*)smem;
+  if (tid == 0) *last = arrive(kp.word, splits);
+  __syncthreads();
+  if (!*last) return;
+  for (int idx = tid; idx < live * (D / 4); idx += 64 * NW) {
+    const int q = idx / (D / 4), d = idx % (D / 4) * 4;
+    float M = -__builtin_inff(), L = 0.0f;
+    f32x4 acc = {0, 0, 0, 0};
+    for (int s0 = 0; s0 < splits; s0 += 4) {
+      f32x2 ml[4];
+      f32x4 o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = min(s0 + i, splits - 1) * kp.bytes;
+        ml[i] = __builtin_bit_cast(
+            f32x2, __builtin_amdgcn_raw_buffer_load_b64(kp.rs, (32 * D + 2 * q) * 4, at, kDeviceScope));
+        o[i] = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(kp.rs, (q * D + d) * 4, at, kDeviceScope));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (s0 + i >= splits) continue;
+        const float m = ml[i][0], n = fmaxf(M, m);
+        const float nn = n == -__builtin_inff() ? 0.0f : n;
+        const float fa = __builtin_amdgcn_exp2f(M - nn), fb = __builtin_amdgcn_exp2f(m - nn);
+        L = L * fa + ml[i][1] * fb;
+        acc = acc * fa + o[i] * fb;
+        M = n;
+      }
+    }
+    const int r = tile * 32 + q, rt = r / group, rh = kvh * group + r % group;
+    store4<T>(a, b * a.o_sb + rh * a.o_sh + rt * a.o_ss + d, acc * inverse_sum(L));
+    if (a.lse && d == 0) a.lse[(b * a.heads + rh) * a.tokens + rt] = lse_of(M, L);
   }
 #endif  // __HIP_DEVICE_COMPILE__
 }

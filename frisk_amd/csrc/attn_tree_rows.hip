@@ -205,10 +205,16 @@ hipError_t tree_attn_sum(const TreeAttnArgs& a, const tree::Part& p, hipStream_t
 }
 
 hipError_t tree_attn(const TreeAttnArgs& a, hipStream_t s) {
-  tree::Part p{nullptr, nullptr, a.splits, a.min_blocks};
+  tree::Part p{nullptr, nullptr, a.splits, a.min_blocks, nullptr};
+  const bool keys = a.kernel == plan::TreeKernel::Keys;
   if (a.splits > 1) {
     p.o = (float*)a.workspace;
-    p.ml = p.o + a.batch * a.heads * a.tokens * a.splits * a.cache.head_dim;
+    if (keys) {
+      const int64_t tiles = plan::tree_key_tiles(a.batch, a.heads, a.cache.kv_heads, a.tokens);
+      p.words = (unsigned long long*)(p.o + tiles * a.splits * 32 * (a.cache.head_dim + 2));
+    } else {
+      p.ml = p.o + a.batch * a.heads * a.tokens * a.splits * a.cache.head_dim;
+    }
   }
   hipError_t e;
   switch (a.kernel == plan::TreeKernel::Rows ? 0 : a.cache.head_dim) {
@@ -217,7 +223,7 @@ hipError_t tree_attn(const TreeAttnArgs& a, hipStream_t s) {
     case 128: e = tree_attn_d128(a, p, s); break;
     default: e = tree_attn_rows(a, p, s);
   }
-  if (e != hipSuccess || a.splits <= 1) return e;
+  if (e != hipSuccess || a.splits <= 1 || keys) return e;
   return tree_attn_sum(a, p, s);
 }
 

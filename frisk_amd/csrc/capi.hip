@@ -1003,7 +1003,8 @@ int check_tree(const frisk_tree_attn_desc* d, bool ptrs, bool split, frisk::Tree
 }
 
 int64_t tree_workspace(const frisk::TreeAttnArgs& a) {
-  return frisk::plan::tree_workspace(a.batch * a.heads * a.tokens, a.splits, a.cache.head_dim);
+  return frisk::plan::tree_workspace(frisk::plan::TreePlan{a.kernel, a.splits, a.min_blocks}, a.batch, a.heads,
+                                     a.cache.kv_heads, a.tokens, a.cache.head_dim);
 }
 
 }  // namespace

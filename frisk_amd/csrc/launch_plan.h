@@ -627,8 +627,8 @@ inline int64_t attn_workspace(int64_t batch_heads, int64_t seq_q, int64_t seq_k,
 //
 // Kernel and splits are the pair of least estimated time: 8 us to start, the
 // rounds of workgroups over the CUs, at least the bytes of K and V at 5.3
-// TB/s, and with splits 5 us of second launch and the f32 rows out and back at 3
-// TB/s.  A round is its steps (64 keys, under Keys 64 for each wave) times
+// TB/s, and with splits the f32 rows out and back at 3 TB/s and 5 us of second
+// launch, or 2 us and 0.1 a split where the last workgroup of a tile sums them.  A round is its steps (64 keys, under Keys 64 for each wave) times
 // the us below, fitted to calls with one and with two workgroups on a CU.  us, the choice of each kernel and its best splits:
 //   b8 h32/8 d128 8k keys        Keys        Tile4       Tile8
 //     bf16, 1 token              47.9 (2)    53.3 (8)    56.6 (4)
@@ -678,7 +678,9 @@ inline TreePlan tree_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_
       const int64_t steps = ((blocks + s - 1) / s + k.waves - 1) / k.waves, load = (units * s + cus - 1) / cus;
       const double work = (double)steps * ((load / k.per_cu) * (k.per_cu > 1 ? k.two : k.one) +
                                            (load % k.per_cu ? k.one : 0.0));
-      const double us = std::max(work, bytes_us) + (s > 1 ? 5.0 + 8.0 * all * s * (head_dim + 2) / 3e6 : 0.0);
+      const double out = k.kernel == TreeKernel::Keys ? 2.0 + 0.1 * s : 5.0;
+      // (Fewer workgroups than CUs do not reach HBM's rate, nor even out ragged lengths.)
+      const double us = std::max(work, units * s < cus ? 1.12 * bytes_us : bytes_us) + (s > 1 ? out + 8.0 * all * s * (head_dim + 2) / 3e6 : 0.0);
       if (best_us >= 0 && us >= best_us) continue;
       best_us = us;
       best = TreePlan{k.kernel, s, least};
@@ -686,8 +688,17 @@ inline TreePlan tree_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_
   }
   return best;
 }
-inline int64_t tree_workspace(int64_t rows, int splits, int64_t head_dim) {
-  return splits > 1 ? rows * splits * (head_dim + 2) * 4 : 0;
+// Tiles of 32 query rows of all kv heads.
+inline int64_t tree_key_tiles(int64_t batch, int64_t heads, int64_t kv_heads, int64_t tokens) {
+  return batch * kv_heads * ((tokens * (heads / kv_heads) + 31) / 32);
+}
+// f32 rows and their statistics for every split; Keys: of whole tiles, and an
+// arrival word for each.
+inline int64_t tree_workspace(const TreePlan& p, int64_t batch, int64_t heads, int64_t kv_heads, int64_t tokens,
+                              int64_t head_dim) {
+  if (p.splits <= 1) return 0;
+  if (p.kernel != TreeKernel::Keys) return batch * heads * tokens * p.splits * (head_dim + 2) * 4;
+  return tree_key_tiles(batch, heads, kv_heads, tokens) * (p.splits * 32 * (head_dim + 2) * 4 + 8);
 }
 
 // ---------------------------------------------------------------------------
