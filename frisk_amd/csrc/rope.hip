@@ -9,10 +9,14 @@
 // whose sine and cosine are Taylor polynomials (degrees 9 and 10: the first
 // terms left out are 1.8e-9 and 1.1e-10 at pi / 4, below half a step of f32).
 //
-// The work.  16 B of each half of a pair per lane; a thread takes the same
-// pairs of several heads, so the angle's ~40 instructions a pair are paid once
-// for them, and the loads of up to four heads are in flight together.  HBM
-// bounds it.
+// The work.  A thread takes 16 B of each half of its pairs, or 16 B of interleaved
+// pairs, of several heads, so the angle's ~40 instructions a pair are paid once
+// for them and the loads of up to 8 pieces are in flight together.  HBM
+// bounds it.  Outputs beyond the L2s' 32 MB are stored past them where a wave
+// stores whole 128-B lines (they would be written back at the kernel's end, and
+// nobody reads them there): q and k of 8192 tokens, h32/8 d128 bf16, 45 -> 34 us;
+// rows of 192 + 128 B, which leave parts of lines, are faster through L2 (11
+// against 13 us).
 
 #include "common.h"
 #include "kernels.h"
@@ -62,16 +66,19 @@ template <Elt E, int P> __device__ __forceinline__ void put(typename Piece<E, P>
   else v[i] = (typename EltInfo<E>::T)f;
 }
 
-// P pairs per thread and head: two pieces of P elements.  A token has
-// `pair_chunks` of those and `copy_chunks` pieces of dims to copy, times
-// `lanes` threads that share its heads.
-template <Elt E, int P, bool INTER>
+// Pieces of P elements.  Pairs in halves: a chunk is P pairs, a piece of each
+// half; interleaved: a chunk is one piece of P / 2 pairs (P == 1: two pieces, one
+// pair).  A token has `pair_chunks` of those and `copy_chunks` pieces of dims to
+// copy, times `lanes` threads that share its heads.
+template <Elt E, int P, bool INTER, bool PAST_L2>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pair_chunks, int copy_chunks,
                                                    int lanes, int tokens_per_block,
                                                    int blocks_per_token) {
   using V = typename Piece<E, P>::V;
   using T = typename EltInfo<E>::T;
-  constexpr int HB = 4;  // heads in flight
+  constexpr int NV = INTER && P > 1 ? 1 : 2;          // pieces of a chunk
+  constexpr int NP = INTER && P > 1 ? P / 2 : P;      // pairs of a chunk
+  constexpr int HB = 8 / NV;                          // heads in flight
   const int chunks = pair_chunks + copy_chunks, n = chunks * lanes;
   int64_t token;
   int item;
@@ -100,12 +107,20 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pair_chunks, 
   auto out_row = [&](int h) {
     return h < h0 ? out0 + h * a.t[0].osh : out1 + (h - h0) * a.t[1].osh;
   };
+  auto store = [&](T* p, V v) {
+    if constexpr (PAST_L2) __builtin_nontemporal_store(v, (V*)p);
+    else *(V*)p = v;
+  };
+  auto load = [&](const T* p) {
+    if constexpr (PAST_L2) return __builtin_nontemporal_load((const V*)p);
+    else return *(const V*)p;
+  };
 
   if (chunk >= pair_chunks) {  // dims that are not rotated
     const int at = a.rot_dim + (chunk - pair_chunks) * P;
     for (int h = first; h < heads; h += lanes) {
       if (h < h0 ? a.t[0].x == a.t[0].out : a.t[1].x == a.t[1].out) continue;  // in place
-      *(V*)(out_row(h) + at) = *(const V*)(in_row(h) + at);
+      store(out_row(h) + at, load(in_row(h) + at));
     }
     return;
   }
@@ -113,106 +128,100 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pair_chunks, 
   if (!a.positions) p += s;
   else if (a.position_bits == 64) p += ((const int64_t*)a.positions)[b * a.pos_sb + s * a.pos_ss];
   else p += ((const int32_t*)a.positions)[b * a.pos_sb + s * a.pos_ss];
-  float cs[P], sn[P];
+  float cs[NP], sn[NP];
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const SinCos r = sincos_turns((uint64_t)p * a.freq[chunk * P + i]);
+  for (int i = 0; i < NP; ++i) {
+    const SinCos r = sincos_turns((uint64_t)p * a.freq[chunk * NP + i]);
     cs[i] = r.c * a.amplitude;
     sn[i] = (a.backward ? -r.s : r.s) * a.amplitude;
   }
-  const int at0 = INTER ? chunk * 2 * P : chunk * P;
-  const int at1 = INTER ? at0 + P : at0 + a.rot_dim / 2;
+  const int at0 = INTER ? chunk * 2 * NP : chunk * NP;
+  const int at1 = INTER ? at0 + 1 : at0 + a.rot_dim / 2;  // (the second piece, if any)
   for (int base = first; base < heads; base += HB * lanes) {
-    V x0[HB], x1[HB];
+    V x[HB][NV];
 #pragma unroll
     for (int j = 0; j < HB; ++j) {
       const int h = base + j * lanes;
       if (h < heads) {
         const T* row = in_row(h);
-        x0[j] = *(const V*)(row + at0);
-        x1[j] = *(const V*)(row + at1);
+        x[j][0] = load(row + at0);
+        if constexpr (NV == 2) x[j][1] = load(row + at1);
       }
     }
 #pragma unroll
     for (int j = 0; j < HB; ++j) {
       const int h = base + j * lanes;
       if (h >= heads) continue;
-      V y0, y1;
+      V y[NV];
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        // Pair i is (x0[i], x1[i]), or interleaved elements 2i and 2i + 1 of x0, x1.
-        const int e0 = INTER ? 2 * i : i, e1 = INTER ? 2 * i + 1 : i;
-        const float u = !INTER || e0 < P ? get<E, P>(x0[j], e0) : get<E, P>(x1[j], e0 - P);
-        const float w = !INTER ? get<E, P>(x1[j], e1)
-                        : e1 < P ? get<E, P>(x0[j], e1) : get<E, P>(x1[j], e1 - P);
-        const float yu = __builtin_fmaf(u, cs[i], -(w * sn[i]));
-        const float yw = __builtin_fmaf(u, sn[i], w * cs[i]);
-        if (!INTER) {
-          put<E, P>(y0, i, yu);
-          put<E, P>(y1, i, yw);
-        } else {
-          if (e0 < P) put<E, P>(y0, e0, yu); else put<E, P>(y1, e0 - P, yu);
-          if (e1 < P) put<E, P>(y0, e1, yw); else put<E, P>(y1, e1 - P, yw);
-        }
+      for (int i = 0; i < NP; ++i) {
+        const int e0 = NV == 1 ? 2 * i : i, e1 = NV == 1 ? 2 * i + 1 : i;
+        const float u = get<E, P>(x[j][0], e0), w = get<E, P>(x[j][NV - 1], e1);
+        put<E, P>(y[0], e0, __builtin_fmaf(u, cs[i], -(w * sn[i])));
+        put<E, P>(y[NV - 1], e1, __builtin_fmaf(u, sn[i], w * cs[i]));
       }
       T* row = out_row(h);
-      *(V*)(row + at0) = y0;
-      *(V*)(row + at1) = y1;
+      store(row + at0, y[0]);
+      if constexpr (NV == 2) store(row + at1, y[1]);
     }
   }
 }
 
-template <Elt E, int P>
+template <Elt E, int P, bool INTER>
 hipError_t launch_rope(const RopeArgs& a, hipStream_t stream) {
+  constexpr int NP = INTER && P > 1 ? P / 2 : P, es = EltInfo<E>::bytes;
   const int heads = a.t[0].heads + a.t[1].heads;
   const bool copies = a.t[0].x != a.t[0].out || (a.t[1].heads && a.t[1].x != a.t[1].out);
-  const int pair_chunks = a.rot_dim / 2 / P;
+  const int pair_chunks = a.rot_dim / 2 / NP;
   const int copy_chunks = copies ? (a.head_dim - a.rot_dim) / P : 0;
   const int chunks = pair_chunks + copy_chunks;
-  // A thread takes up to 8 heads once that leaves two workgroups' threads for
-  // every CU.
+  // A thread takes as many heads as it has in flight at once, where that leaves
+  // two workgroups' threads for every CU.
+  constexpr int kMost = INTER && P > 1 ? 8 : 4;
   const int64_t tokens = a.batch * a.seq;
   const int64_t spare = tokens * chunks * heads / ((int64_t)device_cus() * 512);
-  const int per = (int)std::min<int64_t>(std::max<int64_t>(spare, 1), 8);
+  const int per = (int)std::min<int64_t>(std::max<int64_t>(spare, 1), kMost);
   const int lanes = (heads + per - 1) / per;
   const int64_t n = (int64_t)chunks * lanes;
   const int tpb = n < 256 ? (int)(256 / n) : 1, bpt = (int)((n + 255) / 256);
   const int64_t blocks = n < 256 ? (tokens + tpb - 1) / tpb : tokens * bpt;
   if (blocks > UINT32_MAX / 256) return hipErrorInvalidConfiguration;
-  if (a.interleaved)
-    hipLaunchKernelGGL((rope_kernel<E, P, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a,
-                       pair_chunks, copy_chunks, lanes, tpb, bpt);
-  else
-    hipLaunchKernelGGL((rope_kernel<E, P, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a,
-                       pair_chunks, copy_chunks, lanes, tpb, bpt);
+  const int64_t run = INTER ? a.rot_dim : a.rot_dim / 2;  // elements that neighbouring lanes store
+  const bool past_l2 = run * es % 128 == 0 && (a.head_dim - a.rot_dim) * es % 128 == 0 &&
+                       tokens * heads * a.head_dim * es > (32ll << 20);
+  auto kern = rope_kernel<E, P, INTER, false>;
+  if constexpr (P * es == 16)
+    if (past_l2) kern = rope_kernel<E, P, INTER, true>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, a, pair_chunks, copy_chunks, lanes,
+                     tpb, bpt);
   return hipGetLastError();
 }
 
-// The widest pieces, up to 16 B, that divide the pairs, the copied dims and
-// every stride, and that the pointers are aligned to.
-template <Elt E>
+// The widest pieces, up to 16 B, that divide the rotated dims (in halves: a
+// half), the copied dims and every stride, and that the pointers are aligned to.
+template <Elt E, bool INTER>
 hipError_t rope_type(const RopeArgs& a, hipStream_t stream) {
   constexpr int es = EltInfo<E>::bytes;
-  uint64_t bits = (uint64_t)(a.rot_dim / 2) | (uint64_t)(a.head_dim - a.rot_dim);
+  uint64_t bits = (uint64_t)(INTER ? a.rot_dim : a.rot_dim / 2) | (uint64_t)(a.head_dim - a.rot_dim);
   for (int i = 0; i < (a.t[1].heads ? 2 : 1); ++i) {
     const RopeTensor& t = a.t[i];
     bits |= (uint64_t)t.sb | (uint64_t)t.sh | (uint64_t)t.ss | (uint64_t)t.osb | (uint64_t)t.osh |
             (uint64_t)t.oss | (uint64_t)t.x / es | (uint64_t)t.out / es;
   }
   if constexpr (es == 2)
-    if (bits % 8 == 0) return launch_rope<E, 8>(a, stream);
-  if (bits % 4 == 0) return launch_rope<E, 4>(a, stream);
-  if (bits % 2 == 0) return launch_rope<E, 2>(a, stream);
-  return launch_rope<E, 1>(a, stream);
+    if (bits % 8 == 0) return launch_rope<E, 8, INTER>(a, stream);
+  if (bits % 4 == 0) return launch_rope<E, 4, INTER>(a, stream);
+  if (bits % 2 == 0) return launch_rope<E, 2, INTER>(a, stream);
+  return launch_rope<E, 1, INTER>(a, stream);
 }
 
 }  // namespace
 
 hipError_t rope(const RopeArgs& a, hipStream_t s) {
   switch (a.dtype) {
-    case Elt::F32: return rope_type<Elt::F32>(a, s);
-    case Elt::F16: return rope_type<Elt::F16>(a, s);
-    case Elt::BF16: return rope_type<Elt::BF16>(a, s);
+    case Elt::F32: return a.interleaved ? rope_type<Elt::F32, true>(a, s) : rope_type<Elt::F32, false>(a, s);
+    case Elt::F16: return a.interleaved ? rope_type<Elt::F16, true>(a, s) : rope_type<Elt::F16, false>(a, s);
+    case Elt::BF16: return a.interleaved ? rope_type<Elt::BF16, true>(a, s) : rope_type<Elt::BF16, false>(a, s);
     default: return hipErrorInvalidValue;
   }
 }
