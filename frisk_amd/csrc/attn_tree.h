@@ -23,21 +23,14 @@ struct Part {
   unsigned long long* words;
 };
 
-// Blocks per split of a sequence with `keys` keys: the launch's splits, or
-// fewer where they would fall short.
 __device__ __forceinline__ int blocks_per_split(const Part& p, int blocks) {
-  return max(p.min_blocks, (blocks + p.splits - 1) / p.splits);
+  return blocks_per_split(p.splits, p.min_blocks, blocks);
 }
 
 // Whether new token t sees draft j.
 __device__ __forceinline__ bool sees(const TreeAttnArgs& a, int64_t b, int t, int j) {
   if (!a.mask) return j <= t;
   return (a.mask[b * a.mask_sb + t * a.mask_st + (j >> 6)] >> (j & 63)) & 1;
-}
-
-// Keys of sequence b that exist: up to the last new one, and the capacity.
-__device__ __forceinline__ int keys_of(const TreeAttnArgs& a, const kv::Span& sp) {
-  return (int)min(sp.ctx + sp.fresh, a.cache.capacity);
 }
 
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }

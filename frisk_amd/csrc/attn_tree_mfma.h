@@ -148,26 +148,25 @@ TREE_INLINE void read_k(const char* ks, int h0, int l32, int half, i32x4 (&kf)[2
   }
 }
 
-// Lane offsets of the transposing reads of V^T (attn.h and gemm_tile.h derive
+// Lane offset of the transposing reads of V^T (attn.h and gemm_tile.h derive
 // them): the fragment of key step kk and dim tile dt holds, in lane (l32,
 // half), V[16 kk + (e < 4 ? 4 half + e : 4 + 4 half + e)][32 dt + l32], e = 0 .. 7.
-template <Elt C, int D> TREE_INLINE void v_offsets(int lane, int (&off)[D / 32]) {
+// A dim tile further is another chunk of the row, an XOR above the swizzle.
+template <Elt C, int D> TREE_INLINE uint32_t v_offset(int lane) {
   using G = Geom<C, D>;
   const int g = lane >> 4, h = g >> 1, dg = g & 1;
-#pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt) {
-    if constexpr (is8(C)) {
-      const int e = (lane >> 1) & 7, b = lane & 1, r = e < 4 ? 4 * h + e : 4 + 4 * h + e;
-      off[dt] = r * G::kRB + (((2 * dt + dg) ^ G::swz_v(r)) << 4) + 8 * b;
-    } else {
-      const int e = (lane >> 2) & 3, q = lane & 3, r = 4 * h + e;
-      off[dt] = r * G::kRB + (((4 * dt + 2 * dg + (q >> 1)) ^ G::swz_v(r)) << 4) + 8 * (q & 1);
-    }
+  if constexpr (is8(C)) {
+    const int e = (lane >> 1) & 7, b = lane & 1, r = e < 4 ? 4 * h + e : 4 + 4 * h + e;
+    return r * G::kRB + ((dg ^ G::swz_v(r)) << 4) + 8 * b;
+  } else {
+    const int e = (lane >> 2) & 3, q = lane & 3, r = 4 * h + e;
+    return r * G::kRB + (((2 * dg + (q >> 1)) ^ G::swz_v(r)) << 4) + 8 * (q & 1);
   }
 }
-template <Elt T, Elt C, int D> TREE_INLINE i32x4 read_v(const char* vs, int off, int kk) {
+// `at`: v_offset and the offset of V's tile (a multiple of 1 KiB) in lds.
+template <Elt T, Elt C, int D> TREE_INLINE i32x4 read_v(const char* lds, uint32_t at, int kk, int dt) {
   using G = Geom<C, D>;
-  const char* p = vs + off + kk * 16 * G::kRB;
+  const char* p = lds + (at ^ (uint32_t)(dt << (is8(C) ? 5 : 6))) + kk * 16 * G::kRB;
   if constexpr (is8(C)) {
     const i32x2 w = lds_read_tr8(p);
     return widen8<T, C>(w[0], w[1]);
@@ -178,58 +177,11 @@ template <Elt T, Elt C, int D> TREE_INLINE i32x4 read_v(const char* vs, int off,
   }
 }
 
-// ---- where keys lie ------------------------------------------------------------
-
-// Byte offset of a key's row and element offset of its scale, for one head.
-struct Place {
-  int64_t row;
-  int64_t scale;
-  bool there;
-};
-// The table entry of key n (any value without a table), n < the capacity.
-TREE_INLINE int entry_of(const TreeAttnArgs& a, int64_t b, int n) {
-  const int32_t* p = a.cache.table ? a.cache.table + b * a.cache.table_stride + (n >> a.cache.page_shift)
-                                   : a.ctx_len + b;
-  return *p;
-}
-template <Elt C>
-TREE_INLINE Place place_of(const TreeAttnArgs& a, int64_t b, int kvh, int n, int keys, int entry) {
-  const KvCache& c = a.cache;
-  const int page = c.table ? entry : (int)b;
-  const int slot = c.table ? n & ((1 << c.page_shift) - 1) : n;
-  Place p;
-  p.there = n < keys && page >= 0 && page < c.pages;
-  const int64_t pg = p.there ? page : 0, sl = p.there ? slot : 0;
-  p.row = (pg * c.sp + sl * c.ss + kvh * c.sh) * bytes_of(C);
-  p.scale = pg * c.scp + sl * c.scs + kvh * c.sch;
-  return p;
-}
-
 // ---- masks -----------------------------------------------------------------------
 
-// Which keys of the block from key n0 a token sees, as bits (all of the context;
-// `there`: keys that exist).
-TREE_INLINE uint64_t seen_bits(const TreeAttnArgs& a, int64_t b, int t, int64_t ctx, int n0,
-                               uint64_t there) {
-  const int64_t j0 = n0 - ctx;  // draft number of the first key
-  if (j0 + kBlock <= 0) return there;
-  uint64_t bits;
-  if (!a.mask) {
-    const int64_t n = t - j0 + 1;  // the first n keys
-    bits = n >= 64 ? ~0ull : n <= 0 ? 0 : (1ull << n) - 1;
-  } else {
-    const uint64_t* w = a.mask + (b * a.mask_sb + t * a.mask_st);
-    const int words = (a.tokens + 63) >> 6;
-    if (j0 < 0) {
-      const int n = (int)-j0;  // context keys in front, 1 .. 63
-      bits = ((1ull << n) - 1) | (w[0] << n);
-    } else {
-      const int i = (int)(j0 >> 6), s = (int)(j0 & 63);
-      bits = i < words ? w[i] >> s : 0;
-      if (s && i + 1 < words) bits |= w[i + 1] << (64 - s);
-    }
-  }
-  return bits & there;
+// seen_bits of token t of sequence b.
+TREE_INLINE uint64_t seen_bits(const TreeAttnArgs& a, int64_t b, int t, int64_t ctx, int n0, uint64_t there) {
+  return seen_bits(a.mask ? a.mask + (b * a.mask_sb + t * a.mask_st) : nullptr, a.tokens, t, ctx, n0, there);
 }
 // A copy of the bits that the compiler takes for another value, so that the 32
 // conditions of one use are not kept in scalar registers for the next.
@@ -503,7 +455,7 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
   const kv::Span sp = kv::span_of(a.ctx_len, a.new_len, a.tokens, b);
   const int rows = sp.fresh * group;
   if (sp.ctx < 0 || tile * 32 >= rows) return;
-  int keys = keys_of(a, sp);
+  int keys = keys_of(a.cache.capacity, sp);
   const int blocks_all = (keys + kBlock - 1) / kBlock;
   const int per = blocks_per_split(part, blocks_all);
   if (split > 0 && split * per >= blocks_all) return;
@@ -529,19 +481,18 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
                                        16, 0, 0);
     }
   };
-  int vt[D / 32];
-  v_offsets<C, D>(lane, vt);
+  const uint32_t v_at = (uint32_t)(vs - smem) + v_offset<C, D>(lane);
   State<D> st;
   clear(st);
 
-  // The key this lane looks up for block kb.
-  auto my_key = [&](int kb) { return min(kb * kBlock + lane, (int)a.cache.capacity - 1); };
+  // The table entry of this lane's key of block kb.
+  auto my_entry = [&](int kb) { return entry_of(a.cache, a.ctx_len, b, kb * kBlock + lane); };
   int kb = split * per + wave;
   int entry = 0;
   uint64_t there = 0, there_next = 0;
   float ksc = 0.0f, vsc = 0.0f;
   auto place = [&](int block, int e) __attribute__((always_inline)) {
-    const Place p = place_of<C>(a, b, kvh, block * kBlock + lane, keys, e);
+    const Place p = place_of(a.cache, bytes_of(C), b, kvh, block * kBlock + lane, keys, e);
     offs[lane] = p.row;
     if constexpr (k8) {
       ksc = a.cache.k_scale[p.scale];
@@ -551,8 +502,8 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
   };
   // Table entries of the first two blocks; Q has landed with them, on every
   // path into the loop, so that nothing in it waits for a load by accident.
-  const int first = entry_of(a, b, my_key(max(0, min(kb, end - 1))));
-  entry = entry_of(a, b, my_key(max(0, min(kb + NW, end - 1))));
+  const int first = my_entry(max(0, min(kb, end - 1)));
+  entry = my_entry(max(0, min(kb + NW, end - 1)));
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) asm volatile("" ::"v"(qf[i]), "v"(first), "v"(entry));
   __builtin_amdgcn_s_waitcnt(0);
@@ -589,7 +540,7 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
     __builtin_amdgcn_s_waitcnt(0xC07F);
     if (more) {
       there_next = place(kb + NW, entry);
-      entry = entry_of(a, b, my_key(min(kb + 2 * NW, end - 1)));
+      entry = my_entry(min(kb + 2 * NW, end - 1));
       __builtin_amdgcn_sched_barrier(0);
       issue(kbase, ks, false);
     }
@@ -618,7 +569,7 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
-        st.o[dt] = mfma<T>(read_v<T, C, D>(vs, vt[dt], kk), pf[kk], st.o[dt]);
+        st.o[dt] = mfma<T>(read_v<T, C, D>(smem, v_at, kk, dt), pf[kk], st.o[dt]);
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(0xC07F);
     if (more) issue(vbase, vs, true);
@@ -760,7 +711,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
   const kv::Span sp = kv::span_of(a.ctx_len, a.new_len, a.tokens, b);
   const int rows = sp.fresh * group;
   if (sp.ctx < 0 || rb * 32 * NW >= rows) return;
-  const int keys = keys_of(a, sp);
+  const int keys = keys_of(a.cache.capacity, sp);
   const int blocks_all = (keys + kBlock - 1) / kBlock;
   const int per = blocks_per_split(part, blocks_all);
   if (split > 0 && split * per >= blocks_all) return;
@@ -782,11 +733,11 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
   const char* kbase = (const char*)a.cache.k;
   const char* vbase = (const char*)a.cache.v;
 
-  auto my_key = [&](int kb) { return max(0, min(kb * kBlock + lane, (int)a.cache.capacity - 1)); };
+  auto my_entry = [&](int kb) { return entry_of(a.cache, a.ctx_len, b, kb * kBlock + lane); };
   int64_t my_scale = 0;
   // Row offsets of a block, by wave 0 for all; every wave keeps which keys exist.
   auto place = [&](int kb, int entry) __attribute__((always_inline)) {
-    const Place p = place_of<C>(a, b, kvh, kb * kBlock + lane, keys, entry);
+    const Place p = place_of(a.cache, bytes_of(C), b, kvh, kb * kBlock + lane, keys, entry);
     if (wave == 0) offs[(kb & 1) * 64 + lane] = p.row;
     my_scale = p.scale;
     return __builtin_amdgcn_ballot_w64(p.there);
@@ -827,9 +778,13 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
   };
   auto widen = [&](int kb) __attribute__((always_inline)) {
     char* dst = smem + (kb & 1) * kBuf;
+    // Its LDS addresses are formed here, a block at a time: kept over the loop
+    // they would take registers that it does not have.
+    int first = tid;
+    asm volatile("" : "+v"(first));
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      const int p = i * 64 * NW + tid;
+      const int p = i * 64 * NW + first;
       if (kPieces % (64 * NW) && p >= kPieces) continue;
       const int r = p / kC8, c = 2 * (p % kC8);
 #pragma unroll
@@ -843,14 +798,13 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
     if (wave < 2) scales[(kb & 1) * 128 + wave * 64 + lane] = wave == 0 ? my_value * scale_log2 : my_value;
   };
 
-  int vt[D / 32];
-  v_offsets<T, D>(lane, vt);
+  const uint32_t v_lane = v_offset<T, D>(lane);
   State<D> st;
   clear(st);
   // Table entries of the first blocks; Q has landed with them, on every path
   // into the loop, so that nothing in it waits for a load by accident.
-  const int entry0 = entry_of(a, b, my_key(begin)), entry1 = entry_of(a, b, my_key(begin + 1));
-  int entry = entry_of(a, b, my_key(begin + 2));
+  const int entry0 = my_entry(begin), entry1 = my_entry(begin + 1);
+  int entry = my_entry(begin + 2);
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) asm volatile("" ::"v"(qf[i]), "v"(entry0), "v"(entry1), "v"(entry));
   __builtin_amdgcn_s_waitcnt(0);
@@ -876,6 +830,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
     const bool more = kb + 1 < end;
     const char* ks = smem + (kb & 1) * kBuf;
     char* vs = smem + (kb & 1) * kBuf + G::kTile;
+    const uint32_t v_at = (uint32_t)((kb & 1) * kBuf + G::kTile) + v_lane;
     const bool masked = there != ~0ull || (int64_t)(kb + 1) * kBlock > sp.ctx;
     // The same in every wave: all of them look at the same tile.
     uint64_t bad = 0;
@@ -915,7 +870,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(vs, vt[dt], kk);
+          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(smem, v_at, kk, dt);
 #pragma unroll
         for (int i = 0; i < H1; ++i)
 #pragma unroll
@@ -923,7 +878,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
 #pragma unroll
         for (int kk = 2; kk < kEarly; ++kk)
 #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(vs, vt[dt], kk);
+          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(smem, v_at, kk, dt);
       }
       __builtin_amdgcn_sched_barrier(0);
       i32x4 pf[4];
@@ -940,13 +895,13 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
 #pragma unroll
         for (int kk = 0; kk < kEarly; ++kk)
 #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(vs, vt[dt], kk);
+          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(smem, v_at, kk, dt);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kk = kEarly; kk < 4; ++kk)
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(vs, vt[dt], kk);
+        for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(smem, v_at, kk, dt);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
@@ -957,7 +912,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
     // Offsets of the block after the next, whose place in LDS this block's had.
     there = there1;
     there1 = place(kb + 2, entry);
-    entry = entry_of(a, b, my_key(kb + 3));
+    entry = my_entry(kb + 3);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
   }

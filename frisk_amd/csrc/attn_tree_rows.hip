@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeAttnArgs a, tree::Pa
   const int h = (int)(bh - b * a.heads), kvh = h / (a.heads / a.cache.kv_heads);
   const kv::Span sp = kv::span_of(a.ctx_len, a.new_len, a.tokens, b);
   if (sp.ctx < 0 || t >= sp.fresh) return;
-  const int keys = tree::keys_of(a, sp), blocks = (keys + tree::kBlock - 1) / tree::kBlock;
+  const int keys = tree::keys_of(a.cache.capacity, sp), blocks = (keys + tree::kBlock - 1) / tree::kBlock;
   const int per = tree::blocks_per_split(part, blocks), split = blockIdx.y;
   if (split > 0 && split * per >= blocks) return;
   const int end = min(keys, (split + 1) * per * tree::kBlock);
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256) void tree_sum_kernel(TreeAttnArgs a, tree::Par
   const int h = (int)(bh - b * a.heads);
   const kv::Span sp = kv::span_of(a.ctx_len, a.new_len, a.tokens, b);
   if (sp.ctx < 0 || t >= sp.fresh) return;
-  const int blocks = (tree::keys_of(a, sp) + tree::kBlock - 1) / tree::kBlock;
+  const int blocks = (tree::keys_of(a.cache.capacity, sp) + tree::kBlock - 1) / tree::kBlock;
   const int per = tree::blocks_per_split(part, blocks);
   if (per >= blocks) return;  // written by its workgroup
   const int n = (blocks + per - 1) / per;

@@ -78,15 +78,16 @@ class Setup:
         rt.tree_attn(self.q, self.cache, self.ctx_len, o, mask=mask, new_len=self.new_len, lse=l, **kw)
         return o, l
 
-    def check(self, o, lse, seen=None, scale=None, rows=None):
-        """`seen` bool [batch, tokens, tokens], or None: causal."""
+    def check(self, o, lse, seen=None, scale=None, rows=None, heads=None, seqs=None):
+        """`seen` bool [batch, tokens, tokens], or None: causal.  rows, heads,
+        seqs: the ones looked at (None: all)."""
         h = torch.finfo(DT[self.dt]).eps / 2
         out_h = h if o.dtype == DT[self.dt] else 0.0
         scale = self.d ** -0.5 if scale is None else scale
         group = self.heads // self.kv
         qd, od = self.q.double().cpu().numpy(), o.double().cpu().numpy()
         ld = None if lse is None else lse.double().cpu().numpy()
-        for i in range(self.batch):
+        for i in seqs or range(self.batch):
             live = self.new[i] if self.ctx[i] >= 0 else 0
             assert (od[i, :, live:] == 5.0).all() and (ld is None or (ld[i, :, live:] == 5.0).all())
             if not live:
@@ -94,7 +95,7 @@ class Setup:
             k, v = self.rows(i)
             vis = np.ones((live, self.ctx[i] + live), bool)
             vis[:, self.ctx[i]:] = np.tril(np.ones((live, live), bool)) if seen is None else seen[i][:live, :live]
-            for head in range(self.heads):
+            for head in heads or range(self.heads):
                 pick = range(live) if rows is None else sorted({0, live - 1, *(r % live for r in rows)})
                 pick = list(pick)
                 wo, wl, wa = C.attention(qd[i, head, pick], k[head // group], v[head // group], vis[pick], scale)
@@ -147,6 +148,115 @@ def test_trees(batch, heads, kv, tokens, d, page, ctx, dt, kind):
 def test_chunks(batch, heads, kv, tokens, d, page, ctx, dt, kind):
     s = Setup(batch, heads, kv, tokens, d, dt, kind, page, ctx, seed=tokens)
     s.check(*s.run(), rows=(1, 31, 32, 63, 64, 127, 128, 200))
+
+
+EDGES = (1, 30, 31, 32, 33, 127, 128, 255, 256, 300, 383, 500)
+
+
+@pytest.mark.parametrize("dt,kind", KINDS)
+@pytest.mark.parametrize("batch,d", [(4, 128), (8, 128), (4, 64), (4, 32)])
+@pytest.mark.parametrize("masked", [False, True], ids=["causal", "tree"])
+def test_many_rows(batch, d, masked, dt, kind):
+    # Sizes at which the rule takes 4 and 8 tiles of rows over shared keys.
+    ctx = [(300 if d > 32 else 100, 0, 37, 69)[i % 4] for i in range(batch)]
+    new = [(512, 500, 257, 1)[i % 4] for i in range(batch)]
+    s = Setup(batch, 16, 4, 512, d, dt, kind, 16, ctx, new=new, seed=batch + d)
+    mask, seen = tree(batch, 512, 7) if masked else (None, None)
+    o, lse = s.run(mask)
+    s.check(o, lse, seen, rows=EDGES, heads=(0, 6, 15), seqs=(0, 1, 2, 3))
+    assert torch.equal(o, s.run(mask)[0])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("batch,ctx", [(8, 4096), (2, 8192)])
+def test_many_rows_and_splits(batch, ctx, kind):
+    lens = [ctx - 700 * i for i in range(batch)]
+    s = Setup(batch, 32, 8, 64, 128, "bf16", kind, 64, [max(0, c) for c in lens], seed=batch)
+    mask, seen = tree(batch, 64, 2)
+    s.check(*s.run(mask), seen, rows=(1, 7, 40), heads=(0, 31), seqs=(0, 1, batch - 1))
+
+
+@pytest.mark.parametrize("dt,kind", KINDS)
+@pytest.mark.parametrize("batch,d", [(4, 64), (4, 128), (8, 128)])
+def test_many_rows_hidden_values(batch, d, dt, kind):
+    # Not finite in drafts nobody sees, in one that some see, and behind the end.
+    t = 512
+    s = Setup(batch, 16, 4, t, d, dt, kind, 16, [300] * batch, new=[t - 5] * batch, spare=20, seed=3)
+    rng = np.random.default_rng(2)
+    one = rng.random((t, t)) < 0.3
+    one[:, 200:203] = False
+    one[:, 290] = np.arange(t) % 64 == 63
+    one[0, 0] = True
+    seen = np.stack([one] * batch)
+    mask = torch.from_numpy(C.words_of(one).view(np.int64)).cuda()
+    bad = [500, 501, 502] + list(range(300 + t - 5, 300 + t + 20))
+    for i in range(batch):
+        for n, at in enumerate(bad):
+            p, r = int(s.table[i, at // 16]), at % 16
+            v = (float("nan"), float("inf"), -float("inf"))[n % 3]
+            if kind in C.TOP:
+                s.cache.k_scale[p, :, r] = v
+                s.cache.v_scale[p, :, r] = v
+            else:
+                s.cache.k[p, :, r] = v
+                s.cache.v[p, :, r] = v
+    o, lse = s.run(mask)
+    s.check(o, lse, seen, rows=EDGES, heads=(0, 15), seqs=(0, batch - 1))
+    p, r = int(s.table[0, 590 // 16]), 590 % 16
+    if kind in C.TOP:
+        s.cache.v_scale[p, :, r] = float("nan")
+    else:
+        s.cache.v[p, :, r] = float("nan")
+    o2, _ = s.run(mask)
+    sees = torch.from_numpy(one[:t - 5, 290]).cuda()
+    assert torch.isnan(o2[0][:, :t - 5][:, sees]).all()
+    assert torch.equal(o2[0][:, :t - 5][:, ~sees], o[0][:, :t - 5][:, ~sees])
+    assert torch.equal(o2[1:], o[1:])
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "i8"])
+@pytest.mark.parametrize("tokens", [1, 20])
+def test_value_scales_of_every_size(tokens, kind):
+    # Value scales from 2^-60 to 2^15 in any order: f16 weights times a scale
+    # stay in range.
+    s = Setup(1, 8, 2, tokens, 128, "f16", kind, 16, (700,), seed=8)
+    p = torch.randint(-60, 16, s.cache.v_scale.shape, generator=torch.Generator().manual_seed(4))
+    s.cache.v_scale.copy_(torch.ldexp(torch.ones(()), p))
+    s.cache.v_scale[int(s.table[0, 2]), :, 3] = 2.0 ** 15
+    o, lse = s.run(out=torch.float32)
+    s.check(o, lse)
+
+
+def test_two_streams():
+    # Calls at once on two streams, each with scratch of its own.
+    a = Setup(1, 8, 2, 1, 128, "bf16", "bf16", 64, (20000,), seed=1)
+    b = Setup(2, 8, 2, 3, 128, "bf16", "e4m3", 64, (15000, 300), seed=2)
+    want = [s.run()[0] for s in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(4):
+        for s, st in zip((a, b), streams):
+            with torch.cuda.stream(st):
+                got.append(s.run()[0])
+    o = torch.empty_like(a.q)
+    rt.tree_attn(a.q, a.cache, a.ctx_len, o, stream=streams[0])
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert torch.equal(x, want[i % 2])
+    assert torch.equal(o, want[0])
+
+
+def test_a_workspace_of_any_contents():
+    s = Setup(1, 8, 2, 2, 128, "bf16", "bf16", 64, (9000,), seed=1)
+    want, _ = s.run()
+    need = rt.tree_attn_workspace_bytes(rt.tree_attn_desc(s.q, s.cache, s.ctx_len, torch.empty_like(s.q)))
+    assert need > 0
+    for byte in (0x00, 0xFF, 0x7F, 0x3C):
+        ws = torch.full((need + 64,), byte, dtype=torch.uint8, device="cuda")
+        for _ in range(3):
+            assert torch.equal(s.run(workspace=ws)[0], want)
+        assert (ws[need:] == byte).all()
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
