@@ -63,8 +63,9 @@ FRISK_INDEX int blocks_per_split(int splits, int min_blocks, int blocks) {
 // The table entry that names key n's page (any value without a table); n is
 // held inside the capacity.
 template <typename Cache>
-FRISK_INDEX int entry_of(const Cache& c, const int32_t* ctx_len, int64_t b, int64_t n) {
-  n = n < 0 ? 0 : n < c.capacity ? n : c.capacity - 1;
+FRISK_INDEX int entry_of(const Cache& c, const int32_t* ctx_len, int64_t b, int n) {
+  const int last = (int)c.capacity - 1;  // (the capacity fits)
+  n = n < 0 ? 0 : n < last ? n : last;
   return c.table ? c.table[b * c.table_stride + (n >> c.page_shift)] : ctx_len[b];
 }
 
@@ -77,7 +78,7 @@ struct Place {
 };
 template <typename Cache>
 FRISK_INDEX Place place_of(const Cache& c, int bytes, int64_t b, int kvh, int n, int keys, int entry) {
-  const int64_t page = c.table ? entry : b;
+  const int page = c.table ? entry : (int)b;
   const int slot = c.table ? n & ((1 << c.page_shift) - 1) : n;
   Place p;
   p.there = n < keys && page >= 0 && page < c.pages;

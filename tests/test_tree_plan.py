@@ -91,7 +91,7 @@ int main(int, char** v) {
   for (int64_t b = 0; b < 2; ++b)
     for (int64_t n : {-1ll, 0ll, 7ll, 8ll, 15ll, 16ll, 19ll, 20ll, 23ll, 24ll, 31ll, 32ll, 1ll << 40}) {
       const auto s = frisk::kv::slot_of(c, b, n);
-      const int entry = frisk::tree::entry_of(c, ctx.data(), b, n);
+      const int entry = frisk::tree::entry_of(c, ctx.data(), b, (int)(n > 1000 ? 1000 : n));
       const auto p = frisk::tree::place_of(c, 2, b, 1, (int)(n < 0 ? 0 : n > 1000 ? 1000 : n), (int)c.capacity, entry);
       printf("%lld %lld %lld %lld %d %lld %lld\\n", (long long)b, (long long)n, (long long)s.elem, (long long)s.scale,
              (int)p.there, (long long)p.row, (long long)p.scale);
