@@ -12,9 +12,9 @@
 // 8-bit rows: codes widen to q's type exactly (4 or 8 significant bits), the
 // key's scale multiplies its score column and the value's scale its column of
 // P, in f32; nothing is rounded that a 16-bit cache would not round.  In f16
-// P times a scale could leave the type's range, so those columns are in units
-// of u, a power of two near the largest scale a row has seen, which moves like
-// the maximum does.
+// P times a scale could leave the type's range, so there the maximum that P is
+// taken from is that of score + log2(scale): P times scale stays below 2^8, and
+// P and its sum (f32) below 2^68, since scales below 2^-60 count as that.
 //
 // Where a key lies is computed once per key and block (a page number from the
 // table, loaded a block ahead), into LDS, as a 64-bit offset; the row loads go
@@ -39,7 +39,7 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef __attribute__((address_space(1))) const void* global_ptr;
 
 constexpr float kSlack = 8.0f;      // log2 headroom before the running maximum moves
-constexpr float kUnitSlack = 16.0f;  // headroom before the unit of P moves
+constexpr float kLeastLog = -60.0f;  // of a value scale, where P is taken from score + log2(scale)
 
 template <Elt T> TREE_INLINE f32x16 mfma(i32x4 a, i32x4 b, f32x16 c) {
   if constexpr (T == Elt::BF16)
@@ -163,7 +163,7 @@ template <Elt C, int D> TREE_INLINE uint32_t v_offset(int lane) {
     return r * G::kRB + (((2 * dg + (q >> 1)) ^ G::swz_v(r)) << 4) + 8 * (q & 1);
   }
 }
-// `at`: v_offset and the offset of V's tile (a multiple of 1 KiB) in lds.
+// `at`: v_offset and the offset of V's tile (a multiple of 256 B) in lds.
 template <Elt T, Elt C, int D> TREE_INLINE i32x4 read_v(const char* lds, uint32_t at, int kk, int dt) {
   using G = Geom<C, D>;
   const char* p = lds + (at ^ (uint32_t)(dt << (is8(C) ? 5 : 6))) + kk * 16 * G::kRB;
@@ -195,26 +195,32 @@ constexpr int key_of(int kt, int r) { return kt * 32 + 8 * (r >> 2) + (r & 3); }
 
 // ---- softmax of one block -----------------------------------------------------------
 
-// A row's running state; u: unit of P and O over codes in f16, else 1.
+// A row's running state.
 template <int D> struct State {
   f32x16 o[D / 32];
-  float m, l, u;
+  float m, l;
 };
 template <int D> TREE_INLINE void clear(State<D>& st) {
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = f32x16{};
   st.m = -__builtin_inff();
   st.l = 0.0f;
-  st.u = 0x1p-126f;
+}
+
+// The logarithm that a value scale counts with (0 for one that is not finite: its
+// row is NaN where it is seen).
+TREE_INLINE float scale_log(float v) {
+  return v < __builtin_inff() ? fmaxf(__log2f(v), kLeastLog) : 0.0f;
 }
 
 // Scores s to P (in place, f32, and packed in pf).  seen: bits of the row's
 // keys shifted down by 4 half, read if masked (uniform).  sc: the block's 64 key
-// scales times scale_log2, then 64 value scales, over codes.
+// scales times scale_log2, then 64 value scales, over codes; in f16 then their
+// logarithms (scale_log).
 template <Elt T, Elt C, int D>
 TREE_INLINE void softmax(f32x16 (&s)[2], i32x4 (&pf)[4], State<D>& st, float scale_log2,
                          const float* sc, int half, bool masked, uint64_t seen) {
-  constexpr bool k8 = is8(C), unit = k8 && T == Elt::F16;
+  constexpr bool k8 = is8(C), shift = k8 && T == Elt::F16;
   if constexpr (k8) {
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -236,7 +242,12 @@ TREE_INLINE void softmax(f32x16 (&s)[2], i32x4 (&pf)[4], State<D>& st, float sca
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kt][r]);
+    for (int g = 0; g < 4; ++g) {
+      f32x4 by = {0, 0, 0, 0};
+      if constexpr (shift) by = *(const f32x4*)(sc + 128 + kt * 32 + 8 * g + 4 * half);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, shift ? s[kt][4 * g + i] + by[i] : s[kt][4 * g + i]);
+    }
   top = pair_max(top);
   if constexpr (!k8) top *= scale_log2;
   const bool move = top > st.m + kSlack;
@@ -263,40 +274,13 @@ TREE_INLINE void softmax(f32x16 (&s)[2], i32x4 (&pf)[4], State<D>& st, float sca
     for (int r = 0; r < 16; ++r) l += s[kt][r];
   st.l = l;
   if constexpr (k8) {
-    float inv = 1.0f;
-    if constexpr (unit) {
-      float big = 0.0f;
-      const uint64_t bits = again(masked ? seen : ~0ull);
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 f = *(const f32x4*)(sc + 64 + kt * 32 + 8 * g + 4 * half);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            // (A hidden key's scale may be anything.)
-            const bool counts = f[i] < __builtin_inff() && ((bits >> key_of(kt, 4 * g + i)) & 1);
-            big = fmaxf(big, counts ? f[i] : 0.0f);
-          }
-        }
-      big = pair_max(big);
-      const bool grow = big > st.u * kUnitSlack;
-      if (__builtin_amdgcn_ballot_w64(grow)) {
-        const float next = grow ? __builtin_ldexpf(1.0f, __builtin_amdgcn_frexp_expf(big)) : st.u;
-        const float by = st.u / next;
-        st.u = next;
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= by;
-      }
-      inv = 1.0f / st.u;
-    }
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 f = *(const f32x4*)(sc + 64 + kt * 32 + 8 * g + 4 * half);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[kt][4 * g + i] *= unit ? f[i] * inv : f[i];
+        for (int i = 0; i < 4; ++i) s[kt][4 * g + i] *= f[i];
       }
     if (masked) {  // a hidden key's scale may be NaN
       const uint64_t bits = again(seen);
@@ -389,7 +373,7 @@ TREE_INLINE void place_unit(int pid, int units, int tiles, int& unit, int& tile)
 
 // Waves per workgroup: K and V tiles of all waves in LDS.
 template <Elt C, int D> constexpr int kKeyWaves = plan::tree_key_waves(D);
-constexpr int kExtra = 1024;  // per wave: 64 row offsets (8 B), 2 x 64 scales
+constexpr int kExtra = 1280;  // per wave: 64 row offsets (8 B), 64 scales of K and of V, 64 logarithms
 template <Elt C, int D> constexpr int keys_lds() {
   const int tiles = kKeyWaves<C, D> * (2 * Geom<C, D>::kTile + kExtra);
   const int sum = kKeyWaves<C, D> * 32 * (D + 4 + 2) * 4;
@@ -524,6 +508,7 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
     if constexpr (k8) {
       sc[lane] = ksc * scale_log2;
       sc[64 + lane] = vsc;
+      if constexpr (T == Elt::F16) sc[128 + lane] = scale_log(vsc);
     }
     f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
@@ -577,7 +562,6 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
     __builtin_amdgcn_sched_barrier(0);
   }
   const float l = pair_sum(st.l);
-  const float u = k8 && T == Elt::F16 ? st.u : 1.0f;
 
   // Combine the waves: O_w as padded rows, then m and l.
   __syncthreads();
@@ -591,7 +575,7 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *(f32x4*)(w + dt * 32 + 8 * g + 4 * half) =
-            f32x4{st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]} * u;
+            f32x4{st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]};
     if (half == 0) {
       pm[(wave * 32 + l32) * 2] = st.m;
       pm[(wave * 32 + l32) * 2 + 1] = l;
@@ -699,7 +683,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
   constexpr int kBuf = 2 * G::kTile;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   int64_t* offs = (int64_t*)(smem + 2 * kBuf);  // [2][64]
-  float* scales = (float*)(offs + 128);         // [2][128]
+  float* scales = (float*)(offs + 128);         // [2][192]
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int unit, rb;
@@ -795,7 +779,9 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
             widen8<T, C>(vw[i][2 * e], vw[i][2 * e + 1]);
       }
     }
-    if (wave < 2) scales[(kb & 1) * 128 + wave * 64 + lane] = wave == 0 ? my_value * scale_log2 : my_value;
+    float* sc = scales + (kb & 1) * 192 + lane;
+    if (wave < 2) sc[wave * 64] = wave == 0 ? my_value * scale_log2 : my_value;
+    if (T == Elt::F16 && wave == 1) sc[128] = scale_log(my_value);
   };
 
   const uint32_t v_lane = v_offset<T, D>(lane);
@@ -884,7 +870,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
       i32x4 pf[4];
       uint64_t seen = 0;
       if (masked) seen = seen_bits(a, b, t, sp.ctx, kb * kBlock, there) >> (4 * half);
-      softmax<T, C, D>(s, pf, st, scale_log2, scales + (kb & 1) * 128, half, masked, seen);
+      softmax<T, C, D>(s, pf, st, scale_log2, scales + (kb & 1) * 192, half, masked, seen);
       if (bad) {
         for (uint64_t left = bad; left; left &= left - 1)
           add_key<T, T, D>(vs, __builtin_ctzll(left), s, seen, l32, half, st);
@@ -919,7 +905,6 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
 
   // Each lane holds half of its row's dims.
   const float l = pair_sum(st.l);
-  const float u = k8 && T == Elt::F16 ? st.u : 1.0f;
   if (row0 + l32 >= rows) return;
   const int64_t id = (b * a.heads + h) * a.tokens + t;
   if (per < blocks_all) {
@@ -929,11 +914,11 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *(f32x4*)(part.o + at * D + dt * 32 + 8 * g + 4 * half) =
-            f32x4{st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]} * u;
+            f32x4{st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]};
     if (half == 0) part.ml[2 * at] = st.m, part.ml[2 * at + 1] = l;
     return;
   }
-  const float f = inverse_sum(l) * u;
+  const float f = inverse_sum(l);
   const int64_t o_row = b * a.o_sb + h * a.o_sh + t * a.o_ss;
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
@@ -948,7 +933,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
 template <Elt T, Elt C, int D, int NW>
 static hipError_t launch_tile(const TreeAttnArgs& a, const Part& p, hipStream_t stream) {
   auto kern = tree_tile_kernel<T, C, D, NW>;
-  constexpr int lds = 4 * Geom<T, D>::kTile + 2048;
+  constexpr int lds = 4 * Geom<T, D>::kTile + 1024 + 1536;
   static const hipError_t attr =
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (attr != hipSuccess) return attr;
