@@ -210,7 +210,7 @@ template <int D> TREE_INLINE void clear(State<D>& st) {
 // The logarithm that a value scale counts with (0 for one that is not finite: its
 // row is NaN where it is seen).
 TREE_INLINE float scale_log(float v) {
-  return v < __builtin_inff() ? fmaxf(__log2f(v), kLeastLog) : 0.0f;
+  return fabsf(v) < __builtin_inff() ? fmaxf(__log2f(fabsf(v)), kLeastLog) : 0.0f;
 }
 
 // Scores s to P (in place, f32, and packed in pf).  seen: bits of the row's

@@ -908,6 +908,11 @@ int check_kv(const frisk_kv_desc* d, const char* fn, bool write, frisk::KvArgs& 
       if (!write && n[i] > 1 && st[j][i] < d->cache.head_dim)
         return fail(FRISK_EINVAL, "%s: the rows of k or v overlap", fn);
     }
+  if (write && d->cache.k == d->cache.v)
+    return fail(FRISK_EINVAL, "%s: the cache's k and v must be two tensors", fn);
+  if (!write && rows_share(Rows{d->k, {n[0], n[1], n[2]}, {st[0][0], st[0][1], st[0][2]}},
+                           Rows{d->v, {n[0], n[1], n[2]}, {st[1][0], st[1][1], st[1][2]}}, d->cache.head_dim, 2))
+    return fail(FRISK_EINVAL, "%s: k and v overlap", fn);
   if (d->tokens > (((int64_t)1 << 46) / d->batch) / d->cache.kv_heads)
     return fail(FRISK_EUNSUP, "%s: sizes beyond the kernels' index range", fn);
   a.dtype = (frisk::Elt)d->dtype;

@@ -593,6 +593,15 @@ _rope_pack = _packer(RopeDesc)
 _kv_pack = _packer(KvDesc, "cache")
 _tree_pack = _packer(TreeAttnDesc, "cache")
 _ws_pack = struct.Struct("@Pq")
+
+
+def _pack(packer, *values) -> bytes:
+    try:
+        return packer.pack(*values)
+    except (OverflowError, struct.error) as e:
+        raise ValueError(f"argument out of range: {e}") from None
+
+
 _raw: dict = {}
 
 
@@ -677,7 +686,7 @@ def rope(x, out, positions, table, *, k=None, k_out=None, start=None, interleave
         st = positions.stride()
         at = (positions.data_ptr(), bits, *((0, st[0]) if len(st) == 1 else st))
     dev = _same_device(x, out, k, k_out, positions, table, start)
-    desc = _rope_pack.pack(b, s, h, kh, d, 2 * table.shape[0], torch_dtype_code(x.dtype),
+    desc = _pack(_rope_pack, b, s, h, kh, d, 2 * table.shape[0], torch_dtype_code(x.dtype),
                            bool(interleaved), bool(backward), amplitude,
                            x.data_ptr(), xs[0], xs[1], xs[2], out.data_ptr(), outs[0], outs[1], outs[2],
                            *second, *at, _lengths(start, b, "start"), table.data_ptr())
@@ -754,7 +763,7 @@ def _kv(name, k, v, cache, ctx_len, new_len, stream):
         raise ValueError(f"k and v must be [batch, {csh[1]}, tokens, {csh[3]}] of one dtype "
                          f"(got {tuple(k.shape)} and {tuple(v.shape)})")
     dev = cache._check(b, k, v, ctx_len, new_len)
-    desc = _kv_pack.pack(b, t, torch_dtype_code(k.dtype), k.data_ptr(), ks[0], ks[1], ks[2],
+    desc = _pack(_kv_pack, b, t, torch_dtype_code(k.dtype), k.data_ptr(), ks[0], ks[1], ks[2],
                          v.data_ptr(), vs[0], vs[1], vs[2], _lengths(ctx_len, b, "ctx_len"),
                          _lengths(new_len, b, "new_len")) + cache._packed
     _run(name, desc, dev, stream)
@@ -864,7 +873,7 @@ def tree_attn(q, cache, ctx_len, o, *, mask=None, new_len=None, sm_scale=None, l
         with torch.cuda.device(dev):
             return tree_attn(q, cache, ctx_len, o, mask=mask, new_len=new_len, sm_scale=sm_scale,
                              lse=lse, max_ctx=max_ctx, workspace=workspace, stream=stream)
-    head = _tree_pack.pack(*values) + cache._packed
+    head = _pack(_tree_pack, *values) + cache._packed
     ws, tail = None, bytes(16)
     if workspace is not False:
         need = _raw_fn("frisk_tree_attn_workspace_size")(head + tail)

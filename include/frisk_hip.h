@@ -433,8 +433,9 @@ typedef struct frisk_kv_cache {
 /*
  * frisk_kv_append writes rows [batch, kv_heads, tokens, head_dim] of k and v
  * (bf16 or f16) into the cache: token t < new_len[b] (all, if new_len is NULL)
- * of sequence b becomes key ctx_len[b] + t.  frisk_kv_read is its inverse:
- * those keys, as code * scale rounded to dtype, into k and v; rows from
+ * of sequence b becomes key ctx_len[b] + t; keys behind the capacity or on a
+ * page that is none are dropped.  frisk_kv_read is its inverse: those keys, as
+ * code * scale rounded to dtype, into k and v, which must not overlap; rows from
  * new_len[b] on, and of keys the cache does not hold, are left as they were.
  * A sequence with ctx_len[b] < 0 takes no part.
  * A row x of an 8-bit cache, with top Q = 448 (e4m3) or 127 (i8): a = max |x|
@@ -478,7 +479,7 @@ int frisk_tree_mask(int64_t batch, int64_t tokens, const int32_t* parents, uint6
  * given, [batch, heads, tokens] contiguous f32 natural-log sums.  A 16-bit
  * cache has q's dtype.  A token that sees no key has o = 0 and lse = -inf.
  * What a hidden key or its value holds does not matter, NaN and infinities
- * included.  Tokens from new_len[b] on, and sequences with ctx_len[b] < 0,
+ * included.  o may be q itself.  Tokens from new_len[b] on, and sequences with ctx_len[b] < 0,
  * are left as they were.  ctx_len and new_len are read on the device;
  * max_ctx (0: the cache's capacity) is a hint of the largest ctx_len that
  * only places the work.  head_dim is a multiple of 16 up to 256; 32, 64 and

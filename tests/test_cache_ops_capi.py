@@ -22,7 +22,7 @@ def cache_desc(**over):
 
 def kv_call(name, cache=None, **over):
     d = dict(batch=2, tokens=3, dtype=rt.BF16, k=16, k_stride_b=384, k_stride_h=192, k_stride_s=64,
-             v=16, v_stride_b=384, v_stride_h=192, v_stride_s=64, ctx_len=64, new_len=None)
+             v=1 << 16, v_stride_b=384, v_stride_h=192, v_stride_s=64, ctx_len=64, new_len=None)
     d.update(over)
     desc = rt.KvDesc(**d, cache=cache_desc(**(cache or {})))
     lib = rt.load()
@@ -70,6 +70,14 @@ def test_kv_refusals(name, over, code, msg):
 def test_read_refuses_rows_that_overlap():
     rc, err = kv_call("frisk_kv_read", k_stride_s=0)
     assert rc == rt.EINVAL and "overlap" in err
+    for at in (16, 16 + 128, 16 + 2 * 383):  # v among k's rows
+        rc, err = kv_call("frisk_kv_read", v=at & ~15)
+        assert rc == rt.EINVAL and "k and v overlap" in err
+
+
+def test_append_refuses_one_tensor_for_both():
+    rc, err = kv_call("frisk_kv_append", cache=dict(v=4096))
+    assert rc == rt.EINVAL and "must be two tensors" in err
 
 
 def tree_call(cache=None, fn="frisk_tree_attn", **over):
