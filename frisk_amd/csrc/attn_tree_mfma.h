@@ -9,13 +9,13 @@
 // from transposing LDS reads in the matching key order.  The row sum is kept
 // over the unrounded P, so that the log-sum-exp is exact to f32.
 //
-// 8-bit rows: codes widen to q's type exactly (4 or 8 significant bits), the
-// key's scale multiplies its score column and the value's scale its column of
-// P, in f32; nothing is rounded that a 16-bit cache would not round.  In f16
-// P times a scale could leave the type's range, so there the maximum that P is
-// taken from is that of score + log2(scale): P times scale stays below 2^8, and
-// P and its sum (f32) below 2^68, since scales below 2^-60 count as that.
-//
+// 8-bit rows: codes widen to q's type exactly (4 or 8 significant bits).  A key's
+// score is its column of S times the key's scale, and P is taken from score +
+// log2(value's scale) in one fused multiply-add, so that it is the weight times
+// the value's scale, below 2^8 whatever the scales are; the row sum adds P over
+// the value's scale, in another.  Nothing is rounded that a 16-bit cache would
+// not round.
+
 // Where a key lies is computed once per key and block (a page number from the
 // table, loaded a block ahead), into LDS, as a 64-bit offset; the row loads go
 // straight to LDS from 64-bit addresses, so neither pages nor long caches
@@ -39,7 +39,7 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef __attribute__((address_space(1))) const void* global_ptr;
 
 constexpr float kSlack = 8.0f;      // log2 headroom before the running maximum moves
-constexpr float kLeastLog = -60.0f;  // of a value scale, where P is taken from score + log2(scale)
+constexpr float kLeastLog = -96.0f;  // of a value scale: P over it, and the sum of that, stay in range
 
 template <Elt T> TREE_INLINE f32x16 mfma(i32x4 a, i32x4 b, f32x16 c) {
   if constexpr (T == Elt::BF16)
@@ -207,28 +207,36 @@ template <int D> TREE_INLINE void clear(State<D>& st) {
   st.l = 0.0f;
 }
 
-// The logarithm that a value scale counts with (0 for one that is not finite: its
-// row is NaN where it is seen).
-TREE_INLINE float scale_log(float v) {
-  return fabsf(v) < __builtin_inff() ? fmaxf(__log2f(fabsf(v)), kLeastLog) : 0.0f;
+// What a block's scales are kept as: the key's times scale_log2, the logarithm of
+// the value's and one over it.  A value scale that is not finite has the
+// logarithm NaN and one over it 0: NaN where it is seen, nothing where not.
+TREE_INLINE void put_scales(float* sc, int lane, float value, bool of_key, float scale_log2) {
+  if (of_key) {
+    sc[lane] = value * scale_log2;
+  } else {
+    const bool finite = value < __builtin_inff();  // (NaN is not)
+    const float log = fmaxf(__log2f(value), kLeastLog);
+    sc[64 + lane] = finite ? log : __builtin_nanf("");
+    sc[128 + lane] = finite ? __builtin_amdgcn_exp2f(-log) : 0.0f;
+  }
 }
 
 // Scores s to P (in place, f32, and packed in pf).  seen: bits of the row's
-// keys shifted down by 4 half, read if masked (uniform).  sc: the block's 64 key
-// scales times scale_log2, then 64 value scales, over codes; in f16 then their
-// logarithms (scale_log).
+// keys shifted down by 4 half, read if masked (uniform).  sc: the block's scales
+// (put_scales), over codes.
 template <Elt T, Elt C, int D>
 TREE_INLINE void softmax(f32x16 (&s)[2], i32x4 (&pf)[4], State<D>& st, float scale_log2,
                          const float* sc, int half, bool masked, uint64_t seen) {
-  constexpr bool k8 = is8(C), shift = k8 && T == Elt::F16;
+  constexpr bool k8 = is8(C);
   if constexpr (k8) {
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 f = *(const f32x4*)(sc + kt * 32 + 8 * g + 4 * half);
+        const f32x4 by = *(const f32x4*)(sc + kt * 32 + 8 * g + 4 * half);
+        const f32x4 log = *(const f32x4*)(sc + 64 + kt * 32 + 8 * g + 4 * half);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[kt][4 * g + i] *= f[i];
+        for (int i = 0; i < 4; ++i) s[kt][4 * g + i] = __builtin_fmaf(s[kt][4 * g + i], by[i], log[i]);
       }
   }
   if (masked) {
@@ -242,12 +250,7 @@ TREE_INLINE void softmax(f32x16 (&s)[2], i32x4 (&pf)[4], State<D>& st, float sca
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      f32x4 by = {0, 0, 0, 0};
-      if constexpr (shift) by = *(const f32x4*)(sc + 128 + kt * 32 + 8 * g + 4 * half);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, shift ? s[kt][4 * g + i] + by[i] : s[kt][4 * g + i]);
-    }
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kt][r]);
   top = pair_max(top);
   if constexpr (!k8) top *= scale_log2;
   const bool move = top > st.m + kSlack;
@@ -271,25 +274,14 @@ TREE_INLINE void softmax(f32x16 (&s)[2], i32x4 (&pf)[4], State<D>& st, float sca
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) l += s[kt][r];
-  st.l = l;
-  if constexpr (k8) {
+    for (int g = 0; g < 4; ++g) {
+      f32x4 over = {1.0f, 1.0f, 1.0f, 1.0f};
+      if constexpr (k8) over = *(const f32x4*)(sc + 128 + kt * 32 + 8 * g + 4 * half);
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 f = *(const f32x4*)(sc + 64 + kt * 32 + 8 * g + 4 * half);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[kt][4 * g + i] *= f[i];
-      }
-    if (masked) {  // a hidden key's scale may be NaN
-      const uint64_t bits = again(seen);
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[kt][r] = (bits >> key_of(kt, r)) & 1 ? s[kt][r] : 0.0f;
+      for (int i = 0; i < 4; ++i)
+        l = k8 ? __builtin_fmaf(s[kt][4 * g + i], over[i], l) : l + s[kt][4 * g + i];
     }
-  }
+  st.l = l;
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
@@ -506,9 +498,8 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
     __builtin_amdgcn_s_waitcnt((nv & 15) | ((nv >> 4) << 14) | (7 << 4) | (15 << 8));
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (k8) {
-      sc[lane] = ksc * scale_log2;
-      sc[64 + lane] = vsc;
-      if constexpr (T == Elt::F16) sc[128 + lane] = scale_log(vsc);
+      put_scales(sc, lane, ksc, true, scale_log2);
+      put_scales(sc, lane, vsc, false, scale_log2);
     }
     f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
@@ -779,9 +770,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
             widen8<T, C>(vw[i][2 * e], vw[i][2 * e + 1]);
       }
     }
-    float* sc = scales + (kb & 1) * 192 + lane;
-    if (wave < 2) sc[wave * 64] = wave == 0 ? my_value * scale_log2 : my_value;
-    if (T == Elt::F16 && wave == 1) sc[128] = scale_log(my_value);
+    if (wave < 2) put_scales(scales + (kb & 1) * 192, lane, my_value, wave == 0, scale_log2);
   };
 
   const uint32_t v_lane = v_offset<T, D>(lane);
