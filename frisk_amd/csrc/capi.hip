@@ -752,6 +752,34 @@ struct Rows {
   int64_t n[3], s[3];
 };
 
+typedef __int128 Wide;  // a size of 2^31 times a stride of 2^40
+
+// Whether the ranges of two tensors, from the first row's start to the last
+// one's end (row bytes, element bytes), share memory.
+bool spans_share(const Rows& a, int64_t row_a, int es_a, const Rows& b, int64_t row_b, int es_b) {
+  Wide ea = row_a, eb = row_b;
+  for (int i = 0; i < 3; ++i) {
+    ea += (Wide)(a.n[i] - 1) * a.s[i] * es_a;
+    eb += (Wide)(b.n[i] - 1) * b.s[i] * es_b;
+  }
+  const Wide pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+  return pa < pb + eb && pb < pa + ea;
+}
+
+// Whether rows of one tensor may share memory: they do not if each stride
+// holds all that the smaller ones reach (any permuted or sliced tensor).
+bool rows_overlap(const int64_t (&n)[3], const int64_t (&s)[3], int64_t row) {
+  int d[3] = {0, 1, 2};
+  std::sort(d, d + 3, [&](int i, int j) { return s[i] < s[j]; });
+  Wide below = row;
+  for (const int i : d) {
+    if (n[i] == 1) continue;
+    if (s[i] < below) return true;
+    below += (Wide)(n[i] - 1) * s[i];
+  }
+  return false;
+}
+
 // Whether i * strides of a and j * strides of b, `gap` apart, meet within a
 // row: the dims d[0 .. k) by falling stride, equal in both.
 bool rows_meet(int64_t gap, const Rows& a, const Rows& b, const int* d, int k, int64_t row) {
@@ -767,10 +795,8 @@ bool rows_meet(int64_t gap, const Rows& a, const Rows& b, const int* d, int k, i
 // each at least the extent of the dims below it (heads of one buffer); other
 // tensors must not reach into each other's range.
 bool rows_share(const Rows& a, const Rows& b, int64_t row, int es) {
-  int64_t ea = row, eb = row;
-  for (int i = 0; i < 3; ++i) ea += (a.n[i] - 1) * a.s[i], eb += (b.n[i] - 1) * b.s[i];
   const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
-  if (pa >= pb + (uintptr_t)(eb * es) || pb >= pa + (uintptr_t)(ea * es)) return false;
+  if (!spans_share(a, row * es, es, b, row * es, es)) return false;
   const int64_t bytes = (int64_t)(pb - pa);
   int d[3], k = 0;
   for (int i = 0; i < 3; ++i) {
@@ -779,15 +805,16 @@ bool rows_share(const Rows& a, const Rows& b, int64_t row, int es) {
     d[k++] = i;
   }
   std::sort(d, d + k, [&](int i, int j) { return a.s[i] > a.s[j]; });
-  int64_t below = row;
+  Wide below = row;
   for (int i = k - 1; i >= 0; --i) {
     if (a.s[d[i]] < below) return true;
-    below += (std::max(a.n[d[i]], b.n[d[i]]) - 1) * a.s[d[i]];
+    below += (Wide)(std::max(a.n[d[i]], b.n[d[i]]) - 1) * a.s[d[i]];
   }
   if (bytes % es) return true;
   return rows_meet(bytes / es, a, b, d, k, row);
 }
-// Sizes that keep every offset the kernels form inside 63 bits.
+
+// Sizes and strides that every product of an index the kernels form fits.
 constexpr int64_t kMaxDim = (int64_t)1 << 31, kMaxStride = (int64_t)1 << 40;
 
 int check_rope_tensor(const char* name, int64_t batch, int64_t heads, int64_t seq, int64_t head_dim,
@@ -800,10 +827,9 @@ int check_rope_tensor(const char* name, int64_t batch, int64_t heads, int64_t se
   for (int i = 0; i < 3; ++i) {
     if (xs[i] < 0 || os[i] < 0 || xs[i] > kMaxStride || os[i] > kMaxStride)
       return fail(FRISK_EINVAL, "frisk_rope: strides must be non-negative, up to 2^40 elements");
-    if (n[i] > 1 && os[i] < head_dim)
-      return fail(FRISK_EINVAL, "frisk_rope: the rows of %s's output overlap (stride %lld < head_dim %lld)",
-                  name, (long long)os[i], (long long)head_dim);
   }
+  if (rows_overlap(n, os, head_dim))
+    return fail(FRISK_EINVAL, "frisk_rope: the rows of %s's output overlap", name);
   bool same = x == out;
   for (int i = 0; i < 3; ++i) same = same && (n[i] == 1 || xs[i] == os[i]);
   const Rows in{x, {batch, heads, seq}, {xs[0], xs[1], xs[2]}};
@@ -867,6 +893,8 @@ int check_cache(const frisk_kv_cache& d, const char* fn, bool ptrs, int64_t batc
   }
   if (c.capacity > INT32_MAX - 8192)
     return fail(FRISK_EUNSUP, "%s: a sequence of more than 2^31 - 8193 keys", fn);
+  if (rows_overlap(n, st, d.head_dim) || (k8 && rows_overlap(n, sc, 1)))
+    return fail(FRISK_EINVAL, "%s: the cache's rows or scales overlap", fn);
   c.kind = (frisk::Elt)d.dtype;
   c.pages = (int)d.pages;
   c.kv_heads = (int)d.kv_heads;
@@ -905,11 +933,20 @@ int check_kv(const frisk_kv_desc* d, const char* fn, bool write, frisk::KvArgs& 
       if (st[j][i] < 0 || st[j][i] > kMaxStride || st[j][i] % 8)
         return fail(FRISK_EINVAL, "%s: strides must be non-negative multiples of 8 elements, up to "
                                   "2^40", fn);
-      if (!write && n[i] > 1 && st[j][i] < d->cache.head_dim)
-        return fail(FRISK_EINVAL, "%s: the rows of k or v overlap", fn);
     }
-  if (write && d->cache.k == d->cache.v)
+  if (!write && (rows_overlap(n, st[0], d->cache.head_dim) || rows_overlap(n, st[1], d->cache.head_dim)))
+    return fail(FRISK_EINVAL, "%s: the rows of k or v overlap", fn);
+  const frisk_kv_cache& c = d->cache;
+  auto held = [&](const void* p, int64_t sp, int64_t sh, int64_t ss) {
+    return Rows{p, {c.pages, c.kv_heads, c.page_size}, {sp, sh, ss}};
+  };
+  if (write && rows_share(held(c.k, c.stride_page, c.stride_head, c.stride_slot),
+                          held(c.v, c.stride_page, c.stride_head, c.stride_slot), c.head_dim, esize(c.dtype)))
     return fail(FRISK_EINVAL, "%s: the cache's k and v must be two tensors", fn);
+  if (write && c.k_scale &&
+      rows_share(held(c.k_scale, c.scale_stride_page, c.scale_stride_head, c.scale_stride_slot),
+                 held(c.v_scale, c.scale_stride_page, c.scale_stride_head, c.scale_stride_slot), 1, 4))
+    return fail(FRISK_EINVAL, "%s: k_scale and v_scale must be two tensors", fn);
   if (!write && rows_share(Rows{d->k, {n[0], n[1], n[2]}, {st[0][0], st[0][1], st[0][2]}},
                            Rows{d->v, {n[0], n[1], n[2]}, {st[1][0], st[1][1], st[1][2]}}, d->cache.head_dim, 2))
     return fail(FRISK_EINVAL, "%s: k and v overlap", fn);
@@ -974,8 +1011,17 @@ int check_tree(const frisk_tree_attn_desc* d, bool ptrs, bool split, frisk::Tree
   for (int i = 0; i < 3; ++i) {
     if (qs[i] < 0 || os[i] < 0 || qs[i] > kMaxStride || os[i] > kMaxStride || qs[i] % 8 || os[i] % 8)
       return fail(FRISK_EINVAL, "%s: strides must be non-negative multiples of 8 elements, up to 2^40", fn);
-    if (n[i] > 1 && os[i] < d->cache.head_dim)
-      return fail(FRISK_EINVAL, "%s: the rows of o overlap", fn);
+  }
+  if (rows_overlap(n, os, d->cache.head_dim)) return fail(FRISK_EINVAL, "%s: the rows of o overlap", fn);
+  if (ptrs) {
+    const Rows q{d->q, {n[0], n[1], n[2]}, {qs[0], qs[1], qs[2]}};
+    const Rows o{d->o, {n[0], n[1], n[2]}, {os[0], os[1], os[2]}};
+    bool same = d->q == d->o && d->dtype == d->o_dtype;
+    for (int i = 0; i < 3; ++i) same = same && (n[i] == 1 || qs[i] == os[i]);
+    const int64_t row = d->cache.head_dim;
+    if (!same && (d->dtype == d->o_dtype ? rows_share(q, o, row, 2)
+                                         : spans_share(q, row * 2, 2, o, row * 4, 4)))
+      return fail(FRISK_EINVAL, "%s: q and o overlap (in place: one pointer, dtype and strides)", fn);
   }
   if (d->mask && (d->mask_stride_b < 0 || d->mask_stride_t < 0 || d->mask_stride_b > kMaxStride ||
                   d->mask_stride_t > kMaxStride))
@@ -996,7 +1042,8 @@ int check_tree(const frisk_tree_attn_desc* d, bool ptrs, bool split, frisk::Tree
   a.ctx_len = d->ctx_len;
   a.new_len = d->new_len;
   a.mask = d->mask; a.mask_sb = d->mask_stride_b; a.mask_st = d->mask_stride_t;
-  const int64_t keys = d->max_ctx ? std::min(d->max_ctx + d->tokens, a.cache.capacity) : a.cache.capacity;
+  const int64_t cap = a.cache.capacity;
+  const int64_t keys = d->max_ctx ? std::min(std::min(d->max_ctx, cap) + d->tokens, cap) : cap;
   const frisk::plan::TreePlan p = frisk::plan::tree_plan(
       d->batch, d->heads, d->cache.kv_heads, d->tokens, d->cache.head_dim, esize(d->cache.dtype) == 1, keys,
       split, frisk::device_cus());
@@ -1164,6 +1211,8 @@ int frisk_tree_attn(const frisk_tree_attn_desc* d, void* stream) {
   }
   clear_stale_error();
   const hipError_t e = frisk::tree_attn(a, (hipStream_t)stream);
+  if (e == hipErrorInvalidConfiguration)
+    return fail(FRISK_EUNSUP, "frisk_tree_attn: more rows than one launch takes");
   if (e != hipSuccess) return hip_fail(e, "frisk_tree_attn launch");
   return FRISK_OK;
 }

@@ -748,6 +748,12 @@ class KvCache:
             ks, vs = (torch.empty(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
         return cls(k, v, ks, vs, block_table)
 
+    def __setattr__(self, name, value):
+        # The calls take the descriptor that __init__ packed.
+        if hasattr(self, "_packed"):
+            raise AttributeError("a KvCache's tensors are fixed: write into them, or make another one")
+        object.__setattr__(self, name, value)
+
     def _check(self, batch: int, *ts) -> int:
         """The device of the cache and `ts`, for a batch that fits the block table."""
         if self.block_table is not None and self.block_table.shape[0] != batch:
@@ -881,6 +887,8 @@ def tree_attn(q, cache, ctx_len, o, *, mask=None, new_len=None, sm_scale=None, l
             _check(need, "frisk_tree_attn_workspace_size")
         if need > 0:
             ws = workspace if workspace is not True else _scratch(need, o.device, stream)
+            if ws.get_device() != dev or not ws.is_contiguous():
+                raise ValueError("workspace must be a contiguous tensor on q's device")
             tail = _ws_pack.pack(ws.data_ptr(), ws.numel() * ws.element_size())
     _check(_raw_fn("frisk_tree_attn")(head + tail, _stream_handle(stream)), "frisk_tree_attn")
     return o

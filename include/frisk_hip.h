@@ -409,13 +409,15 @@ int frisk_rope_frequencies(int64_t rot_dim, double base, int32_t scaling, double
  * head_dim] with the strides below (elements, shared by k and v; head_dim
  * stride 1).  dtype bf16 or f16 holds them as they are; e4m3 or i8 holds
  * codes and an f32 scale for each row (page, head, slot) of k and of v: a
- * value is code * scale.
+ * value is code * scale.  Scales are above 0, or NaN (frisk_tree_attn takes a
+ * value's scale below 2^-96 as 2^-96).
  * Key n of sequence b is slot n % page_size of page block_table[b *
  * table_stride + n / page_size] (page_size a power of two), or without a
  * table slot n of page b; a sequence holds capacity = max_pages * page_size
  * (without a table page_size) keys.  A page number outside 0 .. pages - 1 is
  * no page: keys there are not written, not read and not seen.  Bases, and row
- * and stride bytes, are multiples of 16.
+ * and stride bytes, are multiples of 16.  Rows do not overlap: each stride
+ * holds what the smaller ones reach.
  */
 typedef struct frisk_kv_cache {
   int64_t pages, kv_heads, page_size, head_dim;
@@ -442,7 +444,8 @@ typedef struct frisk_kv_cache {
  * held at least 2^-126 Q, scale = a / Q, code = x Q / a rounded to nearest
  * even.  A row that holds an infinity or a NaN has scale NaN and codes 0: it
  * reads back as NaN.  A 16-bit cache takes and gives its own dtype.
- * Pages written by one call must be distinct between its sequences.
+ * Pages written by one call must be distinct between its sequences, and k, v
+ * and the cache four tensors (six with the scales) that share no memory.
  */
 typedef struct frisk_kv_desc {
   int64_t batch, tokens;
@@ -479,7 +482,8 @@ int frisk_tree_mask(int64_t batch, int64_t tokens, const int32_t* parents, uint6
  * given, [batch, heads, tokens] contiguous f32 natural-log sums.  A 16-bit
  * cache has q's dtype.  A token that sees no key has o = 0 and lse = -inf.
  * What a hidden key or its value holds does not matter, NaN and infinities
- * included.  o may be q itself.  Tokens from new_len[b] on, and sequences with ctx_len[b] < 0,
+ * included.  o may be q itself (its dtype and strides); other than that, o, lse and
+ * workspace share no memory with each other or with what is read.  Tokens from new_len[b] on, and sequences with ctx_len[b] < 0,
  * are left as they were.  ctx_len and new_len are read on the device;
  * max_ctx (0: the cache's capacity) is a hint of the largest ctx_len that
  * only places the work.  head_dim is a multiple of 16 up to 256; 32, 64 and

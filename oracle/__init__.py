@@ -13,6 +13,9 @@ Contents
                 reference's strict/fp64 D64 tile oracle with its ordered FP32
                 sum tree and f16 P boundary, its analytic fixtures, and the
                 64x16 fixed-ABI attention oracle with its 15 input cases.
+  cache_ops.py  fp64 rotary positions and their gradient, codes and scales of
+                8-bit cache rows, ancestors of drafted trees, attention over
+                a cache.
   oracle.c      the same fp64 GEMM / attention in C (OpenMP), built into
                 oracle/liboracle.so by oracle/Makefile; bench.py times it as
                 the CPU baseline.

@@ -80,6 +80,26 @@ def test_append_refuses_one_tensor_for_both():
     assert rc == rt.EINVAL and "must be two tensors" in err
 
 
+def test_append_refuses_a_cache_that_meets_itself():
+    # k and v a page apart in one buffer of 8, and two slots of one scale.
+    rc, err = kv_call("frisk_kv_append", cache=dict(v=4096 + 2 * 2048))
+    assert rc == rt.EINVAL and "the cache's k and v must be two tensors" in err
+    codes = dict(dtype=rt.I8, v=1 << 20, k_scale=1 << 21)
+    rc, err = kv_call("frisk_kv_append", cache=dict(codes, v_scale=(1 << 21) + 4))
+    assert rc == rt.EINVAL and "k_scale and v_scale must be two tensors" in err
+    for over in (dict(stride_head=64), dict(stride_page=1024 + 15 * 64), dict(dtype=rt.I8, scale_stride_head=15)):
+        rc, err = kv_call("frisk_kv_append", cache=dict(codes, v_scale=1 << 22, **over) if "dtype" in over else over)
+        assert rc == rt.EINVAL and "the cache's rows or scales overlap" in err, err
+
+
+def test_a_cache_keeps_its_tensors():
+    c = rt.KvCache.__new__(rt.KvCache)
+    c.k = 1
+    c._packed = b""
+    with pytest.raises(AttributeError, match="fixed"):
+        c.block_table = None
+
+
 def tree_call(cache=None, fn="frisk_tree_attn", **over):
     d = dict(batch=2, heads=4, tokens=3, dtype=rt.BF16, o_dtype=rt.BF16, sm_scale=0.125,
              q=16, q_stride_b=768, q_stride_h=192, q_stride_s=64, o=16, o_stride_b=768,
@@ -111,6 +131,22 @@ def test_tree_cache_refusals(cache, code, msg):
 def test_tree_refusals(over, code, msg):
     rc, err = tree_call(**over)
     assert rc == code and err.startswith(f"frisk_tree_attn: {msg}"), err
+
+
+@pytest.mark.parametrize("over", [
+    dict(o=16 + 128), dict(o=16 + 16), dict(o_stride_s=256, o_stride_h=64), dict(o_dtype=rt.F32),
+    dict(o=16 + 2 * 1000, o_dtype=rt.F32), dict(o=16 + 2 * 1528)])
+def test_tree_refuses_an_output_among_the_queries(over):
+    rc, err = tree_call(**over)
+    assert rc == rt.EINVAL and "q and o overlap" in err, err
+
+
+def test_tree_output_rows_and_hints_of_any_size():
+    rc, err = tree_call(o=1 << 20, o_stride_h=128)  # the heads of a token inside the next one's
+    assert rc == rt.EINVAL and "the rows of o overlap" in err
+    big = dict(block_table=64, max_pages=1 << 16, table_stride=1 << 16)
+    size = "frisk_tree_attn_workspace_size"
+    assert tree_call(big, size, max_ctx=(1 << 63) - 1)[0] == tree_call(big, size)[0] > 0
 
 
 def test_tree_workspace():
