@@ -595,11 +595,11 @@ _tree_pack = _packer(TreeAttnDesc, "cache")
 _ws_pack = struct.Struct("@Pq")
 
 
-def _pack(packer, *values) -> bytes:
-    try:
-        return packer.pack(*values)
-    except (OverflowError, struct.error) as e:
-        raise ValueError(f"argument out of range: {e}") from None
+_RANGE = (OverflowError, struct.error)
+
+
+def _range_error(e) -> ValueError:
+    return ValueError(f"argument out of range: {e}")
 
 
 _raw: dict = {}
@@ -635,22 +635,43 @@ def _same_device(*ts) -> int:
 
 def _lengths(t, batch: int, name: str) -> int:
     """The pointer of an int32 [batch] device tensor, or 0."""
-    import torch
     if t is None:
         return 0
+    import torch
     if t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous() or not t.is_cuda:
         raise ValueError(f"{name} must be a contiguous int32 device tensor of {batch} elements")
     return t.data_ptr()
 
 
+_accessors: list = []
+
+
+def _current(dev: int, stream):
+    """The handle of `stream` (None: the current one of device `dev`), or None
+    if `dev` is not the current device."""
+    if not _accessors:
+        import torch
+        # torch's raw accessors, without the Python layers of the public ones.
+        _accessors[:] = [getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device),
+                         getattr(torch._C, "_cuda_getCurrentRawStream", None)]
+    device, raw = _accessors
+    if dev != device():
+        return None
+    return raw(dev) if stream is None and raw is not None else _stream_handle(stream)
+
+
 def _run(name: str, desc: bytes, dev: int, stream):
     """The library's `name` on a packed descriptor, with device `dev` current."""
-    import torch
-    if dev != torch.cuda.current_device():
+    handle = _current(dev, stream)
+    if handle is None:
+        import torch
         with torch.cuda.device(dev):
-            _check(_raw_fn(name)(desc, _stream_handle(stream)), name)
+            handle = _stream_handle(stream)
+            rc = _raw_fn(name)(desc, handle)
     else:
-        _check(_raw_fn(name)(desc, _stream_handle(stream)), name)
+        rc = _raw_fn(name)(desc, handle)
+    if rc:
+        _check(rc, name)
 
 
 def rope(x, out, positions, table, *, k=None, k_out=None, start=None, interleaved=False,
@@ -686,10 +707,14 @@ def rope(x, out, positions, table, *, k=None, k_out=None, start=None, interleave
         st = positions.stride()
         at = (positions.data_ptr(), bits, *((0, st[0]) if len(st) == 1 else st))
     dev = _same_device(x, out, k, k_out, positions, table, start)
-    desc = _pack(_rope_pack, b, s, h, kh, d, 2 * table.shape[0], torch_dtype_code(x.dtype),
-                           bool(interleaved), bool(backward), amplitude,
-                           x.data_ptr(), xs[0], xs[1], xs[2], out.data_ptr(), outs[0], outs[1], outs[2],
-                           *second, *at, _lengths(start, b, "start"), table.data_ptr())
+    start = _lengths(start, b, "start")
+    try:
+        desc = _rope_pack.pack(b, s, h, kh, d, 2 * table.shape[0], torch_dtype_code(x.dtype),
+                               bool(interleaved), bool(backward), amplitude,
+                               x.data_ptr(), xs[0], xs[1], xs[2], out.data_ptr(), outs[0], outs[1], outs[2],
+                               *second, *at, start, table.data_ptr())
+    except _RANGE as e:
+        raise _range_error(e) from None
     _run("frisk_rope", desc, dev, stream)
     return out if k is None else (out, k_out)
 
@@ -769,10 +794,13 @@ def _kv(name, k, v, cache, ctx_len, new_len, stream):
         raise ValueError(f"k and v must be [batch, {csh[1]}, tokens, {csh[3]}] of one dtype "
                          f"(got {tuple(k.shape)} and {tuple(v.shape)})")
     dev = cache._check(b, k, v, ctx_len, new_len)
-    desc = _pack(_kv_pack, b, t, torch_dtype_code(k.dtype), k.data_ptr(), ks[0], ks[1], ks[2],
-                         v.data_ptr(), vs[0], vs[1], vs[2], _lengths(ctx_len, b, "ctx_len"),
-                         _lengths(new_len, b, "new_len")) + cache._packed
-    _run(name, desc, dev, stream)
+    ctx, new = _lengths(ctx_len, b, "ctx_len"), _lengths(new_len, b, "new_len")
+    try:
+        desc = _kv_pack.pack(b, t, torch_dtype_code(k.dtype), k.data_ptr(), ks[0], ks[1], ks[2],
+                             v.data_ptr(), vs[0], vs[1], vs[2], ctx, new)
+    except _RANGE as e:
+        raise _range_error(e) from None
+    _run(name, desc + cache._packed, dev, stream)
 
 
 def kv_append(k, v, cache, ctx_len, *, new_len=None, stream=None):
@@ -873,13 +901,17 @@ def tree_attn(q, cache, ctx_len, o, *, mask=None, new_len=None, sm_scale=None, l
     `workspace`: True allocates the scratch of the key splits (torch's
     caching allocator, on the call's stream), a device tensor supplies it,
     False runs unsplit."""
-    import torch
     dev, values = _tree_values(q, cache, ctx_len, o, mask, new_len, sm_scale, lse, max_ctx)
-    if dev != torch.cuda.current_device():
+    handle = _current(dev, stream)
+    if handle is None:
+        import torch
         with torch.cuda.device(dev):
             return tree_attn(q, cache, ctx_len, o, mask=mask, new_len=new_len, sm_scale=sm_scale,
                              lse=lse, max_ctx=max_ctx, workspace=workspace, stream=stream)
-    head = _pack(_tree_pack, *values) + cache._packed
+    try:
+        head = _tree_pack.pack(*values) + cache._packed
+    except _RANGE as e:
+        raise _range_error(e) from None
     ws, tail = None, bytes(16)
     if workspace is not False:
         need = _raw_fn("frisk_tree_attn_workspace_size")(head + tail)
@@ -890,5 +922,7 @@ def tree_attn(q, cache, ctx_len, o, *, mask=None, new_len=None, sm_scale=None, l
             if ws.get_device() != dev or not ws.is_contiguous():
                 raise ValueError("workspace must be a contiguous tensor on q's device")
             tail = _ws_pack.pack(ws.data_ptr(), ws.numel() * ws.element_size())
-    _check(_raw_fn("frisk_tree_attn")(head + tail, _stream_handle(stream)), "frisk_tree_attn")
+    rc = _raw_fn("frisk_tree_attn")(head + tail, handle)
+    if rc:
+        _check(rc, "frisk_tree_attn")
     return o
