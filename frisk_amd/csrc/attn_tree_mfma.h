@@ -667,10 +667,11 @@ static hipError_t launch_keys(const TreeAttnArgs& a, const Part& p, hipStream_t 
 
 // NW tiles of 32 rows per workgroup, one a wave; K and V of a key block in LDS
 // for all of them, in q's type (codes are widened once, on their way), double
-// buffered.  LDS and the matrix cores bound it alike: of a block, eight waves read 256 KB
-// (2048 cycles) and two waves of a SIMD take 2048 cycles of products.  512 tokens of b2 h32/8 d128
+// buffered.  Of a block, two waves of a SIMD take 2048 cycles of products and 1800 (8-bit rows:
+// 3000) of vector instructions, eight waves 2048 of LDS reads, of 4400 (6000) in all: the
+// barrier keeps the waves in step, so they overlap little.  512 tokens of b2 h32/8 d128
 // bf16 over 32k keys: 550 us, 990 TFLOP/s, matrix cores busy 48% of the cycles; 64 tokens of b8
-// over 16k keys of e4m3, which read scales too: 192 us, 717 TFLOP/s.
+// over 16k keys of e4m3: 192 us, 717 TFLOP/s.
 template <Elt T, Elt C, int D, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, Part part, int row_blocks,
                                                             int units) {

@@ -174,6 +174,29 @@ def test_bad_pages_and_capacity():
     assert (raw[[1, 2, 4]] == FILL).all()
 
 
+def test_keys_and_values_of_one_buffer():
+    """k and v side by side in one tensor, and their scales: rows that never meet."""
+    b, t, kv, d, page = 2, 37, 3, 64, 16
+    x = torch.randn((2, b, kv, t, d), generator=torch.Generator().manual_seed(5)).cuda().bfloat16()
+    table = torch.arange(2 * 3, dtype=torch.int32, device="cuda").flip(0).reshape(2, 3)
+    start = torch.zeros(b, dtype=torch.int32, device="cuda")
+    for dt in (torch.bfloat16, torch.int8):
+        buf = torch.zeros((6, page, 2, kv, d), dtype=dt, device="cuda")
+        scales = torch.zeros((6, page, 2, kv), device="cuda")
+        k, v = (buf[:, :, i].transpose(1, 2) for i in (0, 1))
+        ks, vs = (scales[:, :, i].transpose(1, 2) for i in (0, 1)) if dt == torch.int8 else (None, None)
+        both = rt.KvCache(k, v, ks, vs, table)
+        apart = rt.KvCache.empty(6, kv, page, d, dt, block_table=table)
+        outs = []
+        for cache in (both, apart):
+            rt.kv_append(x[0], x[1], cache, start)
+            out = torch.zeros_like(x)
+            rt.kv_read(cache, out[0], out[1], start)
+            outs.append(out)
+        assert torch.equal(outs[0], outs[1])
+        assert dt == torch.int8 or torch.equal(outs[0], x)
+
+
 def test_offsets_beyond_32_bits():
     # A sequence's page 5 GB into the cache.
     pages, size = 1300, 4096

@@ -369,6 +369,32 @@ def test_f32_output_scale_and_layouts(tokens):
     assert none is None and torch.equal(o, o2)
 
 
+@pytest.mark.parametrize("batch,tokens,d,ctx,dt,kind", [
+    (1, 1, 128, 4000, "bf16", "bf16"), (2, 33, 64, 1500, "f16", "i8"), (1, 150, 128, 3001, "bf16", "e4m3"),
+    (4, 300, 128, 64, "bf16", "bf16"), (2, 3, 80, 700, "f16", "f16"), (2, 40, 32, 0, "bf16", "bf16")])
+def test_output_in_place_of_the_queries(batch, tokens, d, ctx, dt, kind):
+    s = Setup(batch, 8, 2, tokens, d, dt, kind, 16, [ctx] * batch, seed=6)
+    want, lse = s.run()
+    q = s.q.clone(memory_format=torch.preserve_format)
+    assert q.stride() == s.q.stride()
+    l = torch.empty_like(lse)
+    rt.tree_attn(q, s.cache, s.ctx_len, q, lse=l)
+    assert torch.equal(q, want) and torch.equal(l, lse)
+
+
+def test_refuses_workspaces_it_cannot_write():
+    s = Setup(1, 32, 8, 1, 128, "bf16", "bf16", 64, (30000,), seed=6)
+    o = torch.empty_like(s.q)
+    need = rt.tree_attn_workspace_bytes(rt.tree_attn_desc(s.q, s.cache, s.ctx_len, o))
+    assert need > 0
+    one = torch.empty(1, dtype=torch.uint8, device="cuda")
+    for ws in (torch.empty(need, dtype=torch.uint8), one.expand(need)):
+        with pytest.raises(ValueError, match="workspace must be a contiguous tensor"):
+            rt.tree_attn(s.q, s.cache, s.ctx_len, o, workspace=ws)
+    with pytest.raises(ValueError, match="workspace of"):
+        rt.tree_attn(s.q, s.cache, s.ctx_len, o, workspace=one)
+
+
 def test_long_cache_beyond_32_bits():
     # Keys of one sequence over 6 GB of cache.
     pages, size, d = 3, 1 << 20, 128
