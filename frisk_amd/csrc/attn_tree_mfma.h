@@ -9,12 +9,15 @@
 // from transposing LDS reads in the matching key order.  The row sum is kept
 // over the unrounded P, so that the log-sum-exp is exact to f32.
 //
-// 8-bit rows: codes widen to q's type exactly (4 or 8 significant bits).  A key's
-// score is its column of S times the key's scale, and P is taken from score +
-// log2(value's scale) in one fused multiply-add, so that it is the weight times
-// the value's scale, below 2^8 whatever the scales are; the row sum adds P over
-// the value's scale, in another.  Nothing is rounded that a 16-bit cache would
-// not round.
+// 8-bit rows: codes widen exactly (4 or 8 significant bits), a key's to q's type,
+// a value's to bf16.  A key's score is its column of S times the key's scale, and
+// P is taken from score + log2(value's scale) in one fused multiply-add, so that it
+// is the weight times the value's scale, below 2^8 whatever the scales are; the row
+// sum adds P over the value's scale, in another.  P needs bf16's range: f16 would
+// round a key to nothing whose value scale is 2^-25 of another's, though it alone
+// may feed a dim.  With q in bf16 P is rounded once, as over a 16-bit cache; with q
+// in f16 it is the sum of two bf16 numbers, 16 bits (f16 has 11), and the second
+// product is taken twice.
 //
 // Where a key lies is computed once per key and block (a page number from the
 // table, loaded a block ahead), into LDS, as a 64-bit offset; the row loads go
@@ -64,6 +67,9 @@ TREE_INLINE float pair_sum(float x) {
 
 constexpr bool is8(Elt c) { return c == Elt::E4M3 || c == Elt::I8; }
 constexpr int bytes_of(Elt c) { return is8(c) ? 1 : 2; }
+// Type of the second product, and the parts that P enters it in (pack_p).
+template <Elt T, Elt C> constexpr Elt kProduct = is8(C) ? Elt::BF16 : T;
+template <Elt T, Elt C> constexpr int kParts = is8(C) && T == Elt::F16 ? 2 : 1;
 
 // LDS geometry of 64 rows (keys) of D elements: rows of kRB bytes, kKC chunks of
 // 16 B, chunk c of row r stored at c ^ swz(r).
@@ -221,12 +227,11 @@ TREE_INLINE void put_scales(float* sc, int lane, float value, bool of_key, float
   }
 }
 
-// Scores s to P (in place, f32, and packed in pf).  seen: bits of the row's
-// keys shifted down by 4 half, read if masked (uniform).  sc: the block's scales
-// (put_scales), over codes.
-template <Elt T, Elt C, int D>
-TREE_INLINE void softmax(f32x16 (&s)[2], i32x4 (&pf)[4], State<D>& st, float scale_log2,
-                         const float* sc, int half, bool masked, uint64_t seen) {
+// Scores s to P (in place, f32).  seen: bits of the row's keys shifted down by 4
+// half, read if masked (uniform).  sc: the block's scales (put_scales), over codes.
+template <Elt C, int D>
+TREE_INLINE void softmax(f32x16 (&s)[2], State<D>& st, float scale_log2, const float* sc, int half, bool masked,
+                         uint64_t seen) {
   constexpr bool k8 = is8(C);
   if constexpr (k8) {
 #pragma unroll
@@ -282,13 +287,20 @@ TREE_INLINE void softmax(f32x16 (&s)[2], i32x4 (&pf)[4], State<D>& st, float sca
         l = k8 ? __builtin_fmaf(s[kt][4 * g + i], over[i], l) : l + s[kt][4 * g + i];
     }
   st.l = l;
+}
+
+// P of key step kk as the B operand of the second product.
+template <Elt T, Elt C> TREE_INLINE void pack_p(const f32x16 (&s)[2], int kk, i32x4 (&pf)[kParts<T, C>]) {
 #pragma unroll
-  for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = 8 * (kk & 1) + 2 * e;
-      pf[kk][e] = (int)pack16<T>(s[kk >> 1][r], s[kk >> 1][r + 1]);
-    }
+  for (int e = 0; e < 4; ++e) {
+    const int r = 8 * (kk & 1) + 2 * e;
+    const float x = s[kk >> 1][r], y = s[kk >> 1][r + 1];
+    const uint32_t w = pack16<kProduct<T, C>>(x, y);
+    pf[0][e] = (int)w;
+    if constexpr (kParts<T, C> == 2)
+      pf[1][e] = (int)pack16<Elt::BF16>(x - __builtin_bit_cast(float, w << 16),
+                                        y - __builtin_bit_cast(float, w & 0xffff0000u));
+  }
 }
 
 // ---- V rows that are not finite ----------------------------------------------------
@@ -526,12 +538,22 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
     __builtin_amdgcn_sched_barrier(0);
 
     const bool masked = there != ~0ull || (int64_t)(kb + 1) * kBlock > sp.ctx;
-    i32x4 pf[4];
+    constexpr int kp = kParts<T, C>;
+    i32x4 pf[4][kp];
     uint64_t seen = 0;
     if (masked) seen = seen_bits(a, b, t, sp.ctx, kb * kBlock, there) >> (4 * half);
-    softmax<T, C, D>(s, pf, st, scale_log2, sc, half, masked, seen);
+    softmax<C, D>(s, st, scale_log2, sc, half, masked, seen);
+    // P before the wait; in two parts, which take twice the registers, they are
+    // made as the products need them.
+    if constexpr (kp == 1) {
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) asm volatile("" ::"v"(pf[kk]));  // P before the wait
+      for (int kk = 0; kk < 4; ++kk) {
+        pack_p<T, C>(s, kk, pf[kk]);
+        asm volatile("" ::"v"(pf[kk][0]));
+      }
+    } else {
+      asm volatile("" ::"v"(s[0]), "v"(s[1]));
+    }
     // V landed (only the next block's K may be in flight).
     __builtin_amdgcn_sched_barrier(0);
     if (more) __builtin_amdgcn_s_waitcnt((nv & 15) | ((nv >> 4) << 14) | (7 << 4) | (15 << 8));
@@ -545,10 +567,15 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
       }
     }
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
+    for (int kk = 0; kk < 4; ++kk) {
+      if constexpr (kp > 1) pack_p<T, C>(s, kk, pf[kk]);
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-        st.o[dt] = mfma<T>(read_v<T, C, D>(smem, v_at, kk, dt), pf[kk], st.o[dt]);
+      for (int dt = 0; dt < D / 32; ++dt) {
+        const i32x4 vf = read_v<kProduct<T, C>, C, D>(smem, v_at, kk, dt);
+#pragma unroll
+        for (int i = 0; i < kp; ++i) st.o[dt] = mfma<kProduct<T, C>>(vf, pf[kk][i], st.o[dt]);
+      }
+    }
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(0xC07F);
     if (more) issue(vbase, vs, true);
@@ -678,6 +705,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
 #if defined(__HIP_DEVICE_COMPILE__)
   using G = Geom<T, D>;
   constexpr bool k8 = is8(C);
+  constexpr Elt VT = kProduct<T, C>;  // of V in LDS
   constexpr int kBuf = 2 * G::kTile;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   int64_t* offs = (int64_t*)(smem + 2 * kBuf);  // [2][64]
@@ -774,7 +802,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
         *(i32x4*)(dst + r * G::kRB + (((c + e) ^ G::swz_k(r)) << 4)) =
             widen8<T, C>(kw[i][2 * e], kw[i][2 * e + 1]);
         *(i32x4*)(dst + G::kTile + r * G::kRB + (((c + e) ^ G::swz_v(r)) << 4)) =
-            widen8<T, C>(vw[i][2 * e], vw[i][2 * e + 1]);
+            widen8<VT, C>(vw[i][2 * e], vw[i][2 * e + 1]);
       }
     }
     if (wave < 2) put_scales(scales + (kb & 1) * 192, lane, my_value, wave == 0, scale_log2);
@@ -816,7 +844,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
     const bool masked = there != ~0ull || (int64_t)(kb + 1) * kBlock > sp.ctx;
     // The same in every wave: all of them look at the same tile.
     uint64_t bad = 0;
-    if (masked) bad = not_finite<T, T, D>(vs, lane);
+    if (masked) bad = not_finite<VT, VT, D>(vs, lane);
     if (more) {
       if constexpr (k8) fetch(kb + 1);
       else issue(kb + 1);
@@ -852,7 +880,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(smem, v_at, kk, dt);
+          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<VT, VT, D>(smem, v_at, kk, dt);
 #pragma unroll
         for (int i = 0; i < H1; ++i)
 #pragma unroll
@@ -860,16 +888,19 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
 #pragma unroll
         for (int kk = 2; kk < kEarly; ++kk)
 #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(smem, v_at, kk, dt);
+          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<VT, VT, D>(smem, v_at, kk, dt);
       }
       __builtin_amdgcn_sched_barrier(0);
-      i32x4 pf[4];
+      constexpr int kp = kParts<T, C>;
+      i32x4 pf[4][kp];
       uint64_t seen = 0;
       if (masked) seen = seen_bits(a, b, t, sp.ctx, kb * kBlock, there) >> (4 * half);
-      softmax<T, C, D>(s, pf, st, scale_log2, scales + (kb & 1) * 192, half, masked, seen);
+      softmax<C, D>(s, st, scale_log2, scales + (kb & 1) * 192, half, masked, seen);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) pack_p<T, C>(s, kk, pf[kk]);
       if (bad) {
         for (uint64_t left = bad; left; left &= left - 1)
-          add_key<T, T, D>(vs, __builtin_ctzll(left), s, seen, l32, half, st);
+          add_key<VT, VT, D>(vs, __builtin_ctzll(left), s, seen, l32, half, st);
         __syncthreads();
         if (wave == 0)
           for (uint64_t left = bad; left; left &= left - 1) clear_key<T, D>(vs, __builtin_ctzll(left), lane);
@@ -877,17 +908,19 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
 #pragma unroll
         for (int kk = 0; kk < kEarly; ++kk)
 #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(smem, v_at, kk, dt);
+          for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<VT, VT, D>(smem, v_at, kk, dt);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kk = kEarly; kk < 4; ++kk)
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<T, T, D>(smem, v_at, kk, dt);
+        for (int dt = 0; dt < D / 32; ++dt) vf[kk][dt] = read_v<VT, VT, D>(smem, v_at, kk, dt);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) st.o[dt] = mfma<T>(vf[kk][dt], pf[kk], st.o[dt]);
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int i = 0; i < kp; ++i) st.o[dt] = mfma<VT>(vf[kk][dt], pf[kk][i], st.o[dt]);
     }
     if constexpr (k8)
       if (more) widen(kb + 1);
