@@ -11,13 +11,11 @@
 //
 // 8-bit rows: codes widen exactly (4 or 8 significant bits), a key's to q's type,
 // a value's to bf16.  A key's score is its column of S times the key's scale, and
-// P is taken from score + log2(value's scale) in one fused multiply-add, so that it
-// is the weight times the value's scale, below 2^8 whatever the scales are; the row
-// sum adds P over the value's scale, in another.  P needs bf16's range: f16 would
-// round a key to nothing whose value scale is 2^-25 of another's, though it alone
-// may feed a dim.  With q in bf16 P is rounded once, as over a 16-bit cache; with q
-// in f16 it is the sum of two bf16 numbers, 16 bits (f16 has 11), and the second
-// product is taken twice.
+// P is the weight times the value's scale, in f32; the row sum is of the weights.
+// P needs bf16's range: f16 would round a key to nothing whose value scale is 2^-25
+// of another's, though it alone may feed a dim.  With q in bf16 P is rounded once,
+// as over a 16-bit cache; with q in f16 it is the sum of two bf16 numbers, 16 bits
+// (f16 has 11), and the second product is taken twice.
 //
 // Where a key lies is computed once per key and block (a page number from the
 // table, loaded a block ahead), into LDS, as a 64-bit offset; the row loads go
@@ -26,8 +24,8 @@
 // the cache's first row and hidden.
 //
 // Hidden keys must not matter whatever they hold, and 0 * NaN is NaN: in blocks
-// with a hidden key a V row that is not finite is taken out of the product and
-// added by itself to the rows that see it.
+// with a hidden key a V row that is not finite, or whose scale is not, is taken out
+// of the product and added by itself to the rows that see it.
 #pragma once
 
 #include "attn_tree.h"
@@ -41,8 +39,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef __attribute__((address_space(1))) const void* global_ptr;
 
-constexpr float kSlack = 8.0f;      // log2 headroom before the running maximum moves
-constexpr float kLeastLog = -96.0f;  // of a value scale: P over it, and the sum of that, stay in range
+constexpr float kSlack = 8.0f;  // log2 headroom before the running maximum moves
 
 template <Elt T> TREE_INLINE f32x16 mfma(i32x4 a, i32x4 b, f32x16 c) {
   if constexpr (T == Elt::BF16)
@@ -189,13 +186,6 @@ template <Elt T, Elt C, int D> TREE_INLINE i32x4 read_v(const char* lds, uint32_
 TREE_INLINE uint64_t seen_bits(const TreeAttnArgs& a, int64_t b, int t, int64_t ctx, int n0, uint64_t there) {
   return seen_bits(a.mask ? a.mask + (b * a.mask_sb + t * a.mask_st) : nullptr, a.tokens, t, ctx, n0, there);
 }
-// A copy of the bits that the compiler takes for another value, so that the 32
-// conditions of one use are not kept in scalar registers for the next.
-TREE_INLINE uint64_t again(uint64_t bits) {
-  uint32_t lo = (uint32_t)bits, hi = (uint32_t)(bits >> 32);
-  asm volatile("" : "+v"(lo), "+v"(hi));
-  return (uint64_t)hi << 32 | lo;
-}
 // Key of score register r (of 16) of tile kt, less 4 half.
 constexpr int key_of(int kt, int r) { return kt * 32 + 8 * (r >> 2) + (r & 3); }
 
@@ -213,35 +203,50 @@ template <int D> TREE_INLINE void clear(State<D>& st) {
   st.l = 0.0f;
 }
 
-// What a block's scales are kept as: the key's times scale_log2, the logarithm of
-// the value's and one over it.  A value scale that is not finite has the
-// logarithm NaN and one over it 0: NaN where it is seen, nothing where not.
-TREE_INLINE void put_scales(float* sc, int lane, float value, bool of_key, float scale_log2) {
-  if (of_key) {
-    sc[lane] = value * scale_log2;
-  } else {
-    const bool finite = value < __builtin_inff();  // (NaN is not)
-    const float log = fmaxf(__log2f(value), kLeastLog);
-    sc[64 + lane] = finite ? log : __builtin_nanf("");
-    sc[128 + lane] = finite ? __builtin_amdgcn_exp2f(-log) : 0.0f;
-  }
+// The running maximum of rows whose block's `top`, counted from it (from 0 where it
+// is none), is `move` too high; what the block's scores are lowered by.
+template <int D> TREE_INLINE float raise(State<D>& st, bool move, float top) {
+  const bool none = st.m == -__builtin_inff();
+  const float from = none ? 0.0f : st.m, to = from + top;
+  const float by = move ? to - from : 0.0f;
+  const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(-by);  // (without a maximum l and o are 0)
+  st.m = move ? to : st.m;
+  st.l *= alpha;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= alpha;
+  return by;
 }
 
-// Scores s to P (in place, f32).  seen: bits of the row's keys shifted down by 4
-// half, read if masked (uniform).  sc: the block's scales (put_scales), over codes.
+// What a block's scales are kept as: the key's times scale_log2, then the value's.
+// In a block with a hidden key a value scale that is not finite counts as 0, and
+// add_key adds what the rows that see it get: NaN.
+TREE_INLINE void put_scale(float* sc, int lane, float value, bool of_key, float scale_log2, bool masked) {
+  if (of_key) sc[lane] = value * scale_log2;
+  else sc[64 + lane] = masked && !(fabsf(value) < __builtin_inff()) ? 0.0f : value;
+}
+// Bits of the keys whose value scale is not finite (lane = key).
+TREE_INLINE uint64_t nan_scales(float value) {
+  return __builtin_amdgcn_ballot_w64(!(fabsf(value) < __builtin_inff()));
+}
+
+// Scores s to P (in place, f32): the weights, over codes times the value's scale.
+// seen: bits of the row's keys shifted down by 4 half, read if masked (uniform).
+// sc: over codes, the block's scales (put_scale).  The row sum and the maximum
+// are of the weights alone.
 template <Elt C, int D>
 TREE_INLINE void softmax(f32x16 (&s)[2], State<D>& st, float scale_log2, const float* sc, int half, bool masked,
                          uint64_t seen) {
   constexpr bool k8 = is8(C);
-  if constexpr (k8) {
+  // A row that has seen no key keeps m = -inf: p = 0, not NaN.
+  float nm = st.m == -__builtin_inff() ? 0.0f : -st.m;
+  if constexpr (k8) {  // counted from the maximum, which seldom moves
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 by = *(const f32x4*)(sc + kt * 32 + 8 * g + 4 * half);
-        const f32x4 log = *(const f32x4*)(sc + 64 + kt * 32 + 8 * g + 4 * half);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[kt][4 * g + i] = __builtin_fmaf(s[kt][4 * g + i], by[i], log[i]);
+        for (int i = 0; i < 4; ++i) s[kt][4 * g + i] = __builtin_fmaf(s[kt][4 * g + i], by[i], nm);
       }
   }
   if (masked) {
@@ -257,36 +262,46 @@ TREE_INLINE void softmax(f32x16 (&s)[2], State<D>& st, float scale_log2, const f
 #pragma unroll
     for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kt][r]);
   top = pair_max(top);
-  if constexpr (!k8) top *= scale_log2;
-  const bool move = top > st.m + kSlack;
-  if (__builtin_amdgcn_ballot_w64(move)) {
-    const float alpha = move ? __builtin_amdgcn_exp2f(st.m - top) : 1.0f;
-    st.m = move ? top : st.m;
-    st.l *= alpha;
+  if constexpr (k8) {
+    const bool move = st.m == -__builtin_inff() ? top > st.m : top > kSlack;
+    if (__builtin_amdgcn_ballot_w64(move)) {
+      const float by = raise(st, move, top);
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= alpha;
-  }
-  // A row that has seen no key keeps m = -inf: p = 0, not NaN.
-  const float nm = st.m == -__builtin_inff() ? 0.0f : -st.m;
+      for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-  for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float x = k8 ? s[kt][r] + nm : __builtin_fmaf(s[kt][r], scale_log2, nm);
-      s[kt][r] = __builtin_amdgcn_exp2f(x);
+        for (int r = 0; r < 16; ++r) s[kt][r] -= by;
     }
+  } else {
+    top *= scale_log2;
+    const bool move = top > st.m + kSlack;
+    if (__builtin_amdgcn_ballot_w64(move)) {
+      const float alpha = move ? __builtin_amdgcn_exp2f(st.m - top) : 1.0f;
+      st.m = move ? top : st.m;
+      st.l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) st.o[dt] *= alpha;
+    }
+    nm = st.m == -__builtin_inff() ? 0.0f : -st.m;
+  }
   float l = st.l;
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      f32x4 over = {1.0f, 1.0f, 1.0f, 1.0f};
-      if constexpr (k8) over = *(const f32x4*)(sc + 128 + kt * 32 + 8 * g + 4 * half);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        l = k8 ? __builtin_fmaf(s[kt][4 * g + i], over[i], l) : l + s[kt][4 * g + i];
+    for (int r = 0; r < 16; ++r) {
+      s[kt][r] = __builtin_amdgcn_exp2f(k8 ? s[kt][r] : __builtin_fmaf(s[kt][r], scale_log2, nm));
+      l += s[kt][r];
     }
   st.l = l;
+  if constexpr (k8) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 by = *(const f32x4*)(sc + 64 + kt * 32 + 8 * g + 4 * half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[kt][4 * g + i] *= by[i];
+      }
+  }
 }
 
 // P of key step kk as the B operand of the second product.
@@ -326,18 +341,24 @@ template <Elt T, Elt C, int D> TREE_INLINE uint64_t not_finite(const char* vs, i
   return __builtin_amdgcn_ballot_w64(bad != 0);
 }
 
-// o += p V of key `key` alone, for rows that see it.
+// o += p V of key `key` alone, for rows that see it; NaN if its scale is.
 template <Elt T, Elt C, int D>
-TREE_INLINE void add_key(const char* vs, int key, const f32x16 (&p)[2], uint64_t seen, int l32, int half,
+TREE_INLINE void add_key(const char* vs, int key, const f32x16 (&p)[2], uint64_t seen, bool nan, int l32, int half,
                          State<D>& st) {
   using G = Geom<C, D>;
   float w = 0.0f;
+  // w = p of the key, one condition at a time: 32 at once would take the scalar
+  // registers that the loop over keys has.
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) w = key_of(kt, r) == (key & ~4) ? p[kt][r] : w;
+    for (int r = 0; r < 16; ++r)
+      asm("v_cmp_eq_u32_e32 vcc, %1, %2\n\tv_cndmask_b32_e32 %0, %0, %3, vcc"
+          : "+v"(w)
+          : "n"(key_of(kt, r)), "v"(key & ~4), "v"(p[kt][r])
+          : "vcc");
   const int from = l32 + 32 * ((key >> 2) & 1);  // the half that holds the key
-  w = __shfl(w, from);
+  w = nan ? __builtin_nanf("") : __shfl(w, from);
   const bool sees_it = __shfl((int)((seen >> (key & ~4)) & 1), from);
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
@@ -377,7 +398,7 @@ TREE_INLINE void place_unit(int pid, int units, int tiles, int& unit, int& tile)
 
 // Waves per workgroup: K and V tiles of all waves in LDS.
 template <Elt C, int D> constexpr int kKeyWaves = plan::tree_key_waves(D);
-constexpr int kExtra = 1280;  // per wave: 64 row offsets (8 B), 64 scales of K and of V, 64 logarithms
+constexpr int kExtra = 1024;  // per wave: 64 row offsets (8 B), 64 scales of K and of V
 template <Elt C, int D> constexpr int keys_lds() {
   const int tiles = kKeyWaves<C, D> * (2 * Geom<C, D>::kTile + kExtra);
   const int sum = kKeyWaves<C, D> * 32 * (D + 4 + 2) * 4;
@@ -506,6 +527,7 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
   }
   for (; kb < end; kb += NW) {
     const bool more = kb + NW < end;
+    const bool masked = there != ~0ull || (int64_t)(kb + 1) * kBlock > sp.ctx;
     // K landed (V's loads may still be in flight), and with it the scales and
     // the table entry, which were asked for before.
     constexpr int nv = G::kLoads;
@@ -513,9 +535,10 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
     __builtin_amdgcn_s_waitcnt((nv & 15) | ((nv >> 4) << 14) | (7 << 4) | (15 << 8));
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (k8) {
-      put_scales(sc, lane, ksc, true, scale_log2);
-      put_scales(sc, lane, vsc, false, scale_log2);
+      put_scale(sc, lane, ksc, true, scale_log2, masked);
+      put_scale(sc, lane, vsc, false, scale_log2, masked);
     }
+    const float value_scale = vsc;
     f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
     for (int h0 = 0; h0 < D / 16; h0 += 2) {
@@ -537,7 +560,6 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
     }
     __builtin_amdgcn_sched_barrier(0);
 
-    const bool masked = there != ~0ull || (int64_t)(kb + 1) * kBlock > sp.ctx;
     constexpr int kp = kParts<T, C>;
     i32x4 pf[4][kp];
     uint64_t seen = 0;
@@ -560,9 +582,10 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
     else __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));
     __builtin_amdgcn_sched_barrier(0);
     if (masked) {
-      for (uint64_t bad = not_finite<T, C, D>(vs, lane); bad; bad &= bad - 1) {
+      const uint64_t nans = k8 ? nan_scales(value_scale) : 0;
+      for (uint64_t bad = not_finite<T, C, D>(vs, lane) | nans; bad; bad &= bad - 1) {
         const int key = __builtin_ctzll(bad);
-        add_key<T, C, D>(vs, key, s, seen, l32, half, st);
+        add_key<T, C, D>(vs, key, s, seen, (nans >> key) & 1, l32, half, st);
         clear_key<C, D>(vs, key, lane);
       }
     }
@@ -709,7 +732,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
   constexpr int kBuf = 2 * G::kTile;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   int64_t* offs = (int64_t*)(smem + 2 * kBuf);  // [2][64]
-  float* scales = (float*)(offs + 128);         // [2][192]
+  float* scales = (float*)(offs + 128);         // [2][192]: put_scale's, then the value's as they are
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int unit, rb;
@@ -786,7 +809,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
     }
     if (wave < 2) my_value = (wave == 0 ? a.cache.k_scale : a.cache.v_scale)[my_scale];
   };
-  auto widen = [&](int kb) __attribute__((always_inline)) {
+  auto widen = [&](int kb, bool masked) __attribute__((always_inline)) {
     char* dst = smem + (kb & 1) * kBuf;
     // Its LDS addresses are formed here, a block at a time: kept over the loop
     // they would take registers that it does not have.
@@ -805,8 +828,13 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
             widen8<VT, C>(vw[i][2 * e], vw[i][2 * e + 1]);
       }
     }
-    if (wave < 2) put_scales(scales + (kb & 1) * 192, lane, my_value, wave == 0, scale_log2);
+    float* sc = scales + (kb & 1) * 192;
+    if (wave < 2) put_scale(sc, lane, my_value, wave == 0, scale_log2, masked);
+    if (wave == 1) sc[128 + lane] = my_value;
   };
+
+  // Whether some row may not see all keys of a block.
+  auto masked_of = [&](int kb, uint64_t there) { return there != ~0ull || (int64_t)(kb + 1) * kBlock > sp.ctx; };
 
   const uint32_t v_lane = v_offset<T, D>(lane);
   State<D> st;
@@ -829,7 +857,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
       my_scale = scale0;
       fetch(begin);
       my_scale = scale1;
-      widen(begin);
+      widen(begin, masked_of(begin, there));
     } else {
       issue(begin);
     }
@@ -841,10 +869,13 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
     const char* ks = smem + (kb & 1) * kBuf;
     char* vs = smem + (kb & 1) * kBuf + G::kTile;
     const uint32_t v_at = (uint32_t)((kb & 1) * kBuf + G::kTile) + v_lane;
-    const bool masked = there != ~0ull || (int64_t)(kb + 1) * kBlock > sp.ctx;
+    const bool masked = masked_of(kb, there);
     // The same in every wave: all of them look at the same tile.
-    uint64_t bad = 0;
-    if (masked) bad = not_finite<VT, VT, D>(vs, lane);
+    uint64_t bad = 0, nans = 0;
+    if (masked) {
+      if constexpr (k8) nans = nan_scales(scales[(kb & 1) * 192 + 128 + lane]);
+      bad = not_finite<VT, VT, D>(vs, lane) | nans;
+    }
     if (more) {
       if constexpr (k8) fetch(kb + 1);
       else issue(kb + 1);
@@ -900,7 +931,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
       for (int kk = 0; kk < 4; ++kk) pack_p<T, C>(s, kk, pf[kk]);
       if (bad) {
         for (uint64_t left = bad; left; left &= left - 1)
-          add_key<VT, VT, D>(vs, __builtin_ctzll(left), s, seen, l32, half, st);
+          add_key<VT, VT, D>(vs, __builtin_ctzll(left), s, seen, (nans >> __builtin_ctzll(left)) & 1, l32, half, st);
         __syncthreads();
         if (wave == 0)
           for (uint64_t left = bad; left; left &= left - 1) clear_key<T, D>(vs, __builtin_ctzll(left), lane);
@@ -923,7 +954,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
           for (int i = 0; i < kp; ++i) st.o[dt] = mfma<VT>(vf[kk][dt], pf[kk][i], st.o[dt]);
     }
     if constexpr (k8)
-      if (more) widen(kb + 1);
+      if (more) widen(kb + 1, masked_of(kb + 1, there1));
     // Offsets of the block after the next, whose place in LDS this block's had.
     there = there1;
     there1 = place(kb + 2, entry);

@@ -409,8 +409,8 @@ int frisk_rope_frequencies(int64_t rot_dim, double base, int32_t scaling, double
  * head_dim] with the strides below (elements, shared by k and v; head_dim
  * stride 1).  dtype bf16 or f16 holds them as they are; e4m3 or i8 holds
  * codes and an f32 scale for each row (page, head, slot) of k and of v: a
- * value is code * scale.  Scales are above 0, or NaN (frisk_tree_attn takes a
- * value's scale below 2^-96 as 2^-96).
+ * value is code * scale.  Scales are finite and above 0, or NaN (a value that is
+ * NaN makes the o of tokens that see it NaN, not their lse).
  * Key n of sequence b is slot n % page_size of page block_table[b *
  * table_stride + n / page_size] (page_size a power of two), or without a
  * table slot n of page b; a sequence holds capacity = max_pages * page_size

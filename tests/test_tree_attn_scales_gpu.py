@@ -2,11 +2,9 @@
 weights, their sum and its logarithm depend on the scores only, and a result's dim
 only on the keys whose values feed it.  Tolerances as in test_tree_attn_gpu.py
 (per dim: A is the sum of weight * |v| of that dim)."""
-import numpy as np
 import pytest
 import torch
 
-from oracle import cache_ops as C
 from tests.test_tree_attn_gpu import Setup
 
 pytestmark = pytest.mark.gpu
@@ -17,10 +15,6 @@ KINDS8 = [("bf16", "e4m3"), ("f16", "e4m3"), ("bf16", "i8"), ("f16", "i8")]
 SIZES = [(1, 8, 2, 1, 128, 700), (2, 4, 4, 33, 64, 257), (1, 4, 1, 20, 32, 130), (1, 4, 2, 5, 80, 90),
          (4, 16, 4, 512, 64, 300), (4, 16, 4, 512, 128, 300), (8, 16, 4, 512, 128, 300)]
 ROWS = (1, 31, 32, 200, 383)
-
-
-def codes(s, which):
-    return s.cache.k if which == "k" else s.cache.v
 
 
 @pytest.mark.parametrize("dt,kind", KINDS8)
@@ -36,3 +30,38 @@ def test_dims_that_small_scales_feed(batch, heads, kv, tokens, d, ctx, dt, kind)
         s.cache.v_scale[:, :, ::4] *= 2.0 ** k
         o, lse = s.run(out=torch.float32)
         s.check(o, lse, rows=ROWS, heads=(0, heads - 1), seqs=(0, batch - 1))
+
+
+@pytest.mark.parametrize("dt,kind", KINDS8)
+@pytest.mark.parametrize("batch,heads,kv,tokens,d,ctx", SIZES)
+def test_weights_do_not_depend_on_value_scales(batch, heads, kv, tokens, d, ctx, dt, kind):
+    # Value scales of 2^-60 to 2^60, and zero rows with the least scale there is.
+    s = Setup(batch, heads, kv, tokens, d, dt, kind, 16, (ctx,) * batch, seed=3 * d + tokens)
+    s.cache.v_scale.fill_(1.0)
+    _, want = s.run(out=torch.float32)
+    gen = torch.Generator().manual_seed(tokens)
+    s.cache.v_scale.copy_(torch.exp2(torch.randint(-60, 61, s.cache.v_scale.shape, generator=gen).float()))
+    s.cache.v_scale[:, :, 5::6] = 2.0 ** -126
+    s.cache.v.view(torch.uint8)[:, :, 5::6] = 0
+    o, lse = s.run(out=torch.float32)
+    assert torch.equal(lse, want)
+    s.check(o, lse, rows=ROWS, heads=(0, heads - 1), seqs=(0, batch - 1))
+
+
+@pytest.mark.parametrize("dt,kind", KINDS8)
+@pytest.mark.parametrize("batch,heads,kv,tokens,d,ctx", SIZES)
+def test_a_value_scale_that_is_nan(batch, heads, kv, tokens, d, ctx, dt, kind):
+    # The scale of a row with an infinity: NaN results for the tokens that see it,
+    # the same sums as without for all.
+    s = Setup(batch, heads, kv, tokens, d, dt, kind, 16, (ctx,) * batch, seed=d + tokens)
+    o0, l0 = s.run()
+    assert torch.isfinite(l0).all()
+    for key, first in ((11, 0), (ctx + tokens // 2, tokens // 2)):  # of the context, a draft
+        p, r = int(s.table[0, key // 16]), key % 16
+        keep = s.cache.v_scale[p, :, r].clone()
+        s.cache.v_scale[p, :, r] = float("nan")
+        o, lse = s.run()
+        s.cache.v_scale[p, :, r] = keep
+        assert torch.equal(lse, l0)
+        assert torch.isnan(o[0, :, first:]).all()
+        assert torch.equal(o[0, :, :first], o0[0, :, :first]) and torch.equal(o[1:], o0[1:])
