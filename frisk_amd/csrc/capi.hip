@@ -18,6 +18,7 @@
 
 #include "../../include/frisk_hip.h"
 #include "kernels.h"
+#include "row_overlap.h"
 
 namespace {
 
@@ -746,73 +747,10 @@ int frisk_probe_lds_transpose(int bits, uint16_t* out, int64_t out_elems, void* 
 
 namespace {
 
-// Sizes n and strides of three dims around rows of one length (elements).
-struct Rows {
-  const void* p;
-  int64_t n[3], s[3];
-};
-
-typedef __int128 Wide;  // a size of 2^31 times a stride of 2^40
-
-// Whether the ranges of two tensors, from the first row's start to the last
-// one's end (row bytes, element bytes), share memory.
-bool spans_share(const Rows& a, int64_t row_a, int es_a, const Rows& b, int64_t row_b, int es_b) {
-  Wide ea = row_a, eb = row_b;
-  for (int i = 0; i < 3; ++i) {
-    ea += (Wide)(a.n[i] - 1) * a.s[i] * es_a;
-    eb += (Wide)(b.n[i] - 1) * b.s[i] * es_b;
-  }
-  const Wide pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
-  return pa < pb + eb && pb < pa + ea;
-}
-
-// Whether rows of one tensor may share memory: they do not if each stride
-// holds all that the smaller ones reach (any permuted or sliced tensor).
-bool rows_overlap(const int64_t (&n)[3], const int64_t (&s)[3], int64_t row) {
-  int d[3] = {0, 1, 2};
-  std::sort(d, d + 3, [&](int i, int j) { return s[i] < s[j]; });
-  Wide below = row;
-  for (const int i : d) {
-    if (n[i] == 1) continue;
-    if (s[i] < below) return true;
-    below += (Wide)(n[i] - 1) * s[i];
-  }
-  return false;
-}
-
-// Whether i * strides of a and j * strides of b, `gap` apart, meet within a
-// row: the dims d[0 .. k) by falling stride, equal in both.
-bool rows_meet(int64_t gap, const Rows& a, const Rows& b, const int* d, int k, int64_t row) {
-  if (k == 0) return gap < row && gap > -row;
-  const int64_t s = a.s[*d];
-  const int64_t q = gap >= 0 ? gap / s : -((-gap + s - 1) / s);
-  for (const int64_t i : {q, q + 1})  // index in a less index in b
-    if (i < a.n[*d] && -i < b.n[*d] && rows_meet(gap - i * s, a, b, d + 1, k - 1, row)) return true;
-  return false;
-}
-
-// Whether the rows of two tensors may share memory.  Exact for equal strides
-// each at least the extent of the dims below it (heads of one buffer); other
-// tensors must not reach into each other's range.
-bool rows_share(const Rows& a, const Rows& b, int64_t row, int es) {
-  const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
-  if (!spans_share(a, row * es, es, b, row * es, es)) return false;
-  const int64_t bytes = (int64_t)(pb - pa);
-  int d[3], k = 0;
-  for (int i = 0; i < 3; ++i) {
-    if (a.n[i] == 1 && b.n[i] == 1) continue;
-    if (a.s[i] != b.s[i] || a.s[i] == 0) return true;
-    d[k++] = i;
-  }
-  std::sort(d, d + k, [&](int i, int j) { return a.s[i] > a.s[j]; });
-  Wide below = row;
-  for (int i = k - 1; i >= 0; --i) {
-    if (a.s[d[i]] < below) return true;
-    below += (Wide)(std::max(a.n[d[i]], b.n[d[i]]) - 1) * a.s[d[i]];
-  }
-  if (bytes % es) return true;
-  return rows_meet(bytes / es, a, b, d, k, row);
-}
+using frisk::Rows;
+using frisk::rows_overlap;
+using frisk::rows_share;
+using frisk::spans_share;
 
 // Sizes and strides that every product of an index the kernels form fits.
 constexpr int64_t kMaxDim = (int64_t)1 << 31, kMaxStride = (int64_t)1 << 40;

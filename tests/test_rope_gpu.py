@@ -150,3 +150,18 @@ def test_graph_replay_and_streams():
         want = torch.empty_like(x)
         rt.rope(x, want, None, table, start=start)
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("stride", [64, 384, 1])
+def test_in_place_with_one_kv_head(stride):
+    # A projection of 4 + 1 + 1 heads: k's dim of one head has a stride of its own.
+    qkv = randn((2, 3, 6 * 64), 3).to(torch.bfloat16)
+    before = qkv.clone()
+    table = rt.rope_table(64)
+    q = qkv[..., :256].view(2, 3, 4, 64).transpose(1, 2)
+    k = torch.as_strided(qkv, (2, 1, 3, 64), (3 * 384, stride, 384, 1), 256)
+    rt.rope(q, q, None, table, k=k, k_out=k)
+    pos = np.arange(3)[None, None]
+    check(q, before[..., :256].view(2, 3, 4, 64).transpose(1, 2), pos, table, "bf16")
+    check(k, before[..., 256:320].view(2, 3, 1, 64).transpose(1, 2), pos, table, "bf16")
+    assert torch.equal(qkv[..., 320:], before[..., 320:])
