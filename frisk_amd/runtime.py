@@ -251,17 +251,23 @@ def _stream_handle(stream) -> int:
     return int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
 
 
-def _scratch(nbytes: int, device, stream):
-    """A call's scratch, allocated on the stream its kernels run on: the
-    allocator may hand it out again as soon as it is dropped, to work of that
-    stream only."""
+def _empty(shape, dtype, device, stream):
+    """A new tensor, allocated on the stream that the call's kernels run on: the
+    allocator may have had its memory in use by, and may hand it out again to,
+    work of that stream only."""
     import torch
     if stream is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return torch.empty(shape, dtype=dtype, device=device)
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
     with torch.cuda.stream(stream):
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _scratch(nbytes: int, device, stream):
+    """A call's scratch."""
+    import torch
+    return _empty(nbytes, torch.uint8, device, stream)
 
 
 def _row_major(t, name: str) -> int:
@@ -825,7 +831,7 @@ def tree_mask(parents, mask=None, depth=None, *, stream=None):
     drafted token each one continues, -1: the context) to the int64 words
     [batch, tokens, ceil(tokens / 64)] that tree_attn takes, and the int32
     number of drafted tokens before each ([batch, tokens]; its position is
-    ctx_len + depth)."""
+    ctx_len + depth).  Tensors it makes are of the call's stream."""
     import torch
     if parents.dtype != torch.int32 or parents.dim() != 2 or not parents.is_contiguous() or \
             not parents.is_cuda:
@@ -833,11 +839,11 @@ def tree_mask(parents, mask=None, depth=None, *, stream=None):
     b, t = parents.shape
     words = (t + 63) // 64
     if mask is None:
-        mask = torch.empty((b, t, words), dtype=torch.int64, device=parents.device)
+        mask = _empty((b, t, words), torch.int64, parents.device, stream)
     elif mask.dtype != torch.int64 or mask.shape != (b, t, words) or not mask.is_contiguous():
         raise ValueError(f"mask must be a contiguous int64 tensor [{b}, {t}, {words}]")
     if depth is None:
-        depth = torch.empty((b, t), dtype=torch.int32, device=parents.device)
+        depth = _empty((b, t), torch.int32, parents.device, stream)
     elif depth.dtype != torch.int32 or depth.shape != (b, t) or not depth.is_contiguous():
         raise ValueError(f"depth must be a contiguous int32 tensor [{b}, {t}]")
     dev = _same_device(parents, mask, depth)

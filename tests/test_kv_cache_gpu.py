@@ -228,3 +228,18 @@ def test_tree_mask(t):
         seen, deep = C.ancestors(parents[i])
         assert np.array_equal(words[i].cpu().numpy().view(np.uint64), C.words_of(seen))
         assert np.array_equal(depth[i].cpu().numpy(), deep)
+
+
+@pytest.mark.parametrize("raw", [False, True])
+def test_tree_mask_allocates_on_its_stream(raw):
+    # Memory that the current stream's pool hands out may still be in use there.
+    side = torch.cuda.Stream()
+    parents = torch.arange(-1, 99, dtype=torch.int32, device="cuda").expand(2, 100).contiguous()
+    torch.cuda.synchronize()
+    mask, depth = rt.tree_mask(parents, stream=side.cuda_stream if raw else side)
+    torch.cuda.synchronize()
+    for t in (mask, depth):
+        owner = [s["stream"] for s in torch.cuda.memory_snapshot()
+                 if s["address"] <= t.data_ptr() < s["address"] + s["total_size"]]
+        assert owner == [side.cuda_stream]
+    assert torch.equal(depth[0].cpu(), torch.arange(100, dtype=torch.int32))
