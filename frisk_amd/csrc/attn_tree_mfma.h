@@ -707,7 +707,7 @@ static hipError_t launch_keys(const TreeAttnArgs& a, const Part& p, hipStream_t 
   const int group = a.heads / a.cache.kv_heads;
   const int64_t tiles = ((int64_t)a.tokens * group + 31) / 32;
   const int64_t units = a.batch * a.cache.kv_heads * p.splits;
-  if (units * tiles > UINT32_MAX / 512) return hipErrorInvalidConfiguration;
+  if (units * tiles > UINT32_MAX / threads) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL(kern, dim3((unsigned)(units * tiles)), dim3(threads), lds, stream, a, p, (int)tiles,
                      (int)units);
   return hipGetLastError();
@@ -1000,7 +1000,7 @@ static hipError_t launch_tile(const TreeAttnArgs& a, const Part& p, hipStream_t 
   const int group = a.heads / a.cache.kv_heads;
   const int64_t blocks = ((int64_t)a.tokens * group + 32 * NW - 1) / (32 * NW);
   const int64_t units = a.batch * a.cache.kv_heads * p.splits;
-  if (units * blocks > UINT32_MAX / 512) return hipErrorInvalidConfiguration;
+  if (units * blocks > UINT32_MAX / (64 * NW)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL(kern, dim3((unsigned)(units * blocks)), dim3(64 * NW), lds, stream, a, p, (int)blocks,
                      (int)units);
   return hipGetLastError();

@@ -656,15 +656,16 @@ inline TreePlan tree_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_
   struct Kind {
     TreeKernel kernel;
     int tile, waves, per_cu;  // rows and key-dividing waves of a workgroup, workgroups on a CU
+    int threads;              // of a workgroup
     double one, two;          // us a step
   };
   const bool d128 = head_dim == 128;
   const Kind kinds[] = {
       {TreeKernel::Keys, 32, tree_key_waves(head_dim), bits8 || head_dim == 32 ? 2 : 1,
-       d128 ? (bits8 ? 2.0 : 2.2) : bits8 ? 1.8 : 1.6, d128 ? 3.1 : head_dim == 64 ? 4.5 : bits8 ? 3.6 : 2.3},
-      {TreeKernel::Tile4, 128, 1, 2, d128 ? (bits8 ? 1.9 : 1.5) : bits8 ? 1.15 : 0.85,
+       64 * tree_key_waves(head_dim), d128 ? (bits8 ? 2.0 : 2.2) : bits8 ? 1.8 : 1.6, d128 ? 3.1 : head_dim == 64 ? 4.5 : bits8 ? 3.6 : 2.3},
+      {TreeKernel::Tile4, 128, 1, 2, 256, d128 ? (bits8 ? 1.9 : 1.5) : bits8 ? 1.15 : 0.85,
        d128 ? (bits8 ? 2.7 : 2.5) : bits8 ? 1.7 : 1.35},
-      {TreeKernel::Tile8, 256, 1, 1, bits8 ? 2.3 : 2.1, 0.0}};
+      {TreeKernel::Tile8, 256, 1, 1, 512, bits8 ? 2.3 : 2.1, 0.0}};
   const int64_t rows = tokens * (heads / kv_heads);  // of a kv head
   const double bytes_us = 2.0 * batch * kv_heads * keys * head_dim * (bits8 ? 1 : 2) / 5.3e6;
   TreePlan best{TreeKernel::Keys, 1, 1};
@@ -675,6 +676,8 @@ inline TreePlan tree_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_
     const int least = k.kernel == TreeKernel::Keys ? k.waves : 4;
     for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
       if (s > 1 && (!split || blocks < (int64_t)least * s)) break;
+      // (A launch has fewer than 2^32 threads: Tile4's never has more without splits.)
+      if (units * s > (int64_t)UINT32_MAX / k.threads) break;
       const int64_t steps = ((blocks + s - 1) / s + k.waves - 1) / k.waves, load = (units * s + cus - 1) / cus;
       const double work = (double)steps * ((load / k.per_cu) * (k.per_cu > 1 ? k.two : k.one) +
                                            (load % k.per_cu ? k.one : 0.0));

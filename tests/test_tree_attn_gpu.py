@@ -483,3 +483,14 @@ def test_a_drafting_step(kind):
     # What a token saw as a branch it sees as a chain: the same keys.
     both = o.gather(2, path[:, None, :, None].expand(b, heads, 4, d)).float()
     assert (both - o2.float()).abs().max() <= 2.0 ** -5 * both.abs().max()
+
+
+@pytest.mark.parametrize("batch,heads,d", [((1 << 23) + 5, 1, 32), (1 << 18, 40, 16)])
+def test_millions_of_sequences(batch, heads, d):
+    # More query rows than a launch has workgroups of 512 threads: one key each,
+    # whose value is the result.
+    k = torch.ones((batch, heads, 1, d), dtype=torch.bfloat16, device="cuda")
+    v = randn((batch, 1, 1, d), 4).to(torch.bfloat16).expand(batch, heads, 1, d).contiguous()
+    o = torch.empty_like(k)
+    rt.tree_attn(k, rt.KvCache(k, v), torch.zeros(batch, dtype=torch.int32, device="cuda"), o)
+    assert torch.equal(o, v)

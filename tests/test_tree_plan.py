@@ -158,3 +158,18 @@ int main(int, char**) {
     for splits, least, blocks, per in run():
         used = max(1, -(-blocks // per))
         assert per >= least and used <= splits and used * per >= blocks
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("batch,heads,kv,tokens", [
+    ((1 << 24) - 1, 1, 1, 1), ((1 << 23) + 1, 1, 1, 1), (1 << 23, 1, 1, 1), (1 << 18, 60, 30, 1), (1 << 19, 31, 31, 1),
+    (1 << 22, 3, 3, 1), (255, 65535, 65535, 1), (1, 1, 1, (1 << 24) - 1), (1, 4, 2, 1 << 21)])
+def test_every_call_fits_a_launch(plan, batch, heads, kv, tokens, d):
+    # Up to 2^24 - 1 query rows are taken: a launch has fewer than 2^32 threads.
+    for keys in (1, 100, 5000):
+        for bits8 in (0, 1):
+            kernel, splits, *_ = plan(batch, heads, kv, tokens, d, bits8, keys)
+            tile, threads = {ROWS: (1, 256), KEYS: (32, 256 if d == 128 else 512), TILE4: (128, 256),
+                             TILE8: (256, 512)}[kernel]
+            units = batch * heads * tokens if kernel == ROWS else batch * kv * -(-tokens * (heads // kv) // tile)
+            assert units * splits * threads < 2 ** 32
