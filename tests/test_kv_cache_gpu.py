@@ -243,3 +243,26 @@ def test_tree_mask_allocates_on_its_stream(raw):
                  if s["address"] <= t.data_ptr() < s["address"] + s["total_size"]]
         assert owner == [side.cuda_stream]
     assert torch.equal(depth[0].cpu(), torch.arange(100, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "i8"])
+def test_all_quotients_of_bf16(kind):
+    # Every significand of the row's largest value against every smaller value's,
+    # at each power of two that leaves a code: 128 rows of 9 * 128 values.
+    m = torch.arange(128, 256, dtype=torch.float64)
+    x = (m[None, :, None] * 2.0 ** -torch.arange(9.0, dtype=torch.float64)).reshape(1, -1).repeat(128, 1)
+    x[x > m[:, None]] *= 0.5  # (at the largest power only those up to the largest value fit)
+    x = x.reshape(128, -1, 64)  # 18 chunks of 64 values to a row of 80 with the largest value first
+    rows = torch.zeros(128, x.shape[1], 80, dtype=torch.float64)
+    rows[..., 0] = m[:, None]
+    rows[..., 1:65] = x
+    sign = torch.where(torch.rand(rows.shape, generator=torch.Generator().manual_seed(1)) < 0.5, -1.0, 1.0)
+    rows = (rows * sign / 256).reshape(1, 1, -1, 80)
+    half = rows.to(torch.bfloat16)
+    assert torch.equal(half.double(), rows)
+    n = rows.shape[2]
+    cache = rt.KvCache.empty(1, 1, n, 80, DT[kind])
+    rt.kv_append(half.cuda(), half.cuda(), cache, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    codes, scale = C.quantise(rows[0].numpy(), kind)
+    assert (decode(cache.k[0]) == codes).all() and (decode(cache.v[0]) == codes).all()
+    assert (cache.k_scale[0].cpu().numpy() == scale).all()
