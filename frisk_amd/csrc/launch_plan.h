@@ -625,18 +625,30 @@ inline int64_t attn_workspace(int64_t batch_heads, int64_t seq_q, int64_t seq_k,
 // The keys are split so that every CU has workgroups; `keys` is the most a
 // sequence may hold, and the kernels use fewer splits for shorter ones.
 //
-// Kernel and splits are the pair of least estimated time: 8 us to start, the
-// rounds of workgroups over the CUs, at least the bytes of K and V at 5.3
-// TB/s, and with splits the f32 rows out and back at 3 TB/s and 5 us of second
-// launch, or 2 us and 0.1 a split where the last workgroup of a tile sums them.  A round is its steps (64 keys, under Keys 64 for each wave) times
-// the us below, fitted to calls with one and with two workgroups on a CU.  us, the choice of each kernel and its best splits:
+// Kernel and splits are the pair of least estimated time, counted from the
+// launch's start: the rounds of workgroups over the CUs, at least the bytes of K
+// and V at 5.3 TB/s, and with splits the f32 rows out and back at 3 TB/s and 5 us
+// of second launch.  Where the last workgroup of a tile sums them (Keys) that is 2
+// us and 0.1 a split instead, and 0.0025 (s - 4)^2 for each tile: its s workgroups
+// try the same word up to s times each, over words next to each other.  A round is
+// its steps (64 keys, under Keys 64 for each wave) times the us below, fitted to
+// calls with one and with two workgroups on a CU.  Up to 32 rows of a kv head are
+// Keys' alone: all but one wave of a tiled workgroup would have none.
+// us, the choice of each kernel and its best splits:
 //   b8 h32/8 d128 8k keys        Keys        Tile4       Tile8
 //     bf16, 1 token              47.9 (2)    53.3 (8)    56.6 (4)
 //     bf16, 64 tokens            152 (1)     105 (4)     98 (4)
 //     e4m3, 16 tokens            43.4 (4)    62.7 (8)    75.3 (4)
 //     e4m3, 64 tokens            106 (1)     109 (4)     103 (4)
+//   b1 h32/8 d128, 1 token
+//     bf16, 32k keys             39.0 (12)   46.5 (32)   46.6 (32)
+//     bf16, 128k keys            111 (24)    117 (32)    115 (32)
+//     e4m3, 32k keys             34.8 (12)   55.7 (32)   54.4 (32)
 //   b1 h32/8 d128 4k keys, 128 tokens: bf16 32.2 (2), 34.4 (8), 39.3 (8)
 //   b4 h16/16 d64 4k keys, 128 tokens: bf16 22.8 (1), 33.2 (4)
+// and of Keys by its splits:
+//   b1 h32/8 d128 32k keys, 1 token, bf16: 45.5 (8), 39.2 (12), 40.1 (16), 48.8 (24), 63.9 (32)
+//   b4 h16/16 d64 5k keys, 33 tokens, i8: 27.6 (1), 20.3 (2), 29.8 (3), 27.4 (4: two on a CU)
 // ---------------------------------------------------------------------------
 constexpr int kTreeBlock = 64;  // keys per block
 enum class TreeKernel { Rows, Keys, Tile4, Tile8 };
@@ -671,6 +683,7 @@ inline TreePlan tree_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_
   TreePlan best{TreeKernel::Keys, 1, 1};
   double best_us = -1.0;
   for (const Kind& k : kinds) {
+    if (rows <= 32 && best_us >= 0) break;  // Keys fits a launch
     if (k.kernel == TreeKernel::Tile8 && !d128) continue;
     const int64_t units = batch * kv_heads * ((rows + k.tile - 1) / k.tile);
     const int least = k.kernel == TreeKernel::Keys ? k.waves : 4;
@@ -681,9 +694,12 @@ inline TreePlan tree_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_
       const int64_t steps = ((blocks + s - 1) / s + k.waves - 1) / k.waves, load = (units * s + cus - 1) / cus;
       const double work = (double)steps * ((load / k.per_cu) * (k.per_cu > 1 ? k.two : k.one) +
                                            (load % k.per_cu ? k.one : 0.0));
-      const double out = k.kernel == TreeKernel::Keys ? 2.0 + 0.1 * s : 5.0;
-      // (Fewer workgroups than CUs do not reach HBM's rate, nor even out ragged lengths.)
-      const double us = std::max(work, units * s < cus ? 1.12 * bytes_us : bytes_us) + (s > 1 ? out + 8.0 * all * s * (head_dim + 2) / 3e6 : 0.0);
+      const double more = std::max(0, s - 4);
+      const double out = k.kernel == TreeKernel::Keys ? 2.0 + 0.1 * s + 0.0025 * units * more * more : 5.0;
+      // (Fewer workgroups than CUs do not reach HBM's rate, nor even out ragged lengths; below half less still.)
+      const double share = 2 * units * s < cus ? 1.2 : units * s < cus ? 1.12 : 1.0;
+      const double us = std::max(work, share * bytes_us) +
+                        (s > 1 ? out + 8.0 * all * s * (head_dim + 2) / 3e6 : 0.0);
       if (best_us >= 0 && us >= best_us) continue;
       best_us = us;
       best = TreePlan{k.kernel, s, least};
