@@ -445,9 +445,9 @@ TREE_INLINE int arrive(unsigned long long* word, int n) {
 // One tile of 32 rows per workgroup; each wave takes every NW-th key block of
 // the split with K and V tiles of its own: no barrier in the loop, and a block's
 // bytes of loads in flight per wave.  One token of b16 h32/8 d128 bf16, up to 8192 keys,
-// is bound by HBM: 412 MB in 80 us, 5.1 TB/s.  33 tokens of b4 h16/16 d64 over i8 take 23.5
-// us (36 MB): at most 5 blocks a wave, whose widening, scales and softmax have few products
-// to hide behind.
+// is bound by HBM: 412 MB in 80 us, 5.1 TB/s.  33 tokens of b4 h16/16 d64, f16 over i8, take
+// 24.6 us (36 MB): two tiles, which both read and widen all keys, up to 5 blocks a wave whose
+// widening, scales and softmax have few products to hide behind.
 template <Elt T, Elt C, int D>
 __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeAttnArgs a, Part part,
                                                                          int row_tiles, int units) {
@@ -716,12 +716,12 @@ static hipError_t launch_keys(const TreeAttnArgs& a, const Part& p, hipStream_t 
 // ---- many rows: the waves share the keys ----------------------------------------------
 
 // NW tiles of 32 rows per workgroup, one a wave; K and V of a key block in LDS
-// for all of them, in q's type (codes are widened once, on their way), double
+// for all of them, in 16 bits (codes are widened once, on their way), double
 // buffered.  Of a block, two waves of a SIMD take 2048 cycles of products and 1800 (8-bit rows:
-// 3000) of vector instructions, eight waves 2048 of LDS reads, of 4400 (6000) in all: the
+// 2500) of vector instructions, eight waves 2048 of LDS reads, of 4400 (5600) in all: the
 // barrier keeps the waves in step, so they overlap little.  512 tokens of b2 h32/8 d128
 // bf16 over 32k keys: 550 us, 990 TFLOP/s, matrix cores busy 48% of the cycles; 64 tokens of b8
-// over 16k keys of e4m3: 192 us, 717 TFLOP/s.
+// over 16k keys of e4m3: 190 us, 723 TFLOP/s (with f16 queries, two second products: 241).
 template <Elt T, Elt C, int D, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, Part part, int row_blocks,
                                                             int units) {

@@ -354,7 +354,8 @@ int frisk_fill(const frisk_fill_desc* desc, void* stream);
  * tensors [batch, heads, seq, head_dim] of one dtype (f32, f16 or bf16), unit
  * innermost stride, other strides in elements.  out may be x itself (the same
  * pointer and strides); no other rows of the four tensors may overlap an
- * output.  The position of row (b, s) is
+ * output.  Rows of tensors with the same strides (a dim of one row has any) are told
+ * apart where they lie between each other, others by the ranges they reach.  The position of row (b, s) is
  * start[b] (0 if start is NULL) + positions[b * pos_stride_b + s *
  * pos_stride_s] (s if positions is NULL).
  */
@@ -434,8 +435,9 @@ typedef struct frisk_kv_cache {
 
 /*
  * frisk_kv_append writes rows [batch, kv_heads, tokens, head_dim] of k and v
- * (bf16 or f16) into the cache: token t < new_len[b] (all, if new_len is NULL)
- * of sequence b becomes key ctx_len[b] + t; keys behind the capacity or on a
+ * (bf16 or f16; bases and stride bytes are multiples of 16) into the cache:
+ * token t < new_len[b] (all, if new_len is NULL) of sequence b becomes key
+ * ctx_len[b] + t; keys behind the capacity or on a
  * page that is none are dropped.  frisk_kv_read is its inverse: those keys, as
  * code * scale rounded to dtype, into k and v, which must not overlap; rows from
  * new_len[b] on, and of keys the cache does not hold, are left as they were.
@@ -478,7 +480,8 @@ int frisk_tree_mask(int64_t batch, int64_t tokens, const int32_t* parents, uint6
  *   o[b,h,t,:] = softmax_n(sm_scale q[b,h,t,:] . K[b,h / group,n,:]) . V[b,h / group,n,:]
  * with group = heads / cache.kv_heads.  One token is a decode step, a mask
  * from frisk_tree_mask a step of drafted trees, no mask a prompt's chunk.
- * q is bf16 or f16 [batch, heads, tokens, head_dim]; o is that dtype or f32; lse, if
+ * q is bf16 or f16 [batch, heads, tokens, head_dim]; o is that dtype or f32 (bases
+ * multiples of 16 bytes, strides of 8 elements); lse, if
  * given, [batch, heads, tokens] contiguous f32 natural-log sums.  A 16-bit
  * cache has q's dtype.  A token that sees no key has o = 0 and lse = -inf.
  * What a hidden key or its value holds does not matter, NaN and infinities
