@@ -582,10 +582,10 @@ __global__ __launch_bounds__((64 * kKeyWaves<C, D>)) void tree_keys_kernel(TreeA
     else __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));
     __builtin_amdgcn_sched_barrier(0);
     if (masked) {
-      const uint64_t nans = k8 ? nan_scales(value_scale) : 0;
+      const uint64_t nans = k8 ? nan_scales(value_scale) & there : 0;
       for (uint64_t bad = not_finite<T, C, D>(vs, lane) | nans; bad; bad &= bad - 1) {
         const int key = __builtin_ctzll(bad);
-        add_key<T, C, D>(vs, key, s, seen, (nans >> key) & 1, l32, half, st);
+        if ((there >> key) & 1) add_key<T, C, D>(vs, key, s, seen, (nans >> key) & 1, l32, half, st);
         clear_key<C, D>(vs, key, lane);
       }
     }
@@ -873,7 +873,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
     // The same in every wave: all of them look at the same tile.
     uint64_t bad = 0, nans = 0;
     if (masked) {
-      if constexpr (k8) nans = nan_scales(scales[(kb & 1) * 192 + 128 + lane]);
+      if constexpr (k8) nans = nan_scales(scales[(kb & 1) * 192 + 128 + lane]) & there;
       bad = not_finite<VT, VT, D>(vs, lane) | nans;
     }
     if (more) {
@@ -930,7 +930,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_tile_kernel(TreeAttnArgs a, P
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) pack_p<T, C>(s, kk, pf[kk]);
       if (bad) {
-        for (uint64_t left = bad; left; left &= left - 1)
+        for (uint64_t left = bad & there; left; left &= left - 1)
           add_key<VT, VT, D>(vs, __builtin_ctzll(left), s, seen, (nans >> __builtin_ctzll(left)) & 1, l32, half, st);
         __syncthreads();
         if (wave == 0)

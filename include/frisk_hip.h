@@ -411,7 +411,9 @@ int frisk_rope_frequencies(int64_t rot_dim, double base, int32_t scaling, double
  * stride 1).  dtype bf16 or f16 holds them as they are; e4m3 or i8 holds
  * codes and an f32 scale for each row (page, head, slot) of k and of v: a
  * value is code * scale.  Scales are finite and above 0, or NaN (a value that is
- * NaN makes the o of tokens that see it NaN, not their lse).
+ * NaN makes the o of tokens that see it NaN, not their lse).  Attention may take
+ * the product of a weight and a value's scale as 0 below 2^-126, and sums in f32
+ * values up to 256 times as large as they are: beyond 2^119 they may overflow.
  * Key n of sequence b is slot n % page_size of page block_table[b *
  * table_stride + n / page_size] (page_size a power of two), or without a
  * table slot n of page b; a sequence holds capacity = max_pages * page_size

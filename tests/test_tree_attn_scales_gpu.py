@@ -65,3 +65,23 @@ def test_a_value_scale_that_is_nan(batch, heads, kv, tokens, d, ctx, dt, kind):
         assert torch.equal(lse, l0)
         assert torch.isnan(o[0, :, first:]).all()
         assert torch.equal(o[0, :, :first], o0[0, :, :first]) and torch.equal(o[1:], o0[1:])
+
+
+@pytest.mark.parametrize("dt,kind", KINDS8 + [("bf16", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("batch,heads,kv,tokens,d,ctx", SIZES)
+def test_a_first_row_that_is_nan(batch, heads, kv, tokens, d, ctx, dt, kind):
+    # Keys that do not exist are loaded from the cache's first row and hidden:
+    # NaN there, in a page that is no sequence's, changes no bit.
+    s = Setup(batch, heads, kv, tokens, d, dt, kind, 16, (ctx,) * batch, seed=d + tokens)
+    free = (set(range(s.cache.k.shape[0])) - set(s.table.flatten().tolist())).pop()
+    s.cache.block_table[s.cache.block_table == 0] = free  # that page's sequence takes the free one
+    o0, l0 = s.run()
+    for t in (s.cache.k, s.cache.v):
+        if t.element_size() == 2:
+            t[0] = float("nan")
+        elif kind == "e4m3":
+            t.view(torch.uint8)[0] = 0x7F
+    if s.cache.k_scale is not None:
+        s.cache.k_scale[0] = s.cache.v_scale[0] = float("nan")
+    o, lse = s.run()
+    assert torch.isfinite(lse).all() and torch.equal(o, o0) and torch.equal(lse, l0)
