@@ -779,6 +779,24 @@ int check_rope_tensor(const char* name, int64_t batch, int64_t heads, int64_t se
   return FRISK_OK;
 }
 
+// Scales of a page and head.
+int64_t scale_slots(const frisk_kv_cache& d) {
+  return d.scale_block > 1 ? (d.page_size + d.scale_block - 1) / d.scale_block : d.page_size;
+}
+
+// Whether two tensors of a cache, k and v or their scales, share memory.
+bool cache_tensors_share(const frisk_kv_cache& c, bool scales) {
+  auto held = [&](const void* p, int64_t slots, int64_t sp, int64_t sh, int64_t ss) {
+    return Rows{p, {c.pages, c.kv_heads, slots}, {sp, sh, ss}};
+  };
+  if (!scales)
+    return rows_share(held(c.k, c.page_size, c.stride_page, c.stride_head, c.stride_slot),
+                      held(c.v, c.page_size, c.stride_page, c.stride_head, c.stride_slot), c.head_dim, esize(c.dtype));
+  const int64_t n = scale_slots(c);
+  return rows_share(held(c.k_scale, n, c.scale_stride_page, c.scale_stride_head, c.scale_stride_slot),
+                    held(c.v_scale, n, c.scale_stride_page, c.scale_stride_head, c.scale_stride_slot), 1, 4);
+}
+
 // Checks of a cache; 0 or an error code.
 int check_cache(const frisk_kv_cache& d, const char* fn, bool ptrs, int64_t batch, frisk::KvCache& c) {
   if (d.pages <= 0 || d.kv_heads <= 0 || d.page_size <= 0 || d.head_dim <= 0)
@@ -796,11 +814,18 @@ int check_cache(const frisk_kv_cache& d, const char* fn, bool ptrs, int64_t batc
   const int64_t n[3] = {d.pages, d.kv_heads, d.page_size};
   const int64_t st[3] = {d.stride_page, d.stride_head, d.stride_slot};
   const int64_t sc[3] = {d.scale_stride_page, d.scale_stride_head, d.scale_stride_slot};
+  if (d.scale_block < 0 || d.scale_block > 256 || (d.scale_block & (d.scale_block - 1)))
+    return fail(FRISK_EINVAL, "%s: scale_block must be a power of two up to 256 (got %lld)", fn,
+                (long long)d.scale_block);
+  if (d.scale_block > 1 && !k8) return fail(FRISK_EINVAL, "%s: scale_block is for 8-bit caches", fn);
+  if (d.scale_block > 1 && d.block_table && d.scale_block > d.page_size)
+    return fail(FRISK_EINVAL, "%s: scale_block %lld is larger than a page", fn, (long long)d.scale_block);
+  const int64_t ns[3] = {d.pages, d.kv_heads, scale_slots(d)};
   for (int i = 0; i < 3; ++i) {
     if (st[i] < 0 || st[i] > kMaxStride || (st[i] * es) % 16 || (n[i] > 1 && st[i] < d.head_dim))
       return fail(FRISK_EINVAL, "%s: cache strides must be multiples of 16 bytes, at least head_dim "
                                 "and up to 2^40 elements", fn);
-    if (k8 && (sc[i] < 0 || sc[i] > kMaxStride || (n[i] > 1 && sc[i] < 1)))
+    if (k8 && (sc[i] < 0 || sc[i] > kMaxStride || (ns[i] > 1 && sc[i] < 1)))
       return fail(FRISK_EINVAL, "%s: scale strides must be 1 to 2^40 elements", fn);
   }
   if (ptrs && (!d.k || !d.v)) return fail(FRISK_EINVAL, "%s: null cache", fn);
@@ -831,7 +856,7 @@ int check_cache(const frisk_kv_cache& d, const char* fn, bool ptrs, int64_t batc
   }
   if (c.capacity > INT32_MAX - 8192)
     return fail(FRISK_EUNSUP, "%s: a sequence of more than 2^31 - 8193 keys", fn);
-  if (rows_overlap(n, st, d.head_dim) || (k8 && rows_overlap(n, sc, 1)))
+  if (rows_overlap(n, st, d.head_dim) || (k8 && rows_overlap(ns, sc, 1)))
     return fail(FRISK_EINVAL, "%s: the cache's rows or scales overlap", fn);
   c.kind = (frisk::Elt)d.dtype;
   c.pages = (int)d.pages;
@@ -841,6 +866,8 @@ int check_cache(const frisk_kv_cache& d, const char* fn, bool ptrs, int64_t batc
   c.sp = st[0]; c.sh = st[1]; c.ss = st[2];
   c.k_scale = d.k_scale; c.v_scale = d.v_scale;
   c.scp = sc[0]; c.sch = sc[1]; c.scs = sc[2];
+  c.scale_shift = 0;
+  while ((1ll << c.scale_shift) < d.scale_block) ++c.scale_shift;
   c.table = d.block_table;
   c.table_stride = d.table_stride;
   return FRISK_OK;
@@ -874,16 +901,9 @@ int check_kv(const frisk_kv_desc* d, const char* fn, bool write, frisk::KvArgs& 
     }
   if (!write && (rows_overlap(n, st[0], d->cache.head_dim) || rows_overlap(n, st[1], d->cache.head_dim)))
     return fail(FRISK_EINVAL, "%s: the rows of k or v overlap", fn);
-  const frisk_kv_cache& c = d->cache;
-  auto held = [&](const void* p, int64_t sp, int64_t sh, int64_t ss) {
-    return Rows{p, {c.pages, c.kv_heads, c.page_size}, {sp, sh, ss}};
-  };
-  if (write && rows_share(held(c.k, c.stride_page, c.stride_head, c.stride_slot),
-                          held(c.v, c.stride_page, c.stride_head, c.stride_slot), c.head_dim, esize(c.dtype)))
+  if (write && cache_tensors_share(d->cache, false))
     return fail(FRISK_EINVAL, "%s: the cache's k and v must be two tensors", fn);
-  if (write && c.k_scale &&
-      rows_share(held(c.k_scale, c.scale_stride_page, c.scale_stride_head, c.scale_stride_slot),
-                 held(c.v_scale, c.scale_stride_page, c.scale_stride_head, c.scale_stride_slot), 1, 4))
+  if (write && d->cache.k_scale && cache_tensors_share(d->cache, true))
     return fail(FRISK_EINVAL, "%s: k_scale and v_scale must be two tensors", fn);
   if (!write && rows_share(Rows{d->k, {n[0], n[1], n[2]}, {st[0][0], st[0][1], st[0][2]}},
                            Rows{d->v, {n[0], n[1], n[2]}, {st[1][0], st[1][1], st[1][2]}}, d->cache.head_dim, 2))
@@ -992,6 +1012,91 @@ int check_tree(const frisk_tree_attn_desc* d, bool ptrs, bool split, frisk::Tree
   return FRISK_OK;
 }
 
+// A contiguous array; whether two share memory.
+struct Span {
+  const void* p;
+  int64_t bytes;
+};
+bool overlap(const Span& a, const Span& b) {
+  const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+  return x && y && x < y + b.bytes && y < x + a.bytes;
+}
+// Whether one of the outputs overlaps another or an input.
+template <size_t N, size_t M> bool outputs_overlap(const Span (&out)[N], const Span (&in)[M]) {
+  for (size_t i = 0; i < N; ++i) {
+    for (size_t j = 0; j < i; ++j)
+      if (overlap(out[i], out[j])) return true;
+    for (size_t j = 0; j < M; ++j)
+      if (overlap(out[i], in[j])) return true;
+  }
+  return false;
+}
+
+// Checks of the entry that verifies drafts; 0 or an error code.  With ptrs == false the
+// tensors are not required.
+int check_verify(const frisk_tree_verify_desc* d, bool ptrs, frisk::VerifyArgs& a) {
+  const char* fn = "frisk_tree_verify";
+  namespace plan = frisk::plan;
+  if (!d) return fail(FRISK_EINVAL, "%s: null descriptor", fn);
+  if (d->batch <= 0 || d->tokens <= 0 || d->vocab <= 0) return fail(FRISK_EINVAL, "%s: sizes must be positive", fn);
+  if (d->dtype != FRISK_F32 && d->dtype != FRISK_F16 && d->dtype != FRISK_BF16)
+    return fail(FRISK_EINVAL, "%s: dtype must be f32, f16 or bf16 (got %s)", fn, dtype_name(d->dtype));
+  if (d->tokens > plan::kVerifyNodes || d->vocab > plan::kVerifyVocab)
+    return fail(FRISK_EUNSUP, "%s: up to %lld nodes a tree and a vocabulary of 2^24", fn,
+                (long long)plan::kVerifyNodes);
+  const int es = esize(d->dtype);
+  if (d->batch > INT32_MAX / 4) return fail(FRISK_EUNSUP, "%s: more trees than one launch takes", fn);
+  const plan::VerifyPlan p = plan::verify_plan(d->batch, d->tokens, d->vocab, es);
+  if (d->batch > (int64_t)(UINT32_MAX / 256) / (d->tokens * p.chunks))
+    return fail(FRISK_EUNSUP, "%s: more rows of logits than one launch takes", fn);
+  const int64_t st[4] = {d->stride_b, d->stride_t, d->draft_probs ? d->draft_stride_b : 0,
+                         d->draft_probs ? d->draft_stride_t : 0};
+  for (const int64_t s : st)
+    if (s < 0 || s > kMaxStride) return fail(FRISK_EINVAL, "%s: strides must be non-negative, up to 2^40", fn);
+  if (ptrs && (!d->logits || !d->drafts || !d->parents || !d->uniform || !d->final_uniform || !d->path ||
+               !d->count || !d->token))
+    return fail(FRISK_EINVAL, "%s: null tensor", fn);
+  if ((uintptr_t)d->logits % es || (uintptr_t)d->drafts % 4 || (uintptr_t)d->parents % 4 ||
+      (uintptr_t)d->uniform % 4 || (uintptr_t)d->final_uniform % 4 || (uintptr_t)d->draft_probs % 4 ||
+      (uintptr_t)d->temperature % 4 || (uintptr_t)d->new_len % 4 || (uintptr_t)d->path % 4 ||
+      (uintptr_t)d->count % 4 || (uintptr_t)d->token % 4 || (uintptr_t)d->probs % 4)
+    return fail(FRISK_EINVAL, "%s: pointers must be element-aligned", fn);
+  a.dtype = (frisk::Elt)d->dtype;
+  a.batch = d->batch;
+  a.tokens = (int)d->tokens;
+  a.vocab = (int)d->vocab;
+  a.logits = d->logits; a.sb = d->stride_b; a.st = d->stride_t;
+  a.drafts = d->drafts;
+  a.parents = d->parents;
+  a.uniform = d->uniform;
+  a.final_uniform = d->final_uniform;
+  a.draft_probs = d->draft_probs; a.qb = d->draft_stride_b; a.qt = d->draft_stride_t;
+  a.temperature = d->temperature;
+  a.new_len = d->new_len;
+  a.path = d->path;
+  a.count = d->count;
+  a.token = d->token;
+  a.probs = d->probs;
+  a.pieces = p.pieces;
+  a.chunks = (int)p.chunks;
+  a.workspace = d->workspace;
+  if (!ptrs) return FRISK_OK;
+  const int64_t need = frisk::verify_workspace(d->batch, d->tokens, p.chunks), n = d->batch * 4, all = n * d->tokens;
+  if (!d->workspace || d->workspace_bytes < need)
+    return fail(FRISK_EINVAL, "%s: workspace of %lld bytes, this call takes %lld", fn,
+                (long long)(d->workspace ? d->workspace_bytes : 0), (long long)need);
+  if (!aligned16(d->workspace)) return fail(FRISK_EINVAL, "%s: workspace must be 16-byte aligned", fn);
+  auto rows = [&](int64_t sb, int64_t sr, int bytes) {
+    return ((d->batch - 1) * sb + (d->tokens - 1) * sr + d->vocab) * bytes;
+  };
+  const Span out[] = {{d->path, all}, {d->count, n}, {d->token, n}, {d->probs, all}, {d->workspace, need}};
+  const Span in[] = {{d->logits, rows(st[0], st[1], es)}, {d->draft_probs, rows(st[2], st[3], 4)},
+                     {d->drafts, all}, {d->parents, all}, {d->uniform, all}, {d->final_uniform, n},
+                     {d->temperature, n}, {d->new_len, n}};
+  if (outputs_overlap(out, in)) return fail(FRISK_EINVAL, "%s: an output overlaps another tensor", fn);
+  return FRISK_OK;
+}
+
 int64_t tree_workspace(const frisk::TreeAttnArgs& a) {
   return frisk::plan::tree_workspace(frisk::plan::TreePlan{a.kernel, a.splits, a.min_blocks}, a.batch, a.heads,
                                      a.cache.kv_heads, a.tokens, a.cache.head_dim);
@@ -1024,6 +1129,11 @@ int frisk_rope(const frisk_rope_desc* d, void* stream) {
     return fail(FRISK_EINVAL, "frisk_rope: positions must be element-aligned");
   if ((uintptr_t)d->start % 4) return fail(FRISK_EINVAL, "frisk_rope: start must be 4-byte aligned");
   if (d->pos_stride_b < 0 || d->pos_stride_s < 0 || d->pos_stride_b > kMaxStride || d->pos_stride_s > kMaxStride)
+    return fail(FRISK_EINVAL, "frisk_rope: position strides must be non-negative, up to 2^40");
+  if (d->pair_axis && (d->axes < 1 || d->axes > 4))
+    return fail(FRISK_EUNSUP, "frisk_rope: positions of 1 to 4 axes (got %lld)", (long long)d->axes);
+  if (d->pair_axis && !d->positions) return fail(FRISK_EINVAL, "frisk_rope: pair_axis needs positions");
+  if (d->pair_axis && (d->pos_stride_a < 0 || d->pos_stride_a > kMaxStride))
     return fail(FRISK_EINVAL, "frisk_rope: position strides must be non-negative, up to 2^40");
   if (d->batch >= kMaxDim || d->seq >= kMaxDim || d->batch * d->seq >= ((int64_t)1 << 40) ||
       d->heads > 32767 || (d->k && d->k_heads > 32767) || d->head_dim > 4096)
@@ -1059,6 +1169,9 @@ int frisk_rope(const frisk_rope_desc* d, void* stream) {
   a.pos_sb = d->pos_stride_b; a.pos_ss = d->pos_stride_s;
   a.start = d->start;
   a.freq = d->frequencies;
+  a.pair_axis = d->pair_axis;
+  a.axes = d->pair_axis ? (int)d->axes : 1;
+  a.pos_sa = d->pair_axis ? d->pos_stride_a : 0;
   clear_stale_error();
   const hipError_t e = frisk::rope(a, (hipStream_t)stream);
   if (e == hipErrorInvalidConfiguration)
@@ -1123,6 +1236,130 @@ int frisk_tree_mask(int64_t batch, int64_t tokens, const int32_t* parents, uint6
   clear_stale_error();
   const hipError_t e = frisk::tree_mask(batch, (int)tokens, parents, mask, depth, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "frisk_tree_mask launch");
+  return FRISK_OK;
+}
+
+int frisk_kv_compact(const frisk_kv_compact_desc* d, void* stream) {
+  const char* fn = "frisk_kv_compact";
+  g_last_error.clear();
+  if (!d) return fail(FRISK_EINVAL, "%s: null descriptor", fn);
+  if (d->batch <= 0 || d->tokens <= 0) return fail(FRISK_EINVAL, "%s: sizes must be positive", fn);
+  if (d->batch >= kMaxDim || d->tokens >= kMaxDim)
+    return fail(FRISK_EUNSUP, "%s: sizes beyond the kernels' index range", fn);
+  frisk::KvCompactArgs a;
+  const int rc = check_cache(d->cache, fn, true, d->batch, a.cache);
+  if (rc) return rc;
+  if (a.cache.scale_shift)
+    return fail(FRISK_EUNSUP, "%s: rows that share scales cannot move (append them again)", fn);
+  if (cache_tensors_share(d->cache, false) || (d->cache.k_scale && cache_tensors_share(d->cache, true)))
+    return fail(FRISK_EINVAL, "%s: k and v, and their scales, must be two tensors", fn);
+  if (!d->path || !d->ctx_len || !d->count) return fail(FRISK_EINVAL, "%s: null tensor", fn);
+  if ((uintptr_t)d->path % 4 || (uintptr_t)d->ctx_len % 4 || (uintptr_t)d->count % 4)
+    return fail(FRISK_EINVAL, "%s: path, ctx_len and count must be 4-byte aligned", fn);
+  if (d->path_stride < 0 || d->path_stride > kMaxStride)
+    return fail(FRISK_EINVAL, "%s: path_stride must be non-negative, up to 2^40", fn);
+  a.batch = d->batch;
+  a.tokens = (int)d->tokens;
+  a.path = d->path;
+  a.path_stride = d->path_stride;
+  a.ctx_len = d->ctx_len;
+  a.count = d->count;
+  clear_stale_error();
+  const hipError_t e = frisk::kv_compact(a, (hipStream_t)stream);
+  if (e == hipErrorInvalidConfiguration) return fail(FRISK_EUNSUP, "%s: more sequences than one launch takes", fn);
+  if (e != hipSuccess) return hip_fail(e, "frisk_kv_compact launch");
+  return FRISK_OK;
+}
+
+int frisk_kv_copy_pages(const frisk_kv_copy_pages_desc* d, void* stream) {
+  const char* fn = "frisk_kv_copy_pages";
+  g_last_error.clear();
+  if (!d) return fail(FRISK_EINVAL, "%s: null descriptor", fn);
+  if (d->pairs <= 0) return fail(FRISK_EINVAL, "%s: sizes must be positive", fn);
+  frisk::KvCopyPagesArgs a;
+  const int rc = check_cache(d->cache, fn, true, 1, a.cache);
+  if (rc) return rc;
+  if (cache_tensors_share(d->cache, false) || (d->cache.k_scale && cache_tensors_share(d->cache, true)))
+    return fail(FRISK_EINVAL, "%s: k and v, and their scales, must be two tensors", fn);
+  if (!d->src || !d->dst) return fail(FRISK_EINVAL, "%s: null tensor", fn);
+  if ((uintptr_t)d->src % 4 || (uintptr_t)d->dst % 4 || (uintptr_t)d->rows % 4)
+    return fail(FRISK_EINVAL, "%s: src, dst and rows must be 4-byte aligned", fn);
+  if (d->pairs >= kMaxDim) return fail(FRISK_EUNSUP, "%s: more pages than one launch takes", fn);
+  a.pairs = d->pairs;
+  a.src = d->src;
+  a.dst = d->dst;
+  a.rows = d->rows;
+  a.page_size = d->cache.page_size;
+  clear_stale_error();
+  const hipError_t e = frisk::kv_copy_pages(a, (hipStream_t)stream);
+  if (e == hipErrorInvalidConfiguration) return fail(FRISK_EUNSUP, "%s: more pages than one launch takes", fn);
+  if (e != hipSuccess) return hip_fail(e, "frisk_kv_copy_pages launch");
+  return FRISK_OK;
+}
+
+int frisk_kv_pages(const frisk_kv_pages_desc* d, void* stream) {
+  const char* fn = "frisk_kv_pages";
+  g_last_error.clear();
+  if (!d) return fail(FRISK_EINVAL, "%s: null descriptor", fn);
+  if (d->batch <= 0 || d->max_pages <= 0 || d->pages <= 0 || d->page_size <= 0)
+    return fail(FRISK_EINVAL, "%s: sizes must be positive", fn);
+  if (d->page_size & (d->page_size - 1))
+    return fail(FRISK_EINVAL, "%s: page_size must be a power of two (got %lld)", fn, (long long)d->page_size);
+  if (d->pages >= kMaxDim || d->batch >= kMaxDim || frisk::kv_pages_lds(d->batch, d->pages) > frisk::kMaxLds)
+    return fail(FRISK_EUNSUP, "%s: more pages and sequences than the kernel has memory for", fn);
+  if (d->page_size >= kMaxDim || d->max_pages > (kMaxDim - 1) / d->batch || d->max_pages > kMaxDim / d->page_size)
+    return fail(FRISK_EUNSUP, "%s: a table of 2^31 entries, or sequences of more than 2^31 keys", fn);
+  if (d->table_stride < 0 || d->table_stride > kMaxStride || d->out_stride < 0 || d->out_stride > kMaxStride ||
+      (d->batch > 1 && (d->table_stride < d->max_pages || d->out_stride < d->max_pages)))
+    return fail(FRISK_EINVAL, "%s: rows of table and out must be at least max_pages apart", fn);
+  if (!d->table || !d->out || !d->keep) return fail(FRISK_EINVAL, "%s: null tensor", fn);
+  if ((uintptr_t)d->table % 4 || (uintptr_t)d->out % 4 || (uintptr_t)d->parent % 4 || (uintptr_t)d->keep % 4 ||
+      (uintptr_t)d->want % 4 || (uintptr_t)d->src % 4 || (uintptr_t)d->dst % 4 || (uintptr_t)d->rows % 4 ||
+      (uintptr_t)d->lacking % 4)
+    return fail(FRISK_EINVAL, "%s: pointers must be element-aligned", fn);
+  const int64_t n = d->batch * 4;
+  auto table = [&](int64_t stride) { return ((d->batch - 1) * stride + d->max_pages) * 4; };
+  const Span out[] = {{d->out, table(d->out_stride)}, {d->src, n}, {d->dst, n}, {d->rows, n}, {d->lacking, 4}};
+  const Span in[] = {{d->table, table(d->table_stride)}, {d->parent, n}, {d->keep, n}, {d->want, n},
+                     {d->held, d->pages}};
+  if (outputs_overlap(out, in)) return fail(FRISK_EINVAL, "%s: an output overlaps another tensor", fn);
+  frisk::KvPagesArgs a;
+  a.batch = (int)d->batch;
+  a.max_pages = (int)d->max_pages;
+  a.pages = (int)d->pages;
+  a.page_shift = 0;
+  while (((int64_t)1 << a.page_shift) < d->page_size) ++a.page_shift;
+  a.table = d->table; a.table_stride = d->table_stride;
+  a.out = d->out; a.out_stride = d->out_stride;
+  a.parent = d->parent;
+  a.keep = d->keep;
+  a.want = d->want;
+  a.held = d->held;
+  a.src = d->src;
+  a.dst = d->dst;
+  a.rows = d->rows;
+  a.lacking = d->lacking;
+  clear_stale_error();
+  const hipError_t e = frisk::kv_pages(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "frisk_kv_pages launch");
+  return FRISK_OK;
+}
+
+int64_t frisk_tree_verify_workspace_size(const frisk_tree_verify_desc* d) {
+  g_last_error.clear();
+  frisk::VerifyArgs a;
+  const int rc = check_verify(d, false, a);
+  return rc ? rc : frisk::verify_workspace(a.batch, a.tokens, a.chunks);
+}
+
+int frisk_tree_verify(const frisk_tree_verify_desc* d, void* stream) {
+  g_last_error.clear();
+  frisk::VerifyArgs a;
+  const int rc = check_verify(d, true, a);
+  if (rc) return rc;
+  clear_stale_error();
+  const hipError_t e = frisk::tree_verify(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "frisk_tree_verify launch");
   return FRISK_OK;
 }
 

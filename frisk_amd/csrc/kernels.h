@@ -215,6 +215,9 @@ struct RopeArgs {
   int64_t pos_sb, pos_ss;
   const int32_t* start;  // null: 0
   const uint64_t* freq;
+  const uint8_t* pair_axis;  // null: one axis
+  int axes;                  // of positions, pos_sa apart
+  int64_t pos_sa;
 };
 hipError_t rope(const RopeArgs& a, hipStream_t s);
 
@@ -224,6 +227,7 @@ struct KvCache {
   Elt kind;  // BF16, F16, E4M3 or I8
   int pages, kv_heads, head_dim;
   int page_shift;    // log2 of the page size with a table
+  int scale_shift;   // log2 of the rows that share a scale
   int64_t capacity;  // keys a sequence holds
   void* k;
   void* v;
@@ -246,6 +250,8 @@ struct KvArgs {
   KvCache cache;
 };
 hipError_t kv_append(const KvArgs& a, hipStream_t s);
+// The append of an 8-bit cache whose rows share scales (kvblock.hip).
+hipError_t kv_append_blocks(const KvArgs& a, hipStream_t s);
 hipError_t kv_read(const KvArgs& a, hipStream_t s);
 hipError_t tree_mask(int64_t batch, int tokens, const int32_t* parents, uint64_t* mask,
                      int32_t* depth, hipStream_t s);
@@ -273,6 +279,71 @@ struct TreeAttnArgs {
   void* workspace;  // plan::tree_workspace bytes
 };
 hipError_t tree_attn(const TreeAttnArgs& a, hipStream_t s);
+
+// Pages of a cache (kvpages.hip).
+struct KvCompactArgs {
+  int64_t batch;
+  int tokens;  // of a path
+  const int32_t* path;
+  int64_t path_stride;
+  const int32_t* ctx_len;
+  const int32_t* count;
+  KvCache cache;
+};
+hipError_t kv_compact(const KvCompactArgs& a, hipStream_t s);
+struct KvCopyPagesArgs {
+  int64_t pairs;
+  const int32_t* src;
+  const int32_t* dst;
+  const int32_t* rows;  // null: all slots
+  int64_t page_size;
+  KvCache cache;
+};
+hipError_t kv_copy_pages(const KvCopyPagesArgs& a, hipStream_t s);
+struct KvPagesArgs {
+  int batch, max_pages, pages, page_shift;
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t* out;
+  int64_t out_stride;
+  const int32_t* parent;  // null: each row itself
+  const int32_t* keep;
+  const int32_t* want;  // null: keep
+  const uint8_t* held;  // null: none
+  int32_t* src;         // these four may be null
+  int32_t* dst;
+  int32_t* rows;
+  int32_t* lacking;
+};
+// Bytes of LDS that kv_pages takes, up to kMaxLds.
+constexpr int64_t kMaxLds = 160 * 1024;
+int64_t kv_pages_lds(int64_t batch, int64_t pages);
+hipError_t kv_pages(const KvPagesArgs& a, hipStream_t s);
+
+// Verification of drafted tokens (verify.hip).
+struct VerifyArgs {
+  Elt dtype;  // of the logits: F32, F16 or BF16
+  int64_t batch;
+  int tokens, vocab;
+  const void* logits;
+  int64_t sb, st;
+  const int32_t* drafts;
+  const int32_t* parents;
+  const float* uniform;
+  const float* final_uniform;
+  const float* draft_probs;  // null: drafts are certain
+  int64_t qb, qt;
+  const float* temperature;  // null: 1
+  const int32_t* new_len;    // null: tokens
+  int32_t* path;
+  int32_t* count;
+  int32_t* token;
+  float* probs;  // may be null
+  int pieces, chunks;  // plan::verify_plan
+  void* workspace;     // verify_workspace bytes
+};
+int64_t verify_workspace(int64_t batch, int64_t tokens, int64_t chunks);
+hipError_t tree_verify(const VerifyArgs& a, hipStream_t s);
 
 // MFMA fragment-layout probe (probe.hip): atom 0 = bf16 32x32x16,
 // 1 = bf16 16x16x32, 2 = i8 32x32x32; `out` holds mfma_probe_floats(atom)

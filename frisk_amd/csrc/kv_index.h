@@ -24,6 +24,13 @@ FRISK_INDEX Span span_of(const int32_t* ctx_len, const int32_t* new_len, int tok
   return {ctx_len[b], n};
 }
 
+// The scale of row `row` of a page: each one's own, or one for 2^scale_shift rows
+// (a Cache without that member has one for each).
+template <typename Cache> FRISK_INDEX auto scale_row(const Cache& c, int64_t row, int) -> decltype(c.scale_shift, int64_t()) {
+  return row >> c.scale_shift;
+}
+template <typename Cache> FRISK_INDEX int64_t scale_row(const Cache&, int64_t row, long) { return row; }
+
 // Element and scale offsets of one key's row of head 0; elem < 0: the cache
 // does not hold the key.
 struct Slot {
@@ -40,7 +47,7 @@ template <typename Cache> FRISK_INDEX Slot slot_of(const Cache& c, int64_t b, in
   const int page = page_of(c, b, n);
   if (page < 0) return {-1, -1};
   const int64_t row = c.table ? n & ((1ll << c.page_shift) - 1) : n;
-  return {page * c.sp + row * c.ss, page * c.scp + row * c.scs};
+  return {page * c.sp + row * c.ss, page * c.scp + scale_row(c, row, 0) * c.scs};
 }
 
 }  // namespace kv
@@ -84,7 +91,7 @@ FRISK_INDEX Place place_of(const Cache& c, int bytes, int64_t b, int kvh, int n,
   p.there = n < keys && page >= 0 && page < c.pages;
   const int64_t pg = p.there ? page : 0, sl = p.there ? slot : 0;
   p.row = (pg * c.sp + sl * c.ss + kvh * c.sh) * bytes;
-  p.scale = pg * c.scp + sl * c.scs + kvh * c.sch;
+  p.scale = pg * c.scp + kv::scale_row(c, sl, 0) * c.scs + kvh * c.sch;
   return p;
 }
 

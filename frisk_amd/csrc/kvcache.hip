@@ -207,7 +207,9 @@ __global__ __launch_bounds__(256) void tree_mask_kernel(int tokens, const int32_
 
 }  // namespace
 
-hipError_t kv_append(const KvArgs& a, hipStream_t s) { return kv_dispatch<true>(a, s); }
+hipError_t kv_append(const KvArgs& a, hipStream_t s) {
+  return a.cache.scale_shift ? kv_append_blocks(a, s) : kv_dispatch<true>(a, s);
+}
 hipError_t kv_read(const KvArgs& a, hipStream_t s) { return kv_dispatch<false>(a, s); }
 
 hipError_t tree_mask(int64_t batch, int tokens, const int32_t* parents, uint64_t* mask,

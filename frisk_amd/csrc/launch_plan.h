@@ -617,6 +617,22 @@ inline int64_t attn_workspace(int64_t batch_heads, int64_t seq_q, int64_t seq_k,
 }
 
 // ---------------------------------------------------------------------------
+// Verification of drafted tokens (verify.hip): nodes of a tree at most, and how a
+// row of `vocab` logits of `bytes` is cut into chunks of 256 threads with
+// `pieces` 16-B pieces each.
+constexpr int64_t kVerifyNodes = 1024;
+constexpr int64_t kVerifyVocab = 1 << 24;
+struct VerifyPlan {
+  int pieces;
+  int64_t chunks;
+};
+inline VerifyPlan verify_plan(int64_t batch, int64_t tokens, int64_t vocab, int bytes) {
+  const int64_t whole = std::max<int64_t>(vocab * bytes / 16, 1);
+  auto chunks = [&](int pieces) { return (whole + 256 * pieces - 1) / (256 * pieces); };
+  const int pieces = batch * tokens * chunks(4) >= 512 ? 4 : 1;
+  return {pieces, chunks(pieces)};
+}
+
 // Attention of new tokens over a cache (attn_tree_mfma.h, attn_tree_rows.hip).
 // Rows: one query row a workgroup, head dims without a matrix-core kernel.
 // Keys: a tile of 32 query rows of a kv head a workgroup, whose waves divide the

@@ -25,6 +25,8 @@ namespace frisk {
 
 namespace {
 
+constexpr int kRopeAxes = 4;  // most axes of positions
+
 struct SinCos {
   float s, c;
 };
@@ -70,7 +72,8 @@ template <Elt E, int P> __device__ __forceinline__ void put(typename Piece<E, P>
 // half; interleaved: a chunk is one piece of P / 2 pairs (P == 1: two pieces, one
 // pair).  A token has `pair_chunks` of those and `copy_chunks` pieces of dims to
 // copy, times `lanes` threads that share its heads.
-template <Elt E, int P, bool INTER, bool PAST_L2>
+// AXES: a pair's position is that of its axis.
+template <Elt E, int P, bool INTER, bool PAST_L2, bool AXES>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pair_chunks, int copy_chunks,
                                                    int lanes, int tokens_per_block,
                                                    int blocks_per_token) {
@@ -124,14 +127,26 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pair_chunks, 
     }
     return;
   }
-  int64_t p = a.start ? a.start[b] : 0;
-  if (!a.positions) p += s;
-  else if (a.position_bits == 64) p += ((const int64_t*)a.positions)[b * a.pos_sb + s * a.pos_ss];
-  else p += ((const int32_t*)a.positions)[b * a.pos_sb + s * a.pos_ss];
+  const int64_t start = a.start ? a.start[b] : 0, place = b * a.pos_sb + s * a.pos_ss;
+  auto position = [&](int64_t at) {
+    return start + (a.position_bits == 64 ? ((const int64_t*)a.positions)[at] : ((const int32_t*)a.positions)[at]);
+  };
+  int64_t p[AXES ? kRopeAxes : 1];
+  p[0] = a.positions ? position(place) : start + s;
+  if constexpr (AXES) {
+#pragma unroll
+    for (int x = 1; x < kRopeAxes; ++x) p[x] = x < a.axes ? position(place + x * a.pos_sa) : p[0];
+  }
   float cs[NP], sn[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const SinCos r = sincos_turns((uint64_t)p * a.freq[chunk * NP + i]);
+    int64_t mine = p[0];
+    if constexpr (AXES) {
+      const int axis = a.pair_axis[chunk * NP + i];
+#pragma unroll
+      for (int x = 1; x < kRopeAxes; ++x) mine = axis == x ? p[x] : mine;
+    }
+    const SinCos r = sincos_turns((uint64_t)mine * a.freq[chunk * NP + i]);
     cs[i] = r.c * a.amplitude;
     sn[i] = (a.backward ? -r.s : r.s) * a.amplitude;
   }
@@ -167,7 +182,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pair_chunks, 
   }
 }
 
-template <Elt E, int P, bool INTER>
+template <Elt E, int P, bool INTER, bool AXES>
 hipError_t launch_rope(const RopeArgs& a, hipStream_t stream) {
   constexpr int NP = INTER && P > 1 ? P / 2 : P, es = EltInfo<E>::bytes;
   const int heads = a.t[0].heads + a.t[1].heads;
@@ -189,9 +204,9 @@ hipError_t launch_rope(const RopeArgs& a, hipStream_t stream) {
   const int64_t run = INTER ? a.rot_dim : a.rot_dim / 2;  // elements that neighbouring lanes store
   const bool past_l2 = run * es % 128 == 0 && (a.head_dim - a.rot_dim) * es % 128 == 0 &&
                        tokens * heads * a.head_dim * es > (32ll << 20);
-  auto kern = rope_kernel<E, P, INTER, false>;
+  auto kern = rope_kernel<E, P, INTER, false, AXES>;
   if constexpr (P * es == 16)
-    if (past_l2) kern = rope_kernel<E, P, INTER, true>;
+    if (past_l2) kern = rope_kernel<E, P, INTER, true, AXES>;
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, a, pair_chunks, copy_chunks, lanes,
                      tpb, bpt);
   return hipGetLastError();
@@ -208,11 +223,15 @@ hipError_t rope_type(const RopeArgs& a, hipStream_t stream) {
     bits |= (uint64_t)t.sb | (uint64_t)t.sh | (uint64_t)t.ss | (uint64_t)t.osb | (uint64_t)t.osh |
             (uint64_t)t.oss | (uint64_t)t.x / es | (uint64_t)t.out / es;
   }
-  if constexpr (es == 2)
-    if (bits % 8 == 0) return launch_rope<E, 8, INTER>(a, stream);
-  if (bits % 4 == 0) return launch_rope<E, 4, INTER>(a, stream);
-  if (bits % 2 == 0) return launch_rope<E, 2, INTER>(a, stream);
-  return launch_rope<E, 1, INTER>(a, stream);
+  auto launch = [&](auto axes) {
+    constexpr bool AXES = decltype(axes)::value;
+    if constexpr (es == 2)
+      if (bits % 8 == 0) return launch_rope<E, 8, INTER, AXES>(a, stream);
+    if (bits % 4 == 0) return launch_rope<E, 4, INTER, AXES>(a, stream);
+    if (bits % 2 == 0) return launch_rope<E, 2, INTER, AXES>(a, stream);
+    return launch_rope<E, 1, INTER, AXES>(a, stream);
+  };
+  return a.pair_axis ? launch(std::true_type{}) : launch(std::false_type{});
 }
 
 }  // namespace

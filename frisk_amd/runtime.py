@@ -3,7 +3,8 @@
 This is the Python side of the C-ABI: it fills the descriptors from torch
 device tensors and calls frisk_gemm / frisk_attn_fwd / frisk_reduce /
 frisk_copy / frisk_fill, and frisk_rope / frisk_kv_append / frisk_kv_read /
-frisk_tree_mask / frisk_tree_attn, on the current HIP stream.  There is no fallback: if the library is missing or a call fails,
+frisk_tree_mask / frisk_tree_attn / frisk_tree_verify / frisk_kv_compact /
+frisk_kv_copy_pages / frisk_kv_pages, on the current HIP stream.  There is no fallback: if the library is missing or a call fails,
 a RuntimeError (or ValueError for rejected requests, matching the
 reference's ValueError on contract violations, ffi/ir.cpp:333-341) is raised.
 """
@@ -28,9 +29,11 @@ EXPORTS = ("frisk_gemm", "frisk_gemm_workspace_size", "frisk_gemm_plan", "frisk_
            "frisk_copy", "frisk_fill",
            "frisk_rope", "frisk_rope_frequencies", "frisk_kv_append", "frisk_kv_read",
            "frisk_tree_mask", "frisk_tree_attn", "frisk_tree_attn_workspace_size",
+           "frisk_kv_compact", "frisk_kv_copy_pages", "frisk_kv_pages",
+           "frisk_tree_verify", "frisk_tree_verify_workspace_size",
            "frisk_last_error", "frisk_abi_version", "frisk_probe_mfma_layout",
            "frisk_probe_lds_transpose")
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 REDUCE_SUM, REDUCE_MAX, REDUCE_MIN = 0, 1, 2
 REDUCE_KINDS = {"sum": REDUCE_SUM, "add": REDUCE_SUM, "max": REDUCE_MAX, "min": REDUCE_MIN}
@@ -115,6 +118,7 @@ class RopeDesc(ctypes.Structure):
         ("k", _ptr), *_strides("k", "bhs"), ("k_out", _ptr), *_strides("k_out", "bhs"),
         ("positions", _ptr), ("position_bits", _i32), *_strides("pos", "bs"),
         ("start", _ptr), ("frequencies", _ptr),
+        ("axes", _i64), ("pos_stride_a", _i64), ("pair_axis", _ptr),
     ]
 
 
@@ -125,7 +129,7 @@ class KvCacheDesc(ctypes.Structure):
         ("stride_page", _i64), ("stride_head", _i64), ("stride_slot", _i64),
         ("k_scale", _ptr), ("v_scale", _ptr),
         ("scale_stride_page", _i64), ("scale_stride_head", _i64), ("scale_stride_slot", _i64),
-        ("block_table", _ptr), ("table_stride", _i64), ("max_pages", _i64),
+        ("block_table", _ptr), ("table_stride", _i64), ("max_pages", _i64), ("scale_block", _i64),
     ]
 
 
@@ -143,6 +147,36 @@ class TreeAttnDesc(ctypes.Structure):
         ("sm_scale", ctypes.c_float), ("q", _ptr), *_strides("q", "bhs"),
         ("o", _ptr), *_strides("o", "bhs"), ("lse", _ptr), ("ctx_len", _ptr), ("new_len", _ptr),
         ("mask", _ptr), *_strides("mask", "bt"), ("max_ctx", _i64), ("cache", KvCacheDesc),
+        ("workspace", _ptr), ("workspace_bytes", _i64),
+    ]
+
+
+class KvCompactDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("tokens", _i64), ("path", _ptr), ("path_stride", _i64),
+        ("ctx_len", _ptr), ("count", _ptr), ("cache", KvCacheDesc),
+    ]
+
+
+class KvCopyPagesDesc(ctypes.Structure):
+    _fields_ = [("pairs", _i64), ("src", _ptr), ("dst", _ptr), ("rows", _ptr), ("cache", KvCacheDesc)]
+
+
+class KvPagesDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("max_pages", _i64), ("pages", _i64), ("page_size", _i64),
+        ("table", _ptr), ("table_stride", _i64), ("out", _ptr), ("out_stride", _i64),
+        *((n, _ptr) for n in ("parent", "keep", "want", "held", "src", "dst", "rows", "lacking")),
+    ]
+
+
+class TreeVerifyDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("tokens", _i64), ("vocab", _i64), ("dtype", _i32),
+        ("logits", _ptr), ("stride_b", _i64), ("stride_t", _i64),
+        *((n, _ptr) for n in ("drafts", "parents", "uniform", "final_uniform", "draft_probs")),
+        ("draft_stride_b", _i64), ("draft_stride_t", _i64),
+        *((n, _ptr) for n in ("temperature", "new_len", "path", "count", "token", "probs")),
         ("workspace", _ptr), ("workspace_bytes", _i64),
     ]
 
@@ -197,6 +231,12 @@ def load() -> ctypes.CDLL:
     lib.frisk_tree_attn.restype = ctypes.c_int
     lib.frisk_tree_attn_workspace_size.argtypes = [ctypes.POINTER(TreeAttnDesc)]
     lib.frisk_tree_attn_workspace_size.restype = ctypes.c_int64
+    for fn, desc in ((lib.frisk_kv_compact, KvCompactDesc), (lib.frisk_kv_copy_pages, KvCopyPagesDesc),
+                     (lib.frisk_kv_pages, KvPagesDesc), (lib.frisk_tree_verify, TreeVerifyDesc)):
+        fn.argtypes = [ctypes.POINTER(desc), ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+    lib.frisk_tree_verify_workspace_size.argtypes = [ctypes.POINTER(TreeVerifyDesc)]
+    lib.frisk_tree_verify_workspace_size.restype = ctypes.c_int64
     lib.frisk_last_error.argtypes = []
     lib.frisk_last_error.restype = ctypes.c_char_p
     lib.frisk_abi_version.argtypes = []
@@ -579,6 +619,21 @@ def rope_table(rot_dim, base=10000.0, *, scaling="none", factor=1.0, trained=0.0
     return torch.tensor([v - (1 << 64) if v >> 63 else v for v in buf], dtype=torch.int64).to(device)
 
 
+def rope_axes(sections, *, interleaved=False, device="cuda"):
+    """The uint8 [rot_dim / 2] axes of pairs that rope() takes with positions of
+    several axes: sections[a] pairs turn by axis a's position, axis after axis,
+    or, if `interleaved`, in turn (an axis drops out when its pairs are dealt)."""
+    import torch
+    sections = [int(n) for n in sections]
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) < 1:
+        raise ValueError(f"sections are the pairs of 1 to 4 axes (got {sections})")
+    if interleaved:
+        out = [a for i in range(max(sections)) for a, n in enumerate(sections) if i < n]
+    else:
+        out = [a for a, n in enumerate(sections) for _ in range(n)]
+    return torch.tensor(out, dtype=torch.uint8).to(device)
+
+
 # The calls below fill their descriptors with struct.pack, which takes a fifth
 # of the time of a ctypes.Structure's fields (a decode step's launches are short).
 
@@ -598,6 +653,10 @@ def _packer(cls, until=None):
 _rope_pack = _packer(RopeDesc)
 _kv_pack = _packer(KvDesc, "cache")
 _tree_pack = _packer(TreeAttnDesc, "cache")
+_compact_pack = _packer(KvCompactDesc, "cache")
+_copy_pages_pack = _packer(KvCopyPagesDesc, "cache")
+_pages_pack = _packer(KvPagesDesc)
+_verify_pack = _packer(TreeVerifyDesc, "workspace")
 _ws_pack = struct.Struct("@Pq")
 
 
@@ -680,15 +739,17 @@ def _run(name: str, desc: bytes, dev: int, stream):
         _check(rc, name)
 
 
-def rope(x, out, positions, table, *, k=None, k_out=None, start=None, interleaved=False,
-         amplitude=1.0, backward=False, stream=None):
+def rope(x, out, positions, table, *, k=None, k_out=None, start=None, pair_axis=None,
+         interleaved=False, amplitude=1.0, backward=False, stream=None):
     """out = x [batch, heads, seq, head_dim] with its first 2 * len(table) dims
     rotated to their positions, and k_out = k (its own number of heads)
     likewise, in one launch.  out may be x.  `positions` (int32 or int64,
     [seq] or [batch, seq], or None: 0 .. seq - 1) are counted from `start`
-    (int32 [batch], or None: 0).  Pairs are dims (i, i + rot_dim / 2), or
-    (2i, 2i + 1) if `interleaved`.  backward=True is the gradient: the
-    transposed rotation."""
+    (int32 [batch], or None: 0).  With `pair_axis` (uint8 [len(table)],
+    rope_axes) they have 1 to 4 axes, [axes, seq] or [axes, batch, seq], and
+    pair i turns by that of axis pair_axis[i].  Pairs are dims (i, i +
+    rot_dim / 2), or (2i, 2i + 1) if `interleaved`.  backward=True is the
+    gradient: the transposed rotation."""
     import torch
     (b, h, s, d), xs = _heads(x, "x")
     osh, outs = _heads(out, "out")
@@ -705,20 +766,30 @@ def rope(x, out, positions, table, *, k=None, k_out=None, start=None, interleave
         if (kb, ks_, kd) != (b, s, d) or kosh != k.shape or k.dtype != x.dtype or k_out.dtype != x.dtype:
             raise ValueError("k and k_out must have one shape, and x's dtype, batch, seq and head_dim")
         second = (k.data_ptr(), ks[0], ks[1], ks[2], k_out.data_ptr(), kos[0], kos[1], kos[2])
-    at = (0, 0, 0, 0)
+    at, axes = (0, 0, 0, 0), (0, 0, 0)
     if positions is not None:
         bits = 64 if positions.dtype == torch.int64 else 32
-        if (bits == 32 and positions.dtype != torch.int32) or positions.shape not in ((s,), (b, s)):
+        shape, st = positions.shape, positions.stride()
+        if pair_axis is not None:
+            if pair_axis.dtype != torch.uint8 or pair_axis.shape != table.shape or \
+                    not pair_axis.is_contiguous():
+                raise ValueError(f"pair_axis must be a contiguous uint8 device tensor [{table.shape[0]}] (rope_axes)")
+            if len(shape) not in (2, 3):
+                raise ValueError("with pair_axis positions are [axes, seq] or [axes, batch, seq]")
+            axes = (shape[0], st[0], pair_axis.data_ptr())
+            shape, st = shape[1:], st[1:]
+        if (bits == 32 and positions.dtype != torch.int32) or shape not in ((s,), (b, s)):
             raise ValueError("positions must be an int32 or int64 device tensor [seq] or [batch, seq]")
-        st = positions.stride()
         at = (positions.data_ptr(), bits, *((0, st[0]) if len(st) == 1 else st))
-    dev = _same_device(x, out, k, k_out, positions, table, start)
+    elif pair_axis is not None:
+        raise ValueError("pair_axis needs positions")
+    dev = _same_device(x, out, k, k_out, positions, table, start, pair_axis)
     start = _lengths(start, b, "start")
     try:
         desc = _rope_pack.pack(b, s, h, kh, d, 2 * table.shape[0], torch_dtype_code(x.dtype),
                                bool(interleaved), bool(backward), amplitude,
                                x.data_ptr(), xs[0], xs[1], xs[2], out.data_ptr(), outs[0], outs[1], outs[2],
-                               *second, *at, start, table.data_ptr())
+                               *second, *at, start, table.data_ptr(), *axes)
     except _RANGE as e:
         raise _range_error(e) from None
     _run("frisk_rope", desc, dev, stream)
@@ -729,12 +800,14 @@ class KvCache:
     """A cache of keys and values (frisk_kv_cache) over tensors the caller
     owns: k and v [pages, kv_heads, page_size, head_dim] of one layout, in
     bf16 / f16, or in float8_e4m3fn / int8 with f32 k_scale and v_scale
-    [pages, kv_heads, page_size].  `block_table` (int32 [batch, max_pages])
+    [pages, kv_heads, page_size].  With `scale_block` (a power of two, 2 to
+    256) that many slots share a scale, and the scales are [pages, kv_heads,
+    ceil(page_size / scale_block)].  `block_table` (int32 [batch, max_pages])
     names the pages of each sequence; without it page b is sequence b's."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "block_table", "desc", "_packed", "_device")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "block_table", "scale_block", "desc", "_packed", "_device")
 
-    def __init__(self, k, v, k_scale=None, v_scale=None, block_table=None):
+    def __init__(self, k, v, k_scale=None, v_scale=None, block_table=None, *, scale_block=1):
         import torch
         ksh, kst = _heads(k, "k")
         vsh, vst = _heads(v, "v")
@@ -745,10 +818,14 @@ class KvCache:
         if (k_scale is None) != (k.element_size() == 2) or (v_scale is None) != (k_scale is None):
             raise ValueError("an 8-bit cache has k_scale and v_scale, a 16-bit one none")
         sst = (0, 0, 0)
+        if scale_block < 1 or (scale_block > 1 and k_scale is None):
+            raise ValueError(f"scale_block must be 1 or more, and is for 8-bit caches (got {scale_block})")
         if k_scale is not None:
+            shape = (ksh[0], ksh[1], -(-ksh[2] // scale_block))
             for t in (k_scale, v_scale):
-                if t.dtype != torch.float32 or tuple(t.shape) != tuple(ksh[:3]) or not t.is_cuda:
-                    raise ValueError("scales must be f32 device tensors [pages, kv_heads, page_size]")
+                if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_cuda:
+                    raise ValueError(f"scales must be f32 device tensors {list(shape)}: [pages, kv_heads, "
+                                     f"page_size], or one for scale_block slots")
             sst = k_scale.stride()
             if v_scale.stride() != sst:
                 raise ValueError("k_scale and v_scale must have one layout")
@@ -759,25 +836,28 @@ class KvCache:
                              "stride along the pages")
         self._device = _same_device(k, v, k_scale, v_scale, block_table)
         self.k, self.v, self.k_scale, self.v_scale, self.block_table = k, v, k_scale, v_scale, block_table
+        self.scale_block = scale_block
         self.desc = KvCacheDesc(
             *ksh, torch_dtype_code(k.dtype), k.data_ptr(), v.data_ptr(), *kst[:3],
             None if k_scale is None else k_scale.data_ptr(),
             None if v_scale is None else v_scale.data_ptr(), *sst,
             None if block_table is None else block_table.data_ptr(),
             0 if block_table is None else block_table.stride(0),
-            0 if block_table is None else block_table.shape[1])
+            0 if block_table is None else block_table.shape[1], scale_block)
         self._packed = bytes(self.desc)
 
     @classmethod
-    def empty(cls, pages, kv_heads, page_size, head_dim, dtype, *, block_table=None, device="cuda"):
+    def empty(cls, pages, kv_heads, page_size, head_dim, dtype, *, block_table=None, scale_block=1,
+              device="cuda"):
         """A cache over new tensors (their contents undefined until written)."""
         import torch
         shape = (pages, kv_heads, page_size, head_dim)
         k, v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
         ks = vs = None
         if k.element_size() == 1:
-            ks, vs = (torch.empty(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
-        return cls(k, v, ks, vs, block_table)
+            scales = (pages, kv_heads, -(-page_size // scale_block))
+            ks, vs = (torch.empty(scales, dtype=torch.float32, device=device) for _ in range(2))
+        return cls(k, v, ks, vs, block_table, scale_block=scale_block)
 
     def __setattr__(self, name, value):
         # The calls take the descriptor that __init__ packed.
@@ -813,7 +893,9 @@ def kv_append(k, v, cache, ctx_len, *, new_len=None, stream=None):
     """Write k and v [batch, kv_heads, tokens, head_dim] (bf16 or f16) into the
     KvCache as keys ctx_len[b] .. of each sequence (int32 [batch] on the
     device; negative: the sequence takes no part), the first new_len[b]
-    tokens of it.  An 8-bit cache quantises each row by its largest value."""
+    tokens of it.  An 8-bit cache quantises each row by its largest value, or
+    a block's rows by theirs: a block's scale grows with its rows, and the codes
+    before them follow (frisk_kv_append)."""
     _kv("frisk_kv_append", k, v, cache, ctx_len, new_len, stream)
     return cache
 
@@ -824,6 +906,77 @@ def kv_read(cache, k, v, ctx_len, *, new_len=None, stream=None):
     rows are left as they were."""
     _kv("frisk_kv_read", k, v, cache, ctx_len, new_len, stream)
     return k, v
+
+
+def kv_compact(cache, path, ctx_len, count, *, stream=None):
+    """Move the rows of an accepted branch behind its context: key ctx_len[b] + i
+    becomes the one that was ctx_len[b] + path[b, i], for i < count[b] (path
+    int32 [batch, tokens] and count int32 [batch] of tree_verify, on the device;
+    ctx_len negative: the sequence takes no part).  Not for a cache with
+    scale_block, whose rows are appended again instead."""
+    import torch
+    if path.dtype != torch.int32 or path.dim() != 2 or not path.is_cuda or \
+            (path.stride(1) != 1 and path.shape[1] > 1):
+        raise ValueError("path must be an int32 device tensor [batch, tokens] with unit stride along the tokens")
+    b, t = path.shape
+    dev = cache._check(b, path, ctx_len, count)
+    desc = _compact_pack.pack(b, t, path.data_ptr(), path.stride(0) if b > 1 else t,
+                              _lengths(ctx_len, b, "ctx_len"), _lengths(count, b, "count"))
+    _run("frisk_kv_compact", desc + cache._packed, dev, stream)
+    return cache
+
+
+def kv_copy_pages(cache, src, dst, *, rows=None, stream=None):
+    """Copy pages src[i] of the cache to pages dst[i] (int32 [pairs] on the device;
+    a pair with a page outside the cache is left out), the first rows[i] slots
+    of them (None: all).  No page is copied to twice, or copied to and from."""
+    n = src.shape[0] if src.dim() == 1 else 0
+    dev = _same_device(cache.k, src, dst, rows)
+    desc = _copy_pages_pack.pack(n, _lengths(src, n, "src"), _lengths(dst, n, "dst"), _lengths(rows, n, "rows"))
+    _run("frisk_kv_copy_pages", desc + cache._packed, dev, stream)
+    return cache
+
+
+def kv_pages(table, keep, want, page_size, pages, *, parent=None, held=None, out=None, src=None, dst=None,
+             rows=None, lacking=None, stream=None):
+    """(out, src, dst, rows, lacking): the block table of the next step, from `table`
+    (int32 [batch, max_pages]) of a cache of `pages` pages.  Row b takes over the pages of the first
+    keep[b] keys of row parent[b] (None: its own; outside the batch: sequence b has ended, and its
+    pages are free) and has room for want[b] keys (None: keep[b]).  Sequences share whole
+    pages; one that would write a shared page gets a copy of it: page dst[b]
+    of src[b], the first rows[b] slots (-1, -1, 0: none), which kv_copy_pages makes in every
+    layer's cache.  New pages are the lowest-numbered ones that no row has and that
+    `held` (uint8 or bool [pages]) does not keep back; lacking[0] counts the entries
+    that are -1 because there were too few.  keep, want, parent, src, dst, rows: int32
+    [batch]; lacking: int32 [1].  `out` must be another tensor than `table`; a program with one table
+    copies it back."""
+    import torch
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_cuda or \
+            (table.stride(1) != 1 and table.shape[1] > 1):
+        raise ValueError("table must be an int32 device tensor [batch, max_pages] with unit stride along the pages")
+    b, n = table.shape
+    if out is None:
+        out = _empty((b, n), torch.int32, table.device, stream)
+    elif out.dtype != torch.int32 or out.shape != table.shape or (out.stride(1) != 1 and n > 1):
+        raise ValueError(f"out must be an int32 tensor [{b}, {n}] with unit stride along the pages")
+    if held is not None and (held.dtype not in (torch.uint8, torch.bool) or held.shape != (pages,) or
+                             not held.is_contiguous()):
+        raise ValueError(f"held must be a contiguous uint8 or bool device tensor [{pages}]")
+    src, dst, rows = (_empty((b,), torch.int32, table.device, stream) if x is None else x
+                      for x in (src, dst, rows))
+    if lacking is None:
+        lacking = _empty((1,), torch.int32, table.device, stream)
+    dev = _same_device(table, out, keep, want, parent, held, src, dst, rows, lacking)
+    try:
+        desc = _pages_pack.pack(
+            b, n, pages, page_size, table.data_ptr(), table.stride(0) if b > 1 else n, out.data_ptr(),
+            out.stride(0) if b > 1 else n, _lengths(parent, b, "parent"), _lengths(keep, b, "keep"),
+            _lengths(want, b, "want"), 0 if held is None else held.data_ptr(), _lengths(src, b, "src"),
+            _lengths(dst, b, "dst"), _lengths(rows, b, "rows"), _lengths(lacking, 1, "lacking"))
+    except _RANGE as e:
+        raise _range_error(e) from None
+    _run("frisk_kv_pages", desc, dev, stream)
+    return out, src, dst, rows, lacking
 
 
 def tree_mask(parents, mask=None, depth=None, *, stream=None):
@@ -932,3 +1085,96 @@ def tree_attn(q, cache, ctx_len, o, *, mask=None, new_len=None, sm_scale=None, l
     if rc:
         _check(rc, "frisk_tree_attn")
     return o
+
+
+def _words(t, shape, dtype, name: str) -> int:
+    """The pointer of a contiguous device tensor of that shape and dtype, or 0."""
+    if t is None:
+        return 0
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"{name} must be a contiguous {dtype} device tensor {list(shape)}")
+    return t.data_ptr()
+
+
+def _vocab(t, shape, name: str):
+    """Strides of a [batch, tokens, vocab] device tensor."""
+    st = t.stride()
+    if t.shape != shape or not t.is_cuda or (st[2] != 1 and shape[2] > 1):
+        raise ValueError(f"{name} must be a device tensor {list(shape)} with unit stride along the vocabulary")
+    return st
+
+
+def tree_verify(logits, drafts, parents, uniform, final, *, draft_probs=None, temperature=None, new_len=None,
+                path=None, count=None, token=None, probs=None, workspace=True, stream=None):
+    """(path, count, token): which drafted tokens of each tree the target accepts, and
+    the token after them.  Node 0 of a tree is the last token that is decided, node
+    t the draft drafts[b, t] (int32 [batch, tokens]) that continues node parents[b, t] (int32,
+    tree_mask's); logits [batch, tokens, vocab] (f32, f16 or bf16) are the target's behind
+    each node, at `temperature` (f32 [batch], None: 1, 0: the largest logit).  uniform
+    (f32 [batch, tokens]) decides about each draft, final (f32 [batch]) draws the last
+    token; both are of [0, 1).  draft_probs (f32 [batch, tokens, vocab]): row n holds the
+    probabilities that node n's children were drawn from; None: drafts are certain
+    ones.  With one node a tree this samples from its logits.
+    path (int32 [batch, tokens]) lists the accepted nodes from 0 on, then -1, count (int32 [batch])
+    their number, token (int32 [batch]) is -1 where logits hold a NaN or +infinity; probs (f32 [batch, tokens],
+    optional) takes the target's probability of each draft.  Trees have new_len[b]
+    nodes (int32 [batch], None: all; 0: left as they were).  Frees no page and
+    moves no row: kv_compact and kv_pages do.
+    `workspace`: True allocates it (torch's caching allocator, on the call's
+    stream), a device tensor of tree_verify_workspace_bytes supplies it."""
+    import torch
+    if logits.dim() != 3:
+        raise ValueError("logits must be a device tensor [batch, tokens, vocab]")
+    b, t, v = shape = logits.shape
+    ls = _vocab(logits, shape, "logits")
+    qs = (0, 0)
+    if draft_probs is not None:
+        if draft_probs.dtype != torch.float32:
+            raise ValueError("draft_probs must be f32")
+        qs = _vocab(draft_probs, shape, "draft_probs")
+    handle = _current(logits.get_device(), stream)
+    if handle is None:
+        with torch.cuda.device(logits.get_device()):
+            return tree_verify(logits, drafts, parents, uniform, final, draft_probs=draft_probs,
+                               temperature=temperature, new_len=new_len, path=path, count=count, token=token,
+                               probs=probs, workspace=workspace, stream=stream)
+    if path is None:
+        path = _empty((b, t), torch.int32, logits.device, stream)
+    if count is None:
+        count = _empty((b,), torch.int32, logits.device, stream)
+    if token is None:
+        token = _empty((b,), torch.int32, logits.device, stream)
+    dev = _same_device(logits, drafts, parents, uniform, final, draft_probs, temperature, new_len, path, count,
+                       token, probs)
+    i32, f32 = torch.int32, torch.float32
+    try:
+        head = _verify_pack.pack(
+            b, t, v, torch_dtype_code(logits.dtype), logits.data_ptr(), ls[0], ls[1],
+            _words(drafts, (b, t), i32, "drafts"), _words(parents, (b, t), i32, "parents"),
+            _words(uniform, (b, t), f32, "uniform"), _words(final, (b,), f32, "final"),
+            0 if draft_probs is None else draft_probs.data_ptr(), qs[0], qs[1],
+            _words(temperature, (b,), f32, "temperature"), _lengths(new_len, b, "new_len"),
+            _words(path, (b, t), i32, "path"), _words(count, (b,), i32, "count"),
+            _words(token, (b,), i32, "token"), _words(probs, (b, t), f32, "probs"))
+    except _RANGE as e:
+        raise _range_error(e) from None
+    if workspace is True:
+        need = _raw_fn("frisk_tree_verify_workspace_size")(head + bytes(16))
+        if need < 0:
+            _check(need, "frisk_tree_verify_workspace_size")
+        workspace = _scratch(need, logits.device, stream)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on the logits' device")
+    tail = _ws_pack.pack(workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    rc = _raw_fn("frisk_tree_verify")(head + tail, handle)
+    if rc:
+        _check(rc, "frisk_tree_verify")
+    return path, count, token
+
+
+def tree_verify_workspace_bytes(batch: int, tokens: int, vocab: int, dtype) -> int:
+    """Bytes of workspace that tree_verify takes for logits [batch, tokens, vocab] of a torch dtype."""
+    d = TreeVerifyDesc(batch=batch, tokens=tokens, vocab=vocab, dtype=torch_dtype_code(dtype))
+    need = int(load().frisk_tree_verify_workspace_size(ctypes.byref(d)))
+    _check(need if need < 0 else OK, "frisk_tree_verify_workspace_size")
+    return need

@@ -51,7 +51,7 @@
 extern "C" {
 #endif
 
-#define FRISK_ABI_VERSION 8
+#define FRISK_ABI_VERSION 9
 
 /* Element types (the dtype strings of ffi/ir.cpp:399-411 plus bf16/i8/i32). */
 typedef enum frisk_dtype {
@@ -358,6 +358,10 @@ int frisk_fill(const frisk_fill_desc* desc, void* stream);
  * apart where they lie between each other, others by the ranges they reach.  The position of row (b, s) is
  * start[b] (0 if start is NULL) + positions[b * pos_stride_b + s *
  * pos_stride_s] (s if positions is NULL).
+ * Positions of several axes (time, height and width of an image's or a video's
+ * tokens): with pair_axis (device) a row has a position on each of `axes` (1 to
+ * 4) axes, pos_stride_a apart in positions, and pair i turns by that of
+ * axis pair_axis[i]; an axis outside 0 .. axes - 1 counts as 0.
  */
 typedef struct frisk_rope_desc {
   int64_t batch, seq, heads, k_heads, head_dim, rot_dim;
@@ -377,6 +381,8 @@ typedef struct frisk_rope_desc {
   int64_t pos_stride_b, pos_stride_s;
   const int32_t* start; /* optional, [batch] */
   const uint64_t* frequencies;
+  int64_t axes, pos_stride_a; /* with pair_axis */
+  const uint8_t* pair_axis;   /* optional, [rot_dim / 2] */
 } frisk_rope_desc;
 
 int frisk_rope(const frisk_rope_desc* desc, void* stream);
@@ -414,6 +420,9 @@ int frisk_rope_frequencies(int64_t rot_dim, double base, int32_t scaling, double
  * NaN makes the o of tokens that see it NaN, not their lse).  Attention may take
  * the product of a weight and a value's scale as 0 below 2^-126, and sums in f32
  * values up to 256 times as large as they are: beyond 2^119 they may overflow.
+ * With scale_block = 2^s above 1 (up to 256; with a table at most page_size) the
+ * rows of 2^s slots share a scale: k_scale and v_scale are [pages, kv_heads,
+ * ceil(page_size / scale_block)], and slot i's is entry i / scale_block.
  * Key n of sequence b is slot n % page_size of page block_table[b *
  * table_stride + n / page_size] (page_size a power of two), or without a
  * table slot n of page b; a sequence holds capacity = max_pages * page_size
@@ -433,6 +442,7 @@ typedef struct frisk_kv_cache {
   int64_t scale_stride_page, scale_stride_head, scale_stride_slot;
   const int32_t* block_table; /* optional */
   int64_t table_stride, max_pages;
+  int64_t scale_block; /* slots that share a scale; 0 or 1: each has its own */
 } frisk_kv_cache;
 
 /*
@@ -448,6 +458,13 @@ typedef struct frisk_kv_cache {
  * held at least 2^-126 Q, scale = a / Q, code = x Q / a rounded to nearest
  * even.  A row that holds an infinity or a NaN has scale NaN and codes 0: it
  * reads back as NaN.  A 16-bit cache takes and gives its own dtype.
+ * Slots that share a scale (scale_block): a block that takes new rows x has, from
+ * the largest |x| of those, a and scale as above, or the scale s that it had if
+ * that is larger and the block holds keys before ctx_len[b]; a code is x (1 /
+ * scale), both f32, rounded to nearest even.  Where the scale grows the codes c of
+ * those keys become c (s (1 / scale)), in f32, rounded likewise.  An infinity or
+ * NaN makes the block's scale NaN, and all of its keys read back as NaN.
+ * What the block holds behind the new rows has no meaning afterwards.
  * Pages written by one call must be distinct between its sequences, and k, v
  * and the cache four tensors (six with the scales) that share no memory.
  */
@@ -519,6 +536,131 @@ typedef struct frisk_tree_attn_desc {
 
 int frisk_tree_attn(const frisk_tree_attn_desc* desc, void* stream);
 int64_t frisk_tree_attn_workspace_size(const frisk_tree_attn_desc* desc);
+
+/*
+ * Pages of a cache.
+ *
+ * frisk_kv_compact moves the rows of an accepted branch (frisk_tree_verify's path
+ * and count) behind the context they continue: for i = 0 .. count[b] - 1 in order,
+ * key ctx_len[b] + i becomes the key that was ctx_len[b] + path[b][i].  path [batch,
+ * tokens] (row stride path_stride) holds rising draft numbers; an entry
+ * below its place i ends the path.  count[b] is held in 0 .. tokens; ctx_len[b] < 0:
+ * the sequence takes no part.  A key that the cache does not hold is not moved,
+ * nor moved to.  Rows keep their bits; a cache whose slots share scales (scale_block)
+ * is FRISK_EUNSUP (append the rows again).
+ */
+typedef struct frisk_kv_compact_desc {
+  int64_t batch, tokens;
+  const int32_t* path;
+  int64_t path_stride;
+  const int32_t* ctx_len; /* [batch] */
+  const int32_t* count;   /* [batch] */
+  frisk_kv_cache cache;
+} frisk_kv_compact_desc;
+
+int frisk_kv_compact(const frisk_kv_compact_desc* desc, void* stream);
+
+/* Copies pages src[i] to dst[i] (i < pairs): k, v and their scales, the first
+ * rows[i] slots (all, if rows is NULL; with scale_block the scales of the blocks that
+ * these lie in); the other slots are left as they were.  A pair with a page outside 0 .. pages
+ * - 1 is left out.  Pages copied to must be distinct, and none is copied from. */
+typedef struct frisk_kv_copy_pages_desc {
+  int64_t pairs;
+  const int32_t* src; /* [pairs] */
+  const int32_t* dst;
+  const int32_t* rows; /* optional, [pairs] */
+  frisk_kv_cache cache;
+} frisk_kv_copy_pages_desc;
+
+int frisk_kv_copy_pages(const frisk_kv_copy_pages_desc* desc, void* stream);
+
+/*
+ * The block table of the next step: sequences fork, end, go back and grow.  Row b of
+ * `out` continues row parent[b] (its own, if parent is NULL; one outside 0 .. batch - 1:
+ * sequence b has ended, its row holds no page): it takes over the pages of that
+ * row's first keep[b] keys and has room for want[b] (keep[b], if less, or if want is
+ * NULL); both are held in 0 .. max_pages * page_size (keep[b] < 0: the sequence has
+ * ended).  Several rows may take over a page.  A last page that is not full,
+ * where a row's next keys go, must be its own: where others take that page over in
+ * full, or it is held, the row gets a copy, a new page; where several rows would
+ * write it, all but the first do.  src[b], dst[b] and rows[b] are that copy's pages and its keys
+ * (frisk_kv_copy_pages makes it, for every layer's cache), or -1, -1 and 0.  Every entry with
+ * room that has no page gets a new one: in the order of rows and places, the lowest
+ * numbers that no row takes over and that are not held (held, optional: [pages] bytes,
+ * not 0: a page that is in use elsewhere).  If they do not suffice the last entries
+ * are -1 and lacking[0] says how many.  Entries behind the room are -1.  A page
+ * that no row has is free: there is no other state.
+ * table and out are [batch, max_pages], row strides at least that, and share no memory; lengths
+ * and outputs are device arrays.  page_size is a power of two.  FRISK_EUNSUP beyond the kernel's
+ * memory: pages / 4 + 8 batch bytes up to 155 KB.
+ */
+typedef struct frisk_kv_pages_desc {
+  int64_t batch, max_pages, pages, page_size;
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t* out;
+  int64_t out_stride;
+  const int32_t* parent; /* optional, [batch] */
+  const int32_t* keep;   /* [batch] */
+  const int32_t* want;   /* optional, [batch] */
+  const uint8_t* held;   /* optional, [pages] */
+  int32_t* src;          /* optional, [batch], as the next two */
+  int32_t* dst;
+  int32_t* rows;
+  int32_t* lacking; /* optional, [1] */
+} frisk_kv_pages_desc;
+
+int frisk_kv_pages(const frisk_kv_pages_desc* desc, void* stream);
+
+/*
+ * Verification of drafted tokens.  A tree's node 0 is a token that is decided (the
+ * last one of the step before); node t > 0 is the draft drafts[b][t] that continues
+ * node parents[b][t] < t (others are never reached).  logits[b][t] (f32, f16 or bf16
+ * [batch, tokens, vocab], unit stride along the vocabulary) are the target's behind node t,
+ * p = softmax(logits / temperature[b]) (1, if NULL; 0 or below: the first largest logit has p = 1).
+ *
+ * From node 0 on, a node's children are tried in order: with a = p, child t with
+ * token x is accepted, and the walk goes on from it, if
+ *   uniform[b][t] q(x) < a(x);
+ * else a becomes max(a - q, 0) over its sum (and stays if that is 0).  q is draft_probs[b][node]
+ * (f32 [batch, tokens, vocab], finite and at least 0), from which all of the node's children were drawn, or,
+ * if NULL, certain drafts: q(x) = 1 for the child's own token.  When no child is
+ * left, token[b] is the first v at which a summed over 0 .. v passes final_uniform[b]
+ * times its whole sum.  Random numbers are of [0, 1).  Probabilities are computed in 64 bits.
+ *
+ * path[b] ([tokens]) lists the nodes of the walk, node 0 first, then -1; count[b] is their
+ * number.  probs[b][t] (optional) is p of a node's token given its parent, 0 for nodes without
+ * one.  A row with a NaN, with +infinity or without a logit above -infinity gives no
+ * probabilities (probs NaN): the walk ends there and token[b] is -1.  A draft outside the vocabulary
+ * is never accepted.  Only the first new_len[b] nodes take part (all, if NULL; below 1: the tree's
+ * outputs are left as they were).  drafts, parents, uniform, path and probs are contiguous [batch, tokens],
+ * final_uniform, temperature, new_len, count and token [batch].  tokens <= 1024, vocab <= 2^24.
+ * workspace (16-byte aligned): at least frisk_tree_verify_workspace_size bytes; its contents before
+ * a call do not matter, and calls that share one must not overlap in time.  No output overlaps another tensor.
+ */
+typedef struct frisk_tree_verify_desc {
+  int64_t batch, tokens, vocab;
+  int32_t dtype; /* frisk_dtype of the logits */
+  const void* logits;
+  int64_t stride_b, stride_t;
+  const int32_t* drafts;
+  const int32_t* parents;
+  const float* uniform;
+  const float* final_uniform;
+  const float* draft_probs; /* optional */
+  int64_t draft_stride_b, draft_stride_t;
+  const float* temperature; /* optional */
+  const int32_t* new_len;   /* optional */
+  int32_t* path;
+  int32_t* count;
+  int32_t* token;
+  float* probs; /* optional */
+  void* workspace;
+  int64_t workspace_bytes;
+} frisk_tree_verify_desc;
+
+int frisk_tree_verify(const frisk_tree_verify_desc* desc, void* stream);
+int64_t frisk_tree_verify_workspace_size(const frisk_tree_verify_desc* desc);
 
 /* Description of the last failure on the calling thread ("" if none). */
 const char* frisk_last_error(void);
