@@ -1047,7 +1047,7 @@ int check_verify(const frisk_tree_verify_desc* d, bool ptrs, frisk::VerifyArgs& 
   const int es = esize(d->dtype);
   if (d->batch > INT32_MAX / 4) return fail(FRISK_EUNSUP, "%s: more trees than one launch takes", fn);
   const plan::VerifyPlan p = plan::verify_plan(d->batch, d->tokens, d->vocab, es);
-  if (d->batch > (int64_t)(UINT32_MAX / 256) / (d->tokens * p.chunks))
+  if (d->batch > (int64_t)(UINT32_MAX / 256) / (d->tokens * p.segments))
     return fail(FRISK_EUNSUP, "%s: more rows of logits than one launch takes", fn);
   const int64_t st[4] = {d->stride_b, d->stride_t, d->draft_probs ? d->draft_stride_b : 0,
                          d->draft_probs ? d->draft_stride_t : 0};
@@ -1078,10 +1078,10 @@ int check_verify(const frisk_tree_verify_desc* d, bool ptrs, frisk::VerifyArgs& 
   a.token = d->token;
   a.probs = d->probs;
   a.pieces = p.pieces;
-  a.chunks = (int)p.chunks;
+  a.segments = (int)p.segments;
   a.workspace = d->workspace;
   if (!ptrs) return FRISK_OK;
-  const int64_t need = frisk::verify_workspace(d->batch, d->tokens, p.chunks), n = d->batch * 4, all = n * d->tokens;
+  const int64_t need = frisk::verify_workspace(d->batch, d->tokens, p.segments), n = d->batch * 4, all = n * d->tokens;
   if (!d->workspace || d->workspace_bytes < need)
     return fail(FRISK_EINVAL, "%s: workspace of %lld bytes, this call takes %lld", fn,
                 (long long)(d->workspace ? d->workspace_bytes : 0), (long long)need);
@@ -1349,7 +1349,7 @@ int64_t frisk_tree_verify_workspace_size(const frisk_tree_verify_desc* d) {
   g_last_error.clear();
   frisk::VerifyArgs a;
   const int rc = check_verify(d, false, a);
-  return rc ? rc : frisk::verify_workspace(a.batch, a.tokens, a.chunks);
+  return rc ? rc : frisk::verify_workspace(a.batch, a.tokens, a.segments);
 }
 
 int frisk_tree_verify(const frisk_tree_verify_desc* d, void* stream) {

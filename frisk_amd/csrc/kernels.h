@@ -339,10 +339,10 @@ struct VerifyArgs {
   int32_t* count;
   int32_t* token;
   float* probs;  // may be null
-  int pieces, chunks;  // plan::verify_plan
+  int pieces, segments;  // plan::verify_plan
   void* workspace;     // verify_workspace bytes
 };
-int64_t verify_workspace(int64_t batch, int64_t tokens, int64_t chunks);
+int64_t verify_workspace(int64_t batch, int64_t tokens, int64_t segments);
 hipError_t tree_verify(const VerifyArgs& a, hipStream_t s);
 
 // MFMA fragment-layout probe (probe.hip): atom 0 = bf16 32x32x16,

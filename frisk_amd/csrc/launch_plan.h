@@ -618,19 +618,19 @@ inline int64_t attn_workspace(int64_t batch_heads, int64_t seq_q, int64_t seq_k,
 
 // ---------------------------------------------------------------------------
 // Verification of drafted tokens (verify.hip): nodes of a tree at most, and how a
-// row of `vocab` logits of `bytes` is cut into chunks of 256 threads with
-// `pieces` 16-B pieces each.
+// row of `vocab` logits of `bytes` is cut into segments: a wave's, with `pieces`
+// pieces of 16 B a lane.
 constexpr int64_t kVerifyNodes = 1024;
 constexpr int64_t kVerifyVocab = 1 << 24;
 struct VerifyPlan {
   int pieces;
-  int64_t chunks;
+  int64_t segments;
 };
 inline VerifyPlan verify_plan(int64_t batch, int64_t tokens, int64_t vocab, int bytes) {
   const int64_t whole = std::max<int64_t>(vocab * bytes / 16, 1);
-  auto chunks = [&](int pieces) { return (whole + 256 * pieces - 1) / (256 * pieces); };
-  const int pieces = batch * tokens * chunks(4) >= 512 ? 4 : 1;
-  return {pieces, chunks(pieces)};
+  auto segments = [&](int pieces) { return (whole + 64 * pieces - 1) / (64 * pieces); };
+  const int pieces = batch * tokens * segments(4) >= 2048 ? 4 : 1;
+  return {pieces, segments(pieces)};
 }
 
 // Attention of new tokens over a cache (attn_tree_mfma.h, attn_tree_rows.hip).

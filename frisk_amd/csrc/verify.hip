@@ -2,17 +2,22 @@
 // probabilities accept under given random numbers, and the token after it.
 //
 // Probabilities are compared with random numbers, so they are computed in 64
-// bits: a weight is 2^t, t = (x - max) log2(e) / T, from a polynomial of degree 11
-// on the fraction of t, off by 2^-47 of it, and sums are of doubles.  The vector
-// unit does as many 64-bit as 32-bit multiply-adds, so a weight costs about 20
-// instructions and reading the logits once bounds the work.
+// bits: a weight is 2^t, t = (x - max) log2(e) / T, from a polynomial of degree 9
+// on the fraction of t, off by 2^-45 of it, and sums are of doubles.  The vector
+// unit does as many 64-bit as 32-bit multiply-adds, so a weight costs about 16
+// instructions.
 //
-// Four launches.  (1) The rows of nodes that have children, in chunks: each one's
-// maximum and sum.  (2) A workgroup per tree combines them, takes every node's
-// probability given its parent, and walks from the root.  (3) What is left of the
-// probabilities at the last node, in chunks; chunks that no rejected token lies in
-// have their sums from (1).  (4) The chunk, then the element, in which the sum
-// passes the last random number.
+// Up to four launches.  (1) The rows of nodes that have children, a wave for each
+// segment of a row, without a barrier: its maximum and sum.  (2) A workgroup per tree combines
+// them, takes every node's probability given its parent, and walks from the root.
+// (3) What is left of the probabilities at the last node, by segments: the same kernel as (1),
+// so that its code is in the instruction caches already; segments that no rejected
+// token lies in have their sums from (1).  (4) The segment, then the element, in which the sum
+// passes the last random number.  A tree of one node takes (3) and (4) only.  ((4) by the last
+// workgroup of (3) to arrive took longer: 16 arrivals at a word, each an exchange past the
+// L2 caches, are 15 us one after the other, the launch 5.)
+
+#include <algorithm>
 
 #include "common.h"
 #include "kernels.h"
@@ -22,15 +27,16 @@ namespace frisk {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kWalkers = 1024;  // threads of a walk
 
-// A chunk's or a row's largest logit, its first place, and the sum of weights
+// A segment's or a row's largest logit, its first place, and the sum of weights
 // 2^((x - m) c): NaN if the row gives no probabilities (it holds a NaN or +infinity).
 struct Stat {
   double s;
   float m;
   int at;
 };
-// A chunk of the last node's row: sums of what is left there, and of what was left
+// A segment of the last node's row: sums of what is left there, and of what was left
 // before the last rejection; both relative to m.
 struct Rest {
   double s, whole;
@@ -47,8 +53,8 @@ struct End {
 };
 
 struct Layout {
-  Stat* stats;  // [batch][tokens][chunks]
-  Rest* rest;   // [batch][chunks]
+  Stat* stats;  // [batch][tokens][segments]
+  Rest* rest;   // [batch][segments]
   End* end;     // [batch]
   double* list;  // [batch][tokens] rejected tokens or, of dense drafts, what their rest summed to
 };
@@ -57,34 +63,80 @@ __device__ __forceinline__ Layout layout(const VerifyArgs& a) {
   char* p = (char*)a.workspace;
   Layout l;
   l.stats = (Stat*)p;
-  p += up16((int64_t)a.batch * a.tokens * a.chunks * sizeof(Stat));
+  p += up16((int64_t)a.batch * a.tokens * a.segments * sizeof(Stat));
   l.rest = (Rest*)p;
-  p += up16((int64_t)a.batch * a.chunks * sizeof(Rest));
+  p += up16((int64_t)a.batch * a.segments * sizeof(Rest));
   l.end = (End*)p;
   p += up16((int64_t)a.batch * sizeof(End));
   l.list = (double*)p;
   return l;
 }
 
-// 2^t for t <= 0 (0 below -1100).
-__device__ __forceinline__ double pow2(double t) {
-  t = __builtin_fmax(t, -1100.0);
-  const double k = __builtin_rint(t), f = t - k;
-  // ln(2)^n / n!: the first term left out is 2^-47 of the result at f = 1/2.
-  double p = 4.44553827187081e-10;
-  p = __builtin_fma(p, f, 7.054911620801121e-09);
-  p = __builtin_fma(p, f, 1.0178086009239696e-07);
-  p = __builtin_fma(p, f, 1.3215486790144305e-06);
-  p = __builtin_fma(p, f, 1.5252733804059838e-05);
-  p = __builtin_fma(p, f, 1.5403530393381606e-04);
-  p = __builtin_fma(p, f, 1.3333558146428441e-03);
-  p = __builtin_fma(p, f, 9.618129107628477e-03);
-  p = __builtin_fma(p, f, 5.5504108664821577e-02);
-  p = __builtin_fma(p, f, 2.402265069591007e-01);
-  p = __builtin_fma(p, f, 6.931471805599453e-01);
-  p = __builtin_fma(p, f, 1.0);
-  return __builtin_ldexp(p, (int)k);
+constexpr double kPoly[9] = {1.3259165418921631e-06, 1.5252831553412485e-05, 0.000154034371500767,
+                             0.0013333557934657732,  0.009618129186021637,   0.055504108666170275,
+                             0.2402265069570673,     0.6931471805599285,     1.0};
+constexpr double kLead = 1.0175586973078281e-07;  // the polynomial's first coefficient
+constexpr double kRound = 0x1.8p52;                // t + kRound has rint(t) in its low bits
+
+// 2^f for |f| <= 1/2: 1 + f p(f), p of degree 8 with the least largest relative
+// error of the whole, 2^-45; 1 at f = 0.
+__device__ __forceinline__ double pow2_fraction(double f, double lead = kLead) {
+  double p = lead;
+#pragma unroll
+  for (int i = 0; i < 9; ++i) p = __builtin_fma(p, f, kPoly[i]);
+  return p;
 }
+// x 2^k for the k in the low bits of `shifted`.  (Written out, the 32-bit addition to
+// the exponent's half became six instructions of a 64-bit one.)
+__device__ __forceinline__ double scale_by(double x, double shifted) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, shifted);
+  uint32_t hi = (uint32_t)(u >> 32);
+  asm("v_lshl_add_u32 %0, %1, 20, %0" : "+v"(hi) : "v"(k));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)u);
+}
+// 2^t for t <= 0: the exponent is added to the bits of 2^f.  0 below -1000 and for NaN.
+__device__ __forceinline__ double pow2(double t) {
+  const double held = __builtin_fmax(t, -1000.0), shifted = held + kRound, f = held - (shifted - kRound);
+  const double w = scale_by(pow2_fraction(f), shifted);
+  return t > -1000.0 ? w : 0.0;
+}
+
+// Weights of a segment's elements for their sum: 2^-900 in the place of smaller ones, 16
+// instructions of 64 bits.  A v_fma takes one scalar operand, so the other
+// constants of an operation are kept in vector registers.
+struct Weigh {
+  double top, factor, round, lead, least;
+  __device__ __forceinline__ Weigh(float m, double f)
+      : top((double)m), factor(f), round(kRound), lead(kLead), least(-900.0 / f) {
+    asm volatile("" : "+v"(factor), "+v"(round), "+v"(lead));
+  }
+  // The sum of W elements' weights, step by step for all of them: the steps of one
+  // wait for each other.
+  template <int W> __device__ __forceinline__ double sum(const float* x) const {
+    double f[W], shifted[W], p[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const double d = __builtin_fmax((double)x[k] - top, least);
+      shifted[k] = __builtin_fma(d, factor, round);
+      f[k] = __builtin_fma(d, factor, round - shifted[k]);
+      p[k] = lead;
+    }
+#pragma unroll
+    for (int i = 0; i < 9; ++i) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) p[k] = __builtin_fma(p[k], f[k], kPoly[i]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int k = 0; k < W; ++k) p[k] = scale_by(p[k], shifted[k]);
+#pragma unroll
+    for (int n = W / 2; n; n /= 2)
+#pragma unroll
+      for (int k = 0; k < n; ++k) p[k] += p[k + n];
+    return p[0];
+  }
+};
 
 // log2(e) / T of a tree; 0: its temperature is 0, the largest logit wins.
 __device__ __forceinline__ double factor_of(const VerifyArgs& a, int64_t b) {
@@ -94,6 +146,11 @@ __device__ __forceinline__ double factor_of(const VerifyArgs& a, int64_t b) {
 }
 __device__ __forceinline__ int nodes_of(const VerifyArgs& a, int64_t b) {
   return a.new_len ? min(max(a.new_len[b], 0), a.tokens) : a.tokens;
+}
+// Where a tree's walk ended; of trees of one node, which are not walked: at the root.
+__device__ __forceinline__ End end_of(const VerifyArgs& a, const Layout& l, int64_t b, double factor) {
+  if (a.tokens > 1) return l.end[b];
+  return End{0.0, 0.0f, nodes_of(a, b) < 1 ? -1 : 0, 0, factor == 0.0 ? -2 : -1};
 }
 
 template <Elt E> struct Row {
@@ -113,11 +170,13 @@ template <Elt E> __device__ __forceinline__ Row<E> row_of(const VerifyArgs& a, i
   return r;
 }
 
-// A chunk's elements are PIECES whole pieces a thread, in the order (piece, thread,
-// element); the first chunk's start with the row's head, the last one's end with
-// its tail, one element a thread.
-template <Elt E> __device__ __forceinline__ void load_piece(const Row<E>& r, int piece, float (&x)[Row<E>::N]) {
-  const i32x4 w = *(const i32x4*)(r.p + r.head + (int64_t)piece * Row<E>::N);
+// A segment's elements are PIECES whole pieces of 16 B a lane, in the order (piece,
+// lane, element); the first segment's start with the row's head, the last one's end
+// with its tail, one element a lane.
+template <Elt E> __device__ __forceinline__ i32x4 raw_piece(const Row<E>& r, int piece) {
+  return *(const i32x4*)(r.p + r.head + (int64_t)piece * Row<E>::N);
+}
+template <Elt E> __device__ __forceinline__ void widen_piece(i32x4 w, float (&x)[Row<E>::N]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t word = (uint32_t)w[i];
@@ -132,131 +191,80 @@ template <Elt E> __device__ __forceinline__ void load_piece(const Row<E>& r, int
     }
   }
 }
-// The loose element of a thread in chunk c, or -1: the head's in the first chunk
-// (threads 0 ..), the tail's in the last (threads 128 ..).
-template <Elt E> __device__ __forceinline__ int loose_of(const VerifyArgs& a, const Row<E>& r, int c) {
-  const int tid = threadIdx.x;
-  if (c == 0 && tid < r.head) return tid;
+template <Elt E> __device__ __forceinline__ void load_piece(const Row<E>& r, int piece, float (&x)[Row<E>::N]) {
+  widen_piece<E>(raw_piece<E>(r, piece), x);
+}
+// The loose element of a lane in segment g, or -1: the head's in the first segment
+// (lanes 0 ..), the tail's in the last (lanes 32 ..).
+template <Elt E> __device__ __forceinline__ int loose_of(const VerifyArgs& a, const Row<E>& r, int g, int lane) {
+  if (g == 0 && lane < r.head) return lane;
   const int tail = r.head + r.full * Row<E>::N;
-  if (c == a.chunks - 1 && tid >= 128 && tail + tid - 128 < r.n) return tail + tid - 128;
+  if (g == a.segments - 1 && lane >= 32 && tail + lane - 32 < r.n) return tail + lane - 32;
   return -1;
 }
 
+// ---- sums and so on over a wave ----------------------------------------------------
+
+// The values of two lanes of a pair, the same on both: lanes l ^ 1, l ^ 2, mirrored in
+// 8 and in 16, l ^ 16, l ^ 32.
+template <int STEP> __device__ __forceinline__ uint2 pair_of(uint32_t x) {
+  if constexpr (STEP < 4) {
+    constexpr int kControl[4] = {0xB1, 0x4E, 0x141, 0x140};
+    return {x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kControl[STEP], 0xf, 0xf, true)};
+  } else if constexpr (STEP == 4) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return {(uint32_t)r[0], (uint32_t)r[1]};
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return {(uint32_t)r[0], (uint32_t)r[1]};
+  }
+}
+template <int STEP = 0> __device__ __forceinline__ double wave_sum(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint2 lo = pair_of<STEP>((uint32_t)u), hi = pair_of<STEP>((uint32_t)(u >> 32));
+  x = __builtin_bit_cast(double, (uint64_t)hi.x << 32 | lo.x) + __builtin_bit_cast(double, (uint64_t)hi.y << 32 | lo.y);
+  if constexpr (STEP < 5) return wave_sum<STEP + 1>(x);
+  else return x;
+}
+// NaN if one of them is.
+template <int STEP = 0> __device__ __forceinline__ float wave_max(float x) {
+  const uint2 p = pair_of<STEP>(__builtin_bit_cast(uint32_t, x));
+  x = __builtin_elementwise_maximum(__builtin_bit_cast(float, p.x), __builtin_bit_cast(float, p.y));
+  if constexpr (STEP < 5) return wave_max<STEP + 1>(x);
+  else return x;
+}
+template <int STEP = 0> __device__ __forceinline__ int wave_min(int x) {
+  const uint2 p = pair_of<STEP>((uint32_t)x);
+  x = min((int)p.x, (int)p.y);
+  if constexpr (STEP < 5) return wave_min<STEP + 1>(x);
+  else return x;
+}
 __device__ __forceinline__ double shfl_d(double x, int lane) {
   const uint64_t u = __builtin_bit_cast(uint64_t, x);
   const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)u, lane), hi = (uint32_t)__shfl((int)(u >> 32), lane);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ double wave_sum(double x) {
+// The sum over the lanes up to this one.
+__device__ __forceinline__ double wave_scan(double x) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x += shfl_d(x, lane ^ m);
+  for (int d = 1; d < 64; d <<= 1) {
+    const double y = shfl_d(x, max(lane - d, 0));
+    if (lane >= d) x += y;
+  }
   return x;
 }
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x = fmaxf(x, __shfl_xor(x, m));
-  return x;
+// The value of lane k, the same in all lanes.
+__device__ __forceinline__ float lane_f(float x, int k) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), k));
 }
-__device__ __forceinline__ int wave_min(int x) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x = min(x, __shfl_xor(x, m));
-  return x;
+__device__ __forceinline__ double lane_d(double x, int k) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, k), hi = __builtin_amdgcn_readlane((int)(u >> 32), k);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// The statistics of chunk c of a row, known to all threads afterwards.  skip(index):
-// the element has no weight.
-template <Elt E, int PIECES, typename Skip>
-__device__ __forceinline__ Stat chunk_stat(const VerifyArgs& a, const Row<E>& r, int c, double factor, Skip skip) {
-  constexpr int N = Row<E>::N;
-  __shared__ float ms[kWaves];
-  __shared__ double ss[kWaves];
-  __shared__ int as[kWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int base = c * PIECES * kThreads + tid;
-  float x[PIECES][N];
-  float m = -__builtin_inff();
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < PIECES; ++i) {
-    const int piece = base + i * kThreads;
-    if (piece < r.full) {
-      load_piece<E>(r, piece, x[i]);
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        bad |= x[i][e] != x[i][e];
-        if (skip(r.head + piece * N + e)) x[i][e] = -__builtin_inff();
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) x[i][e] = -__builtin_inff();
-    }
-  }
-  const int loose = loose_of<E>(a, r, c);
-  float extra = -__builtin_inff();
-  if (loose >= 0) {
-    extra = (float)r.p[loose];
-    bad |= extra != extra;
-    if (skip(loose)) extra = -__builtin_inff();
-  }
-#pragma unroll
-  for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-    for (int e = 0; e < N; ++e) m = fmaxf(m, x[i][e]);
-  m = wave_max(fmaxf(m, extra));
-  __syncthreads();
-  if (lane == 0) ms[wave] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ms[w]);
-  double s = 0.0;
-  int at = INT32_MAX;
-  if (m > -__builtin_inff()) {
-    if (factor == 0.0) {
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (x[i][e] == m) at = min(at, r.head + (base + i * kThreads) * N + e);
-      if (extra == m) at = min(at, loose);
-      s = tid == 0 ? 1.0 : 0.0;
-    } else {
-      const double top = (double)m;
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i)
-        if (base + i * kThreads < r.full)
-#pragma unroll
-          for (int e = 0; e < N; ++e) s += pow2(((double)x[i][e] - top) * factor);
-      if (loose >= 0) s += pow2(((double)extra - top) * factor);
-    }
-  }
-  if (bad || m == __builtin_inff()) s = __builtin_nan("");
-  s = wave_sum(s);
-  at = wave_min(at);
-  if (lane == 0) ss[wave] = s, as[wave] = at;
-  __syncthreads();
-  s = 0.0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) s += ss[w], at = min(at, as[w]);
-  return Stat{s, m, at};
-}
-
-template <Elt E, int PIECES> __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
-  uint32_t id = blockIdx.x;
-  const int c = id % a.chunks;
-  id /= a.chunks;
-  const int t = id % a.tokens;
-  const int64_t b = id / a.tokens;
-  const int n = nodes_of(a, b);
-  if (t >= n) return;
-  // A row is needed if its node has a child.
-  bool child = false;
-  for (int i = t + 1 + threadIdx.x; i < n; i += kThreads) child |= a.parents[b * a.tokens + i] == t;
-  if (!__syncthreads_or(child)) return;
-  const Row<E> r = row_of<E>(a, b, t);
-  const Stat st = chunk_stat<E, PIECES>(a, r, c, factor_of(a, b), [](int) { return false; });
-  if (threadIdx.x == 0) layout(a).stats[(b * a.tokens + t) * a.chunks + c] = st;
-}
+// ---- segments of a row --------------------------------------------------------------
 
 // What is left of a probability p after `rounds` children drawn from q were
 // rejected, whose rests summed to z[0 ..]; a rest without mass leaves it as it was.
@@ -267,12 +275,191 @@ __device__ __forceinline__ double left_of(double p, double q, const double* z, i
   }
   return p;
 }
+// The same, and before the last rejection, whose rest has no sum yet.
+struct Left {
+  double now, was;
+};
+__device__ __forceinline__ Left dense_left(double p, float q, const double* z, int rounds) {
+  const double was = left_of(p, (double)q, z, rounds - 1);
+  return {__builtin_fmax(was - (double)q, 0.0), was};
+}
+
+// A segment's elements as they are loaded.
+template <Elt E, int PIECES> struct Held {
+  i32x4 w[PIECES];
+  float extra;
+};
+template <Elt E, int PIECES>
+__device__ __forceinline__ void load_segment(const VerifyArgs& a, const Row<E>& r, int g, Held<E, PIECES>& h) {
+  const int lane = threadIdx.x & 63, base = g * PIECES * 64 + lane;
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i)
+    if (base + i * 64 < r.full) h.w[i] = raw_piece<E>(r, base + i * 64);
+  const int loose = loose_of<E>(a, r, g, lane);
+  h.extra = loose >= 0 ? (float)r.p[loose] : -__builtin_inff();
+}
+
+// The statistics of segment g, known to all lanes, without the tokens list[0 .. gone).
+template <Elt E, int PIECES>
+__device__ __forceinline__ Stat segment_stat(const VerifyArgs& a, const Row<E>& r, int g, const Held<E, PIECES>& h,
+                                             double factor, const double* list, int gone) {
+  constexpr int N = Row<E>::N;
+  const int lane = threadIdx.x & 63, base = g * PIECES * 64 + lane;
+  float x[PIECES][N];
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    if (base + i * 64 < r.full) {
+      widen_piece<E>(h.w[i], x[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[i][e] = -__builtin_inff();
+    }
+  }
+  const int loose = loose_of<E>(a, r, g, lane);
+  float m = -__builtin_inff(), extra = h.extra;
+  for (int k = 0; k < gone; ++k) {
+    const int v = (int)list[k];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (v == r.head + (base + i * 64) * N + e) x[i][e] = m;
+    if (v == loose) extra = m;
+  }
+  // The maximum of a row with a NaN is NaN.
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+    for (int e = 0; e < N; ++e) m = __builtin_elementwise_maximum(m, x[i][e]);
+  m = wave_max(__builtin_elementwise_maximum(m, extra));
+  double s = 0.0;
+  int at = INT32_MAX;
+  if (m > -__builtin_inff()) {
+    if (factor == 0.0) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (x[i][e] == m) at = min(at, r.head + (base + i * 64) * N + e);
+      if (extra == m) at = min(at, loose);
+      at = wave_min(at);
+      s = 1.0;
+    } else {
+      const Weigh weigh(m, factor);
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+        if (base + i * 64 < r.full)
+#pragma unroll
+          for (int e = 0; e < N; e += 4) s += weigh.template sum<4>(x[i] + e);
+      if (loose >= 0) s += weigh.template sum<1>(&extra);
+      s = wave_sum(s);
+    }
+  }
+  if (!(m < __builtin_inff())) s = __builtin_nan("");
+  return Stat{s, m, at};
+}
+
+// Segment g of what dense drafts' rejection left at a tree's last node.
+template <Elt E, int PIECES>
+__device__ __forceinline__ Rest segment_rest(const VerifyArgs& a, const Row<E>& r, int64_t b, int g, const End& e,
+                                             const double* list, double factor) {
+  constexpr int N = Row<E>::N;
+  const int lane = threadIdx.x & 63;
+  const float* q = a.draft_probs + b * a.qb + e.node * a.qt;
+  const double top = (double)e.m;
+  double s = 0.0, whole = 0.0;
+  auto add = [&](float x, int v) {
+    const Left w = dense_left(pow2(((double)x - top) * factor) / e.scale, q[v], list, e.rounds);
+    s += w.now;
+    whole += w.was;
+  };
+#pragma unroll 1
+  for (int i = 0; i < PIECES; ++i) {
+    const int piece = (g * PIECES + i) * 64 + lane;
+    if (piece >= r.full) break;
+    float x[N];
+    load_piece<E>(r, piece, x);
+#pragma unroll
+    for (int k = 0; k < N; ++k) add(x[k], r.head + piece * N + k);
+  }
+  const int loose = loose_of<E>(a, r, g, lane);
+  if (loose >= 0) add((float)r.p[loose], loose);
+  return Rest{wave_sum(s), wave_sum(whole), 0.0f, 0};
+}
+
+// `groups` workgroups have the segments of a row, each wave every (4 groups)-th one, the next
+// one's loads under way: of every row whose node has children (last 0), or of the rows that
+// the walks ended at.
+template <Elt E, int PIECES>
+__global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, int groups, int last) {
+  constexpr int N = Row<E>::N;
+  const int lane = threadIdx.x & 63, step = groups * kWaves;
+  uint32_t id = blockIdx.x;
+  int g = __builtin_amdgcn_readfirstlane((int)(id % groups * kWaves + (threadIdx.x >> 6)));
+  if (g >= a.segments) return;
+  id /= groups;
+  const Layout l = layout(a);
+  const int64_t b = last ? id : id / a.tokens;
+  const double factor = factor_of(a, b);
+  int t = last ? 0 : id % a.tokens, gone = 0;
+  const double* list = l.list + b * a.tokens;
+  Rest* rests = l.rest + b * a.segments;
+  End e = {};
+  if (last) {
+    e = end_of(a, l, b, factor);
+    if (e.node < 0 || e.greedy >= 0) return;
+    t = e.node;
+    gone = e.rounds;
+    if (gone > 0 && a.draft_probs) {
+      const Row<E> r = row_of<E>(a, b, t);
+      for (; g < a.segments; g += step) {
+        const Rest rest = segment_rest<E, PIECES>(a, r, b, g, e, list, factor);
+        if (lane == 0) rests[g] = rest;
+      }
+      return;
+    }
+  } else {
+    // (Every wave looks for itself.)
+    const int n = nodes_of(a, b);
+    uint64_t child = 0;
+    for (int i0 = t + 1; i0 < n && !child; i0 += 64)
+      child = __builtin_amdgcn_ballot_w64(i0 + lane < n && a.parents[b * a.tokens + min(i0 + lane, n - 1)] == t);
+    if (!child) return;
+  }
+  const Row<E> r = row_of<E>(a, b, t);
+  Stat* stats = l.stats + (b * a.tokens + t) * a.segments;
+  Held<E, PIECES> now, next;
+  load_segment<E, PIECES>(a, r, g, now);
+  for (; g < a.segments; g += step) {
+    if (g + step < a.segments) load_segment<E, PIECES>(a, r, g + step, next);
+    bool reuse = false;
+    if (gone > 0) {
+      // One-hot drafts: a segment without a rejected token is as it was.
+      const int lo = g ? r.head + g * PIECES * 64 * N : 0;
+      const int hi = g == a.segments - 1 ? r.n : r.head + (g + 1) * PIECES * 64 * N;
+      uint64_t any = 0;
+      for (int i0 = 0; i0 < gone && !any; i0 += 64) {
+        const int v = i0 + lane < gone ? (int)list[i0 + lane] : -1;
+        any = __builtin_amdgcn_ballot_w64(v >= lo && v < hi);
+      }
+      reuse = !any;
+    }
+    const Stat st = reuse ? stats[g] : segment_stat<E, PIECES>(a, r, g, now, factor, list, gone);
+    if (lane == 0) {
+      if (last) rests[g] = Rest{st.s, st.s, st.m, st.at};
+      else stats[g] = st;
+    }
+    now = next;
+  }
+}
+
+// ---- the walk ----------------------------------------------------------------------
 
 template <Elt E> __device__ __forceinline__ float logit(const VerifyArgs& a, int64_t b, int64_t t, int v) {
   return load_as_f32<E>(a.logits, b * a.sb + t * a.st + v);
 }
 
-template <Elt E> __global__ __launch_bounds__(kThreads) void verify_walk_kernel(VerifyArgs a) {
+template <Elt E> __global__ __launch_bounds__(kWalkers) void verify_walk_kernel(VerifyArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   double* mass = (double*)smem;            // [tokens] sum of a node's row, NaN if it has none
   double* chance = mass + a.tokens;        // [tokens] weight of a node's token in its parent's row
@@ -281,8 +468,11 @@ template <Elt E> __global__ __launch_bounds__(kThreads) void verify_walk_kernel(
   int* firsts = (int*)(tops + a.tokens);   // [tokens]
   int* up = firsts + a.tokens;             // [tokens] parent, -1: none that is reached
   float* qs = (float*)(up + a.tokens);     // [tokens]
-  __shared__ int todo, at_node, at_rounds;
-  __shared__ double sums[kWaves];
+  int* order = (int*)(qs + a.tokens);      // [tokens] the nodes that have children
+  int* tokens = order + a.tokens;          // [tokens] their drafts
+  float* us = (float*)(tokens + a.tokens);  // [tokens]
+  __shared__ int todo, at_node, at_rounds, inner;
+  __shared__ double sums[(kWalkers / 64)];
   const Layout l = layout(a);
   const int64_t b = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -293,49 +483,62 @@ template <Elt E> __global__ __launch_bounds__(kThreads) void verify_walk_kernel(
   }
   const double factor = factor_of(a, b);
   const bool dense = a.draft_probs != nullptr;
-  for (int t = tid; t < a.tokens; t += kThreads) {
-    const int p = t < n ? a.parents[b * a.tokens + t] : -1;
-    up[t] = p >= 0 && p < t ? p : -1;
-    mass[t] = __builtin_nan("");
-    chance[t] = 0.0;
-    if (t > 0) a.path[b * a.tokens + t] = -1;
-    firsts[t] = 0;  // (whether the node has a child, for now)
+  // A thread has a node; what it loads is under way while the rows are combined.
+  static_assert(plan::kVerifyNodes <= kWalkers, "a thread for each node");
+  int parent = -1, token = -1;
+  float x = 0.0f, q = 1.0f;
+  if (tid < a.tokens) {
+    if (tid > 0 && tid < n) parent = a.parents[b * a.tokens + tid], token = a.drafts[b * a.tokens + tid];
+    if (parent >= tid) parent = -1;
+    up[tid] = parent;
+    us[tid] = tid < n ? a.uniform[b * a.tokens + tid] : 0.0f;
+    tokens[tid] = token;
+    if (tid > 0) a.path[b * a.tokens + tid] = -1;
+    mass[tid] = __builtin_nan("");
+    firsts[tid] = 0;  // (whether the node has a child, for now)
+  }
+  if (tid == 0) inner = 0;
+  const bool known = parent >= 0 && token >= 0 && token < a.vocab;
+  if (known) {
+    x = logit<E>(a, b, parent, token);
+    if (dense) q = a.draft_probs[b * a.qb + parent * a.qt + token];
   }
   __syncthreads();
-  for (int t = tid; t < n; t += kThreads)
-    if (up[t] >= 0) firsts[up[t]] = 1;
+  if (parent >= 0) firsts[parent] = 1;
   __syncthreads();
-  for (int t = wave; t < n; t += kWaves) {
-    if (!firsts[t]) continue;
-    const Stat* st = l.stats + (b * a.tokens + t) * a.chunks;
-    float m = -__builtin_inff();
-    for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, st[c].m);
+  if (tid < n && firsts[tid]) order[atomicAdd(&inner, 1)] = tid;
+  __syncthreads();
+  // A wave combines the segments of a row.
+  for (int i = wave; i < inner; i += kWalkers / 64) {
+    const int t = order[i];
+    const Stat* st = l.stats + (b * a.tokens + t) * a.segments;
+    const Stat none = {0.0, -__builtin_inff(), INT32_MAX}, mine = lane < a.segments ? st[lane] : none;
+    float m = mine.m;
+    for (int c = lane + 64; c < a.segments; c += 64) m = __builtin_elementwise_maximum(m, st[c].m);
     m = wave_max(m);
-    double s = 0.0;
-    int at = INT32_MAX;
-    for (int c = lane; c < a.chunks; c += 64) {
+    auto scaled = [&](const Stat& x) {
+      return x.s == 0.0 ? 0.0 : factor == 0.0 ? x.s : x.s * pow2(((double)x.m - (double)m) * factor);
+    };
+    double s = scaled(mine);
+    int at = mine.m == m ? mine.at : INT32_MAX;
+    for (int c = lane + 64; c < a.segments; c += 64) {
       const Stat x = st[c];
-      if (x.m > -__builtin_inff() || x.s != x.s) s += x.s * (factor == 0.0 ? 1.0 : pow2(((double)x.m - (double)m) * factor));
-      if (factor == 0.0 && x.m == m) at = min(at, x.at);
+      s += scaled(x);
+      if (x.m == m) at = min(at, x.at);
     }
     s = wave_sum(s);
     at = wave_min(at);
     if (lane == 0) mass[t] = s > 0.0 && s < __builtin_inf() ? s : __builtin_nan(""), tops[t] = m, firsts[t] = at;
   }
   __syncthreads();
-  for (int t = tid; t < a.tokens; t += kThreads) {
-    const int p = t < n ? up[t] : -1, v = p >= 0 ? a.drafts[b * a.tokens + t] : -1;
-    double w = 0.0;
-    float q = 1.0f;
-    if (p >= 0 && v >= 0 && v < a.vocab) {
-      if (factor == 0.0) w = v == firsts[p] ? mass[p] : 0.0;
-      else w = pow2(((double)logit<E>(a, b, p, v) - (double)tops[p]) * factor);
-      if (dense) q = a.draft_probs[b * a.qb + p * a.qt + v];
-    }
+  if (tid < a.tokens) {
     // (A row without probabilities has none for its tokens either.)
-    chance[t] = w;
-    qs[t] = q;
-    if (a.probs) a.probs[b * a.tokens + t] = p >= 0 ? (float)(w / mass[p]) : 0.0f;
+    double w = 0.0;
+    if (known) w = factor == 0.0 ? token == firsts[parent] ? mass[parent] : 0.0
+                                 : pow2(((double)x - (double)tops[parent]) * factor);
+    chance[tid] = w;
+    qs[tid] = q;
+    if (a.probs) a.probs[b * a.tokens + tid] = parent >= 0 ? (float)(w / mass[parent]) : 0.0f;
   }
   __syncthreads();
 
@@ -353,8 +556,8 @@ template <Elt E> __global__ __launch_bounds__(kThreads) void verify_walk_kernel(
       for (; base < n && !sum; base += sum ? 0 : 64) {
         const int t = base + lane;
         const bool live = t < n;
-        const int parent = live ? up[t] : -1, token = live ? a.drafts[b * a.tokens + t] : -1;
-        const float u = live ? a.uniform[b * a.tokens + t] : 0.0f;
+        const int parent = live ? up[t] : -1, token = live ? tokens[t] : -1;
+        const float u = live ? us[t] : 0.0f;
         double w = live ? chance[t] : 0.0;
         const float q = live ? qs[t] : 0.0f;
         if (!dense)
@@ -370,9 +573,9 @@ template <Elt E> __global__ __launch_bounds__(kThreads) void verify_walk_kernel(
             base = n;
             break;
           }
-          const double wk = shfl_d(w, k);
-          const float uk = __shfl(u, k), qk = __shfl(q, k);
-          const int token_k = __shfl(token, k);
+          const double wk = lane_d(w, k);
+          const float uk = lane_f(u, k), qk = lane_f(q, k);
+          const int token_k = __builtin_amdgcn_readlane(token, k);
           bool taken;
           if (dense && factor != 0.0) {
             if (rounds > 0 && list[rounds - 1] < 0.0) {
@@ -414,7 +617,7 @@ template <Elt E> __global__ __launch_bounds__(kThreads) void verify_walk_kernel(
     const double top = (double)tops[node], scale = mass[node];
     const float* q = a.draft_probs + b * a.qb + node * a.qt;
     double s = 0.0;
-    for (int v = tid; v < a.vocab; v += kThreads) {
+    for (int v = tid; v < a.vocab; v += kWalkers) {
       const double p = pow2(((double)logit<E>(a, b, node, v) - top) * factor) / scale;
       s += __builtin_fmax(left_of(p, (double)q[v], list, done) - (double)q[v], 0.0);
     }
@@ -423,12 +626,12 @@ template <Elt E> __global__ __launch_bounds__(kThreads) void verify_walk_kernel(
     __syncthreads();
     if (tid == 0) {
       double all = 0.0;
-      for (int w = 0; w < kWaves; ++w) all += sums[w];
+      for (int w = 0; w < (kWalkers / 64); ++w) all += sums[w];
       list[done] = all;
     }
     __syncthreads();
   }
-  for (int i = tid; i < at_rounds; i += kThreads) l.list[b * a.tokens + i] = list[i];
+  for (int i = tid; i < at_rounds; i += kWalkers) l.list[b * a.tokens + i] = list[i];
   if (tid == 0) {
     End e;
     e.scale = mass[cur];
@@ -444,254 +647,181 @@ template <Elt E> __global__ __launch_bounds__(kThreads) void verify_walk_kernel(
   }
 }
 
-// Weight of what is left of an element, and before the last rejection, for dense
-// drafts.
-struct Left {
-  double now, was;
-};
-__device__ __forceinline__ Left dense_left(double p, float q, const double* z, int rounds) {
-  const double was = left_of(p, (double)q, z, rounds - 1);
-  return {__builtin_fmax(was - (double)q, 0.0), was};
-}
-
-template <Elt E, int PIECES> __global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a) {
-  constexpr int N = Row<E>::N;
-  const Layout l = layout(a);
-  const int c = blockIdx.x % a.chunks;
-  const int64_t b = blockIdx.x / a.chunks;
-  const End e = l.end[b];
-  if (e.node < 0 || e.greedy >= 0) return;
-  const double factor = factor_of(a, b);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  Rest* out = l.rest + b * a.chunks + c;
-  const Row<E> r = row_of<E>(a, b, e.node);
-  const double* list = l.list + b * a.tokens;
-  if (e.rounds > 0 && a.draft_probs) {
-    __shared__ double ss[kWaves], ws[kWaves];
-    const float* q = a.draft_probs + b * a.qb + e.node * a.qt;
-    const double top = (double)e.m;
-    double s = 0.0, whole = 0.0;
-    auto add = [&](float x, int v) {
-      const Left w = dense_left(pow2(((double)x - top) * factor) / e.scale, q[v], list, e.rounds);
-      s += w.now;
-      whole += w.was;
-    };
-#pragma unroll 1
-    for (int i = 0; i < PIECES; ++i) {
-      const int piece = (c * PIECES + i) * kThreads + tid;
-      if (piece >= r.full) break;
-      float x[N];
-      load_piece<E>(r, piece, x);
-#pragma unroll
-      for (int k = 0; k < N; ++k) add(x[k], r.head + piece * N + k);
-    }
-    const int loose = loose_of<E>(a, r, c);
-    if (loose >= 0) add((float)r.p[loose], loose);
-    s = wave_sum(s);
-    whole = wave_sum(whole);
-    if (lane == 0) ss[wave] = s, ws[wave] = whole;
-    __syncthreads();
-    if (tid == 0) {
-      Rest o = {0.0, 0.0, 0.0f, 0};
-      for (int w = 0; w < kWaves; ++w) o.s += ss[w], o.whole += ws[w];
-      *out = o;
-    }
-    return;
-  }
-  // One-hot drafts: without the rejected tokens.
-  const int lo = c * PIECES * kThreads * N + (c ? r.head : 0);
-  const int hi = c == a.chunks - 1 ? r.n : min(r.head + (c + 1) * PIECES * kThreads * N, r.n);
-  __shared__ uint32_t gone[PIECES * kThreads * N / 32 + 1];
-  bool any = false;
-  if (e.rounds > 0) {
-    for (int i = tid; i < PIECES * kThreads * N / 32 + 1; i += kThreads) gone[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < e.rounds; i += kThreads) {
-      const int v = (int)list[i];
-      if (v >= lo && v < hi) atomicOr(&gone[(v - lo) >> 5], 1u << ((v - lo) & 31)), any = true;
-    }
-    any = __syncthreads_or(any);
-    if (!any) {
-      const Stat st = l.stats[(b * a.tokens + e.node) * a.chunks + c];
-      if (tid == 0) *out = Rest{st.s, st.s, st.m, st.at};
-      return;
-    }
-  }
-  const Stat st = chunk_stat<E, PIECES>(a, r, c, factor, [&](int v) {
-    return any && (gone[(v - lo) >> 5] >> ((v - lo) & 31)) & 1u;
-  });
-  if (tid == 0) *out = Rest{st.s, st.s, st.m, st.at};
-}
+// ---- the token ---------------------------------------------------------------------
 
 template <Elt E, int PIECES> __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   constexpr int N = Row<E>::N;
+  static_assert(PIECES <= kWaves, "a piece of a segment for each wave");
   const Layout l = layout(a);
   const int64_t b = blockIdx.x;
-  const End e = l.end[b];
-  if (e.node == -1) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const double factor = factor_of(a, b);
+  const End e = end_of(a, l, b, factor);
+  if (e.node == -1) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (a.tokens == 1 && tid == 0) {  // (no walk has written these)
+    a.path[b] = 0;
+    a.count[b] = 1;
+    if (a.probs) a.probs[b] = 0.0f;
+  }
   if (e.node < 0 || e.greedy >= 0) {
     if (tid == 0) a.token[b] = e.node < 0 ? -1 : e.greedy;
     return;
   }
-  const Rest* rest = l.rest + b * a.chunks;
+  const Rest* rest = l.rest + b * a.segments;
   const double* list = l.list + b * a.tokens;
   const bool dense = e.rounds > 0 && a.draft_probs;
-  __shared__ int chosen, found, use_whole, token_at, last_at[kWaves];
-  __shared__ double before, goal, sums[kWaves];
+  __shared__ int chosen, use_whole;
+  __shared__ double before, goal;
   __shared__ float top_at;
   if (wave == 0) {
-    float m = -__builtin_inff();
-    for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, rest[c].m);
+    // A lane has a run of segments, the first of them held.
+    const int per = (a.segments + 63) / 64, c0 = lane * per, c1 = min(c0 + per, a.segments);
+    const Rest none = {0.0, 0.0, -__builtin_inff(), INT32_MAX}, held = c0 < c1 ? rest[c0] : none;
+    auto of = [&](int c) { return c == c0 ? held : rest[c]; };
+    float m = held.m;
+    for (int c = c0 + 1; c < c1; ++c) m = __builtin_elementwise_maximum(m, of(c).m);
     m = wave_max(m);
     auto scaled = [&](double s, float mc) {
       return s == 0.0 ? 0.0 : dense ? s : s * pow2(((double)mc - (double)m) * factor);
     };
     if (factor == 0.0) {
       int at = INT32_MAX;
-      bool bad = false;
-      for (int c = lane; c < a.chunks; c += 64) {
-        if (rest[c].m == m) at = min(at, rest[c].at);
-        bad |= rest[c].s != rest[c].s;
+      for (int c = c0; c < c1; ++c) {
+        const Rest x = of(c);
+        if (x.m == m) at = min(at, x.at);
       }
       at = wave_min(at);
-      bad = __builtin_amdgcn_ballot_w64(bad) != 0;
-      if (lane == 0) a.token[b] = bad || at == INT32_MAX ? -1 : at, chosen = -1;
+      const bool none = !(m > -__builtin_inff() && m < __builtin_inff());
+      if (lane == 0) a.token[b] = none ? -1 : at, chosen = -1;
     } else {
       double s = 0.0, w = 0.0;
-      for (int c = lane; c < a.chunks; c += 64) s += scaled(rest[c].s, rest[c].m), w += scaled(rest[c].whole, rest[c].m);
-      s = wave_sum(s);
-      w = wave_sum(w);
-      const bool whole = dense && !(s > 0.0);
-      const double all = whole ? w : s, want = (double)a.final_uniform[b] * all;
+      for (int c = c0; c < c1; ++c) {
+        const Rest x = of(c);
+        s += scaled(x.s, x.m), w += scaled(x.whole, x.m);
+      }
+      const double sums = wave_sum(s), wholes = wave_sum(w);
+      const bool whole = dense && !(sums > 0.0);
+      const double all = whole ? wholes : sums, want = (double)a.final_uniform[b] * all;
       if (!(all > 0.0) || all == __builtin_inf()) {
         // Nothing is left of one-hot drafts: the last one had it all.  Else the
         // row gives no probabilities.
         if (lane == 0) a.token[b] = all == 0.0 && e.rounds > 0 && !dense ? (int)list[e.rounds - 1] : -1, chosen = -1;
       } else {
-        // The first chunk whose end passes `want`; the last one with any mass, if rounding
-        // leaves none.
-        double base = 0.0, at_base = 0.0, last_base = 0.0;
-        int at = -1, last = -1;
-        for (int c0 = 0; c0 < a.chunks && at < 0; c0 += 64) {
-          const int c = c0 + lane;
-          const double mine = c < a.chunks ? scaled(whole ? rest[c].whole : rest[c].s, rest[c].m) : 0.0;
-          double sum = mine;
-#pragma unroll
-          for (int d = 1; d < 64; d <<= 1) {
-            const double y = shfl_d(sum, max(lane - d, 0));
-            if (lane >= d) sum += y;
+        // The first lane, then segment, whose end passes `want`; the last one with any mass, if
+        // rounding leaves none.
+        const double mine = whole ? w : s, upto = wave_scan(mine);
+        const uint64_t some = __builtin_amdgcn_ballot_w64(mine > 0.0);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(mine > 0.0 && upto > want);
+        const int k = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+        if (lane == k) {
+          double base = upto - mine, at = base;
+          int g = -1;
+          for (int c = c0; c < c1; ++c) {
+            const Rest x = of(c);
+            const double here = scaled(whole ? x.whole : x.s, x.m);
+            if (!(here > 0.0)) continue;
+            g = c, at = base;
+            base += here;
+            if (base > want) break;
           }
-          const uint64_t some = __builtin_amdgcn_ballot_w64(mine > 0.0);
-          const uint64_t past = __builtin_amdgcn_ballot_w64(mine > 0.0 && base + sum > want);
-          if (past) {
-            const int k = __builtin_ctzll(past);
-            at = c0 + k;
-            at_base = base + shfl_d(sum, k) - shfl_d(mine, k);
-          } else if (some) {
-            const int k = 63 - __builtin_clzll(some);
-            last = c0 + k;
-            last_base = base + shfl_d(sum, k) - shfl_d(mine, k);
-          }
-          base += shfl_d(sum, 63);
-        }
-        if (lane == 0) {
-          chosen = at >= 0 ? at : last;
-          before = at >= 0 ? at_base : last_base;
-          goal = want;
-          use_whole = whole;
-          top_at = m;
+          chosen = g, before = at, goal = want, use_whole = whole, top_at = m;
         }
       }
     }
   }
-  if (tid == 0) found = INT32_MAX, token_at = -1;
   __syncthreads();
-  const int c = chosen;
-  if (c < 0) return;
-  // The chunk's elements in order: the head, the pieces, the tail.
+  const int g = chosen;
+  if (g < 0) return;
   const Row<E> r = row_of<E>(a, b, e.node);
   const float* q = dense ? a.draft_probs + b * a.qb + e.node * a.qt : nullptr;
   const double top = (double)(dense ? e.m : top_at), want = goal;
   const bool whole = use_whole;
   auto weight = [&](float x, int v) {
     const double p = pow2(((double)x - top) * factor);
-    if (dense) {
-      const Left w = dense_left(p / e.scale, q[v], list, e.rounds);
-      return whole ? w.was : w.now;
-    }
-    for (int i = 0; i < e.rounds; ++i)
-      if (v == (int)list[i]) return 0.0;
-    return p;
+    if (!dense) return p;
+    const Left w = dense_left(p / e.scale, q[v], list, e.rounds);
+    return whole ? w.was : w.now;
   };
-  double base = before;
-  int last = -1;
-  // Step 0: the head, an element a thread; then the pieces; then the tail.
-  const int tail = r.head + r.full * N;
-  for (int step = 0; step < PIECES + 2; ++step) {
-    double w[N], mine = 0.0;
-    int first = 0, n = 0;
-    if (step == 0 || step == PIECES + 1) {
-      first = (step ? tail : 0) + tid;
-      n = (step ? c == a.chunks - 1 && first < r.n : c == 0 && tid < r.head) ? 1 : 0;
-      if (n) mine = w[0] = weight((float)r.p[first], first);
-    } else {
-      const int piece = (c * PIECES + step - 1) * kThreads + tid;
-      if (piece < r.full) {
-        n = N;
-        first = r.head + piece * N;
-        float x[N];
-        load_piece<E>(r, piece, x);
+  // The segment's elements in order: part 0 is the head (the first wave's), 1 + w wave
+  // w's piece of each lane, and the last one the tail (the first wave's).
+  constexpr int kParts = PIECES + 2;
+  __shared__ double parts[kParts];
+  const int piece = g * PIECES * 64 + tid, loose = wave == 0 ? loose_of<E>(a, r, g, lane) : -1;
+  double w[N];
+  float x[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) w[k] = weight(x[k], first + k), mine += w[k];
-      }
+  for (int k = 0; k < N; ++k) x[k] = -__builtin_inff();
+  if (wave < PIECES && piece < r.full) load_piece<E>(r, piece, x);
+  float extra = -__builtin_inff();
+  if (loose >= 0) extra = (float)r.p[loose];
+  const int first = r.head + piece * N;
+  if (!dense)
+    for (int i = 0; i < e.rounds; ++i) {
+      const int v = (int)list[i];
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (v == first + k) x[k] = -__builtin_inff();
+      if (v == loose) extra = -__builtin_inff();
     }
-    double sum = mine;
+  double sum = 0.0;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double y = shfl_d(sum, max(lane - d, 0));
-      if (lane >= d) sum += y;
-    }
-    if (lane == 63) sums[wave] = sum;
-    __syncthreads();
-    double at = base + sum - mine, all = base;
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-      if (k < wave) at += sums[k];
-      all += sums[k];
-    }
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (k < n && w[k] > 0.0) {
-        last = first + k;
-        at += w[k];
-        if (at > want) {
-          atomicMin(&found, first + k);
-          break;
-        }
-      }
-    base = all;
-    __syncthreads();
-    if (found != INT32_MAX) break;
+  for (int k = 0; k < N; ++k) {
+    w[k] = wave < PIECES && piece < r.full ? weight(x[k], first + k) : 0.0;
+    sum += w[k];
   }
-  if (found == INT32_MAX) {  // rounding: the last element with a weight
-    for (int m = 1; m < 64; m <<= 1) last = max(last, __shfl_xor(last, m));
-    if (lane == 0) last_at[wave] = last;
-    __syncthreads();
-    last = max(max(last_at[0], last_at[1]), max(last_at[2], last_at[3]));
+  const double odd = loose >= 0 ? weight(extra, loose) : 0.0, all = wave_sum(sum);
+  const bool in_head = loose >= 0 && loose < r.head;
+  const double heads = wave_sum(in_head ? odd : 0.0), tails = wave_sum(in_head ? 0.0 : odd);
+  if (lane == 0 && wave < PIECES) parts[1 + wave] = all;
+  if (tid == 0) parts[0] = heads, parts[kParts - 1] = tails;
+  __syncthreads();
+  // The part whose end passes `want` (the last one with a weight, if rounding leaves none).
+  double base = before, at = before;
+  int part = -1;
+  for (int k = 0; k < kParts; ++k) {
+    if (!(parts[k] > 0.0)) continue;
+    part = k, at = base;
+    base += parts[k];
+    if (base > want) break;
   }
-  if (tid == 0) a.token[b] = found != INT32_MAX ? found : last;
+  const bool ends = part == 0 || part == kParts - 1;
+  if (part < 0 || wave != (ends ? 0 : part - 1)) return;
+  // Its elements, by lanes: the first that passes, or the last with a weight.
+  if (ends) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) w[k] = 0.0;
+    if (in_head == (part == 0)) w[0] = odd;
+    sum = w[0];
+  }
+  const int start = ends ? loose : first;
+  at += wave_scan(sum) - sum;
+  int found = INT32_MAX, last = -1;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    at += w[k];
+    if (w[k] > 0.0) {
+      last = start + k;
+      if (at > want) found = min(found, start + k);
+    }
+  }
+  found = wave_min(found);
+  last = -wave_min(-last);
+  if (lane == 0) a.token[b] = found != INT32_MAX ? found : last;
 }
 
 template <Elt E, int PIECES> hipError_t launch_pieces(const VerifyArgs& a, hipStream_t s) {
-  const int64_t rows = a.batch * a.tokens * a.chunks, ends = a.batch * a.chunks;
-  if (rows > UINT32_MAX / kThreads) return hipErrorInvalidConfiguration;
-  if (a.tokens > 1)
-    hipLaunchKernelGGL((verify_stats_kernel<E, PIECES>), dim3((unsigned)rows), dim3(kThreads), 0, s, a);
-  hipLaunchKernelGGL((verify_walk_kernel<E>), dim3((unsigned)a.batch), dim3(kThreads),
-                     (unsigned)(a.tokens * 40), s, a);
-  hipLaunchKernelGGL((verify_rest_kernel<E, PIECES>), dim3((unsigned)ends), dim3(kThreads), 0, s, a);
+  const int64_t groups = (a.segments + kWaves - 1) / kWaves;  // a segment a wave
+  if (a.batch * a.tokens * groups > UINT32_MAX / kThreads) return hipErrorInvalidConfiguration;
+  auto rows = verify_rows_kernel<E, PIECES>;
+  if (a.tokens > 1) {
+    // As many segments a wave as leave 32 waves for a CU.
+    const int64_t per = a.batch * a.tokens * groups / (8 * (int64_t)device_cus());
+    const int64_t some = (groups + std::max<int64_t>(per, 1) - 1) / std::max<int64_t>(per, 1);
+    hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * a.tokens * some)), dim3(kThreads), 0, s, a, (int)some, 0);
+    hipLaunchKernelGGL((verify_walk_kernel<E>), dim3((unsigned)a.batch), dim3(kWalkers),
+                       (unsigned)(a.tokens * 52), s, a);
+  }
+  hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * groups)), dim3(kThreads), 0, s, a, (int)groups, 1);
   hipLaunchKernelGGL((verify_pick_kernel<E, PIECES>), dim3((unsigned)a.batch), dim3(kThreads), 0, s, a);
   return hipGetLastError();
 }
@@ -706,8 +836,8 @@ template <Elt E> hipError_t launch_type(const VerifyArgs& a, hipStream_t s) {
 
 }  // namespace
 
-int64_t verify_workspace(int64_t batch, int64_t tokens, int64_t chunks) {
-  return up16(batch * tokens * chunks * (int64_t)sizeof(Stat)) + up16(batch * chunks * (int64_t)sizeof(Rest)) +
+int64_t verify_workspace(int64_t batch, int64_t tokens, int64_t segments) {
+  return up16(batch * tokens * segments * (int64_t)sizeof(Stat)) + up16(batch * segments * (int64_t)sizeof(Rest)) +
          up16(batch * (int64_t)sizeof(End)) + batch * tokens * 8;
 }
 
