@@ -38,8 +38,9 @@ template <Elt T> __device__ __forceinline__ float value_of(i32x4 x, int i) {
 }
 
 // Workgroups in the order (sequence, block, head, k or v).  HOLD: a block is at
-// most kHold pieces a thread, which stay in registers.
-template <Elt T, Elt C, bool HOLD>
+// most kHold pieces a thread, which stay in registers.  PAST_L2: the rows, read once,
+// go past the caches.
+template <Elt T, Elt C, bool HOLD, bool PAST_L2>
 __global__ __launch_bounds__(kThreads) void kv_block_kernel(KvArgs a, int g, int blocks) {
   constexpr float Q = kv::kTop<C>;
   const KvCache& c = a.cache;
@@ -84,13 +85,17 @@ __global__ __launch_bounds__(kThreads) void kv_block_kernel(KvArgs a, int g, int
       top = max(top, max(w & 0xffffu, w >> 16));
     }
   };
+  auto load = [&](const uint16_t* p) {
+    if constexpr (PAST_L2) return __builtin_nontemporal_load((const i32x4*)p);
+    else return *(const i32x4*)p;
+  };
   i32x4 held[kHold];
   if constexpr (HOLD) {
 #pragma unroll
     for (int i = 0; i < kHold; ++i) {
       const int r = row0 + i * rows;
       held[i] = i32x4{0, 0, 0, 0};
-      if (in && r >= old && r < end) held[i] = *(const i32x4*)(x + r * xs);
+      if (in && r >= old && r < end) held[i] = load(x + r * xs);
     }
 #pragma unroll
     for (int i = 0; i < kHold; ++i) larger(held[i]);
@@ -151,7 +156,9 @@ template <Elt T, Elt C> hipError_t launch_blocks(const KvArgs& a, hipStream_t st
   const int64_t per = 2 * (int64_t)a.cache.kv_heads * blocks;
   if (a.batch > (int64_t)(UINT32_MAX / kThreads) / per) return hipErrorInvalidConfiguration;
   const bool hold = size <= (int64_t)kHold * (kThreads >> g);
-  auto kern = hold ? kv_block_kernel<T, C, true> : kv_block_kernel<T, C, false>;
+  const bool past_l2 = a.batch * a.tokens * a.cache.kv_heads * a.cache.head_dim * 4 > (32ll << 20);
+  auto kern = !hold ? kv_block_kernel<T, C, false, false>
+                    : past_l2 ? kv_block_kernel<T, C, true, true> : kv_block_kernel<T, C, true, false>;
   hipLaunchKernelGGL(kern, dim3((unsigned)(a.batch * per)), dim3(kThreads), 0, stream, a, g, (int)blocks);
   return hipGetLastError();
 }

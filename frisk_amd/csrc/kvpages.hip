@@ -121,6 +121,9 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(KvCopyPagesArgs a) {
 // ---- tables ------------------------------------------------------------------------
 
 constexpr int kTableThreads = 1024, kTableWaves = kTableThreads / 64;
+constexpr int kListed = 1024;  // new pages that are looked up
+constexpr int kPieces = 8;  // pieces of four entries that a lane has at once
+typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 // Sum of `x` over the threads before this one; `all`: over all.  wave_sums: LDS.
 __device__ __forceinline__ int before(int x, int* wave_sums, int& all) {
@@ -172,14 +175,15 @@ __device__ __forceinline__ Span span_of(const KvPagesArgs& a, int b) {
 // the first of those that would write it; the others get a copy.  Free pages
 // are then counted off by number to the entries that lack one, by place.
 __global__ __launch_bounds__(kTableThreads) void kv_pages_kernel(KvPagesArgs a) {
-  extern __shared__ uint32_t lds[];
-  const int words = (a.pages + 31) / 32;
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+  const int words = (a.pages + 31) / 32, room = (words + 3) & ~3;
   uint32_t* used = lds;              // [words]
-  uint32_t* twice = used + words;    // [words] pages that several sequences would write
-  int* last = (int*)(twice + words);  // [batch] the page that a row would write, -1: none; then -2 - it: a copy
+  uint32_t* twice = used + room;     // [words] pages that several sequences would write
+  int* last = (int*)(twice + room);  // [batch] the page that a row would write, -1: none; then -2 - it: a copy
   int* need = last + a.batch;        // [batch] entries without a page; then the sum before
   int* ranks = need + a.batch;       // [kTableThreads + 1] free pages before a thread's words
-  int* sums = ranks + kTableThreads + 1;
+  int* list = ranks + kTableThreads + 1;  // [kListed] the first free pages
+  int* sums = list + kListed;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int w = tid; w < words; w += kTableThreads) {
     uint32_t bits = 0;
@@ -190,28 +194,64 @@ __global__ __launch_bounds__(kTableThreads) void kv_pages_kernel(KvPagesArgs a) 
   }
   __syncthreads();
   auto bit = [](const uint32_t* m, int p) { return (m[p >> 5] >> (p & 31)) & 1u; };
-  auto entry = [&](const Span& s, int i) {
-    const int p = a.table[(int64_t)s.parent * a.table_stride + i];
-    return p >= 0 && p < a.pages ? p : -1;
-  };
-  // Pages kept whole; entries that lack one.
-  for (int b = wave; b < a.batch; b += kTableWaves) {
-    const Span s = span_of(a, b);
-    const int whole = s.part ? s.kept - 1 : s.kept;
-    int lack = 0;
-    for (int i = lane; i < whole; i += 64) {
-      const int p = entry(s, i);
-      if (p >= 0) atomicOr(&used[p >> 5], 1u << (p & 31));
-      else ++lack;
-    }
+  // Sixteen lanes have a row, 512 of its entries at a time (entry i0 + 64 j + 4 sub + e is
+  // element e of piece j), so that the loads of four rows are under way together.  An
+  // entry costs the one CU an instruction for every 64 of them: pieces that a row keeps whole are taken
+  // as they are, others and the rest of the row an entry a lane.
+  const int sub = lane & 15;
+  const uint64_t group = 0xffffull << (lane & 48);
+  auto for_rows = [&](auto piece, auto rest) {
+    for (int b0 = wave * 4; b0 < a.batch; b0 += kTableWaves * 4) {
+      const int b = b0 + (lane >> 4);
+      Span s = {-1, 0, 0, 0};
+      if (b < a.batch) s = span_of(a, b);
+      const int whole = s.part ? s.kept - 1 : s.kept;  // pages kept whole
+      const int32_t* row = a.table + (int64_t)max(s.parent, 0) * a.table_stride;
+      bool clean = true;
+      for (int i0 = 0; i0 < a.max_pages; i0 += 64 * kPieces) {
+        i32x4 p[kPieces];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) lack += __shfl_xor(lack, d);
-    if (lane == 0) {
-      const int p = s.part ? entry(s, s.kept - 1) : -1;
-      last[b] = p;
-      need[b] = lack + s.wanted - s.kept + (s.part && p < 0 ? 1 : 0);
+        for (int j = 0; j < kPieces; ++j) {
+          const int i = i0 + 64 * j + 4 * sub;
+          if (i + 4 <= whole) p[j] = *(const i32x4_any*)(row + i);
+        }
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) clean &= piece(b, s, whole, i0 + 64 * j + 4 * sub, p[j]);
+      }
+      const bool all = !(__builtin_amdgcn_ballot_w64(!clean) & group);
+      rest(b, s, whole, row, all);
     }
-  }
+  };
+  auto valid = [&](int p) { return (uint32_t)p < (uint32_t)a.pages; };
+  auto mark = [&](int p) { atomicOr(&used[p >> 5], 1u << (p & 31)); };
+  // Pages kept whole; entries that lack one.
+  int lack = 0;
+  for_rows(
+      [&](int, const Span&, int whole, int i, const i32x4& p) {
+        if (i + 4 > whole) return true;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (valid(p[e])) mark(p[e]);
+          else ++lack;
+        }
+        return true;
+      },
+      [&](int b, const Span& s, int whole, const int32_t* row, bool) {
+        const int i = (whole & ~3) + sub;  // the entries behind the pieces, and the row's last
+        int p = -1;
+        if (i < s.kept && sub < 4) {
+          p = row[i];
+          p = valid(p) ? p : -1;
+          lack += p < 0;
+          if (i < whole && p >= 0) mark(p);
+        }
+        if (b < a.batch && i == whole) last[b] = s.part ? p : -1;
+        int all = lack;
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) all += __shfl_xor(all, d);
+        if (b < a.batch && sub == 0) need[b] = all + s.wanted - s.kept;
+        lack = 0;
+      });
   __syncthreads();
   // Last pages that a sequence keeps whole are copied ...
   for (int b = tid; b < a.batch; b += kTableThreads)
@@ -229,7 +269,11 @@ __global__ __launch_bounds__(kTableThreads) void kv_pages_kernel(KvPagesArgs a) 
     if (b < a.batch) {
       const int p = last[b];
       if (p >= 0 && bit(twice, p))
-        for (int i = 0; i < b && !copies; ++i) copies = last[i] == p || last[i] == -2 - p;
+        for (int i = 0; i < b && !copies; i += 4) {
+          const i32x4 four = *(const i32x4*)(last + i);  // (what lies behind the last row: of `need`)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) copies |= i + e < b && (four[e] == p || four[e] == -2 - p);
+        }
     }
     __syncthreads();
     if (copies) last[b] = -2 - last[b];
@@ -260,9 +304,20 @@ __global__ __launch_bounds__(kTableThreads) void kv_pages_kernel(KvPagesArgs a) 
     if (a.lacking) *a.lacking = max(0, total - have);
   }
   __syncthreads();
+  // The first of them, in order.
+  for (int first = 0; first < a.pages; first += kTableThreads) {
+    const int page = first + tid, w = page >> 5, owner = w / per;
+    if (ranks[(first >> 5) / per] >= min(total, kListed)) break;  // (the same in all threads)
+    if (page >= a.pages || !((free_of(w) >> (page & 31)) & 1)) continue;
+    int n = ranks[owner] + __popc(free_of(w) & ((1u << (page & 31)) - 1));
+    for (int before_w = owner * per; before_w < w; ++before_w) n += __popc(free_of(before_w));
+    if (n < kListed) list[n] = page;
+  }
+  __syncthreads();
   // The n-th free page, or -1.
   auto nth = [&](int n) {
     if (n >= have) return -1;
+    if (n < kListed) return list[n];
     int lo = 0, hi = kTableThreads;  // ranks[lo] <= n < ranks[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
@@ -281,30 +336,47 @@ __global__ __launch_bounds__(kTableThreads) void kv_pages_kernel(KvPagesArgs a) 
     }
     return -1;
   };
-  for (int b = wave; b < a.batch; b += kTableWaves) {
-    const Span s = span_of(a, b);
-    const int page = last[b];
-    int lacks = need[b], copy = -1;
-    for (int i0 = 0; i0 < a.max_pages; i0 += 64) {
-      const int i = i0 + lane;
-      int p = -1;
-      if (i < s.kept) p = s.part && i == s.kept - 1 ? max(page, -1) : entry(s, i);
-      const bool without = i < s.wanted && p < 0;
-      const uint64_t ask = __builtin_amdgcn_ballot_w64(without);
-      if (without) p = nth(lacks + __popcll(ask & ((1ull << lane) - 1)));
-      lacks += __popcll(ask);
-      if (i < a.max_pages) a.out[(int64_t)b * a.out_stride + i] = p;
-      if (page < -1 && i == s.kept - 1) copy = p;
-    }
-    // (The copy's page lies in the lane of its entry.)
-    const int where = s.kept > 0 ? (s.kept - 1) & 63 : 0;
-    copy = __shfl(copy, where);
-    if (lane == 0) {
-      if (a.src) a.src[b] = copy >= 0 ? -2 - page : -1;
-      if (a.dst) a.dst[b] = copy;
-      if (a.rows) a.rows[b] = copy >= 0 ? s.part : 0;
-    }
-  }
+  for_rows(
+      [&](int b, const Span& s, int whole, int i, const i32x4& p) {
+        int32_t* out = a.out + (int64_t)b * a.out_stride + i;
+        if (b >= a.batch) return true;
+        if (i + 4 <= whole) {
+          if (!valid(p[0]) || !valid(p[1]) || !valid(p[2]) || !valid(p[3])) return false;
+          *(i32x4_any*)out = p;
+        } else if (i >= s.wanted && i + 4 <= a.max_pages) {
+          *(i32x4_any*)out = i32x4{-1, -1, -1, -1};
+        }
+        return true;
+      },
+      [&](int b, const Span& s, int whole, const int32_t* row, bool clean) {
+        if (b >= a.batch) return;
+        const int page = last[b], end = s.part ? whole : -1;  // the entry that the row writes
+        int32_t* out = a.out + (int64_t)b * a.out_stride;
+        int lacks = need[b];
+        if (sub == 0 && (end < 0 || page >= -1)) {
+          if (a.src) a.src[b] = -1;
+          if (a.dst) a.dst[b] = -1;
+          if (a.rows) a.rows[b] = 0;
+        }
+        const int stop = min((s.wanted + 3) & ~3, a.max_pages);
+        for (int i0 = clean ? whole & ~3 : 0; i0 < stop; i0 += 16) {
+          const int i = i0 + sub;
+          int p = -1;
+          if (i < s.kept) p = i == end ? max(page, -1) : row[i];
+          const bool without = i < s.wanted && !valid(p);
+          const uint64_t ask = __builtin_amdgcn_ballot_w64(without) & group;
+          if (without) p = nth(lacks + __popcll(ask & ((1ull << lane) - 1)));
+          lacks += __popcll(ask);
+          if (i < stop) out[i] = i < s.wanted ? p : -1;
+          if (i == end && page < -1) {
+            if (a.src) a.src[b] = p >= 0 ? -2 - page : -1;
+            if (a.dst) a.dst[b] = p;
+            if (a.rows) a.rows[b] = p >= 0 ? s.part : 0;
+          }
+        }
+        const int i = (a.max_pages & ~3) + sub;  // a last piece that is none
+        if (i >= stop && i < a.max_pages) out[i] = -1;
+      });
 }
 
 }  // namespace
@@ -324,7 +396,7 @@ hipError_t kv_copy_pages(const KvCopyPagesArgs& a, hipStream_t s) {
 }
 
 int64_t kv_pages_lds(int64_t batch, int64_t pages) {
-  return ((pages + 31) / 32 * 2 + 2 * batch + kTableThreads + 1 + kTableWaves) * 4;
+  return (((pages + 31) / 32 + 3) / 4 * 8 + 2 * batch + kTableThreads + 1 + kListed + kTableWaves) * 4;
 }
 
 hipError_t kv_pages(const KvPagesArgs& a, hipStream_t s) {

@@ -592,7 +592,7 @@ int frisk_kv_copy_pages(const frisk_kv_copy_pages_desc* desc, void* stream);
  * that no row has is free: there is no other state.
  * table and out are [batch, max_pages], row strides at least that, and share no memory; lengths
  * and outputs are device arrays.  page_size is a power of two.  FRISK_EUNSUP beyond the kernel's
- * memory: pages / 4 + 8 batch bytes up to 155 KB.
+ * memory: pages / 4 + 8 batch up to 155000 bytes.
  */
 typedef struct frisk_kv_pages_desc {
   int64_t batch, max_pages, pages, page_size;
