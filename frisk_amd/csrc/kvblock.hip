@@ -3,7 +3,10 @@
 // A workgroup has the rows of one block, head and tensor: it finds the largest of
 // the new ones, and with it the block's scale (include/frisk_hip.h states the
 // arithmetic, each step of it one f32 operation), and writes their codes; only
-// where the scale grows are the codes before them read and written again.
+// where the scale grows are the codes before them read and written again.  HBM
+// bounds it: 4 x 8192 tokens, 8 heads of 128 in int8, 201 MB in 36 us with 32 slots a scale,
+// 32 with 128 (part of it from the last-level cache; with the rows read again 51).  A wave for a block of 32
+// slots took 39, rows past the L2s as long as through them.
 
 #include "kvcache.h"
 
@@ -12,7 +15,6 @@ namespace frisk {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kHold = 8;  // pieces of 8 values that a thread keeps between the passes
 
 // Eight values as two words of codes.
 template <Elt C> __device__ __forceinline__ i32x2 round8(const float (&y)[8]) {
@@ -37,11 +39,11 @@ template <Elt T> __device__ __forceinline__ float value_of(i32x4 x, int i) {
   return T == Elt::BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
 }
 
-// Workgroups in the order (sequence, block, head, k or v).  HOLD: a block is at
-// most kHold pieces a thread, which stay in registers.  PAST_L2: the rows, read once,
-// go past the caches.
-template <Elt T, Elt C, bool HOLD, bool PAST_L2>
-__global__ __launch_bounds__(kThreads) void kv_block_kernel(KvArgs a, int g, int blocks) {
+// Workgroups in the order (sequence, block, head, k or v).  A block is at most
+// HOLD pieces of 8 values a thread, which stay in registers between the passes (0: they are
+// read again).
+template <Elt T, Elt C, int HOLD>
+__global__ __launch_bounds__(kThreads, 4) void kv_block_kernel(KvArgs a, int g, int blocks) {
   constexpr float Q = kv::kTop<C>;
   const KvCache& c = a.cache;
   const int shift = c.scale_shift, size = 1 << shift;
@@ -85,20 +87,16 @@ __global__ __launch_bounds__(kThreads) void kv_block_kernel(KvArgs a, int g, int
       top = max(top, max(w & 0xffffu, w >> 16));
     }
   };
-  auto load = [&](const uint16_t* p) {
-    if constexpr (PAST_L2) return __builtin_nontemporal_load((const i32x4*)p);
-    else return *(const i32x4*)p;
-  };
-  i32x4 held[kHold];
+  i32x4 held[HOLD ? HOLD : 1];
   if constexpr (HOLD) {
 #pragma unroll
-    for (int i = 0; i < kHold; ++i) {
+    for (int i = 0; i < HOLD; ++i) {
       const int r = row0 + i * rows;
       held[i] = i32x4{0, 0, 0, 0};
-      if (in && r >= old && r < end) held[i] = load(x + r * xs);
+      if (in && r >= old && r < end) held[i] = *(const i32x4*)(x + r * xs);
     }
 #pragma unroll
-    for (int i = 0; i < kHold; ++i) larger(held[i]);
+    for (int i = 0; i < HOLD; ++i) larger(held[i]);
   } else {
     for (int r = row0; r < end; r += rows)
       if (in && r >= old) larger(*(const i32x4*)(x + r * xs));
@@ -125,8 +123,10 @@ __global__ __launch_bounds__(kThreads) void kv_block_kernel(KvArgs a, int g, int
   };
   if constexpr (HOLD) {
 #pragma unroll
-    for (int i = 0; i < kHold; ++i) {
+    for (int i = 0; i < HOLD; ++i) {
       const int r = row0 + i * rows;
+      // (Widened here: all f16 pieces at once took 233 registers.)
+      asm volatile("" : "+v"(held[i]));
       if (in && r >= old && r < end) put(r, held[i]);
     }
   } else {
@@ -155,10 +155,10 @@ template <Elt T, Elt C> hipError_t launch_blocks(const KvArgs& a, hipStream_t st
   if (blocks > INT32_MAX / 2) return hipErrorInvalidConfiguration;
   const int64_t per = 2 * (int64_t)a.cache.kv_heads * blocks;
   if (a.batch > (int64_t)(UINT32_MAX / kThreads) / per) return hipErrorInvalidConfiguration;
-  const bool hold = size <= (int64_t)kHold * (kThreads >> g);
-  const bool past_l2 = a.batch * a.tokens * a.cache.kv_heads * a.cache.head_dim * 4 > (32ll << 20);
-  auto kern = !hold ? kv_block_kernel<T, C, false, false>
-                    : past_l2 ? kv_block_kernel<T, C, true, true> : kv_block_kernel<T, C, true, false>;
+  const int64_t pieces = (size + (kThreads >> g) - 1) / (kThreads >> g);
+  auto kern = pieces <= 1 ? kv_block_kernel<T, C, 1> : pieces <= 2 ? kv_block_kernel<T, C, 2>
+            : pieces <= 4 ? kv_block_kernel<T, C, 4> : pieces <= 8 ? kv_block_kernel<T, C, 8>
+                                                                   : kv_block_kernel<T, C, 0>;
   hipLaunchKernelGGL(kern, dim3((unsigned)(a.batch * per)), dim3(kThreads), 0, stream, a, g, (int)blocks);
   return hipGetLastError();
 }
