@@ -633,6 +633,23 @@ inline VerifyPlan verify_plan(int64_t batch, int64_t tokens, int64_t vocab, int 
   return {pieces, segments(pieces)};
 }
 
+// Workgroups of kVerifyTableWaves with a table of weights (bf16) for each row of logits, or 0: none.
+// A table costs a lane 12 weights of 17 instructions, a segment through it saves some 20 of
+// its 32: it pays from two segments a wave on.  us of a call with and without, of b x t nodes in chains:
+//   vocabulary      64 x 32      64 x 8      8 x 64      8 x 8
+//   32000 (16)      74, 71       33.6, 34.1  36.2, 37.3  21.8, 21.8
+//   50304 (25)      82, 98       42, 44      44, 46      24.0, 24.0
+//   65536 (32)      87, 116      43, 48      45, 50      24.9, 23.1
+//   131072 (64)     155, 220     56, 70      56, 72      25.6, 25.7
+// (segments in brackets; workgroups of 16 waves 166, of 4 182 in the last line's first).
+constexpr int kVerifyTableWaves = 8;
+inline int64_t verify_tables(int64_t batch, int64_t tokens, int64_t segments, int cus) {
+  const int64_t whole = (segments + kVerifyTableWaves - 1) / kVerifyTableWaves;  // a segment a wave
+  const int64_t per = batch * tokens * whole / (4 * (int64_t)cus);
+  if (segments < 24 || per < 2) return 0;
+  return std::max<int64_t>(1, whole / per);
+}
+
 // Attention of new tokens over a cache (attn_tree_mfma.h, attn_tree_rows.hip).
 // Rows: one query row a workgroup, head dims without a matrix-core kernel.
 // Keys: a tile of 32 query rows of a kv head a workgroup, whose waves divide the

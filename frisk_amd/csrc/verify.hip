@@ -95,10 +95,14 @@ __device__ __forceinline__ double scale_by(double x, double shifted) {
   asm("v_lshl_add_u32 %0, %1, 20, %0" : "+v"(hi) : "v"(k));
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)u);
 }
+// 2^t for |t| <= 1000.
+__device__ __forceinline__ double pow2_any(double t) {
+  const double shifted = t + kRound;
+  return scale_by(pow2_fraction(t - (shifted - kRound)), shifted);
+}
 // 2^t for t <= 0: the exponent is added to the bits of 2^f.  0 below -1000 and for NaN.
 __device__ __forceinline__ double pow2(double t) {
-  const double held = __builtin_fmax(t, -1000.0), shifted = held + kRound, f = held - (shifted - kRound);
-  const double w = scale_by(pow2_fraction(f), shifted);
+  const double w = pow2_any(__builtin_fmax(t, -1000.0));
   return t > -1000.0 ? w : 0.0;
 }
 
@@ -449,6 +453,108 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, int
       if (last) rests[g] = Rest{st.s, st.s, st.m, st.at};
       else stats[g] = st;
     }
+    now = next;
+  }
+}
+
+// ---- rows of bf16 through a table ------------------------------------------------------
+
+// There are few bf16 numbers: the weights 2^(x c) of all of 2^-16 <= |x| < 2^7 are 5888
+// doubles, which a workgroup computes once, and a logit's is a read of LDS (five 32-bit
+// instructions and an addition of 64 bits in the place of 17 of 64).  c <= 7, so that they stay
+// within a double's range (and x c, up to 900, is off by 2^-44); segments with other numbers are
+// summed as the other types' are.  131072 logits of 32 rows of 8 trees: 33 us without the
+// table, 21 with it, which the reads of LDS and their conflicts bound (bytes: 11).
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+constexpr int kTableWaves = plan::kVerifyTableWaves, kTableThreads = 64 * kTableWaves;
+constexpr uint32_t kTableLeast = (127 - 16) << 7, kTableSize = 23 << 7;  // first magnitude, number of them
+constexpr uint32_t kNegative = 0x8000;  // bytes from a number's weight to its negative's
+constexpr int kTableBytes = kNegative + kTableSize * 8;
+static_assert(kTableSize * 8 <= kNegative, "a half for each sign");
+constexpr double kTableSteepest = 7.0;  // c
+
+// The statistics of segment g, if the table has all of its numbers.
+template <int PIECES>
+__device__ __forceinline__ bool table_stat(const VerifyArgs& a, const Row<Elt::BF16>& r, int g,
+                                           const Held<Elt::BF16, PIECES>& h, double factor, const char* table,
+                                           Stat& st) {
+  // (The first and the last segment may have a head or a tail.)
+  if (g == 0 || (g + 1) * PIECES * 64 > r.full || g == a.segments - 1) return false;
+  u16x2 least = {0xffff, 0xffff}, most = {0, 0};
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const u16x2 m = __builtin_bit_cast(u16x2, (uint32_t)h.w[i][k] & 0x7fff7fffu);
+      least = __builtin_elementwise_min(least, m);
+      most = __builtin_elementwise_max(most, m);
+    }
+  const bool out = min(least[0], least[1]) < kTableLeast || max(most[0], most[1]) >= kTableLeast + kTableSize;
+  if (__builtin_amdgcn_ballot_w64(out)) return false;
+  float m = -__builtin_inff();
+  double s[4] = {0.0, 0.0, 0.0, 0.0}, read[2][8];
+#pragma unroll
+  for (int i = 0; i <= PIECES; ++i) {
+    // A piece's reads, then the additions of the one before.
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (i == PIECES) continue;
+      const uint32_t w = (uint32_t)h.w[i][k];
+      m = __builtin_elementwise_maximum(m, __builtin_elementwise_maximum(
+                 __builtin_bit_cast(float, w << 16), __builtin_bit_cast(float, w & 0xffff0000u)));
+      const u16x2 at = (__builtin_bit_cast(u16x2, w & 0x7fff7fffu) - (unsigned short)kTableLeast) << (unsigned short)3;
+      const uint32_t both = (w & 0x80008000u) | __builtin_bit_cast(uint32_t, at);
+      read[i & 1][2 * k] = *(const double*)(table + (both & 0xffff));
+      read[i & 1][2 * k + 1] = *(const double*)(table + (both >> 16));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (i == 0) continue;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] += read[(i + 1) & 1][2 * k] + read[(i + 1) & 1][2 * k + 1];
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  m = wave_max(m);
+  // The sum relative to the maximum, as the other segments' are.
+  const double sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
+  st = Stat{sum * pow2_any(-(double)m * factor), m, INT32_MAX};
+  return true;
+}
+
+// As verify_rows_kernel for the rows of nodes that have children.
+template <int PIECES>
+__global__ __launch_bounds__(kTableThreads) void verify_table_kernel(VerifyArgs a, int groups) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, step = groups * kTableWaves;
+  uint32_t id = blockIdx.x;
+  int g = __builtin_amdgcn_readfirstlane((int)(id % groups * kTableWaves + (tid >> 6)));
+  id /= groups;
+  const int t = id % a.tokens;
+  const int64_t b = id / a.tokens;
+  const int n = nodes_of(a, b);
+  uint64_t child = 0;  // (every wave looks for itself: all of them find the same)
+  for (int i0 = t + 1; i0 < n && !child; i0 += 64)
+    child = __builtin_amdgcn_ballot_w64(i0 + lane < n && a.parents[b * a.tokens + min(i0 + lane, n - 1)] == t);
+  if (!child) return;
+  const double factor = factor_of(a, b);
+  const Row<Elt::BF16> r = row_of<Elt::BF16>(a, b, t);
+  Stat* stats = layout(a).stats + (b * a.tokens + t) * a.segments;
+  Held<Elt::BF16, PIECES> now, next;
+  if (g < a.segments) load_segment<Elt::BF16, PIECES>(a, r, g, now);
+  const bool tabled = factor > 0.0 && factor <= kTableSteepest;
+  if (tabled) {
+    for (uint32_t i = tid; i < 2 * kTableSize; i += kTableThreads) {
+      const uint32_t magnitude = kTableLeast + (i >> 1);
+      const float x = bf16_bits_to_f32((uint16_t)((i & 1) << 15 | magnitude));
+      *(double*)(smem + (i & 1) * kNegative + (i >> 1) * 8) = pow2_any((double)x * factor);
+    }
+  }
+  __syncthreads();
+  for (; g < a.segments; g += step) {
+    if (g + step < a.segments) load_segment<Elt::BF16, PIECES>(a, r, g + step, next);
+    Stat st;
+    if (!tabled || !table_stat<PIECES>(a, r, g, now, factor, smem, st))
+      st = segment_stat<Elt::BF16, PIECES>(a, r, g, now, factor, nullptr, 0);
+    if (lane == 0) stats[g] = st;
     now = next;
   }
 }
@@ -817,7 +923,16 @@ template <Elt E, int PIECES> hipError_t launch_pieces(const VerifyArgs& a, hipSt
     // As many segments a wave as leave 32 waves for a CU.
     const int64_t per = a.batch * a.tokens * groups / (8 * (int64_t)device_cus());
     const int64_t some = (groups + std::max<int64_t>(per, 1) - 1) / std::max<int64_t>(per, 1);
-    hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * a.tokens * some)), dim3(kThreads), 0, s, a, (int)some, 0);
+    if constexpr (E == Elt::BF16 && PIECES == 4) {
+      const int64_t tables = plan::verify_tables(a.batch, a.tokens, a.segments, device_cus());
+      if (tables)
+        hipLaunchKernelGGL(verify_table_kernel<PIECES>, dim3((unsigned)(a.batch * a.tokens * tables)),
+                           dim3(kTableThreads), kTableBytes, s, a, (int)tables);
+      else
+        hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * a.tokens * some)), dim3(kThreads), 0, s, a, (int)some, 0);
+    } else {
+      hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * a.tokens * some)), dim3(kThreads), 0, s, a, (int)some, 0);
+    }
     hipLaunchKernelGGL((verify_walk_kernel<E>), dim3((unsigned)a.batch), dim3(kWalkers),
                        (unsigned)(a.tokens * 52), s, a);
   }

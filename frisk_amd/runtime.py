@@ -1088,10 +1088,10 @@ def tree_attn(q, cache, ctx_len, o, *, mask=None, new_len=None, sm_scale=None, l
 
 
 def _words(t, shape, dtype, name: str) -> int:
-    """The pointer of a contiguous device tensor of that shape and dtype, or 0."""
+    """The pointer of a contiguous tensor of that shape and dtype, or 0."""
     if t is None:
         return 0
-    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or not t.is_cuda:
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} device tensor {list(shape)}")
     return t.data_ptr()
 
@@ -1146,16 +1146,16 @@ def tree_verify(logits, drafts, parents, uniform, final, *, draft_probs=None, te
         token = _empty((b,), torch.int32, logits.device, stream)
     dev = _same_device(logits, drafts, parents, uniform, final, draft_probs, temperature, new_len, path, count,
                        token, probs)
-    i32, f32 = torch.int32, torch.float32
+    i32, f32, one, all_ = torch.int32, torch.float32, shape[:1], shape[:2]
     try:
         head = _verify_pack.pack(
             b, t, v, torch_dtype_code(logits.dtype), logits.data_ptr(), ls[0], ls[1],
-            _words(drafts, (b, t), i32, "drafts"), _words(parents, (b, t), i32, "parents"),
-            _words(uniform, (b, t), f32, "uniform"), _words(final, (b,), f32, "final"),
+            _words(drafts, all_, i32, "drafts"), _words(parents, all_, i32, "parents"),
+            _words(uniform, all_, f32, "uniform"), _words(final, one, f32, "final"),
             0 if draft_probs is None else draft_probs.data_ptr(), qs[0], qs[1],
-            _words(temperature, (b,), f32, "temperature"), _lengths(new_len, b, "new_len"),
-            _words(path, (b, t), i32, "path"), _words(count, (b,), i32, "count"),
-            _words(token, (b,), i32, "token"), _words(probs, (b, t), f32, "probs"))
+            _words(temperature, one, f32, "temperature"), _words(new_len, one, i32, "new_len"),
+            _words(path, all_, i32, "path"), _words(count, one, i32, "count"),
+            _words(token, one, i32, "token"), _words(probs, all_, f32, "probs"))
     except _RANGE as e:
         raise _range_error(e) from None
     if workspace is True:

@@ -108,6 +108,25 @@ def test_children_of_one_node(kids):
             t.check(t.run())
 
 
+@pytest.mark.parametrize("shift", [0, 3])
+@pytest.mark.parametrize("temperature", [None, (0.5, 3.0), (0.21, 0.2), (0.0, 1e-3)])
+def test_many_rows_of_a_large_vocabulary(temperature, shift):
+    # Enough rows of bf16 that their weights come from a table, but for numbers that it does not
+    # hold: masked ones, zeros, the tiny and the large.
+    t = Trees(2, 256, 50021, "bf16", branch=1, shift=shift, temperature=temperature, seed=13 + shift)
+    t.check(t.run())
+    t.logits[0, ::3, 48000:] = -torch.inf
+    t.logits[0, 1::3, 3000:3010] = 0.0
+    t.logits[1, ::3, 20000:20100] *= 2.0 ** -20
+    t.logits[1, 1::3, 30000] = -300.0
+    t.logits[1, 2::3, 40000] = 200.0
+    t.check(t.run())
+    t.logits[0, 5, 17] = float("nan")
+    t.logits[1, 7, 45000] = float("inf")
+    t.logits[1, 9, :] = -torch.inf
+    t.check(t.run())
+
+
 def test_many_drafts_of_the_largest_tree():
     t = Trees(2, 1024, 50, branch=3, seed=9)
     t.uniform[0] *= 0.01
