@@ -127,24 +127,26 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pair_chunks, 
     }
     return;
   }
-  const int64_t start = a.start ? a.start[b] : 0, place = b * a.pos_sb + s * a.pos_ss;
-  auto position = [&](int64_t at) {
-    return start + (a.position_bits == 64 ? ((const int64_t*)a.positions)[at] : ((const int32_t*)a.positions)[at]);
-  };
-  int64_t p[AXES ? kRopeAxes : 1];
-  p[0] = a.positions ? position(place) : start + s;
+  int64_t p = a.start ? a.start[b] : 0;
+  [[maybe_unused]] int64_t more[kRopeAxes];  // the positions on the other axes
   if constexpr (AXES) {
 #pragma unroll
-    for (int x = 1; x < kRopeAxes; ++x) p[x] = x < a.axes ? position(place + x * a.pos_sa) : p[0];
+    for (int x = 1; x < kRopeAxes; ++x) {
+      const int64_t at = b * a.pos_sb + s * a.pos_ss + (x < a.axes ? x : 0) * a.pos_sa;
+      more[x] = p + (a.position_bits == 64 ? ((const int64_t*)a.positions)[at] : ((const int32_t*)a.positions)[at]);
+    }
   }
+  if (!a.positions) p += s;
+  else if (a.position_bits == 64) p += ((const int64_t*)a.positions)[b * a.pos_sb + s * a.pos_ss];
+  else p += ((const int32_t*)a.positions)[b * a.pos_sb + s * a.pos_ss];
   float cs[NP], sn[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    int64_t mine = p[0];
+    int64_t mine = p;
     if constexpr (AXES) {
       const int axis = a.pair_axis[chunk * NP + i];
 #pragma unroll
-      for (int x = 1; x < kRopeAxes; ++x) mine = axis == x ? p[x] : mine;
+      for (int x = 1; x < kRopeAxes; ++x) mine = axis == x ? more[x] : mine;
     }
     const SinCos r = sincos_turns((uint64_t)mine * a.freq[chunk * NP + i]);
     cs[i] = r.c * a.amplitude;
