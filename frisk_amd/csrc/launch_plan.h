@@ -619,7 +619,12 @@ inline int64_t attn_workspace(int64_t batch_heads, int64_t seq_q, int64_t seq_k,
 // ---------------------------------------------------------------------------
 // Verification of drafted tokens (verify.hip): nodes of a tree at most, and how a
 // row of `vocab` logits of `bytes` is cut into segments: a wave's, with `pieces`
-// pieces of 16 B a lane.
+// pieces of 16 B a lane.  Four, but one where four leave SIMDs without a wave and a row still has
+// no more than the 64 segments that a wave of the walk and of the last launch takes at once.
+// us of a call with four, with one (batch x nodes):
+//   bf16, 32000:  1 x 1  10.1, 9.2;  8 x 6  21.3, 20.3;  64 x 1  10.8, 11.5;  8 x 16  25.7, 27.2
+//   bf16, 131072: 1 x 1  9.9, 10.4;  1 x 8  19.4, 20.4;  8 x 1   10.4, 11.9;  64 x 1  15.3, 21.5
+//   f32:          16 x 6 of 50257  23.8, 30.0;  64 x 1 of 131072  17.7, 30.2
 constexpr int64_t kVerifyNodes = 1024;
 constexpr int64_t kVerifyVocab = 1 << 24;
 struct VerifyPlan {
@@ -629,7 +634,7 @@ struct VerifyPlan {
 inline VerifyPlan verify_plan(int64_t batch, int64_t tokens, int64_t vocab, int bytes) {
   const int64_t whole = std::max<int64_t>(vocab * bytes / 16, 1);
   auto segments = [&](int pieces) { return (whole + 64 * pieces - 1) / (64 * pieces); };
-  const int pieces = batch * tokens * segments(4) >= 2048 ? 4 : 1;
+  const int pieces = batch * tokens * segments(4) < 1024 && segments(1) <= 64 ? 1 : 4;
   return {pieces, segments(pieces)};
 }
 

@@ -562,7 +562,8 @@ int frisk_kv_compact(const frisk_kv_compact_desc* desc, void* stream);
 
 /* Copies pages src[i] to dst[i] (i < pairs): k, v and their scales, the first
  * rows[i] slots (all, if rows is NULL; with scale_block the scales of the blocks that
- * these lie in); the other slots are left as they were.  A pair with a page outside 0 .. pages
+ * these lie in, so that the other slots of such a block no longer hold what they did); the other
+ * slots are left as they were.  A pair with a page outside 0 .. pages
  * - 1 is left out.  Pages copied to must be distinct, and none is copied from. */
 typedef struct frisk_kv_copy_pages_desc {
   int64_t pairs;
@@ -633,7 +634,7 @@ int frisk_kv_pages(const frisk_kv_pages_desc* desc, void* stream);
  * one.  A row with a NaN, with +infinity or without a logit above -infinity gives no
  * probabilities (probs NaN): the walk ends there and token[b] is -1.  A draft outside the vocabulary
  * is never accepted.  Only the first new_len[b] nodes take part (all, if NULL; below 1: the tree's
- * outputs are left as they were).  drafts, parents, uniform, path and probs are contiguous [batch, tokens],
+ * outputs are left as they were).  temperature is finite.  drafts, parents, uniform, path and probs are contiguous [batch, tokens],
  * final_uniform, temperature, new_len, count and token [batch].  tokens <= 1024, vocab <= 2^24.
  * workspace (16-byte aligned): at least frisk_tree_verify_workspace_size bytes; its contents before
  * a call do not matter, and calls that share one must not overlap in time.  No output overlaps another tensor.

@@ -56,6 +56,26 @@ def test_tables(b, n, page, pages):
         assert got == list(S.next_table(table, keep, want, page, pages, parent, held)), trial
 
 
+@pytest.mark.parametrize("n,page", [(1300, 4), (513, 1), (512, 16), (1024, 2), (515, 8)])
+def test_long_tables(n, page):
+    # More entries than four rows' lanes take at once, some of them no page.
+    rng = np.random.default_rng(n)
+    for wrong in (0.0, 0.01):
+        table = random_tables(rng, 7, n, page, 8 * n, wrong)
+        keep = [0, n * page, n * page - 1, 512 * page, min(513, n) * page, 1, int(rng.integers(0, n * page))]
+        want = [n * page, n * page, 0, 600 * page, n * page, 3 * page, n * page]
+        args = (table, keep, want, page, 8 * n, [1, 1, 2, 2, 5, 6, 0])
+        assert step(*args) == list(S.next_table(*args))
+
+
+def test_more_new_pages_than_are_listed():
+    # 4000 entries of empty rows out of 6000 pages, then out of 3000.
+    for pages in (6000, 3000):
+        held = np.random.default_rng(5).random(pages) < 0.1
+        args = ([[-1] * 100] * 40, [0] * 40, [800] * 40, 8, pages, None, held)
+        assert step(*args) == list(S.next_table(*args))
+
+
 def test_many_sequences_continue_one():
     # All of one parent within a page: the first writes it, the others copy.
     table = random_tables(np.random.default_rng(1), 300, 4, 8, 3000)

@@ -269,6 +269,33 @@ def test_refuses_wrong_arguments():
         rt.tree_verify(**good, temperature=torch.ones(2))
 
 
+def test_two_calls_at_once():
+    # On two streams, from two threads, with workspaces of their own.
+    import threading
+    trees = [Trees(3, 40, 9000, "bf16", dense=d, seed=20 + d) for d in (False, True)]
+    dev = lambda x: torch.as_tensor(x).cuda()  # noqa: E731
+    args = [(t.logits, dev(t.drafts), dev(t.parents), dev(t.uniform), dev(t.final)) for t in trees]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        side = torch.cuda.Stream()
+        for _ in range(20):
+            got[i].append(rt.tree_verify(*args[i], draft_probs=trees[i].q, stream=side))
+        side.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i, t in enumerate(trees):
+        probs = t.run()[3]
+        for out in got[i]:
+            t.check((*(x.cpu().numpy() for x in out), probs)) if out is got[i][0] else None
+            assert all(torch.equal(a, b) for a, b in zip(out, got[i][0]))
+
+
 def test_another_stream_and_a_graph():
     t = Trees(4, 17, 5000, "bf16", dense=True, seed=11)
     dev = lambda x: torch.as_tensor(x).cuda()  # noqa: E731
