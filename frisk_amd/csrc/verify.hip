@@ -464,14 +464,20 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, int
 // instructions and an addition of 64 bits in the place of 17 of 64).  c <= 7, so that they stay
 // within a double's range (and x c, up to 900, is off by 2^-44); segments with other numbers are
 // summed as the other types' are.  131072 logits of 32 rows of 8 trees: 33 us without the
-// table, 21 with it, which the reads of LDS and their conflicts bound (bytes: 11).
+// table, 20 with it, which the reads of LDS and their conflicts bound (bytes: 11).
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef short i16x2 __attribute__((ext_vector_type(2)));
 constexpr int kTableWaves = plan::kVerifyTableWaves, kTableThreads = 64 * kTableWaves;
 constexpr uint32_t kTableLeast = (127 - 16) << 7, kTableSize = 23 << 7;  // first magnitude, number of them
 constexpr uint32_t kNegative = 0x8000;  // bytes from a number's weight to its negative's
 constexpr int kTableBytes = kNegative + kTableSize * 8;
 static_assert(kTableSize * 8 <= kNegative, "a half for each sign");
 constexpr double kTableSteepest = 7.0;  // c
+
+// Where the magnitudes of two numbers lie in the table.
+__device__ __forceinline__ u16x2 place_of(uint32_t w) {
+  return __builtin_bit_cast(u16x2, w & 0x7fff7fffu) - (unsigned short)kTableLeast;
+}
 
 // The statistics of segment g, if the table has all of its numbers.
 template <int PIECES>
@@ -480,18 +486,29 @@ __device__ __forceinline__ bool table_stat(const VerifyArgs& a, const Row<Elt::B
                                            Stat& st) {
   // (The first and the last segment may have a head or a tail.)
   if (g == 0 || (g + 1) * PIECES * 64 > r.full || g == a.segments - 1) return false;
-  u16x2 least = {0xffff, 0xffff}, most = {0, 0};
+  // Magnitudes from the table's first on (smaller ones wrap round), and the largest number as an
+  // integer: right if it is positive.
+  u16x2 most = {0, 0};
+  i16x2 top = {-32768, -32768};
 #pragma unroll
   for (int i = 0; i < PIECES; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const u16x2 m = __builtin_bit_cast(u16x2, (uint32_t)h.w[i][k] & 0x7fff7fffu);
-      least = __builtin_elementwise_min(least, m);
-      most = __builtin_elementwise_max(most, m);
+      const uint32_t w = (uint32_t)h.w[i][k];
+      most = __builtin_elementwise_max(most, place_of(w));
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(i16x2, w));
     }
-  const bool out = min(least[0], least[1]) < kTableLeast || max(most[0], most[1]) >= kTableLeast + kTableSize;
-  if (__builtin_amdgcn_ballot_w64(out)) return false;
-  float m = -__builtin_inff();
+  if (__builtin_amdgcn_ballot_w64(max(most[0], most[1]) >= kTableSize)) return false;
+  uint32_t bits = (uint16_t)max(top[0], top[1]);
+  if (bits & 0x8000) {  // the lane has negative numbers only: the smallest magnitude
+    u16x2 least = {0xffff, 0xffff};
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2, (uint32_t)h.w[i][k]));
+    bits = min(least[0], least[1]);
+  }
+  const float m = wave_max(__builtin_bit_cast(float, bits << 16));
   double s[4] = {0.0, 0.0, 0.0, 0.0}, read[2][8];
 #pragma unroll
   for (int i = 0; i <= PIECES; ++i) {
@@ -500,9 +517,7 @@ __device__ __forceinline__ bool table_stat(const VerifyArgs& a, const Row<Elt::B
     for (int k = 0; k < 4; ++k) {
       if (i == PIECES) continue;
       const uint32_t w = (uint32_t)h.w[i][k];
-      m = __builtin_elementwise_maximum(m, __builtin_elementwise_maximum(
-                 __builtin_bit_cast(float, w << 16), __builtin_bit_cast(float, w & 0xffff0000u)));
-      const u16x2 at = (__builtin_bit_cast(u16x2, w & 0x7fff7fffu) - (unsigned short)kTableLeast) << (unsigned short)3;
+      const u16x2 at = place_of(w) << (unsigned short)3;
       const uint32_t both = (w & 0x80008000u) | __builtin_bit_cast(uint32_t, at);
       read[i & 1][2 * k] = *(const double*)(table + (both & 0xffff));
       read[i & 1][2 * k + 1] = *(const double*)(table + (both >> 16));
@@ -513,7 +528,6 @@ __device__ __forceinline__ bool table_stat(const VerifyArgs& a, const Row<Elt::B
     for (int k = 0; k < 4; ++k) s[k] += read[(i + 1) & 1][2 * k] + read[(i + 1) & 1][2 * k + 1];
     __builtin_amdgcn_sched_barrier(0);
   }
-  m = wave_max(m);
   // The sum relative to the maximum, as the other segments' are.
   const double sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
   st = Stat{sum * pow2_any(-(double)m * factor), m, INT32_MAX};
@@ -523,7 +537,7 @@ __device__ __forceinline__ bool table_stat(const VerifyArgs& a, const Row<Elt::B
 // As verify_rows_kernel for the rows of nodes that have children.
 template <int PIECES>
 __global__ __launch_bounds__(kTableThreads) void verify_table_kernel(VerifyArgs a, int groups) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ __attribute__((aligned(16))) char table[kTableBytes];
   const int tid = threadIdx.x, lane = tid & 63, step = groups * kTableWaves;
   uint32_t id = blockIdx.x;
   int g = __builtin_amdgcn_readfirstlane((int)(id % groups * kTableWaves + (tid >> 6)));
@@ -545,14 +559,14 @@ __global__ __launch_bounds__(kTableThreads) void verify_table_kernel(VerifyArgs 
     for (uint32_t i = tid; i < 2 * kTableSize; i += kTableThreads) {
       const uint32_t magnitude = kTableLeast + (i >> 1);
       const float x = bf16_bits_to_f32((uint16_t)((i & 1) << 15 | magnitude));
-      *(double*)(smem + (i & 1) * kNegative + (i >> 1) * 8) = pow2_any((double)x * factor);
+      *(double*)(table + (i & 1) * kNegative + (i >> 1) * 8) = pow2_any((double)x * factor);
     }
   }
   __syncthreads();
   for (; g < a.segments; g += step) {
     if (g + step < a.segments) load_segment<Elt::BF16, PIECES>(a, r, g + step, next);
     Stat st;
-    if (!tabled || !table_stat<PIECES>(a, r, g, now, factor, smem, st))
+    if (!tabled || !table_stat<PIECES>(a, r, g, now, factor, table, st))
       st = segment_stat<Elt::BF16, PIECES>(a, r, g, now, factor, nullptr, 0);
     if (lane == 0) stats[g] = st;
     now = next;
@@ -927,7 +941,7 @@ template <Elt E, int PIECES> hipError_t launch_pieces(const VerifyArgs& a, hipSt
       const int64_t tables = plan::verify_tables(a.batch, a.tokens, a.segments, device_cus());
       if (tables)
         hipLaunchKernelGGL(verify_table_kernel<PIECES>, dim3((unsigned)(a.batch * a.tokens * tables)),
-                           dim3(kTableThreads), kTableBytes, s, a, (int)tables);
+                           dim3(kTableThreads), 0, s, a, (int)tables);
       else
         hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * a.tokens * some)), dim3(kThreads), 0, s, a, (int)some, 0);
     } else {

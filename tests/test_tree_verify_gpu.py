@@ -127,6 +127,14 @@ def test_many_rows_of_a_large_vocabulary(temperature, shift):
     t.check(t.run())
 
 
+def test_many_rows_of_one_sign():
+    t = Trees(2, 256, 50021, "bf16", branch=1, temperature=(0.7, 1.0), seed=31)
+    t.logits.copy_(t.logits.float().abs() - 25.0)  # all negative, rest and peaks apart
+    t.check(t.run())
+    t.logits.copy_(t.logits.float() + 40.0)
+    t.check(t.run())
+
+
 def test_many_drafts_of_the_largest_tree():
     t = Trees(2, 1024, 50, branch=3, seed=9)
     t.uniform[0] *= 0.01
