@@ -7,15 +7,15 @@
 // unit does as many 64-bit as 32-bit multiply-adds, so a weight costs about 16
 // instructions.
 //
-// Up to four launches.  (1) The rows of nodes that have children, a wave for each
+// Three launches.  (1) The rows of nodes that have children, a wave for each
 // segment of a row, without a barrier: its maximum and sum.  (2) A workgroup per tree combines
 // them, takes every node's probability given its parent, and walks from the root.
-// (3) What is left of the probabilities at the last node, by segments: the same kernel as (1),
-// so that its code is in the instruction caches already; segments that no rejected
-// token lies in have their sums from (1).  (4) The segment, then the element, in which the sum
-// passes the last random number.  A tree of one node takes (3) and (4) only.  ((4) by the last
-// workgroup of (3) to arrive took longer: 16 arrivals at a word, each an exchange past the
-// L2 caches, are 15 us one after the other, the launch 5.)
+// (3) What is left of the probabilities at the last node, by segments: the same kernel as (1);
+// segments that no rejected token lies in have their sums from (1).  The tree's last workgroup to
+// arrive there finds the segment, then the element, in which the sum passes the last random
+// number (a launch of its own took 0.7 us longer).  (2) set the count of arrivals to 0, so that an
+// arrival is one addition; exchanges with a word of any content took 1 us each, one after the
+// other.  A tree of one node takes (3) without arrivals, and that search as a launch.
 
 #include <algorithm>
 
@@ -50,6 +50,7 @@ struct End {
   int node;      // -1: the tree takes no part, -2: no token
   int rounds;    // children rejected there
   int greedy;    // the token, if the temperature is 0 and it is known; -1: sample, -2: largest
+  int arrived;   // workgroups of (3) that have written their rests
 };
 
 struct Layout {
@@ -154,7 +155,7 @@ __device__ __forceinline__ int nodes_of(const VerifyArgs& a, int64_t b) {
 // Where a tree's walk ended; of trees of one node, which are not walked: at the root.
 __device__ __forceinline__ End end_of(const VerifyArgs& a, const Layout& l, int64_t b, double factor) {
   if (a.tokens > 1) return l.end[b];
-  return End{0.0, 0.0f, nodes_of(a, b) < 1 ? -1 : 0, 0, factor == 0.0 ? -2 : -1};
+  return End{0.0, 0.0f, nodes_of(a, b) < 1 ? -1 : 0, 0, factor == 0.0 ? -2 : -1, 0};
 }
 
 template <Elt E> struct Row {
@@ -391,6 +392,171 @@ __device__ __forceinline__ Rest segment_rest(const VerifyArgs& a, const Row<E>& 
   return Rest{wave_sum(s), wave_sum(whole), 0.0f, 0};
 }
 
+// ---- the token ---------------------------------------------------------------------
+
+// Rests pass from one workgroup to another inside a launch, so past the L2 caches.
+__device__ __forceinline__ void write_rest(Rest* p, const Rest& r) {
+  const uint64_t at = (uint64_t)(uint32_t)r.at << 32 | __builtin_bit_cast(uint32_t, r.m);
+  __hip_atomic_store((uint64_t*)p, __builtin_bit_cast(uint64_t, r.s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store((uint64_t*)p + 1, __builtin_bit_cast(uint64_t, r.whole), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store((uint64_t*)p + 2, at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ Rest read_rest(const Rest* p) {
+  const uint64_t s = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const uint64_t w = __hip_atomic_load((const uint64_t*)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const uint64_t at = __hip_atomic_load((const uint64_t*)p + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return {__builtin_bit_cast(double, s), __builtin_bit_cast(double, w), __builtin_bit_cast(float, (uint32_t)at),
+          (int)(at >> 32)};
+}
+
+// The token of tree b, by a workgroup, from the rests of its last node's segments.
+template <Elt E, int PIECES>
+__device__ __forceinline__ void pick(const VerifyArgs& a, const Layout& l, int64_t b, const End& e, double factor) {
+  constexpr int N = Row<E>::N;
+  static_assert(PIECES <= kWaves, "a piece of a segment for each wave");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Rest* rest = l.rest + b * a.segments;
+  const double* list = l.list + b * a.tokens;
+  const bool dense = e.rounds > 0 && a.draft_probs;
+  __shared__ int chosen, use_whole;
+  __shared__ double before, goal;
+  __shared__ float top_at;
+  if (wave == 0) {
+    // A lane has a run of segments, the first of them held.
+    const int per = (a.segments + 63) / 64, c0 = lane * per, c1 = min(c0 + per, a.segments);
+    const Rest none = {0.0, 0.0, -__builtin_inff(), INT32_MAX}, held = c0 < c1 ? read_rest(rest + c0) : none;
+    auto of = [&](int c) { return c == c0 ? held : read_rest(rest + c); };
+    float m = held.m;
+    for (int c = c0 + 1; c < c1; ++c) m = __builtin_elementwise_maximum(m, of(c).m);
+    m = wave_max(m);
+    auto scaled = [&](double s, float mc) {
+      return s == 0.0 ? 0.0 : dense ? s : s * pow2(((double)mc - (double)m) * factor);
+    };
+    if (factor == 0.0) {
+      int at = INT32_MAX;
+      for (int c = c0; c < c1; ++c) {
+        const Rest x = of(c);
+        if (x.m == m) at = min(at, x.at);
+      }
+      at = wave_min(at);
+      const bool none = !(m > -__builtin_inff() && m < __builtin_inff());
+      if (lane == 0) a.token[b] = none ? -1 : at, chosen = -1;
+    } else {
+      double s = 0.0, w = 0.0;
+      for (int c = c0; c < c1; ++c) {
+        const Rest x = of(c);
+        s += scaled(x.s, x.m), w += scaled(x.whole, x.m);
+      }
+      const double sums = wave_sum(s), wholes = wave_sum(w);
+      const bool whole = dense && !(sums > 0.0);
+      const double all = whole ? wholes : sums, want = (double)a.final_uniform[b] * all;
+      if (!(all > 0.0) || all == __builtin_inf()) {
+        // Nothing is left of one-hot drafts: the last one had it all.  Else the
+        // row gives no probabilities.
+        if (lane == 0) a.token[b] = all == 0.0 && e.rounds > 0 && !dense ? (int)list[e.rounds - 1] : -1, chosen = -1;
+      } else {
+        // The first lane, then segment, whose end passes `want`; the last one with any mass, if
+        // rounding leaves none.
+        const double mine = whole ? w : s, upto = wave_scan(mine);
+        const uint64_t some = __builtin_amdgcn_ballot_w64(mine > 0.0);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(mine > 0.0 && upto > want);
+        const int k = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+        if (lane == k) {
+          double base = upto - mine, at = base;
+          int g = -1;
+          for (int c = c0; c < c1; ++c) {
+            const Rest x = of(c);
+            const double here = scaled(whole ? x.whole : x.s, x.m);
+            if (!(here > 0.0)) continue;
+            g = c, at = base;
+            base += here;
+            if (base > want) break;
+          }
+          chosen = g, before = at, goal = want, use_whole = whole, top_at = m;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int g = chosen;
+  if (g < 0) return;
+  const Row<E> r = row_of<E>(a, b, e.node);
+  const float* q = dense ? a.draft_probs + b * a.qb + e.node * a.qt : nullptr;
+  const double top = (double)(dense ? e.m : top_at), want = goal;
+  const bool whole = use_whole;
+  auto weight = [&](float x, int v) {
+    const double p = pow2(((double)x - top) * factor);
+    if (!dense) return p;
+    const Left w = dense_left(p / e.scale, q[v], list, e.rounds);
+    return whole ? w.was : w.now;
+  };
+  // The segment's elements in order: part 0 is the head (the first wave's), 1 + w wave
+  // w's piece of each lane, and the last one the tail (the first wave's).
+  constexpr int kParts = PIECES + 2;
+  __shared__ double parts[kParts];
+  const int piece = g * PIECES * 64 + tid, loose = wave == 0 ? loose_of<E>(a, r, g, lane) : -1;
+  double w[N];
+  float x[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) x[k] = -__builtin_inff();
+  if (wave < PIECES && piece < r.full) load_piece<E>(r, piece, x);
+  float extra = -__builtin_inff();
+  if (loose >= 0) extra = (float)r.p[loose];
+  const int first = r.head + piece * N;
+  if (!dense)
+    for (int i = 0; i < e.rounds; ++i) {
+      const int v = (int)list[i];
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (v == first + k) x[k] = -__builtin_inff();
+      if (v == loose) extra = -__builtin_inff();
+    }
+  double sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    w[k] = wave < PIECES && piece < r.full ? weight(x[k], first + k) : 0.0;
+    sum += w[k];
+  }
+  const double odd = loose >= 0 ? weight(extra, loose) : 0.0, all = wave_sum(sum);
+  const bool in_head = loose >= 0 && loose < r.head;
+  const double heads = wave_sum(in_head ? odd : 0.0), tails = wave_sum(in_head ? 0.0 : odd);
+  if (lane == 0 && wave < PIECES) parts[1 + wave] = all;
+  if (tid == 0) parts[0] = heads, parts[kParts - 1] = tails;
+  __syncthreads();
+  // The part whose end passes `want` (the last one with a weight, if rounding leaves none).
+  double base = before, at = before;
+  int part = -1;
+  for (int k = 0; k < kParts; ++k) {
+    if (!(parts[k] > 0.0)) continue;
+    part = k, at = base;
+    base += parts[k];
+    if (base > want) break;
+  }
+  const bool ends = part == 0 || part == kParts - 1;
+  if (part < 0 || wave != (ends ? 0 : part - 1)) return;
+  // Its elements, by lanes: the first that passes, or the last with a weight.
+  if (ends) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) w[k] = 0.0;
+    if (in_head == (part == 0)) w[0] = odd;
+    sum = w[0];
+  }
+  const int start = ends ? loose : first;
+  at += wave_scan(sum) - sum;
+  int found = INT32_MAX, last = -1;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    at += w[k];
+    if (w[k] > 0.0) {
+      last = start + k;
+      if (at > want) found = min(found, start + k);
+    }
+  }
+  found = wave_min(found);
+  last = -wave_min(-last);
+  if (lane == 0) a.token[b] = found != INT32_MAX ? found : last;
+}
+
 // `groups` workgroups have the segments of a row, each wave every (4 groups)-th one, the next
 // one's loads under way: of every row whose node has children (last 0), or of the rows that
 // the walks ended at.
@@ -400,7 +566,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, int
   const int lane = threadIdx.x & 63, step = groups * kWaves;
   uint32_t id = blockIdx.x;
   int g = __builtin_amdgcn_readfirstlane((int)(id % groups * kWaves + (threadIdx.x >> 6)));
-  if (g >= a.segments) return;
+  if (!last && g >= a.segments) return;
   id /= groups;
   const Layout l = layout(a);
   const int64_t b = last ? id : id / a.tokens;
@@ -411,16 +577,19 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, int
   End e = {};
   if (last) {
     e = end_of(a, l, b, factor);
-    if (e.node < 0 || e.greedy >= 0) return;
+    if (e.node < 0 || e.greedy >= 0) {
+      if (a.tokens > 1 && e.node != -1 && blockIdx.x == b * groups && threadIdx.x == 0)
+        a.token[b] = e.node < 0 ? -1 : e.greedy;
+      return;
+    }
     t = e.node;
     gone = e.rounds;
     if (gone > 0 && a.draft_probs) {
       const Row<E> r = row_of<E>(a, b, t);
       for (; g < a.segments; g += step) {
         const Rest rest = segment_rest<E, PIECES>(a, r, b, g, e, list, factor);
-        if (lane == 0) rests[g] = rest;
+        if (lane == 0) write_rest(rests + g, rest);
       }
-      return;
     }
   } else {
     // (Every wave looks for itself.)
@@ -433,7 +602,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, int
   const Row<E> r = row_of<E>(a, b, t);
   Stat* stats = l.stats + (b * a.tokens + t) * a.segments;
   Held<E, PIECES> now, next;
-  load_segment<E, PIECES>(a, r, g, now);
+  if (g < a.segments) load_segment<E, PIECES>(a, r, g, now);
   for (; g < a.segments; g += step) {
     if (g + step < a.segments) load_segment<E, PIECES>(a, r, g + step, next);
     bool reuse = false;
@@ -450,11 +619,35 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, int
     }
     const Stat st = reuse ? stats[g] : segment_stat<E, PIECES>(a, r, g, now, factor, list, gone);
     if (lane == 0) {
-      if (last) rests[g] = Rest{st.s, st.s, st.m, st.at};
+      if (last) write_rest(rests + g, Rest{st.s, st.s, st.m, st.at});
       else stats[g] = st;
     }
     now = next;
   }
+  // A walked tree's last workgroup to arrive picks the token.
+  if (!last || a.tokens == 1) return;
+  __shared__ int arrived;
+  __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));  // vmcnt(0): the stores are acknowledged
+  __syncthreads();
+  if (threadIdx.x == 0)
+    arrived = __hip_atomic_fetch_add(&l.end[b].arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived == groups - 1) pick<E, PIECES>(a, l, b, e, factor);
+}
+
+// The tokens of trees of one node.
+template <Elt E, int PIECES> __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
+  const Layout l = layout(a);
+  const int64_t b = blockIdx.x;
+  const double factor = factor_of(a, b);
+  const End e = end_of(a, l, b, factor);
+  if (e.node == -1) return;
+  if (threadIdx.x == 0) {  // (no walk has written these)
+    a.path[b] = 0;
+    a.count[b] = 1;
+    if (a.probs) a.probs[b] = 0.0f;
+  }
+  pick<E, PIECES>(a, l, b, e, factor);
 }
 
 // ---- rows of bf16 through a table ------------------------------------------------------
@@ -762,171 +955,10 @@ template <Elt E> __global__ __launch_bounds__(kWalkers) void verify_walk_kernel(
     if (none) e.node = -2;
     // (A node at which no child was rejected has none.)
     if (factor == 0.0) e.greedy = rounds > 0 ? firsts[cur] : -2;
+    e.arrived = 0;
     l.end[b] = e;
     a.count[b] = count;
   }
-}
-
-// ---- the token ---------------------------------------------------------------------
-
-template <Elt E, int PIECES> __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
-  constexpr int N = Row<E>::N;
-  static_assert(PIECES <= kWaves, "a piece of a segment for each wave");
-  const Layout l = layout(a);
-  const int64_t b = blockIdx.x;
-  const double factor = factor_of(a, b);
-  const End e = end_of(a, l, b, factor);
-  if (e.node == -1) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (a.tokens == 1 && tid == 0) {  // (no walk has written these)
-    a.path[b] = 0;
-    a.count[b] = 1;
-    if (a.probs) a.probs[b] = 0.0f;
-  }
-  if (e.node < 0 || e.greedy >= 0) {
-    if (tid == 0) a.token[b] = e.node < 0 ? -1 : e.greedy;
-    return;
-  }
-  const Rest* rest = l.rest + b * a.segments;
-  const double* list = l.list + b * a.tokens;
-  const bool dense = e.rounds > 0 && a.draft_probs;
-  __shared__ int chosen, use_whole;
-  __shared__ double before, goal;
-  __shared__ float top_at;
-  if (wave == 0) {
-    // A lane has a run of segments, the first of them held.
-    const int per = (a.segments + 63) / 64, c0 = lane * per, c1 = min(c0 + per, a.segments);
-    const Rest none = {0.0, 0.0, -__builtin_inff(), INT32_MAX}, held = c0 < c1 ? rest[c0] : none;
-    auto of = [&](int c) { return c == c0 ? held : rest[c]; };
-    float m = held.m;
-    for (int c = c0 + 1; c < c1; ++c) m = __builtin_elementwise_maximum(m, of(c).m);
-    m = wave_max(m);
-    auto scaled = [&](double s, float mc) {
-      return s == 0.0 ? 0.0 : dense ? s : s * pow2(((double)mc - (double)m) * factor);
-    };
-    if (factor == 0.0) {
-      int at = INT32_MAX;
-      for (int c = c0; c < c1; ++c) {
-        const Rest x = of(c);
-        if (x.m == m) at = min(at, x.at);
-      }
-      at = wave_min(at);
-      const bool none = !(m > -__builtin_inff() && m < __builtin_inff());
-      if (lane == 0) a.token[b] = none ? -1 : at, chosen = -1;
-    } else {
-      double s = 0.0, w = 0.0;
-      for (int c = c0; c < c1; ++c) {
-        const Rest x = of(c);
-        s += scaled(x.s, x.m), w += scaled(x.whole, x.m);
-      }
-      const double sums = wave_sum(s), wholes = wave_sum(w);
-      const bool whole = dense && !(sums > 0.0);
-      const double all = whole ? wholes : sums, want = (double)a.final_uniform[b] * all;
-      if (!(all > 0.0) || all == __builtin_inf()) {
-        // Nothing is left of one-hot drafts: the last one had it all.  Else the
-        // row gives no probabilities.
-        if (lane == 0) a.token[b] = all == 0.0 && e.rounds > 0 && !dense ? (int)list[e.rounds - 1] : -1, chosen = -1;
-      } else {
-        // The first lane, then segment, whose end passes `want`; the last one with any mass, if
-        // rounding leaves none.
-        const double mine = whole ? w : s, upto = wave_scan(mine);
-        const uint64_t some = __builtin_amdgcn_ballot_w64(mine > 0.0);
-        const uint64_t past = __builtin_amdgcn_ballot_w64(mine > 0.0 && upto > want);
-        const int k = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
-        if (lane == k) {
-          double base = upto - mine, at = base;
-          int g = -1;
-          for (int c = c0; c < c1; ++c) {
-            const Rest x = of(c);
-            const double here = scaled(whole ? x.whole : x.s, x.m);
-            if (!(here > 0.0)) continue;
-            g = c, at = base;
-            base += here;
-            if (base > want) break;
-          }
-          chosen = g, before = at, goal = want, use_whole = whole, top_at = m;
-        }
-      }
-    }
-  }
-  __syncthreads();
-  const int g = chosen;
-  if (g < 0) return;
-  const Row<E> r = row_of<E>(a, b, e.node);
-  const float* q = dense ? a.draft_probs + b * a.qb + e.node * a.qt : nullptr;
-  const double top = (double)(dense ? e.m : top_at), want = goal;
-  const bool whole = use_whole;
-  auto weight = [&](float x, int v) {
-    const double p = pow2(((double)x - top) * factor);
-    if (!dense) return p;
-    const Left w = dense_left(p / e.scale, q[v], list, e.rounds);
-    return whole ? w.was : w.now;
-  };
-  // The segment's elements in order: part 0 is the head (the first wave's), 1 + w wave
-  // w's piece of each lane, and the last one the tail (the first wave's).
-  constexpr int kParts = PIECES + 2;
-  __shared__ double parts[kParts];
-  const int piece = g * PIECES * 64 + tid, loose = wave == 0 ? loose_of<E>(a, r, g, lane) : -1;
-  double w[N];
-  float x[N];
-#pragma unroll
-  for (int k = 0; k < N; ++k) x[k] = -__builtin_inff();
-  if (wave < PIECES && piece < r.full) load_piece<E>(r, piece, x);
-  float extra = -__builtin_inff();
-  if (loose >= 0) extra = (float)r.p[loose];
-  const int first = r.head + piece * N;
-  if (!dense)
-    for (int i = 0; i < e.rounds; ++i) {
-      const int v = (int)list[i];
-#pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (v == first + k) x[k] = -__builtin_inff();
-      if (v == loose) extra = -__builtin_inff();
-    }
-  double sum = 0.0;
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    w[k] = wave < PIECES && piece < r.full ? weight(x[k], first + k) : 0.0;
-    sum += w[k];
-  }
-  const double odd = loose >= 0 ? weight(extra, loose) : 0.0, all = wave_sum(sum);
-  const bool in_head = loose >= 0 && loose < r.head;
-  const double heads = wave_sum(in_head ? odd : 0.0), tails = wave_sum(in_head ? 0.0 : odd);
-  if (lane == 0 && wave < PIECES) parts[1 + wave] = all;
-  if (tid == 0) parts[0] = heads, parts[kParts - 1] = tails;
-  __syncthreads();
-  // The part whose end passes `want` (the last one with a weight, if rounding leaves none).
-  double base = before, at = before;
-  int part = -1;
-  for (int k = 0; k < kParts; ++k) {
-    if (!(parts[k] > 0.0)) continue;
-    part = k, at = base;
-    base += parts[k];
-    if (base > want) break;
-  }
-  const bool ends = part == 0 || part == kParts - 1;
-  if (part < 0 || wave != (ends ? 0 : part - 1)) return;
-  // Its elements, by lanes: the first that passes, or the last with a weight.
-  if (ends) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) w[k] = 0.0;
-    if (in_head == (part == 0)) w[0] = odd;
-    sum = w[0];
-  }
-  const int start = ends ? loose : first;
-  at += wave_scan(sum) - sum;
-  int found = INT32_MAX, last = -1;
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    at += w[k];
-    if (w[k] > 0.0) {
-      last = start + k;
-      if (at > want) found = min(found, start + k);
-    }
-  }
-  found = wave_min(found);
-  last = -wave_min(-last);
-  if (lane == 0) a.token[b] = found != INT32_MAX ? found : last;
 }
 
 template <Elt E, int PIECES> hipError_t launch_pieces(const VerifyArgs& a, hipStream_t s) {
@@ -951,7 +983,7 @@ template <Elt E, int PIECES> hipError_t launch_pieces(const VerifyArgs& a, hipSt
                        (unsigned)(a.tokens * 52), s, a);
   }
   hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * groups)), dim3(kThreads), 0, s, a, (int)groups, 1);
-  hipLaunchKernelGGL((verify_pick_kernel<E, PIECES>), dim3((unsigned)a.batch), dim3(kThreads), 0, s, a);
+  if (a.tokens == 1) hipLaunchKernelGGL((verify_pick_kernel<E, PIECES>), dim3((unsigned)a.batch), dim3(kThreads), 0, s, a);
   return hipGetLastError();
 }
 
