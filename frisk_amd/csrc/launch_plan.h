@@ -620,9 +620,10 @@ inline int64_t attn_workspace(int64_t batch_heads, int64_t seq_q, int64_t seq_k,
 // Verification of drafted tokens (verify.hip): nodes of a tree at most, and how a
 // row of `vocab` logits of `bytes` is cut into segments: a wave's, with `pieces`
 // pieces of 16 B a lane.  Four, but one where four leave SIMDs without a wave and a row still has
-// no more than the 64 segments that a wave of the walk and of the last launch takes at once.
+// no more than the 64 segments that a wave of the walk and of the last launch takes at once;
+// of trees of one node as many as leave each of a workgroup's 16 waves at most one segment.
 // us of a call with four, with one (batch x nodes):
-//   bf16, 32000:  1 x 1  10.1, 9.2;  8 x 6  21.3, 20.3;  64 x 1  10.8, 11.5;  8 x 16  25.7, 27.2
+//   bf16, 32000:  8 x 6  21.3, 20.3;  8 x 16  25.7, 27.2
 //   bf16, 131072: 1 x 1  9.9, 10.4;  1 x 8  19.4, 20.4;  8 x 1   10.4, 11.9;  64 x 1  15.3, 21.5
 //   f32:          16 x 6 of 50257  23.8, 30.0;  64 x 1 of 131072  17.7, 30.2
 constexpr int64_t kVerifyNodes = 1024;
@@ -634,8 +635,26 @@ struct VerifyPlan {
 inline VerifyPlan verify_plan(int64_t batch, int64_t tokens, int64_t vocab, int bytes) {
   const int64_t whole = std::max<int64_t>(vocab * bytes / 16, 1);
   auto segments = [&](int pieces) { return (whole + 64 * pieces - 1) / (64 * pieces); };
-  const int pieces = batch * tokens * segments(4) < 1024 && segments(1) <= 64 ? 1 : 4;
+  int pieces = batch * tokens * segments(4) < 1024 && segments(1) <= 64 ? 1 : 4;
+  if (tokens == 1) pieces = segments(1) <= 16 ? 1 : 4;
   return {pieces, segments(pieces)};
+}
+
+// Whether trees of one node have a workgroup of 16 waves each and a launch, in place of a
+// workgroup for every four segments and a second launch.  us of a call between other work in a graph, in
+// two launches and in one (segments in brackets):
+//   rows                     1           64          128         256
+//   bf16, 8000 (16, small)   8.0, 5.5    8.8, 6.0    9.0, 5.9    10.8, 6.1
+//   bf16, 32000 (16)         8.4, 9.3    10.6, 9.2   11.6, 9.4   14.8, 9.9
+//   bf16, 65536 (32)         9.8, 10.0   11.8, 12.1  14.2, 12.2  20.6, 12.4
+//   bf16, 131072 (64)        9.9, 17.0   14.3, 18.1  20.1, 17.7  31.9, 18.0
+//   f32, 16000 (16)          6.7, 6.0    9.0, 6.5    10.0, 6.5   11.6, 7.3
+//   f32, 32000 (32)          8.3, 9.0    10.0, 9.4   11.9, 9.6   16.0, 10.4
+//   f32, 65536 (64)          8.2, 15.0   11.7, 15.1  15.9, 15.2  24.4, 16.4
+// Outside of a graph a second launch costs more: one row of 32000 bf16 11.6, 9.4.
+constexpr int64_t kVerifyAlone = 64;
+inline bool verify_alone(int64_t batch, int64_t tokens, int64_t segments, int cus) {
+  return tokens == 1 && segments <= std::min(kVerifyAlone, std::max<int64_t>(16, batch * 128 / cus));
 }
 
 // Workgroups of kVerifyTableWaves with a table of weights (bf16) for each row of logits, or 0: none.

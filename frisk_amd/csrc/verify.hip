@@ -15,7 +15,8 @@
 // arrive there finds the segment, then the element, in which the sum passes the last random
 // number (a launch of its own took 0.7 us longer).  (2) set the count of arrivals to 0, so that an
 // arrival is one addition; exchanges with a word of any content took 1 us each, one after the
-// other.  A tree of one node takes (3) without arrivals, and that search as a launch.
+// other.  Trees of one node: (3) without arrivals and the search as a second launch, or both by
+// one workgroup a row (plan::verify_alone).
 
 #include <algorithm>
 
@@ -28,6 +29,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kWalkers = 1024;  // threads of a walk
+constexpr int kAlone = 1024;    // threads of a row in a launch of its own
 
 // A segment's or a row's largest logit, its first place, and the sum of weights
 // 2^((x - m) c): NaN if the row gives no probabilities (it holds a NaN or +infinity).
@@ -152,10 +154,9 @@ __device__ __forceinline__ double factor_of(const VerifyArgs& a, int64_t b) {
 __device__ __forceinline__ int nodes_of(const VerifyArgs& a, int64_t b) {
   return a.new_len ? min(max(a.new_len[b], 0), a.tokens) : a.tokens;
 }
-// Where a tree's walk ended; of trees of one node, which are not walked: at the root.
-__device__ __forceinline__ End end_of(const VerifyArgs& a, const Layout& l, int64_t b, double factor) {
-  if (a.tokens > 1) return l.end[b];
-  return End{0.0, 0.0f, nodes_of(a, b) < 1 ? -1 : 0, 0, factor == 0.0 ? -2 : -1, 0};
+// The end of a tree of one node, which is not walked.
+__device__ __forceinline__ End root_end(const VerifyArgs& a, int64_t b) {
+  return End{0.0, 0.0f, nodes_of(a, b) < 1 ? -1 : 0, 0, -1, 0};
 }
 
 template <Elt E> struct Row {
@@ -410,13 +411,12 @@ __device__ __forceinline__ Rest read_rest(const Rest* p) {
 }
 
 // The token of tree b, by a workgroup, from the rests of its last node's segments.
-template <Elt E, int PIECES>
-__device__ __forceinline__ void pick(const VerifyArgs& a, const Layout& l, int64_t b, const End& e, double factor) {
+template <Elt E, int PIECES, typename Read>
+__device__ __forceinline__ void pick(const VerifyArgs& a, int64_t b, const End& e, double factor, const double* list,
+                                     const Read& rest) {
   constexpr int N = Row<E>::N;
   static_assert(PIECES <= kWaves, "a piece of a segment for each wave");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Rest* rest = l.rest + b * a.segments;
-  const double* list = l.list + b * a.tokens;
   const bool dense = e.rounds > 0 && a.draft_probs;
   __shared__ int chosen, use_whole;
   __shared__ double before, goal;
@@ -424,8 +424,8 @@ __device__ __forceinline__ void pick(const VerifyArgs& a, const Layout& l, int64
   if (wave == 0) {
     // A lane has a run of segments, the first of them held.
     const int per = (a.segments + 63) / 64, c0 = lane * per, c1 = min(c0 + per, a.segments);
-    const Rest none = {0.0, 0.0, -__builtin_inff(), INT32_MAX}, held = c0 < c1 ? read_rest(rest + c0) : none;
-    auto of = [&](int c) { return c == c0 ? held : read_rest(rest + c); };
+    const Rest none = {0.0, 0.0, -__builtin_inff(), INT32_MAX}, held = c0 < c1 ? rest(c0) : none;
+    auto of = [&](int c) { return c == c0 ? held : rest(c); };
     float m = held.m;
     for (int c = c0 + 1; c < c1; ++c) m = __builtin_elementwise_maximum(m, of(c).m);
     m = wave_max(m);
@@ -484,9 +484,8 @@ __device__ __forceinline__ void pick(const VerifyArgs& a, const Layout& l, int64
   const float* q = dense ? a.draft_probs + b * a.qb + e.node * a.qt : nullptr;
   const double top = (double)(dense ? e.m : top_at), want = goal;
   const bool whole = use_whole;
-  auto weight = [&](float x, int v) {
-    const double p = pow2(((double)x - top) * factor);
-    if (!dense) return p;
+  auto weight = [&](float x) { return pow2(((double)x - top) * factor); };
+  auto left = [&](double p, int v) {
     const Left w = dense_left(p / e.scale, q[v], list, e.rounds);
     return whole ? w.was : w.now;
   };
@@ -511,13 +510,18 @@ __device__ __forceinline__ void pick(const VerifyArgs& a, const Layout& l, int64
         if (v == first + k) x[k] = -__builtin_inff();
       if (v == loose) extra = -__builtin_inff();
     }
-  double sum = 0.0;
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    w[k] = wave < PIECES && piece < r.full ? weight(x[k], first + k) : 0.0;
-    sum += w[k];
+  for (int k = 0; k < N; ++k) w[k] = weight(x[k]);  // (0 of -infinity)
+  double odd = weight(extra), sum = 0.0;
+  if (dense) {
+    if (wave < PIECES && piece < r.full)
+#pragma unroll
+      for (int k = 0; k < N; ++k) w[k] = left(w[k], first + k);
+    if (loose >= 0) odd = left(odd, loose);
   }
-  const double odd = loose >= 0 ? weight(extra, loose) : 0.0, all = wave_sum(sum);
+#pragma unroll
+  for (int k = 0; k < N; ++k) sum += w[k];
+  const double all = wave_sum(sum);
   const bool in_head = loose >= 0 && loose < r.head;
   const double heads = wave_sum(in_head ? odd : 0.0), tails = wave_sum(in_head ? 0.0 : odd);
   if (lane == 0 && wave < PIECES) parts[1 + wave] = all;
@@ -576,7 +580,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, int
   Rest* rests = l.rest + b * a.segments;
   End e = {};
   if (last) {
-    e = end_of(a, l, b, factor);
+    e = a.tokens > 1 ? l.end[b] : root_end(a, b);
     if (e.node < 0 || e.greedy >= 0) {
       if (a.tokens > 1 && e.node != -1 && blockIdx.x == b * groups && threadIdx.x == 0)
         a.token[b] = e.node < 0 ? -1 : e.greedy;
@@ -632,24 +636,27 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, int
   if (threadIdx.x == 0)
     arrived = __hip_atomic_fetch_add(&l.end[b].arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  if (arrived == groups - 1) pick<E, PIECES>(a, l, b, e, factor);
+  if (arrived == groups - 1)
+    pick<E, PIECES>(a, b, e, factor, list, [&](int c) { return read_rest(rests + c); });
 }
 
+// What a walk writes of a tree of one node.
+__device__ __forceinline__ void one_node(const VerifyArgs& a, int64_t b) {
+  a.path[b] = 0;
+  a.count[b] = 1;
+  if (a.probs) a.probs[b] = 0.0f;
+}
 // The tokens of trees of one node.
 template <Elt E, int PIECES> __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   const Layout l = layout(a);
   const int64_t b = blockIdx.x;
   const double factor = factor_of(a, b);
-  const End e = end_of(a, l, b, factor);
-  if (e.node == -1) return;
-  if (threadIdx.x == 0) {  // (no walk has written these)
-    a.path[b] = 0;
-    a.count[b] = 1;
-    if (a.probs) a.probs[b] = 0.0f;
-  }
-  pick<E, PIECES>(a, l, b, e, factor);
+  const End e = root_end(a, b);
+  if (e.node < 0) return;
+  if (threadIdx.x == 0) one_node(a, b);
+  const Rest* rests = l.rest + b * a.segments;
+  pick<E, PIECES>(a, b, e, factor, nullptr, [&](int c) { return read_rest(rests + c); });
 }
-
 // ---- rows of bf16 through a table ------------------------------------------------------
 
 // There are few bf16 numbers: the weights 2^(x c) of all of 2^-16 <= |x| < 2^7 are 5888
@@ -678,7 +685,8 @@ __device__ __forceinline__ bool table_stat(const VerifyArgs& a, const Row<Elt::B
                                            const Held<Elt::BF16, PIECES>& h, double factor, const char* table,
                                            Stat& st) {
   // (The first and the last segment may have a head or a tail.)
-  if (g == 0 || (g + 1) * PIECES * 64 > r.full || g == a.segments - 1) return false;
+  if ((g == 0 && r.head > 0) || (g + 1) * PIECES * 64 > r.full ||
+      (g == a.segments - 1 && r.head + r.full * Row<Elt::BF16>::N < r.n)) return false;
   // Magnitudes from the table's first on (smaller ones wrap round), and the largest number as an
   // integer: right if it is positive.
   u16x2 most = {0, 0};
@@ -727,6 +735,14 @@ __device__ __forceinline__ bool table_stat(const VerifyArgs& a, const Row<Elt::B
   return true;
 }
 
+__device__ __forceinline__ void fill_table(char* table, double factor, int threads) {
+  for (uint32_t i = threadIdx.x; i < 2 * kTableSize; i += threads) {
+    const uint32_t magnitude = kTableLeast + (i >> 1);
+    const float x = bf16_bits_to_f32((uint16_t)((i & 1) << 15 | magnitude));
+    *(double*)(table + (i & 1) * kNegative + (i >> 1) * 8) = pow2_any((double)x * factor);
+  }
+}
+
 // As verify_rows_kernel for the rows of nodes that have children.
 template <int PIECES>
 __global__ __launch_bounds__(kTableThreads) void verify_table_kernel(VerifyArgs a, int groups) {
@@ -749,11 +765,7 @@ __global__ __launch_bounds__(kTableThreads) void verify_table_kernel(VerifyArgs 
   if (g < a.segments) load_segment<Elt::BF16, PIECES>(a, r, g, now);
   const bool tabled = factor > 0.0 && factor <= kTableSteepest;
   if (tabled) {
-    for (uint32_t i = tid; i < 2 * kTableSize; i += kTableThreads) {
-      const uint32_t magnitude = kTableLeast + (i >> 1);
-      const float x = bf16_bits_to_f32((uint16_t)((i & 1) << 15 | magnitude));
-      *(double*)(table + (i & 1) * kNegative + (i >> 1) * 8) = pow2_any((double)x * factor);
-    }
+    fill_table(table, factor, kTableThreads);
   }
   __syncthreads();
   for (; g < a.segments; g += step) {
@@ -764,6 +776,40 @@ __global__ __launch_bounds__(kTableThreads) void verify_table_kernel(VerifyArgs 
     if (lane == 0) stats[g] = st;
     now = next;
   }
+}
+
+// Trees of one node in a launch, a workgroup a row: its latencies and, of long rows, one CU's 64-bit
+// arithmetic bound it.  A row of 32000 bf16 9.4 us, of which 1 us less by the table.
+template <Elt E, int PIECES> __global__ __launch_bounds__(kAlone) void verify_alone_kernel(VerifyArgs a) {
+  const int64_t b = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const double factor = factor_of(a, b);
+  const End e = root_end(a, b);
+  if (e.node < 0) return;
+  constexpr bool kTable = E == Elt::BF16 && PIECES == 4;
+  __shared__ Rest rests[plan::kVerifyAlone];
+  __shared__ __attribute__((aligned(16))) char table[kTable ? kTableBytes : 16];
+  const Row<E> r = row_of<E>(a, b, 0);
+  int g = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  Held<E, PIECES> now;
+  if (g < a.segments) load_segment<E, PIECES>(a, r, g, now);
+  if (threadIdx.x == 0) one_node(a, b);
+  // (A table costs a lane 6 weights: for two waves a SIMD it took 0.5 us longer.)
+  const bool tabled = kTable && a.segments > 8 && factor > 0.0 && factor <= kTableSteepest;
+  if constexpr (kTable) {
+    if (tabled) fill_table(table, factor, kAlone);
+    __syncthreads();
+  }
+  for (; g < a.segments; g += kAlone / 64) {
+    Stat st;
+    bool found = false;
+    if constexpr (kTable) found = tabled && table_stat<PIECES>(a, r, g, now, factor, table, st);
+    if (!found) st = segment_stat<E, PIECES>(a, r, g, now, factor, nullptr, 0);
+    if (lane == 0) rests[g] = Rest{st.s, st.s, st.m, st.at};
+    if (g + kAlone / 64 < a.segments) load_segment<E, PIECES>(a, r, g + kAlone / 64, now);
+  }
+  __syncthreads();
+  pick<E, PIECES>(a, b, e, factor, nullptr, [&](int c) { return rests[c]; });
 }
 
 // ---- the walk ----------------------------------------------------------------------
@@ -964,6 +1010,10 @@ template <Elt E> __global__ __launch_bounds__(kWalkers) void verify_walk_kernel(
 template <Elt E, int PIECES> hipError_t launch_pieces(const VerifyArgs& a, hipStream_t s) {
   const int64_t groups = (a.segments + kWaves - 1) / kWaves;  // a segment a wave
   if (a.batch * a.tokens * groups > UINT32_MAX / kThreads) return hipErrorInvalidConfiguration;
+  if (plan::verify_alone(a.batch, a.tokens, a.segments, device_cus())) {
+    hipLaunchKernelGGL((verify_alone_kernel<E, PIECES>), dim3((unsigned)a.batch), dim3(kAlone), 0, s, a);
+    return hipGetLastError();
+  }
   auto rows = verify_rows_kernel<E, PIECES>;
   if (a.tokens > 1) {
     // As many segments a wave as leave 32 waves for a CU.

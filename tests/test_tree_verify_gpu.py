@@ -127,6 +127,21 @@ def test_many_rows_of_a_large_vocabulary(temperature, shift):
     t.check(t.run())
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("batch,vocab,shift", [(2, 7, 0), (3, 8000, 1), (2, 20000, 3), (2, 32768, 0), (3, 32771, 2),
+                                               (70, 50257, 1), (130, 131072, 0), (260, 65537, 5), (2, 140000, 1)])
+def test_tokens_alone(batch, vocab, shift, dt):
+    # One node a tree: rows that a workgroup has whole, and rows that are cut.
+    t = Trees(batch, 1, vocab, dt, shift=shift, seed=vocab + shift, temperature=[0.3 + 0.2 * (i % 9) for i in range(batch)])
+    t.temperature[::5] = 0.0
+    t.logits[batch // 2, 0, vocab // 3:] = -torch.inf
+    t.check(t.run())
+    t.logits[0, 0, vocab - 1] = float("nan")
+    t.logits[1, 0, :] = -torch.inf
+    t.nodes = [1] * (batch - 1) + [0]
+    t.check(t.run())
+
+
 def test_many_rows_of_one_sign():
     t = Trees(2, 256, 50021, "bf16", branch=1, temperature=(0.7, 1.0), seed=31)
     t.logits.copy_(t.logits.float().abs() - 25.0)  # all negative, rest and peaks apart
