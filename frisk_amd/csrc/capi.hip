@@ -1082,7 +1082,7 @@ int check_verify(const frisk_tree_verify_desc* d, bool ptrs, frisk::VerifyArgs& 
   a.workspace = d->workspace;
   if (!ptrs) return FRISK_OK;
   const int64_t need = frisk::verify_workspace(d->batch, d->tokens, p.segments), n = d->batch * 4, all = n * d->tokens;
-  if (!d->workspace || d->workspace_bytes < need)
+  if (need && (!d->workspace || d->workspace_bytes < need))
     return fail(FRISK_EINVAL, "%s: workspace of %lld bytes, this call takes %lld", fn,
                 (long long)(d->workspace ? d->workspace_bytes : 0), (long long)need);
   if (!aligned16(d->workspace)) return fail(FRISK_EINVAL, "%s: workspace must be 16-byte aligned", fn);

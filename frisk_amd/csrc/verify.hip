@@ -1048,6 +1048,7 @@ template <Elt E> hipError_t launch_type(const VerifyArgs& a, hipStream_t s) {
 }  // namespace
 
 int64_t verify_workspace(int64_t batch, int64_t tokens, int64_t segments) {
+  if (plan::verify_alone(batch, tokens, segments, device_cus())) return 0;
   return up16(batch * tokens * segments * (int64_t)sizeof(Stat)) + up16(batch * segments * (int64_t)sizeof(Rest)) +
          up16(batch * (int64_t)sizeof(End)) + batch * tokens * 8;
 }

@@ -1162,10 +1162,14 @@ def tree_verify(logits, drafts, parents, uniform, final, *, draft_probs=None, te
         need = _raw_fn("frisk_tree_verify_workspace_size")(head + bytes(16))
         if need < 0:
             _check(need, "frisk_tree_verify_workspace_size")
-        workspace = _scratch(need, logits.device, stream)
+        tail = bytes(16)
+        if need:
+            workspace = _scratch(need, logits.device, stream)
+            tail = _ws_pack.pack(workspace.data_ptr(), need)
     elif workspace.get_device() != dev or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous tensor on the logits' device")
-    tail = _ws_pack.pack(workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    else:
+        tail = _ws_pack.pack(workspace.data_ptr(), workspace.numel() * workspace.element_size())
     rc = _raw_fn("frisk_tree_verify")(head + tail, handle)
     if rc:
         _check(rc, "frisk_tree_verify")

@@ -184,7 +184,8 @@ def test_null_descriptors_and_the_workspace_query():
         assert getattr(lib, name)(None, None) == rt.EINVAL
     assert lib.frisk_tree_verify_workspace_size(None) == rt.EINVAL
     assert lib.frisk_tree_verify_workspace_size(ctypes.byref(verify_desc(tokens=0))) == rt.EINVAL
-    small = rt.tree_verify_workspace_bytes(1, 1, 1, torch.float32)
+    assert rt.tree_verify_workspace_bytes(1, 1, 1000, torch.float32) == 0
+    small = rt.tree_verify_workspace_bytes(1, 2, 1, torch.float32)
     large = rt.tree_verify_workspace_bytes(64, 64, 131072, torch.bfloat16)
     assert 0 < small < 1024 and small < large < 64 << 20
     with pytest.raises(ValueError, match="up to 1024"):
