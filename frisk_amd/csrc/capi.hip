@@ -1318,11 +1318,16 @@ int frisk_kv_pages(const frisk_kv_pages_desc* d, void* stream) {
       (uintptr_t)d->lacking % 4)
     return fail(FRISK_EINVAL, "%s: pointers must be element-aligned", fn);
   const int64_t n = d->batch * 4;
-  auto table = [&](int64_t stride) { return ((d->batch - 1) * stride + d->max_pages) * 4; };
-  const Span out[] = {{d->out, table(d->out_stride)}, {d->src, n}, {d->dst, n}, {d->rows, n}, {d->lacking, 4}};
-  const Span in[] = {{d->table, table(d->table_stride)}, {d->parent, n}, {d->keep, n}, {d->want, n},
-                     {d->held, d->pages}};
-  if (outputs_overlap(out, in)) return fail(FRISK_EINVAL, "%s: an output overlaps another tensor", fn);
+  // (The two tables may be interleaved.)
+  auto rows = [&](const void* p, int64_t stride) { return Rows{p, {d->batch, 1, 1}, {stride, 1, 1}}; };
+  auto all = [&](const void* p, int64_t stride) { return Span{p, ((d->batch - 1) * stride + d->max_pages) * 4}; };
+  const Span next[] = {all(d->out, d->out_stride)};
+  const Span lists[] = {{d->src, n}, {d->dst, n}, {d->rows, n}, {d->lacking, 4}};
+  const Span in[] = {{d->parent, n}, {d->keep, n}, {d->want, n}, {d->held, d->pages}};
+  const Span tables[] = {all(d->table, d->table_stride), next[0]};
+  if (outputs_overlap(lists, in) || outputs_overlap(lists, tables) || outputs_overlap(next, in) ||
+      rows_share(rows(d->table, d->table_stride), rows(d->out, d->out_stride), d->max_pages, 4))
+    return fail(FRISK_EINVAL, "%s: an output overlaps another tensor", fn);
   frisk::KvPagesArgs a;
   a.batch = (int)d->batch;
   a.max_pages = (int)d->max_pages;

@@ -136,6 +136,19 @@ def test_strided_tables_and_made_outputs():
         rt.kv_pages(wide, keep, None, 4, 80, held=torch.zeros(79, dtype=torch.bool, device="cuda"))
 
 
+def test_interleaved_tables():
+    rng = np.random.default_rng(6)
+    both = torch.full((5, 2, 6), -7, dtype=torch.int32, device="cuda")
+    both[:, 0] = ints(random_tables(rng, 5, 6, 4, 80))
+    table, out, keep = both[:, 0], both[:, 1], ints([9, 3, 16, 0, 7])
+    before = table.tolist()
+    rt.kv_pages(table, keep, keep + 5, 4, 80, out=out)
+    assert out.tolist() == S.next_table(before, keep.tolist(), (keep + 5).tolist(), 4, 80)[0]
+    assert table.tolist() == before
+    with pytest.raises(ValueError, match="an output overlaps"):
+        rt.kv_pages(both[:, 0], keep, None, 4, 80, out=both.view(5, 12)[:, 5:11])
+
+
 # ---- rows and pages of a cache --------------------------------------------------------
 
 
