@@ -127,6 +127,21 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pair_chunks, 
     }
     return;
   }
+  const int at0 = INTER ? chunk * 2 * NP : chunk * NP;
+  const int at1 = INTER ? at0 + 1 : at0 + a.rot_dim / 2;  // (the second piece, if any)
+  V x[HB][NV];
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int j = 0; j < HB; ++j) {
+      const int h = base + j * lanes;
+      if (h < heads) {
+        const T* row = in_row(h);
+        x[j][0] = load(row + at0);
+        if constexpr (NV == 2) x[j][1] = load(row + at1);
+      }
+    }
+  };
+  fetch(first);  // (beside the loads of positions and frequencies)
   int64_t p = a.start ? a.start[b] : 0;
   [[maybe_unused]] int64_t more[kRopeAxes];  // the positions on the other axes
   if constexpr (AXES) {
@@ -152,19 +167,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pair_chunks, 
     cs[i] = r.c * a.amplitude;
     sn[i] = (a.backward ? -r.s : r.s) * a.amplitude;
   }
-  const int at0 = INTER ? chunk * 2 * NP : chunk * NP;
-  const int at1 = INTER ? at0 + 1 : at0 + a.rot_dim / 2;  // (the second piece, if any)
   for (int base = first; base < heads; base += HB * lanes) {
-    V x[HB][NV];
-#pragma unroll
-    for (int j = 0; j < HB; ++j) {
-      const int h = base + j * lanes;
-      if (h < heads) {
-        const T* row = in_row(h);
-        x[j][0] = load(row + at0);
-        if constexpr (NV == 2) x[j][1] = load(row + at1);
-      }
-    }
+    if (base != first) fetch(base);
 #pragma unroll
     for (int j = 0; j < HB; ++j) {
       const int h = base + j * lanes;
