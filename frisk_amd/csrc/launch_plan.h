@@ -620,14 +620,19 @@ inline int64_t attn_workspace(int64_t batch_heads, int64_t seq_q, int64_t seq_k,
 // Verification of drafted tokens (verify.hip): nodes of a tree at most, and how a
 // row of `vocab` logits of `bytes` is cut into segments: a wave's, with `pieces`
 // pieces of 16 B a lane.  Four, but one where four leave SIMDs without a wave and a row still has
-// no more than the 64 segments that a wave of the walk and of the last launch takes at once;
-// of trees of one node as many as leave each of a workgroup's 16 waves at most one segment.
+// no more than the 64 segments that a wave of the walk and of the last launch takes at once.
 // us of a call with four, with one (batch x nodes):
 //   bf16, 32000:  8 x 6  21.3, 20.3;  8 x 16  25.7, 27.2
 //   bf16, 131072: 1 x 1  9.9, 10.4;  1 x 8  19.4, 20.4;  8 x 1   10.4, 11.9;  64 x 1  15.3, 21.5
 //   f32:          16 x 6 of 50257  23.8, 30.0;  64 x 1 of 131072  17.7, 30.2
 constexpr int64_t kVerifyNodes = 1024;
 constexpr int64_t kVerifyVocab = 1 << 24;
+// And one for rows of at most 16 segments, a workgroup's waves: their walks do the last rows
+// as well, without a launch for these.  us of a call between other work in a graph, with that launch and
+// without it: 8 x 6 of 1000 bf16 15.2, 12.7, of 8000 15.5, 14.1; 8 x 64 of 8000 22.0, 18.9;
+// 64 x 6 of 4000 f32 with draft probabilities 18.6, 16.9.  Of twice these rows the two are
+// even, of longer ones the launch pays.
+constexpr int64_t kVerifyShort = 16;
 struct VerifyPlan {
   int pieces;
   int64_t segments;
@@ -635,8 +640,9 @@ struct VerifyPlan {
 inline VerifyPlan verify_plan(int64_t batch, int64_t tokens, int64_t vocab, int bytes) {
   const int64_t whole = std::max<int64_t>(vocab * bytes / 16, 1);
   auto segments = [&](int pieces) { return (whole + 64 * pieces - 1) / (64 * pieces); };
-  int pieces = batch * tokens * segments(4) < 1024 && segments(1) <= 64 ? 1 : 4;
-  if (tokens == 1) pieces = segments(1) <= 16 ? 1 : 4;
+  const bool one = segments(1) <= kVerifyShort ||
+                   (tokens > 1 && batch * tokens * segments(4) < 1024 && segments(1) <= 64);
+  const int pieces = one ? 1 : 4;
   return {pieces, segments(pieces)};
 }
 

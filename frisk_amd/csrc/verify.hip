@@ -15,8 +15,9 @@
 // arrive there finds the segment, then the element, in which the sum passes the last random
 // number (a launch of its own took 0.7 us longer).  (2) set the count of arrivals to 0, so that an
 // arrival is one addition; exchanges with a word of any content took 1 us each, one after the
-// other.  Trees of one node: (3) without arrivals and the search as a second launch, or both by
-// one workgroup a row (plan::verify_alone).
+// other.  Short rows (plan::kVerifyShort): (3) is a part of (2).  Trees of one node: (3)
+// without arrivals and the search as a second launch, or both by one workgroup a row
+// (plan::verify_alone).
 
 #include <algorithm>
 
@@ -561,6 +562,29 @@ __device__ __forceinline__ void pick(const VerifyArgs& a, int64_t b, const End& 
   if (lane == 0) a.token[b] = found != INT32_MAX ? found : last;
 }
 
+// Segment g of what is left at a tree's last node.  `held`: the segment, as loaded.
+template <Elt E, int PIECES>
+__device__ __forceinline__ Rest last_segment(const VerifyArgs& a, const Row<E>& r, int64_t b, int g, const End& e,
+                                             const double* list, double factor, const Stat* stats,
+                                             const Held<E, PIECES>& held) {
+  constexpr int N = Row<E>::N;
+  const int lane = threadIdx.x & 63;
+  bool reuse = false;
+  if (e.rounds > 0) {
+    // One-hot drafts: a segment without a rejected token is as it was.
+    const int lo = g ? r.head + g * PIECES * 64 * N : 0;
+    const int hi = g == a.segments - 1 ? r.n : r.head + (g + 1) * PIECES * 64 * N;
+    uint64_t any = 0;
+    for (int i0 = 0; i0 < e.rounds && !any; i0 += 64) {
+      const int v = i0 + lane < e.rounds ? (int)list[i0 + lane] : -1;
+      any = __builtin_amdgcn_ballot_w64(v >= lo && v < hi);
+    }
+    reuse = !any;
+  }
+  const Stat st = reuse ? stats[g] : segment_stat<E, PIECES>(a, r, g, held, factor, list, e.rounds);
+  return {st.s, st.s, st.m, st.at};
+}
+
 // `groups` workgroups have the segments of a row, each wave every (4 groups)-th one, the next
 // one's loads under way: of every row whose node has children (last 0), or of the rows that
 // the walks ended at.
@@ -609,22 +633,12 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, int
   if (g < a.segments) load_segment<E, PIECES>(a, r, g, now);
   for (; g < a.segments; g += step) {
     if (g + step < a.segments) load_segment<E, PIECES>(a, r, g + step, next);
-    bool reuse = false;
-    if (gone > 0) {
-      // One-hot drafts: a segment without a rejected token is as it was.
-      const int lo = g ? r.head + g * PIECES * 64 * N : 0;
-      const int hi = g == a.segments - 1 ? r.n : r.head + (g + 1) * PIECES * 64 * N;
-      uint64_t any = 0;
-      for (int i0 = 0; i0 < gone && !any; i0 += 64) {
-        const int v = i0 + lane < gone ? (int)list[i0 + lane] : -1;
-        any = __builtin_amdgcn_ballot_w64(v >= lo && v < hi);
-      }
-      reuse = !any;
-    }
-    const Stat st = reuse ? stats[g] : segment_stat<E, PIECES>(a, r, g, now, factor, list, gone);
-    if (lane == 0) {
-      if (last) write_rest(rests + g, Rest{st.s, st.s, st.m, st.at});
-      else stats[g] = st;
+    if (last) {
+      const Rest rest = last_segment<E, PIECES>(a, r, b, g, e, list, factor, stats, now);
+      if (lane == 0) write_rest(rests + g, rest);
+    } else {
+      const Stat st = segment_stat<E, PIECES>(a, r, g, now, factor, nullptr, 0);
+      if (lane == 0) stats[g] = st;
     }
     now = next;
   }
@@ -818,7 +832,9 @@ template <Elt E> __device__ __forceinline__ float logit(const VerifyArgs& a, int
   return load_as_f32<E>(a.logits, b * a.sb + t * a.st + v);
 }
 
-template <Elt E> __global__ __launch_bounds__(kWalkers) void verify_walk_kernel(VerifyArgs a) {
+// LAST: what is left of the last row, and the token, as well.
+template <Elt E, int PIECES, bool LAST>
+__global__ __launch_bounds__(kWalkers) void verify_walk_kernel(VerifyArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   double* mass = (double*)smem;            // [tokens] sum of a node's row, NaN if it has none
   double* chance = mass + a.tokens;        // [tokens] weight of a node's token in its parent's row
@@ -990,20 +1006,36 @@ template <Elt E> __global__ __launch_bounds__(kWalkers) void verify_walk_kernel(
     }
     __syncthreads();
   }
-  for (int i = tid; i < at_rounds; i += kWalkers) l.list[b * a.tokens + i] = list[i];
-  if (tid == 0) {
-    End e;
-    e.scale = mass[cur];
-    e.m = tops[cur];
-    e.node = cur;
-    e.rounds = rounds;
-    e.greedy = -1;
-    if (none) e.node = -2;
-    // (A node at which no child was rejected has none.)
-    if (factor == 0.0) e.greedy = rounds > 0 ? firsts[cur] : -2;
-    e.arrived = 0;
-    l.end[b] = e;
-    a.count[b] = count;
+  // (Of the first wave.  A node at which no child was rejected has no `firsts`.)
+  End e = {mass[cur], tops[cur], none ? -2 : cur, rounds, factor != 0.0 ? -1 : rounds > 0 ? firsts[cur] : -2, 0};
+  if constexpr (LAST) {
+    __shared__ End end;
+    __shared__ Rest rests[plan::kVerifyShort];
+    if (tid == 0) end = e, a.count[b] = count;
+    __syncthreads();
+    e = end;
+    if (e.node < 0 || e.greedy >= 0) {
+      if (tid == 0) a.token[b] = e.node < 0 ? -1 : e.greedy;
+      return;
+    }
+    const Row<E> r = row_of<E>(a, b, e.node);
+    const Stat* stats = l.stats + (b * a.tokens + e.node) * a.segments;
+    for (int g = __builtin_amdgcn_readfirstlane(wave); g < a.segments; g += kWalkers / 64) {
+      Rest rest;
+      if (dense && e.rounds > 0) {
+        rest = segment_rest<E, PIECES>(a, r, b, g, e, list, factor);
+      } else {
+        Held<E, PIECES> held;
+        load_segment<E, PIECES>(a, r, g, held);
+        rest = last_segment<E, PIECES>(a, r, b, g, e, list, factor, stats, held);
+      }
+      if (lane == 0) rests[g] = rest;
+    }
+    __syncthreads();
+    pick<E, PIECES>(a, b, e, factor, list, [&](int c) { return rests[c]; });
+  } else {
+    for (int i = tid; i < at_rounds; i += kWalkers) l.list[b * a.tokens + i] = list[i];
+    if (tid == 0) l.end[b] = e, a.count[b] = count;
   }
 }
 
@@ -1015,24 +1047,27 @@ template <Elt E, int PIECES> hipError_t launch_pieces(const VerifyArgs& a, hipSt
     return hipGetLastError();
   }
   auto rows = verify_rows_kernel<E, PIECES>;
+  bool last = true;  // the last rows are still to do
   if (a.tokens > 1) {
     // As many segments a wave as leave 32 waves for a CU.
     const int64_t per = a.batch * a.tokens * groups / (8 * (int64_t)device_cus());
     const int64_t some = (groups + std::max<int64_t>(per, 1) - 1) / std::max<int64_t>(per, 1);
+    auto walk = verify_walk_kernel<E, PIECES, false>;
+    int64_t tables = 0;
     if constexpr (E == Elt::BF16 && PIECES == 4) {
-      const int64_t tables = plan::verify_tables(a.batch, a.tokens, a.segments, device_cus());
+      tables = plan::verify_tables(a.batch, a.tokens, a.segments, device_cus());
       if (tables)
         hipLaunchKernelGGL(verify_table_kernel<PIECES>, dim3((unsigned)(a.batch * a.tokens * tables)),
                            dim3(kTableThreads), 0, s, a, (int)tables);
-      else
-        hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * a.tokens * some)), dim3(kThreads), 0, s, a, (int)some, 0);
-    } else {
-      hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * a.tokens * some)), dim3(kThreads), 0, s, a, (int)some, 0);
     }
-    hipLaunchKernelGGL((verify_walk_kernel<E>), dim3((unsigned)a.batch), dim3(kWalkers),
-                       (unsigned)(a.tokens * 52), s, a);
+    if (!tables)
+      hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * a.tokens * some)), dim3(kThreads), 0, s, a, (int)some, 0);
+    if constexpr (PIECES == 1)
+      if (a.segments <= plan::kVerifyShort) walk = verify_walk_kernel<E, PIECES, true>, last = false;
+    hipLaunchKernelGGL(walk, dim3((unsigned)a.batch), dim3(kWalkers), (unsigned)(a.tokens * 52), s, a);
   }
-  hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * groups)), dim3(kThreads), 0, s, a, (int)groups, 1);
+  if (last)
+    hipLaunchKernelGGL(rows, dim3((unsigned)(a.batch * groups)), dim3(kThreads), 0, s, a, (int)groups, 1);
   if (a.tokens == 1) hipLaunchKernelGGL((verify_pick_kernel<E, PIECES>), dim3((unsigned)a.batch), dim3(kThreads), 0, s, a);
   return hipGetLastError();
 }

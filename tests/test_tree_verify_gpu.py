@@ -128,6 +128,22 @@ def test_many_rows_of_a_large_vocabulary(temperature, shift):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dense", [False, True])
+@pytest.mark.parametrize("vocab", [4095, 4097, 8193, 20011, 70001])
+def test_rows_from_short_to_long(vocab, dense, dt):
+    # Rows around what a walk does by itself, and cut ones: greedy trees, masks, several
+    # rejections at a node, trees that end early or take no part.
+    for branch, seed in ((1, 41), (4, 42)):
+        t = Trees(6, 9, vocab, dt, dense=dense, branch=branch, seed=seed, shift=seed % 3,
+                  temperature=(0.0, 0.6, 1.0, 1.5, 0.0, 1.0), nodes=[9, 9, 5, 9, 1, 0])
+        t.check(t.run())
+        t.logits[1, :, vocab // 2:] = -torch.inf
+        t.logits[2, 3, 7] = float("nan")
+        t.uniform[3] = np.float32(1 - 2.0 ** -24)
+        t.check(t.run())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("batch,vocab,shift", [(2, 7, 0), (3, 8000, 1), (2, 20000, 3), (2, 32768, 0), (3, 32771, 2),
                                                (70, 50257, 1), (130, 131072, 0), (260, 65537, 5), (2, 140000, 1)])
 def test_tokens_alone(batch, vocab, shift, dt):
