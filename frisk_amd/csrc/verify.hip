@@ -48,7 +48,7 @@ struct Rest {
 };
 // Where a walk ended.
 struct End {
-  double scale;  // sum of the row's weights
+  double inverse;  // of the sum of the row's weights
   float m;       // its maximum
   int node;      // -1: the tree takes no part, -2: no token
   int rounds;    // children rejected there
@@ -60,7 +60,7 @@ struct Layout {
   Stat* stats;  // [batch][tokens][segments]
   Rest* rest;   // [batch][segments]
   End* end;     // [batch]
-  double* list;  // [batch][tokens] rejected tokens or, of dense drafts, what their rest summed to
+  double* list;  // [batch][tokens] rejected tokens or, of dense drafts, 1 over what their rest summed to
 };
 __host__ __device__ inline int64_t up16(int64_t n) { return (n + 15) & ~15ll; }
 __device__ __forceinline__ Layout layout(const VerifyArgs& a) {
@@ -274,11 +274,12 @@ __device__ __forceinline__ double lane_d(double x, int k) {
 // ---- segments of a row --------------------------------------------------------------
 
 // What is left of a probability p after `rounds` children drawn from q were
-// rejected, whose rests summed to z[0 ..]; a rest without mass leaves it as it was.
+// rejected, whose rests' sums have the inverses z[0 ..]; a rest without mass (0) leaves it as
+// it was.  (With divisions in their place a tree of 8 nodes over 47565 bf16 took 41 us, not 37.)
 __device__ __forceinline__ double left_of(double p, double q, const double* z, int rounds) {
   for (int i = 0; i < rounds; ++i) {
-    const double rest = __builtin_fmax(p - q, 0.0), mass = z[i];
-    if (mass > 0.0) p = rest / mass;
+    const double rest = __builtin_fmax(p - q, 0.0), inverse = z[i];
+    if (inverse > 0.0) p = rest * inverse;
   }
   return p;
 }
@@ -376,7 +377,7 @@ __device__ __forceinline__ Rest segment_rest(const VerifyArgs& a, const Row<E>& 
   const double top = (double)e.m;
   double s = 0.0, whole = 0.0;
   auto add = [&](float x, int v) {
-    const Left w = dense_left(pow2(((double)x - top) * factor) / e.scale, q[v], list, e.rounds);
+    const Left w = dense_left(pow2(((double)x - top) * factor) * e.inverse, q[v], list, e.rounds);
     s += w.now;
     whole += w.was;
   };
@@ -487,7 +488,7 @@ __device__ __forceinline__ void pick(const VerifyArgs& a, int64_t b, const End& 
   const bool whole = use_whole;
   auto weight = [&](float x) { return pow2(((double)x - top) * factor); };
   auto left = [&](double p, int v) {
-    const Left w = dense_left(p / e.scale, q[v], list, e.rounds);
+    const Left w = dense_left(p * e.inverse, q[v], list, e.rounds);
     return whole ? w.was : w.now;
   };
   // The segment's elements in order: part 0 is the head (the first wave's), 1 + w wave
@@ -989,11 +990,11 @@ __global__ __launch_bounds__(kWalkers) void verify_walk_kernel(VerifyArgs a) {
     if (!todo) break;
     // The sum of what `at_rounds` rejected children left of node at_node's row.
     const int node = at_node, done = at_rounds - 1;
-    const double top = (double)tops[node], scale = mass[node];
+    const double top = (double)tops[node], inverse = 1.0 / mass[node];
     const float* q = a.draft_probs + b * a.qb + node * a.qt;
     double s = 0.0;
     for (int v = tid; v < a.vocab; v += kWalkers) {
-      const double p = pow2(((double)logit<E>(a, b, node, v) - top) * factor) / scale;
+      const double p = pow2(((double)logit<E>(a, b, node, v) - top) * factor) * inverse;
       s += __builtin_fmax(left_of(p, (double)q[v], list, done) - (double)q[v], 0.0);
     }
     s = wave_sum(s);
@@ -1002,12 +1003,12 @@ __global__ __launch_bounds__(kWalkers) void verify_walk_kernel(VerifyArgs a) {
     if (tid == 0) {
       double all = 0.0;
       for (int w = 0; w < (kWalkers / 64); ++w) all += sums[w];
-      list[done] = all;
+      list[done] = all > 0x1p-1000 ? 1.0 / all : 0.0;
     }
     __syncthreads();
   }
   // (Of the first wave.  A node at which no child was rejected has no `firsts`.)
-  End e = {mass[cur], tops[cur], none ? -2 : cur, rounds, factor != 0.0 ? -1 : rounds > 0 ? firsts[cur] : -2, 0};
+  End e = {1.0 / mass[cur], tops[cur], none ? -2 : cur, rounds, factor != 0.0 ? -1 : rounds > 0 ? firsts[cur] : -2, 0};
   if constexpr (LAST) {
     __shared__ End end;
     __shared__ Rest rests[plan::kVerifyShort];
