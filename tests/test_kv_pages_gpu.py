@@ -301,8 +301,9 @@ def test_graph_and_stream():
     reset()
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
-    assert [x.tolist() for x in work(side)] == made or side.synchronize()
+    got = work(side)
     side.synchronize()
+    assert [x.tolist() for x in got] == made
     assert same(tensors(cache), want)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
