@@ -274,3 +274,42 @@ def test_a_key_scale_that_is_nan(dt, kind):
         s.cache.k_scale[int(s.table[0, 0])] = float("nan")
         o, lse = s.run()
         assert torch.isnan(o[0]).all() and torch.equal(o[1:], o0[1:])
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "i8"])
+def test_graph_replay_and_streams(kind):
+    # A captured step of append, read and attention: tokens and lengths change between replays.
+    m = Blocks(2, 2, 64, "bf16", kind, 32, 16, 96)
+    k, v = (torch.zeros(2, 3, 2, 64, dtype=torch.bfloat16, device="cuda").transpose(1, 2) for _ in range(2))
+    q, ctx = randn((2, 4, 3, 64), 7).to(torch.bfloat16), ints([0, 0])
+    ko, vo, o = (torch.zeros_like(x) for x in (k, v, q))
+
+    def step(stream=None):
+        rt.kv_append(k, v, m.cache, ctx, stream=stream)
+        rt.kv_read(m.cache, ko, vo, ctx, stream=stream)
+        rt.tree_attn(q, m.cache, ctx, o, stream=stream)
+
+    def load(n):
+        for x, new in zip((k, v), rows(2, 3, 2, 64, "bf16", n, 1.0 + n % 5)):
+            x.copy_(new)
+        ctx.copy_(ints([2 * n, 3 * n + 1]))
+        torch.cuda.synchronize()
+        m.append(k, v, [2 * n, 3 * n + 1], [3, 3])
+
+    side = torch.cuda.Stream()
+    load(0)
+    step(side)
+    side.synchronize()
+    m.check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for n in range(1, 6):
+        load(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        m.check()
+        got = [x.clone() for x in (ko, vo, o)]
+        rt.kv_read(m.cache, ko, vo, ctx)
+        rt.tree_attn(q, m.cache, ctx, o)
+        assert all(torch.equal(x, y) for x, y in zip(got, (ko, vo, o)))

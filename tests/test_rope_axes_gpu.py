@@ -125,3 +125,28 @@ def test_refuses_wrong_arguments():
         rt.rope(x, x, pos[0], table, pair_axis=axis)
     with pytest.raises(ValueError, match="axes"):
         rt.rope(x, x, torch.zeros(5, 4, dtype=torch.int64, device="cuda"), table, pair_axis=axis)
+
+
+def test_graph_replay_streams_and_in_place():
+    x = randn((2, 5, 7, 64), 21)
+    table, axis = rt.rope_table(48), rt.rope_axes([8, 12, 4])
+    pos = torch.zeros(3, 2, 7, dtype=torch.int32, device="cuda")
+    out, side = torch.empty_like(x), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    rt.rope(x, out, pos, table, pair_axis=axis, stream=side)
+    side.synchronize()
+    assert torch.equal(out, x)  # (no turn)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rt.rope(x, out, pos, table, pair_axis=axis)
+    for step in range(3):
+        pos.copy_(torch.randint(-50, 50, pos.shape, generator=torch.Generator().manual_seed(step)))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, x, pos.cpu().numpy(), axis.tolist(), table, "f32")
+    # Heads of one buffer, more of them than a thread has in flight, turned in place.
+    wide = randn((2, 7, 40, 64), 22)
+    before = wide.clone()
+    rt.rope(wide[:, :, :36].transpose(1, 2), wide[:, :, :36].transpose(1, 2), pos, table, pair_axis=axis)
+    check(wide[:, :, :36].transpose(1, 2), before[:, :, :36].transpose(1, 2), pos.cpu().numpy(), axis.tolist(), table, "f32")
+    assert torch.equal(wide[:, :, 36:], before[:, :, 36:])
