@@ -358,3 +358,30 @@ def test_another_stream_and_a_graph():
             x.copy_(torch.as_tensor(y))
         graph.replay()
         n.check((*(x.cpu().numpy() for x in (path, count, token)), probs.double().cpu().numpy()))
+
+
+@pytest.mark.parametrize("batch,tokens,vocab,dense", [(2, 17, 40000, False), (2, 9, 20011, True), (2, 1, 5000, False),
+                                                      (2, 1, 140000, False), (4, 64, 131072, False)])
+def test_graphs_of_every_way(batch, tokens, vocab, dense):
+    # Long rows, one node a tree in one launch and in two, rows through a table; one workspace.
+    first = Trees(batch, tokens, vocab, "bf16", dense=dense, seed=51)
+    dev = lambda x: torch.as_tensor(x).cuda()  # noqa: E731
+    args = (first.logits, dev(first.drafts), dev(first.parents), dev(first.uniform), dev(first.final))
+    need = rt.tree_verify_workspace_bytes(batch, tokens, vocab, torch.bfloat16)
+    ws = torch.full((need + 16,), 255, dtype=torch.uint8, device="cuda")
+    probs = torch.empty(batch, tokens, device="cuda")
+    rt.tree_verify(*args, draft_probs=first.q, workspace=ws)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        path, count, token = rt.tree_verify(*args, draft_probs=first.q, probs=probs, workspace=ws)
+    for seed in (52, 53, 54):
+        n = Trees(batch, tokens, vocab, "bf16", dense=dense, seed=seed)
+        first.logits.copy_(n.logits)
+        if dense:
+            first.q.copy_(n.q)
+        for x, y in zip(args[1:], (n.drafts, n.parents, n.uniform, n.final)):
+            x.copy_(torch.as_tensor(y))
+        ws.fill_(seed)  # (what it holds does not matter)
+        for _ in range(2):
+            graph.replay()
+            n.check((*(x.cpu().numpy() for x in (path, count, token)), probs.double().cpu().numpy()))
