@@ -63,8 +63,6 @@ __global__ __launch_bounds__(kThreads, 4) void kv_block_kernel(KvArgs a, int g, 
   hi = hi < first + size ? hi : first + size;
   hi = hi < c.capacity ? hi : c.capacity;
   if (lo >= hi) return;
-  const kv::Slot at = kv::slot_of(c, b, first);
-  if (at.elem < 0) return;
   const int old = (int)(lo - first), end = (int)(hi - first);
 
   const int sub = threadIdx.x & ((1 << g) - 1), row0 = threadIdx.x >> g, rows = kThreads >> g;
@@ -72,6 +70,18 @@ __global__ __launch_bounds__(kThreads, 4) void kv_block_kernel(KvArgs a, int g, 
   const uint16_t* x = (const uint16_t*)(of_v ? a.v : a.k) + b * (of_v ? a.vsb : a.ksb) + h * (of_v ? a.vsh : a.ksh) +
                       (first - sp.ctx) * (of_v ? a.vss : a.kss) + sub * 8;
   const int64_t xs = of_v ? a.vss : a.kss;
+  // (The new rows' loads are under way while the page is looked up.)
+  i32x4 held[HOLD ? HOLD : 1];
+  if constexpr (HOLD) {
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      const int r = row0 + i * rows;
+      held[i] = i32x4{0, 0, 0, 0};
+      if (in && r >= old && r < end) held[i] = *(const i32x4*)(x + r * xs);
+    }
+  }
+  const kv::Slot at = kv::slot_of(c, b, first);
+  if (at.elem < 0) return;
   char* codes = (char*)(of_v ? c.v : c.k) + at.elem + h * c.sh + sub * 8;
   float* scale_at = (of_v ? c.v_scale : c.k_scale) + at.scale + h * c.sch;
   __shared__ uint32_t tops[kThreads / 64];
@@ -87,14 +97,7 @@ __global__ __launch_bounds__(kThreads, 4) void kv_block_kernel(KvArgs a, int g, 
       top = max(top, max(w & 0xffffu, w >> 16));
     }
   };
-  i32x4 held[HOLD ? HOLD : 1];
   if constexpr (HOLD) {
-#pragma unroll
-    for (int i = 0; i < HOLD; ++i) {
-      const int r = row0 + i * rows;
-      held[i] = i32x4{0, 0, 0, 0};
-      if (in && r >= old && r < end) held[i] = *(const i32x4*)(x + r * xs);
-    }
 #pragma unroll
     for (int i = 0; i < HOLD; ++i) larger(held[i]);
   } else {
