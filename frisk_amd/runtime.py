@@ -291,17 +291,18 @@ def _stream_handle(stream) -> int:
     return int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
 
 
-def _empty(shape, dtype, device, stream):
-    """A new tensor, allocated on the stream that the call's kernels run on: the
-    allocator may have had its memory in use by, and may hand it out again to,
+def _empty(shape, dtype, device, stream, fill=None):
+    """A new tensor, allocated (and filled) on the stream that the call's kernels run on:
+    the allocator may have had its memory in use by, and may hand it out again to,
     work of that stream only."""
     import torch
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        t = torch.empty(shape, dtype=dtype, device=device)
+        return t if fill is None else t.fill_(fill)
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return _empty(shape, dtype, device, None, fill)
 
 
 def _scratch(nbytes: int, device, stream):
@@ -1118,8 +1119,8 @@ def tree_verify(logits, drafts, parents, uniform, final, *, draft_probs=None, te
     path (int32 [batch, tokens]) lists the accepted nodes from 0 on, then -1, count (int32 [batch])
     their number, token (int32 [batch]) is -1 where logits hold a NaN or +infinity; probs (f32 [batch, tokens],
     optional) takes the target's probability of each draft.  Trees have new_len[b]
-    nodes (int32 [batch], None: all; 0: left as they were).  Frees no page and
-    moves no row: kv_compact and kv_pages do.
+    nodes (int32 [batch], None: all; 0: left as they were, -1, 0 and -1 in tensors that
+    the call makes).  Frees no page and moves no row: kv_compact and kv_pages do.
     `workspace`: True allocates it (torch's caching allocator, on the call's
     stream), a device tensor of tree_verify_workspace_bytes supplies it."""
     import torch
@@ -1138,12 +1139,13 @@ def tree_verify(logits, drafts, parents, uniform, final, *, draft_probs=None, te
             return tree_verify(logits, drafts, parents, uniform, final, draft_probs=draft_probs,
                                temperature=temperature, new_len=new_len, path=path, count=count, token=token,
                                probs=probs, workspace=workspace, stream=stream)
+    absent = new_len is not None  # trees of no nodes: nothing is written for them
     if path is None:
-        path = _empty((b, t), torch.int32, logits.device, stream)
+        path = _empty((b, t), torch.int32, logits.device, stream, -1 if absent else None)
     if count is None:
-        count = _empty((b,), torch.int32, logits.device, stream)
+        count = _empty((b,), torch.int32, logits.device, stream, 0 if absent else None)
     if token is None:
-        token = _empty((b,), torch.int32, logits.device, stream)
+        token = _empty((b,), torch.int32, logits.device, stream, -1 if absent else None)
     dev = _same_device(logits, drafts, parents, uniform, final, draft_probs, temperature, new_len, path, count,
                        token, probs)
     i32, f32, one, all_ = torch.int32, torch.float32, shape[:1], shape[:2]

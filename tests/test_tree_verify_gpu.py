@@ -360,6 +360,21 @@ def test_another_stream_and_a_graph():
         n.check((*(x.cpu().numpy() for x in (path, count, token)), probs.double().cpu().numpy()))
 
 
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_made_outputs_of_trees_without_nodes(own_stream):
+    t = Trees(4, 5, 300, seed=61)
+    junk = [torch.full((4096,), 9, dtype=torch.int32, device="cuda") for _ in range(8)]
+    new, side = torch.tensor([5, 0, -3, 1], dtype=torch.int32, device="cuda"), torch.cuda.Stream()
+    dev = lambda x: torch.as_tensor(x).cuda()  # noqa: E731
+    args = (t.logits, dev(t.drafts), dev(t.parents), dev(t.uniform), dev(t.final))
+    del junk
+    torch.cuda.synchronize()
+    path, count, token = rt.tree_verify(*args, new_len=new, stream=side if own_stream else None)
+    torch.cuda.synchronize()
+    assert (path[1:3] == -1).all() and path[3].tolist() == [0, -1, -1, -1, -1]
+    assert count.tolist()[1:] == [0, 0, 1] and token.tolist()[1:3] == [-1, -1] and token[3] >= 0 and token[0] >= 0
+
+
 @pytest.mark.parametrize("batch,tokens,vocab,dense", [(2, 17, 40000, False), (2, 9, 20011, True), (2, 1, 5000, False),
                                                       (2, 1, 140000, False), (4, 64, 131072, False)])
 def test_graphs_of_every_way(batch, tokens, vocab, dense):
