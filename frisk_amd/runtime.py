@@ -916,12 +916,12 @@ def kv_compact(cache, path, ctx_len, count, *, stream=None):
     ctx_len negative: the sequence takes no part).  Not for a cache with
     scale_block, whose rows are appended again instead."""
     import torch
-    if path.dtype != torch.int32 or path.dim() != 2 or not path.is_cuda or \
-            (path.stride(1) != 1 and path.shape[1] > 1):
+    shape, st = path.shape, path.stride()
+    if path.dtype != torch.int32 or len(shape) != 2 or not path.is_cuda or (st[1] != 1 and shape[1] > 1):
         raise ValueError("path must be an int32 device tensor [batch, tokens] with unit stride along the tokens")
-    b, t = path.shape
+    b, t = shape
     dev = cache._check(b, path, ctx_len, count)
-    desc = _compact_pack.pack(b, t, path.data_ptr(), path.stride(0) if b > 1 else t,
+    desc = _compact_pack.pack(b, t, path.data_ptr(), st[0] if b > 1 else t,
                               _lengths(ctx_len, b, "ctx_len"), _lengths(count, b, "count"))
     _run("frisk_kv_compact", desc + cache._packed, dev, stream)
     return cache
