@@ -1047,8 +1047,9 @@ int check_verify(const frisk_tree_verify_desc* d, bool ptrs, frisk::VerifyArgs& 
   const int es = esize(d->dtype);
   if (d->batch > INT32_MAX / 4) return fail(FRISK_EUNSUP, "%s: more trees than one launch takes", fn);
   const plan::VerifyPlan p = plan::verify_plan(d->batch, d->tokens, d->vocab, es);
-  if (d->batch > (int64_t)(UINT32_MAX / 256) / (d->tokens * p.segments))
+  if (d->batch > plan::kVerifySegments / (d->tokens * p.segments))
     return fail(FRISK_EUNSUP, "%s: more rows of logits than one launch takes", fn);
+  if (d->batch > plan::kVerifyTrees) return fail(FRISK_EUNSUP, "%s: more trees than one launch takes", fn);
   const int64_t st[4] = {d->stride_b, d->stride_t, d->draft_probs ? d->draft_stride_b : 0,
                          d->draft_probs ? d->draft_stride_t : 0};
   for (const int64_t s : st)

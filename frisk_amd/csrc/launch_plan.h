@@ -646,6 +646,12 @@ inline VerifyPlan verify_plan(int64_t batch, int64_t tokens, int64_t vocab, int 
   return {pieces, segments(pieces)};
 }
 
+// What a call takes, as a launch has fewer than 2^32 threads: a walk, or a launch for trees of one
+// node, has a workgroup for each tree; a row's segment has a wave, in a workgroup of four.
+constexpr int kVerifyTreeThreads = 1024;
+constexpr int64_t kVerifyTrees = UINT32_MAX / kVerifyTreeThreads;
+constexpr int64_t kVerifySegments = UINT32_MAX / 256;
+
 // Whether trees of one node have a workgroup of 16 waves each and a launch, in place of a
 // workgroup for every four segments and a second launch.  us of a call between other work in a graph, in
 // two launches and in one (segments in brackets):

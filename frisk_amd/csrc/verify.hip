@@ -29,8 +29,8 @@ namespace frisk {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kWalkers = 1024;  // threads of a walk
-constexpr int kAlone = 1024;    // threads of a row in a launch of its own
+constexpr int kWalkers = plan::kVerifyTreeThreads;  // threads of a walk
+constexpr int kAlone = plan::kVerifyTreeThreads;    // threads of a row in a launch of its own
 
 // A segment's or a row's largest logit, its first place, and the sum of weights
 // 2^((x - m) c): NaN if the row gives no probabilities (it holds a NaN or +infinity).
@@ -1042,7 +1042,6 @@ __global__ __launch_bounds__(kWalkers) void verify_walk_kernel(VerifyArgs a) {
 
 template <Elt E, int PIECES> hipError_t launch_pieces(const VerifyArgs& a, hipStream_t s) {
   const int64_t groups = (a.segments + kWaves - 1) / kWaves;  // a segment a wave
-  if (a.batch * a.tokens * groups > UINT32_MAX / kThreads) return hipErrorInvalidConfiguration;
   if (plan::verify_alone(a.batch, a.tokens, a.segments, device_cus())) {
     hipLaunchKernelGGL((verify_alone_kernel<E, PIECES>), dim3((unsigned)a.batch), dim3(kAlone), 0, s, a);
     return hipGetLastError();

@@ -635,7 +635,8 @@ int frisk_kv_pages(const frisk_kv_pages_desc* desc, void* stream);
  * probabilities (probs NaN): the walk ends there and token[b] is -1.  A draft outside the vocabulary
  * is never accepted.  Only the first new_len[b] nodes take part (all, if NULL; below 1: the tree's
  * outputs are left as they were).  temperature is finite.  drafts, parents, uniform, path and probs are contiguous [batch, tokens],
- * final_uniform, temperature, new_len, count and token [batch].  tokens <= 1024, vocab <= 2^24.
+ * final_uniform, temperature, new_len, count and token [batch].  tokens <= 1024, vocab <= 2^24;
+ * fewer than 2^22 trees, and fewer than 2^24 segments (of 1 KiB or more) of their rows.
  * workspace (16-byte aligned): at least frisk_tree_verify_workspace_size bytes, which the current
  * device decides (0, and NULL will do, for trees of one node with short rows or many of them); its contents before
  * a call do not matter, and calls that share one must not overlap in time.  No output overlaps another tensor.
