@@ -1122,7 +1122,8 @@ def tree_verify(logits, drafts, parents, uniform, final, *, draft_probs=None, te
     nodes (int32 [batch], None: all; 0: left as they were, -1, 0 and -1 in tensors that
     the call makes).  Frees no page and moves no row: kv_compact and kv_pages do.
     `workspace`: True allocates it (torch's caching allocator, on the call's
-    stream), a device tensor of tree_verify_workspace_bytes supplies it."""
+    stream), a device tensor of tree_verify_workspace_bytes supplies it, False or None
+    is for calls that take none."""
     import torch
     if logits.dim() != 3:
         raise ValueError("logits must be a device tensor [batch, tokens, vocab]")
@@ -1160,14 +1161,16 @@ def tree_verify(logits, drafts, parents, uniform, final, *, draft_probs=None, te
             _words(token, one, i32, "token"), _words(probs, all_, f32, "probs"))
     except _RANGE as e:
         raise _range_error(e) from None
+    tail = bytes(16)
     if workspace is True:
         need = _raw_fn("frisk_tree_verify_workspace_size")(head + bytes(16))
         if need < 0:
             _check(need, "frisk_tree_verify_workspace_size")
-        tail = bytes(16)
         if need:
             workspace = _scratch(need, logits.device, stream)
             tail = _ws_pack.pack(workspace.data_ptr(), need)
+    elif workspace is False or workspace is None:
+        pass
     elif workspace.get_device() != dev or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous tensor on the logits' device")
     else:
