@@ -819,8 +819,7 @@ class KvCache:
         if (k_scale is None) != (k.element_size() == 2) or (v_scale is None) != (k_scale is None):
             raise ValueError("an 8-bit cache has k_scale and v_scale, a 16-bit one none")
         sst = (0, 0, 0)
-        if scale_block < 1 or (scale_block > 1 and k_scale is None):
-            raise ValueError(f"scale_block must be 1 or more, and is for 8-bit caches (got {scale_block})")
+        self._check_block(scale_block, k.element_size())
         if k_scale is not None:
             shape = (ksh[0], ksh[1], -(-ksh[2] // scale_block))
             for t in (k_scale, v_scale):
@@ -852,6 +851,7 @@ class KvCache:
               device="cuda"):
         """A cache over new tensors (their contents undefined until written)."""
         import torch
+        cls._check_block(scale_block, dtype.itemsize)
         shape = (pages, kv_heads, page_size, head_dim)
         k, v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
         ks = vs = None
@@ -859,6 +859,11 @@ class KvCache:
             scales = (pages, kv_heads, -(-page_size // scale_block))
             ks, vs = (torch.empty(scales, dtype=torch.float32, device=device) for _ in range(2))
         return cls(k, v, ks, vs, block_table, scale_block=scale_block)
+
+    @staticmethod
+    def _check_block(scale_block, bytes_):
+        if scale_block < 1 or (scale_block > 1 and bytes_ != 1):
+            raise ValueError(f"scale_block must be 1 or more, and is for 8-bit caches (got {scale_block})")
 
     def __setattr__(self, name, value):
         # The calls take the descriptor that __init__ packed.
