@@ -948,10 +948,11 @@ def kv_pages(table, keep, want, page_size, pages, *, parent=None, held=None, out
     """(out, src, dst, rows, lacking): the block table of the next step, from `table`
     (int32 [batch, max_pages]) of a cache of `pages` pages.  Row b takes over the pages of the first
     keep[b] keys of row parent[b] (None: its own; outside the batch: sequence b has ended, and its
-    pages are free) and has room for want[b] keys (None: keep[b]).  Sequences share whole
-    pages; one that would write a shared page gets a copy of it: page dst[b]
-    of src[b], the first rows[b] slots (-1, -1, 0: none), which kv_copy_pages makes in every
-    layer's cache.  New pages are the lowest-numbered ones that no row has and that
+    pages are free) and has room for want[b] keys (None: keep[b]).  keep[b] is a length of the
+    parent's row, not of b's own: a program that keeps all of it passes ctx_len[parent[b]], which
+    is b's length from then on.  Sequences share whole pages; one that would write a shared page
+    gets a copy of it: page dst[b] of src[b], the first rows[b] slots (-1, -1, 0: none), which
+    kv_copy_pages makes in every layer's cache.  New pages are the lowest-numbered ones that no row has and that
     `held` (uint8 or bool [pages]) does not keep back; lacking[0] counts the entries
     that are -1 because there were too few.  keep, want, parent, src, dst, rows: int32
     [batch]; lacking: int32 [1].  `out` must be another tensor than `table`; a program with one table

@@ -579,7 +579,8 @@ int frisk_kv_copy_pages(const frisk_kv_copy_pages_desc* desc, void* stream);
  * The block table of the next step: sequences fork, end, go back and grow.  Row b of
  * `out` continues row parent[b] (its own, if parent is NULL; one outside 0 .. batch - 1:
  * sequence b has ended, its row holds no page): it takes over the pages of that
- * row's first keep[b] keys and has room for want[b] (keep[b], if less, or if want is
+ * row's first keep[b] keys (a length of the parent's row: entries of kept places that hold no page
+ * get a new one, whose keys nobody has written) and has room for want[b] (keep[b], if less, or if want is
  * NULL); both are held in 0 .. max_pages * page_size (keep[b] < 0: the sequence has
  * ended).  Several rows may take over a page.  A last page that is not full,
  * where a row's next keys go, must be its own: where others take that page over in
