@@ -2,12 +2,17 @@
 // the conversions of its 8-bit rows.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 #include "kernels.h"
 #include "kv_index.h"
 
 namespace frisk {
 namespace kv {
+
+// (The indexing counts a scale a row for a Cache without this member.)
+static_assert(std::is_same<decltype(KvCache::scale_shift), int>::value, "the log2 of the rows that share a scale");
 
 template <Elt C> constexpr float kTop = C == Elt::E4M3 ? 448.0f : 127.0f;
 
