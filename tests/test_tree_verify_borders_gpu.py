@@ -1,0 +1,54 @@
+"""Decisions close to a border, against the fp64 oracle: what rejected drafts leave is a
+difference, right to 2^-42 of what there was before them.  Here they take all but
+2^-20, and random numbers lie 2^-21 beside the border or farther."""
+import numpy as np
+import pytest
+import torch
+
+from frisk_amd import runtime as rt
+from oracle import serving_ops as S
+from tests.test_tree_verify_gpu import DT
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("stages", [1, 2])
+@pytest.mark.parametrize("dt,batch,tokens,vocab", [
+    ("f32", 48, 4, 3000), ("f16", 48, 4, 8200), ("bf16", 48, 4, 50304),
+    # Rows enough that their weights come from a table.
+    ("bf16", 128, 64, 50304)])
+def test_after_a_likely_draft_is_rejected(dt, batch, tokens, vocab, stages):
+    rng = np.random.default_rng(vocab + stages)
+    logits = np.empty((batch, 1, vocab))
+    drafts, uniform = np.zeros((batch, tokens), np.int32), np.full((batch, tokens), 0.5, np.float32)
+    parents = np.full((batch, tokens), -1, np.int32)
+    parents[:, 1:stages + 2] = 0
+    for b in range(batch):
+        x = 20.0 - np.log(vocab) - 20.0 * np.log(2.0) + rng.normal(0, 0.5, vocab)
+        likely = rng.permutation(vocab)[:stages + 1]
+        # The first draft all but 2^-20, or each of two all but 2^-10 of what there is.
+        x[likely[0]] = 20.0
+        if stages == 2:
+            x[likely[1]] = 20.0 - 10.0 * np.log(2.0)
+        x[likely[-1]] += 6.0
+        logits[b, 0] = torch.from_numpy(x).to(DT[dt]).double().numpy()
+        a = S.probabilities(logits[b, 0])
+        for i in range(stages):
+            drafts[b, 1 + i], uniform[b, 1 + i] = likely[i], np.nextafter(np.float32(1), np.float32(0))
+            assert a[likely[i]] < uniform[b, 1 + i]
+            a[likely[i]] = 0.0
+            a /= a.sum()
+        last = likely[-1]
+        drafts[b, 1 + stages] = last
+        side = 1.0 + (1 if b % 2 else -1) * 2.0 ** -rng.uniform(12, 20)
+        uniform[b, 1 + stages] = a[last] * side
+        assert abs(float(uniform[b, 1 + stages]) / a[last] - 1.0) > 2.0 ** -21
+    final = rng.random(batch, np.float32)
+    path, count, token = rt.tree_verify(
+        torch.from_numpy(logits).to(DT[dt]).cuda().expand(batch, tokens, vocab),
+        *(torch.from_numpy(x).cuda() for x in (drafts, parents, uniform, final)))
+    path, count, token = path.tolist(), count.tolist(), token.tolist()
+    for b in range(batch):
+        want, last, _ = S.verify(np.broadcast_to(logits[b], (tokens, vocab)), drafts[b], parents[b], uniform[b], final[b])
+        assert len(want) == (1 if b % 2 else 2)
+        assert (path[b][:count[b]], token[b]) == (want, last), b
