@@ -273,7 +273,7 @@ __device__ __forceinline__ double lane_d(double x, int k) {
 
 // ---- segments of a row --------------------------------------------------------------
 
-// What is left of a probability p after `rounds` children drawn from q were
+// What is left of a probability p after `rounds` children drawn independently from q were
 // rejected, whose rests' sums have the inverses z[0 ..]; a rest without mass (0) leaves it as
 // it was.  (With divisions in their place a tree of 8 nodes over 47565 bf16 took 41 us, not 37.)
 // A pass of the walk calls it for every element, so many rejections at one node cost their square: 50257

@@ -1120,7 +1120,8 @@ def tree_verify(logits, drafts, parents, uniform, final, *, draft_probs=None, te
     each node, at `temperature` (f32 [batch], None: 1, 0: the largest logit).  uniform
     (f32 [batch, tokens]) decides about each draft, final (f32 [batch]) draws the last
     token; both are of [0, 1).  draft_probs (f32 [batch, tokens, vocab]): row n holds the
-    probabilities that node n's children were drawn from; None: drafts are certain
+    probabilities that node n's children were drawn from, independently (with replacement:
+    else tokens are not distributed as the target's); None: drafts are certain
     ones.  With one node a tree this samples from its logits.
     path (int32 [batch, tokens]) lists the accepted nodes from 0 on, then -1, count (int32 [batch])
     their number, token (int32 [batch]) is -1 where logits hold a NaN or +infinity; probs (f32 [batch, tokens],

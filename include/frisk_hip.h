@@ -625,7 +625,8 @@ int frisk_kv_pages(const frisk_kv_pages_desc* desc, void* stream);
  * token x is accepted, and the walk goes on from it, if
  *   uniform[b][t] q(x) < a(x);
  * else a becomes max(a - q, 0) over its sum (and stays if that is 0).  q is draft_probs[b][node]
- * (f32 [batch, tokens, vocab], finite and at least 0), from which all of the node's children were drawn, or,
+ * (f32 [batch, tokens, vocab], finite and at least 0), from which all of the node's children were drawn independently (with
+ * replacement: of children drawn without it the tokens are not distributed as the target's), or,
  * if NULL, certain drafts: q(x) = 1 for the child's own token.  When no child is
  * left, token[b] is the first v at which a summed over 0 .. v passes final_uniform[b]
  * times its whole sum.  With draft_probs each child of a node that is rejected before its last one costs a pass over
