@@ -901,7 +901,8 @@ def kv_append(k, v, cache, ctx_len, *, new_len=None, stream=None):
     device; negative: the sequence takes no part), the first new_len[b]
     tokens of it.  An 8-bit cache quantises each row by its largest value, or
     a block's rows by theirs: a block's scale grows with its rows, and the codes
-    before them follow (frisk_kv_append)."""
+    before them follow (frisk_kv_append).  Both stay when the rows are drafts that
+    are rejected, and so does NaN; a block appended from its first slot is made anew."""
     _kv("frisk_kv_append", k, v, cache, ctx_len, new_len, stream)
     return cache
 

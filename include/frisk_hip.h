@@ -465,6 +465,10 @@ typedef struct frisk_kv_cache {
  * those keys become c (s (1 / scale)), in f32, rounded likewise.  An infinity or
  * NaN makes the block's scale NaN, and all of its keys read back as NaN.
  * What the block holds behind the new rows has no meaning afterwards.
+ * So drafts that are rejected leave their mark: the scale that they raised, the second rounding of the
+ * codes before them, and NaN if they held a value that is not finite, stay with the block's decided
+ * keys, and what is generated over such a cache may depend on the drafts.  Keys appended again from the
+ * block's first slot on are as if the drafts had never been there.
  * Pages written by one call must be distinct between its sequences, and k, v
  * and the cache four tensors (six with the scales) that share no memory.
  */
