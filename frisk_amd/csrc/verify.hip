@@ -4,8 +4,8 @@
 // Probabilities are compared with random numbers, so they are computed in 64
 // bits: a weight is 2^t, t = (x - max) log2(e) / T, from a polynomial of degree 9
 // on the fraction of t, off by 2^-45 of it, and sums are of doubles.  The vector
-// unit does as many 64-bit as 32-bit multiply-adds, so a weight costs about 16
-// instructions.
+// unit does as many 64-bit as 32-bit multiply-adds, so a weight costs 17
+// instructions, 16 of them of 64 bits.
 //
 // Three launches.  (1) The rows of nodes that have children, a wave for each
 // segment of a row, without a barrier: its maximum and sum.  (2) A workgroup per tree combines
@@ -677,8 +677,8 @@ template <Elt E, int PIECES> __global__ __launch_bounds__(kThreads) void verify_
 // ---- rows of bf16 through a table ------------------------------------------------------
 
 // There are few bf16 numbers: the weights 2^(x c) of all of 2^-16 <= |x| < 2^7 are 5888
-// doubles, which a workgroup computes once, and a logit's is a read of LDS (five 32-bit
-// instructions and an addition of 64 bits in the place of 17 of 64).  c <= 7, so that they stay
+// doubles (46 KiB, in 55 of LDS: each sign begins a half), which a workgroup computes once, and a logit's is a read of LDS (five 32-bit
+// instructions and an addition of 64 bits in the place of 17).  c <= 7, so that they stay
 // within a double's range (and x c, up to 900, is off by 2^-44); segments with other numbers are
 // summed as the other types' are.  131072 logits of 32 rows of 8 trees: 33 us without the
 // table, 20 with it, which the reads of LDS and their conflicts bound (bytes: 11).
