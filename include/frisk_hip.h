@@ -648,7 +648,8 @@ int frisk_kv_pages(const frisk_kv_pages_desc* desc, void* stream);
  * fewer than 2^22 trees, and fewer than 2^24 segments (of 1 KiB or more) of their rows.
  * workspace (16-byte aligned): at least frisk_tree_verify_workspace_size bytes, which the current
  * device decides (0, and NULL will do, for trees of one node with short rows or many of them); its contents before
- * a call do not matter, and calls that share one must not overlap in time.  No output overlaps another tensor.
+ * a call do not matter, and calls that share one must not overlap in time.  No output overlaps another tensor
+ * (the rows of logits and of draft_probs count with what lies between them).
  */
 typedef struct frisk_tree_verify_desc {
   int64_t batch, tokens, vocab;
