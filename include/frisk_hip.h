@@ -636,7 +636,8 @@ int frisk_kv_pages(const frisk_kv_pages_desc* desc, void* stream);
  * times its whole sum.  With draft_probs each child of a node that is rejected before its last one costs a pass over
  * the row by one workgroup, and a pass goes through the rejections before it: time grows with their
  * square (64 rejected children over a vocabulary of 50257: 7 ms).  Random numbers are of [0, 1).  Probabilities are computed in 64 bits, off
- * by less than 2^-42 of themselves, what rejected drafts leave by 2^-42 of what there was before them.
+ * by less than 2^-42 of themselves, what rejected drafts leave by 2^-42 of what there was before them; one below
+ * 2^-1000 of its row's largest counts as 0.
  *
  * path[b] ([tokens]) lists the nodes of the walk, node 0 first, then -1; count[b] is their
  * number.  probs[b][t] (optional) is p of a node's token given its parent, 0 for nodes without

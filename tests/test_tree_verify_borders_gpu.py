@@ -52,3 +52,23 @@ def test_after_a_likely_draft_is_rejected(dt, batch, tokens, vocab, stages):
         want, last, _ = S.verify(np.broadcast_to(logits[b], (tokens, vocab)), drafts[b], parents[b], uniform[b], final[b])
         assert len(want) == (1 if b % 2 else 2)
         assert (path[b][:count[b]], token[b]) == (want, last), b
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("batch", [1, 300])
+def test_the_least_probability(dt, batch):
+    # Weights below 2^-1000 of the largest are none: a random number of 0 picks the first that is
+    # one, and accepts no draft without.  2^-1082, 2^-938 and 1, at T = 1/1024.
+    x = torch.full((batch, 3, 40), -torch.inf)
+    x[:, :, 3], x[:, :, 7], x[:, :, 30] = -750.0 / 1024, -650.0 / 1024, 0.0
+    x = x.to(DT[dt]).cuda()
+    cold = torch.full((batch,), 2.0 ** -10, device="cuda")
+    zeros = torch.zeros(batch, 3, device="cuda")
+    parents = torch.tensor([[-1, 0, 0]] * batch, dtype=torch.int32, device="cuda")
+    for drafts, path, token in (((0, 3, 3), [0, -1, -1], 7), ((0, 3, 7), [0, 2, -1], 7)):
+        got = rt.tree_verify(x, torch.tensor([drafts] * batch, dtype=torch.int32, device="cuda"), parents, zeros,
+                             zeros[:, 0].contiguous(), temperature=cold)
+        assert got[0].tolist() == [path] * batch and got[2].tolist() == [token] * batch
+    # One node a tree.
+    one = [t[:, :1].contiguous() for t in (torch.zeros(batch, 3, dtype=torch.int32, device="cuda"), parents, zeros)]
+    assert rt.tree_verify(x[:, :1], *one, zeros[:, 0].contiguous(), temperature=cold)[2].tolist() == [7] * batch
