@@ -629,15 +629,16 @@ int frisk_kv_pages(const frisk_kv_pages_desc* desc, void* stream);
  * token x is accepted, and the walk goes on from it, if
  *   uniform[b][t] q(x) < a(x);
  * else a becomes max(a - q, 0) over its sum (and stays if that is 0).  q is draft_probs[b][node]
- * (f32 [batch, tokens, vocab], finite and at least 0), from which all of the node's children were drawn independently (with
- * replacement: of children drawn without it the tokens are not distributed as the target's), or,
- * if NULL, certain drafts: q(x) = 1 for the child's own token.  When no child is
+ * (f32 [batch, tokens, vocab], finite and at least 0), from which all of the node's children were
+ * drawn independently (with replacement: of children drawn without it the tokens are not distributed
+ * as the target's), or, if NULL, certain drafts: q(x) = 1 for the child's own token.  When no child is
  * left, token[b] is the first v at which a summed over 0 .. v passes final_uniform[b]
- * times its whole sum.  With draft_probs each child of a node that is rejected before its last one costs a pass over
- * the row by one workgroup, and a pass goes through the rejections before it: time grows with their
- * square (64 rejected children over a vocabulary of 50257: 7 ms).  Random numbers are of [0, 1).  Probabilities are computed in 64 bits, off
- * by less than 2^-42 of themselves, what rejected drafts leave by 2^-42 of what there was before them; one below
- * 2^-1000 of its row's largest counts as 0.
+ * times its whole sum.  Random numbers are of [0, 1).  Probabilities are computed in 64 bits,
+ * off by less than 2^-42 of themselves, what rejected drafts leave by 2^-42 of what there was before
+ * them; one below 2^-1000 of its row's largest counts as 0.
+ * With draft_probs each rejected child of a node but the last costs a pass over the row by one
+ * workgroup, and a pass goes through the rejections before it: time grows with their square (64 over
+ * a vocabulary of 50257: 7 ms; hundreds over a long one: seconds and more).
  *
  * path[b] ([tokens]) lists the nodes of the walk, node 0 first, then -1; count[b] is their
  * number.  probs[b][t] (optional) is p of a node's token given its parent, 0 for nodes without
